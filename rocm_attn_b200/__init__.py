@@ -71,13 +71,17 @@ def attn_forward_batch(qs: Sequence[torch.Tensor], ks: Sequence[torch.Tensor], v
 
 
 def check_status(device: int = 0) -> int:
-    """Synchronise ``device`` and return (and clear) the kernel watchdog
-    status: 0 when every earlier launch completed, non-zero when a kernel gave
-    up on a wait (its output is then invalid)."""
+    """Synchronise ``device`` and return (and clear) the kernel status: 0 when
+    every earlier launch completed; 7 when a kernel gave up on a wait (its
+    output is then invalid); 8 when a kernel of the paged cache met a
+    block-table entry or a length that is out of range (the tokens concerned
+    were left out)."""
     return int(rocm_attn_ext.check_status(int(device)))
 
 
 from .pipeline import attn_forward_pinned  # noqa: E402  (host-resident inputs, transfers overlapped)
+from .paged import attn_decode, kv_append, kv_evict, kv_page_bounds, kv_select_pages  # noqa: E402  (paged key-value cache)
 
-__all__ = ["attn_forward", "attn_forward_batch", "attn_forward_pinned", "check_status", "rocm_attn_ext", "KERNEL_LIB_PATH",
+__all__ = ["attn_forward", "attn_forward_batch", "attn_forward_pinned", "attn_decode", "kv_append", "kv_evict",
+           "kv_page_bounds", "kv_select_pages", "check_status", "rocm_attn_ext", "KERNEL_LIB_PATH",
            "SUPPORTED_HEAD_DIMS", "SUPPORTED_DTYPES", "MAX_HEAD_DIM"]

@@ -3,13 +3,14 @@
 * ``librocm_attn.so``  -- the sm_100a kernels and the C-ABI launcher
   (``csrc/attn_kernel.cu``: tensor-core kernel and dispatch;
   ``csrc/attn_group.cu``: grouped launches of several problems;
-  ``csrc/attn_general.cu``: fp32 / other head dims), compiled by nvcc for
-  ``sm_100a`` only, with the
+  ``csrc/attn_general.cu``: fp32 / other head dims; ``csrc/attn_decode.cu``:
+  attention over a paged key-value cache; ``csrc/kv_cache.cu``: what keeps
+  that cache), compiled by nvcc for ``sm_100a`` only, with the
   CUDA runtime linked statically so the library loads without torch.
 * ``librocm_attn_wdtest.so`` -- the same kernels built with
   RA_WATCHDOG_TEST for the watchdog's GPU test (see WATCHDOG_TEST_LIB).
-* ``rocm_attn_ext*.so`` -- the PyTorch binding (``csrc/attn_torch.cpp``),
-  linked against ``librocm_attn.so`` through an ``$ORIGIN`` rpath.
+* ``rocm_attn_ext*.so`` -- the PyTorch binding (``csrc/attn_torch.cpp``,
+  ``csrc/paged_torch.cpp``), linked against ``librocm_attn.so`` through an ``$ORIGIN`` rpath.
 
 Both land next to this file so they travel with the source tree.  Run as
 ``python rocm_attn_b200/build.py`` (or through ``__graft_entry__.build()``).
@@ -104,13 +105,14 @@ def build_kernel_lib(force: bool = False, verbose: bool = False) -> str:
         # The translation units compile in parallel (each takes about a minute).
         jobs = [("attn_general.cu", "attn_general.o", ()), ("attn_kernel.cu", "attn_kernel.o", ()),
                 ("attn_group.cu", "attn_group.o", ()),
+                ("attn_decode.cu", "attn_decode.o", ()), ("kv_cache.cu", "kv_cache.o", ()),
                 ("attn_kernel.cu", "attn_kernel_wdtest.o", ("RA_WATCHDOG_TEST",))]
         with ThreadPoolExecutor(len(jobs)) as ex:
-            general, kernel, group, wd = ex.map(
+            general, kernel, group, decode, cache, wd = ex.map(
                 lambda j: _compile(os.path.join(CSRC, j[0]), os.path.join(OBJ_DIR, j[1]), defines=j[2],
                                    verbose=verbose), jobs)
-        _link([kernel, group, general], KERNEL_LIB)
-        _link([wd, group, general], WATCHDOG_TEST_LIB)
+        _link([kernel, group, general, decode, cache], KERNEL_LIB)
+        _link([wd, group, general, decode, cache], WATCHDOG_TEST_LIB)
     return KERNEL_LIB
 
 
@@ -122,9 +124,9 @@ def ext_path() -> str | None:
 
 def build_torch_ext(force: bool = False) -> str:
     """Build the PyTorch binding in place (rocm_attn_b200/rocm_attn_ext*.so)."""
-    src = os.path.join(CSRC, "attn_torch.cpp")
+    srcs = [os.path.join(CSRC, f) for f in ("attn_torch.cpp", "paged_torch.cpp")]
     existing = ext_path()
-    if not force and existing and not _newer(existing, [src, KERNEL_LIB, os.path.join(INCLUDE, "attn_kernel.h")]):
+    if not force and existing and not _newer(existing, [*srcs, KERNEL_LIB, os.path.join(INCLUDE, "attn_kernel.h")]):
         return existing
     from setuptools import setup
     from torch.utils.cpp_extension import BuildExtension, CUDAExtension
@@ -132,7 +134,7 @@ def build_torch_ext(force: bool = False) -> str:
     build_temp = os.path.join(PKG_DIR, "_build")
     ext = CUDAExtension(
         name="rocm_attn_b200.rocm_attn_ext",
-        sources=[os.path.relpath(src, REPO_DIR)],
+        sources=[os.path.relpath(s, REPO_DIR) for s in srcs],
         include_dirs=[INCLUDE],
         library_dirs=[PKG_DIR],
         libraries=["rocm_attn"],

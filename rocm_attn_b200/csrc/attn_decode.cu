@@ -1,0 +1,1023 @@
+// Attention of one new token per sequence over a paged key-value cache
+// (launch_attn_decode).
+//
+// For sequence b, query head i of the g heads that read kv head h, and the
+// tokens t of the sequence (all of them, or those of the listed pages):
+//   x_t = scale * log2(e) * (q_i . k_t),  M = max x_t,  L = sum 2^(x_t - M),
+//   o_i = sum 2^(x_t - M) v_t / L,  and 0 where L is 0 (no token),
+//   weights[b, h, t] += sum_i 2^(x_t - M_i - log2 L_i)   when asked for.
+//
+// Every K and V element is used by the g query heads of one token only, so up
+// to about 64 query heads per kv head the floor is the time to read the cache
+// once.  What that asks for:
+//   * The work is cut by tokens, not by sequences.  A unit is one (sequence,
+//     kv head, tile of query heads); its tokens are cut in tiles, and the tiles
+//     of all units in a row are dealt out in equal runs to a grid that fills
+//     the GPU once.  Each CTA works out its own run from seq_lens (a sum over
+//     the batch), so the host needs no lengths, a captured call follows
+//     lengths that change, and a ragged batch loads every SM alike.
+//   * A unit inside one run is finished by its CTA.  A unit cut by the ends of
+//     runs leaves its parts (M, L and the unscaled O, fp32) in the workspace,
+//     and a second small kernel joins them in the order of the tokens, so
+//     results do not depend on timing.  It is launched early and waits on the
+//     grid before it (programmatic launch), which hides its launch.
+//   * Each warp has its own ring of K/V chunks in shared memory filled by
+//     16-byte asynchronous copies, through page ids looked up one chunk ahead;
+//     warps meet only where a unit ends.  The chunk freed last is the scratch
+//     space of that meeting, so the ring stays full meanwhile.
+//
+// Two kernels share that frame: attn_decode_mma_kernel (fp16/bf16, D a
+// multiple of 8, 16-byte rows) on warp-level tensor cores, and
+// attn_decode_simt_kernel (fp32, any D <= 256, any strides).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include <mutex>
+#include <type_traits>
+
+#include "paged_cache.h"
+#include "sm100_ptx.cuh"
+
+namespace ra {
+
+namespace {
+
+__device__ int g_page_fault = 0;
+
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kMmaRows = 16;  // query heads per unit of the tensor-core kernel
+constexpr int kSimtRows = 8;  // ... at most, of the other one
+
+struct DecodeArgs {
+  PagedView c;
+  const void* q;
+  long long q_b, q_h;  // element strides of q over (batch, head)
+  void* out;           // [B, Hq, D] contiguous
+  int Hq, group, rows, row_tiles;  // group = Hq / heads, in row_tiles tiles of `rows` heads
+  float scale_log2;
+  const int* pages;  // [B, heads, n_pages] contiguous, or null
+  int n_pages;
+  float* x;         // [B, Hq, x_stride] scores in the exp2 domain, or null
+  long long x_stride;
+  float* lse2;      // [B, Hq] M + log2 L, or null
+  int4* meta;       // [gridDim.x]: first output row, rows, CTAs that continue the unit begun last
+  float2* part_ml;  // [2 gridDim.x][rows]
+  float* part_o;    // [2 gridDim.x][rows][D4]
+  int D4;           // D rounded up to 4
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+template <bool kBf16>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (kBf16) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+                 "{%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  } else {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+                 "{%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+}
+
+template <typename T> __device__ __forceinline__ float to_f32(T x);
+template <> __device__ __forceinline__ float to_f32<float>(float x) { return x; }
+template <> __device__ __forceinline__ float to_f32<__half>(__half x) { return __half2float(x); }
+template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T> __device__ __forceinline__ T from_f32(float x);
+template <> __device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <> __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) {
+  return __float2bfloat16_rn(x);
+}
+
+// 2^(x - m) for a running maximum that may still be -inf (no token yet).
+__device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.f : m; }
+
+// ---------------------------------------------------------------------------
+// The run of tiles of one CTA
+// ---------------------------------------------------------------------------
+
+// A place in the row of tiles: tile t of the T tiles of unit `hu` (kv head *
+// row_tiles + row tile) of sequence b.
+struct Cursor {
+  int b, hu, t, T, len;
+};
+
+template <int kTile>
+__device__ __forceinline__ int tiles_of(const DecodeArgs& a, int len) {
+  const int n = a.pages ? (len > 0 ? a.n_pages * a.c.page_size : 0) : len;
+  return (n + kTile - 1) / kTile;
+}
+
+template <int kTile>
+__device__ __forceinline__ void advance(const DecodeArgs& a, Cursor& c, int* fault) {
+  if (++c.t < c.T) return;
+  c.t = 0;
+  if (++c.hu < a.c.heads * a.row_tiles) return;
+  c.hu = 0;
+  c.T = 0;
+  while (c.T == 0 && ++c.b < a.c.B) {
+    c.len = paged_len(a.c, c.b, fault);
+    c.T = tiles_of<kTile>(a, c.len);
+  }
+}
+
+struct ScheduleSmem {
+  long long warp_sum[kWarps];
+  Cursor first;
+};
+
+// Works out this CTA's run: its first tile (returned), the number of its
+// tiles *n and the run length of the grid *per.
+template <int kTile>
+__device__ __forceinline__ Cursor schedule(const DecodeArgs& a, ScheduleSmem& s, long long* n, long long* per,
+                                           int* fault) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int seg = (a.c.B + kThreads - 1) / kThreads;
+  const int b0 = min(a.c.B, tid * seg), b1 = min(a.c.B, b0 + seg);
+  long long mine = 0;
+  for (int b = b0; b < b1; ++b) mine += tiles_of<kTile>(a, paged_len(a.c, b, fault));
+  long long upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += y;
+  }
+  if (lane == 31) s.warp_sum[warp] = upto;
+  __syncthreads();
+  long long before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += s.warp_sum[w];
+    total += s.warp_sum[w];
+  }
+  const int units = a.c.heads * a.row_tiles;
+  *per = (total * units + gridDim.x - 1) / gridDim.x;
+  const long long f0 = *per * blockIdx.x;
+  *n = max(0LL, min(*per, total * units - f0));
+  before += upto - mine;
+  if (*n > 0 && f0 >= before * units && f0 < (before + mine) * units) {
+    for (int b = b0; b < b1; ++b) {
+      const int len = paged_len(a.c, b, fault);
+      const int T = tiles_of<kTile>(a, len);
+      if (f0 < (before + T) * units) {
+        const long long in = f0 - before * units;
+        const int hu = static_cast<int>(in / T);
+        s.first = Cursor{b, hu, static_cast<int>(in - static_cast<long long>(hu) * T), T, len};
+        break;
+      }
+      before += T;
+    }
+  }
+  __syncthreads();
+  return s.first;
+}
+
+// Output rows of empty sequences are zeros.
+template <typename T>
+__device__ __forceinline__ void zero_empty_rows(const DecodeArgs& a, int* fault) {
+  const long long per_seq = static_cast<long long>(a.Hq) * a.c.D;
+  for (int b = blockIdx.x; b < a.c.B; b += gridDim.x) {
+    if (paged_len(a.c, b, fault) > 0 && !(a.pages && a.n_pages == 0)) continue;
+    T* o = static_cast<T*>(a.out) + b * per_seq;
+    for (long long i = threadIdx.x; i < per_seq; i += kThreads) o[i] = from_f32<T>(0.f);
+  }
+}
+
+// Where token `pos` of (sequence b, kv head h) lies, pos counting the tokens
+// of the listed pages when there is a list: its page (-1: no such token, or
+// no such page) and its row in that page.
+__device__ __forceinline__ void locate(const DecodeArgs& a, int b, int h, int pos, int len, int* page, int* row,
+                                       int* fault) {
+  const int ps = a.c.page_size;
+  int lp = static_cast<int>(static_cast<unsigned>(pos) / static_cast<unsigned>(ps));
+  *row = pos - lp * ps;
+  *page = -1;
+  if (a.pages) {
+    if (lp >= a.n_pages) return;
+    lp = __ldg(a.pages + (static_cast<long long>(b) * a.c.heads + h) * a.n_pages + lp);
+    // An entry that names no page of the sequence adds nothing.
+    if (lp < 0 || lp >= a.c.table_width) return;
+    pos = lp * ps + *row;
+  }
+  if (pos < len) *page = paged_page(a.c, b, lp, fault);
+}
+
+// Where a unit's result goes: the output when the whole unit was in this
+// CTA's run, otherwise a part of the workspace (the first of the CTA's two
+// for a unit begun earlier, the second for one begun here).
+struct Place {
+  bool whole;
+  long long row0;  // first output row
+  int rows, slot;
+};
+
+__device__ __forceinline__ Place place_of(const DecodeArgs& a, const Cursor& c, bool begun, long long per) {
+  const int h = c.hu / a.row_tiles, rt = c.hu - h * a.row_tiles;
+  Place p;
+  p.rows = min(a.rows, a.group - rt * a.rows);
+  p.row0 = static_cast<long long>(c.b) * a.Hq + h * a.group + rt * a.rows;
+  const bool ends = c.t + 1 == c.T;
+  p.whole = begun && ends;
+  p.slot = 2 * blockIdx.x + (begun ? 1 : 0);
+  if (begun && !ends && threadIdx.x == 0) {
+    const int later = static_cast<int>((c.T - (c.t + 1) + per - 1) / per);
+    // row0 < B * Hq, which the host keeps below 2^31
+    a.meta[blockIdx.x] = make_int4(static_cast<int>(p.row0), p.rows, later, 0);
+  }
+  return p;
+}
+
+// ---------------------------------------------------------------------------
+// Tensor-core kernel
+// ---------------------------------------------------------------------------
+
+// A warp's chunk is kKeys tokens: K rows, then V rows, of kD 16-bit elements,
+// 16-byte columns XOR-swizzled by the row so that ldmatrix reads every bank
+// once.  Its size, 4 kKeys kD bytes, is at least that of the 16 x kD fp32
+// output tile, which is what the freed chunk holds where a unit ends.
+template <int kD>
+struct MmaCfg {
+  static constexpr int kKeys = kD <= 64 ? 32 : 16;
+  static constexpr int kTile = kWarps * kKeys;
+  static constexpr int kCtas = kD <= 128 ? 2 : 1;
+  static constexpr int kStageBytes = kKeys * kD * 4;
+  static constexpr int kStages = 3;
+  static constexpr int kRingBytes = kWarps * kStages * kStageBytes;
+};
+
+template <bool kBf16, int kD, bool kWeights>
+__global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas) attn_decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
+  using C = MmaCfg<kD>;
+  using T = typename std::conditional<kBf16, __nv_bfloat16, __half>::type;
+  constexpr int kKeys = C::kKeys, kTile = C::kTile, kStages = C::kStages;
+  constexpr int kCols = kD / 8;           // 16-byte columns of a row
+  constexpr int kSteps = kD / 16;         // 16-wide steps of the head dim
+  constexpr int kCopies = kKeys * kCols / 32;  // 16-byte copies per lane for K, and for V
+  constexpr bool kQInRegs = kD <= 128;
+
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ ScheduleSmem s_sched;
+  __shared__ float s_m[2][kWarps][kMmaRows], s_l[2][kWarps][kMmaRows];
+  __shared__ uint32_t s_mask[kWarps][kStages];
+  __shared__ __align__(16) uint16_t s_q[kQInRegs ? 1 : kMmaRows * kD];
+
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int fault = 0;
+  if (threadIdx.x == 0) a.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
+  long long n, per;
+  Cursor cur = schedule<kTile>(a, s_sched, &n, &per, &fault);
+  launch_dependents();
+  zero_empty_rows<T>(a, &fault);
+
+  unsigned char* ring = smem + warp * (kStages * C::kStageBytes);
+  const uint32_t ring_addr = smem_addr(ring);
+  const T* kbase = static_cast<const T*>(a.c.k);
+  const T* vbase = static_cast<const T*>(a.c.v);
+
+  // The chunk whose copies go out next: its head, and (lane = token) the
+  // page and row of each token, looked up when the one before was issued.
+  Cursor ahead = cur;
+  long long issued = 0;
+  int page = -1, row = 0, head = 0;
+  auto look_up = [&]() {
+    page = -1;
+    if (issued < n) {
+      head = ahead.hu / a.row_tiles;
+      if (lane < kKeys)
+        locate(a, ahead.b, head, ahead.t * kTile + warp * kKeys + lane, ahead.len, &page, &row, &fault);
+      advance<kTile>(a, ahead, &fault);
+    }
+  };
+  auto issue = [&](int stage) {
+    const uint32_t mask = __ballot_sync(0xffffffffu, page >= 0);
+    if (lane == 0) s_mask[warp][stage] = mask;
+    if (mask != 0) {
+      const uint32_t dst = ring_addr + stage * C::kStageBytes;
+      const long long kh = head * a.c.ks[1], vh = head * a.c.vs[1];
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i) {
+        const int e = i * 32 + lane;
+        const int r = e / kCols, col = e % kCols;
+        const int pg = __shfl_sync(0xffffffffu, page, r), in = __shfl_sync(0xffffffffu, row, r);
+        const bool ok = pg >= 0 && col * 8 < a.c.D;
+        const long long ko = ok ? pg * a.c.ks[0] + kh + in * a.c.ks[2] + col * 8 : 0;
+        const long long vo = ok ? pg * a.c.vs[0] + vh + in * a.c.vs[2] + col * 8 : 0;
+        const uint32_t at = dst + r * (kD * 2) + ((col ^ (r & 7)) << 4);
+        cp_async16(at, kbase + ko, ok);
+        cp_async16(at + kKeys * kD * 2, vbase + vo, ok);
+      }
+    }
+    cp_async_commit();
+    ++issued;
+    look_up();
+  };
+
+  look_up();
+#pragma unroll
+  for (int s = 0; s < kStages; ++s) issue(s);
+
+  uint32_t qf[kQInRegs ? kSteps : 1][4];
+  float o[kD / 8][4];
+  float m[2], l[2];
+  bool begun = cur.t == 0, fresh = true;
+  int parity = 0, stage = 0;
+
+  for (long long i = 0; i < n; ++i) {
+    if (fresh) {
+      // A new unit: its query rows as A fragments (rows behind the last are zero).
+      const int h = cur.hu / a.row_tiles, rt = cur.hu - h * a.row_tiles;
+      const int rows = min(a.rows, a.group - rt * a.rows);
+      const T* q = static_cast<const T*>(a.q) + cur.b * a.q_b + (static_cast<long long>(h) * a.group + rt * a.rows) * a.q_h;
+      if constexpr (kQInRegs) {
+#pragma unroll
+        for (int ks = 0; ks < kSteps; ++ks)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int r = (lane >> 2) + (j & 1) * 8, d = ks * 16 + (j >> 1) * 8 + (lane & 3) * 2;
+            qf[ks][j] = (r < rows && d < a.c.D) ? __ldg(reinterpret_cast<const uint32_t*>(q + r * a.q_h + d)) : 0u;
+          }
+      } else {
+        __syncthreads();
+        for (int e = threadIdx.x; e < kMmaRows * kCols; e += kThreads) {
+          const int r = e / kCols, col = e % kCols;
+          uint4 w = make_uint4(0, 0, 0, 0);
+          if (r < rows && col * 8 < a.c.D) w = __ldg(reinterpret_cast<const uint4*>(q + r * a.q_h + col * 8));
+          *reinterpret_cast<uint4*>(s_q + r * kD + ((col ^ (r & 7)) << 3)) = w;
+        }
+        __syncthreads();
+      }
+#pragma unroll
+      for (int j = 0; j < kD / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+      m[0] = m[1] = -INFINITY;
+      l[0] = l[1] = 0.f;
+      fresh = false;
+    }
+    cp_async_wait<kStages - 1>();
+    __syncwarp();
+    const uint32_t mask = s_mask[warp][stage];
+    const uint32_t kaddr = ring_addr + stage * C::kStageBytes;
+    const uint32_t vaddr = kaddr + kKeys * kD * 2;
+    if (mask != 0 || kWeights) {
+      float s[kKeys / 8][4];
+#pragma unroll
+      for (int j = 0; j < kKeys / 8; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+      if (mask != 0) {
+#pragma unroll
+        for (int ks = 0; ks < kSteps; ++ks) {
+          uint32_t af[4];
+          if constexpr (kQInRegs) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) af[j] = qf[ks][j];
+          } else {
+            const int r = (lane & 7) + ((lane >> 3) & 1) * 8, col = ks * 2 + (lane >> 4);
+            ldsm_x4(smem_addr(s_q) + r * (kD * 2) + ((col ^ (r & 7)) << 4), af);
+          }
+#pragma unroll
+          for (int g = 0; g < kKeys / 16; ++g) {
+            uint32_t kf[4];
+            const int r = g * 16 + (lane >> 4) * 8 + (lane & 7), col = ks * 2 + ((lane >> 3) & 1);
+            ldsm_x4(kaddr + r * (kD * 2) + ((col ^ (r & 7)) << 4), kf);
+            mma16816<kBf16>(s[2 * g], af, kf[0], kf[1]);
+            mma16816<kBf16>(s[2 * g + 1], af, kf[2], kf[3]);
+          }
+        }
+      }
+      // Thread: rows lane / 4 and lane / 4 + 8, tokens 8 j + 2 (lane % 4) + {0, 1}.
+      float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int j = 0; j < kKeys / 8; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int tok = j * 8 + (lane & 3) * 2 + (e & 1);
+          s[j][e] = (mask >> tok & 1u) ? s[j][e] * a.scale_log2 : -INFINITY;
+          mx[e >> 1] = fmaxf(mx[e >> 1], s[j][e]);
+        }
+      if constexpr (kWeights) {
+        const int h = cur.hu / a.row_tiles, rt = cur.hu - h * a.row_tiles;
+        const int rows = min(a.rows, a.group - rt * a.rows);
+        const long long r0 = static_cast<long long>(cur.b) * a.Hq + h * a.group + rt * a.rows;
+        float* x = a.x + r0 * a.x_stride + cur.t * kTile + warp * kKeys + (lane & 3) * 2;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int r = (lane >> 2) + half * 8;
+          if (r < rows)
+#pragma unroll
+            for (int j = 0; j < kKeys / 8; ++j)
+              *reinterpret_cast<float2*>(x + r * a.x_stride + j * 8) = make_float2(s[j][2 * half], s[j][2 * half + 1]);
+        }
+      }
+      if (mask != 0) {
+        float f[2];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 1));
+          mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 2));
+          const float mn = fmaxf(m[half], mx[half]);
+          f[half] = ex2_approx(m[half] - finite_max(mn));
+          m[half] = mn;
+          l[half] *= f[half];
+        }
+        if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
+#pragma unroll
+          for (int j = 0; j < kD / 8; ++j) {
+            o[j][0] *= f[0];
+            o[j][1] *= f[0];
+            o[j][2] *= f[1];
+            o[j][3] *= f[1];
+          }
+        }
+        const float m0 = finite_max(m[0]), m1 = finite_max(m[1]);
+        // P is rounded to the input type for P V (half a step, 2^-9 or 2^-12
+        // of each weight); its sum is taken before the rounding.
+#pragma unroll
+        for (int g = 0; g < kKeys / 16; ++g) {
+          uint32_t pf[4];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float(&sj)[4] = s[2 * g + j];
+            sj[0] = ex2_approx(sj[0] - m0);
+            sj[1] = ex2_approx(sj[1] - m0);
+            sj[2] = ex2_approx(sj[2] - m1);
+            sj[3] = ex2_approx(sj[3] - m1);
+            l[0] += sj[0] + sj[1];
+            l[1] += sj[2] + sj[3];
+            pf[2 * j] = pack2<kBf16>(sj[0], sj[1]);
+            pf[2 * j + 1] = pack2<kBf16>(sj[2], sj[3]);
+          }
+#pragma unroll
+          for (int dt = 0; dt < kSteps; ++dt) {
+            uint32_t vf[4];
+            const int r = g * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), col = dt * 2 + (lane >> 4);
+            ldsm_x4_trans(vaddr + r * (kD * 2) + ((col ^ (r & 7)) << 4), vf);
+            mma16816<kBf16>(o[2 * dt], pf, vf[0], vf[1]);
+            mma16816<kBf16>(o[2 * dt + 1], pf, vf[2], vf[3]);
+          }
+        }
+      }
+    }
+
+    if (cur.t + 1 == cur.T || i + 1 == n) {
+      // The unit, or this CTA's part of it, ends: the warps' parts are scaled
+      // to their common maximum and summed over the chunks just freed.
+      const Place p = place_of(a, cur, begun, per);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
+        l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
+        if ((lane & 3) == 0) {
+          s_m[parity][warp][(lane >> 2) + half * 8] = m[half];
+          s_l[parity][warp][(lane >> 2) + half * 8] = l[half];
+        }
+      }
+      __syncthreads();
+      float* ot = reinterpret_cast<float*>(ring + stage * C::kStageBytes);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int r = (lane >> 2) + half * 8;
+        if (r < p.rows) {
+          float M = s_m[parity][0][r];
+#pragma unroll
+          for (int w = 1; w < kWarps; ++w) M = fmaxf(M, s_m[parity][w][r]);
+          const float f = ex2_approx(m[half] - finite_max(M));
+#pragma unroll
+          for (int j = 0; j < kD / 8; ++j) {
+            const int c4 = (2 * j + ((lane & 3) >> 1)) ^ ((r & 7) << 1);
+            *reinterpret_cast<float2*>(ot + r * kD + c4 * 4 + (lane & 1) * 2) =
+                make_float2(o[j][2 * half] * f, o[j][2 * half + 1] * f);
+          }
+        }
+      }
+      __syncthreads();
+      for (int e = threadIdx.x; e < p.rows * (kD / 4); e += kThreads) {
+        const int r = e / (kD / 4), c4 = e % (kD / 4);
+        if (c4 * 4 >= a.c.D) continue;
+        float M = s_m[parity][0][r], L = 0.f;
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) M = fmaxf(M, s_m[parity][w][r]);
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          L += s_l[parity][w][r] * ex2_approx(s_m[parity][w][r] - finite_max(M));
+          const float4 y = *reinterpret_cast<const float4*>(
+              reinterpret_cast<const float*>(smem + (w * kStages + stage) * C::kStageBytes) + r * kD +
+              ((c4 ^ ((r & 7) << 1)) << 2));
+          sum.x += y.x;
+          sum.y += y.y;
+          sum.z += y.z;
+          sum.w += y.w;
+        }
+        if (p.whole) {
+          const float inv = L == 0.f ? 0.f : 1.f / L;
+          T* out = static_cast<T*>(a.out) + (p.row0 + r) * a.c.D + c4 * 4;
+          *reinterpret_cast<uint2*>(out) =
+              make_uint2(pack2<kBf16>(sum.x * inv, sum.y * inv), pack2<kBf16>(sum.z * inv, sum.w * inv));
+          if (kWeights && c4 == 0) a.lse2[p.row0 + r] = L == 0.f ? INFINITY : M + log2f(L);
+        } else {
+          const long long at = static_cast<long long>(p.slot) * a.rows + r;
+          *reinterpret_cast<float4*>(a.part_o + at * a.D4 + c4 * 4) = sum;
+          if (c4 == 0) a.part_ml[at] = make_float2(M, L);
+        }
+      }
+      __syncthreads();  // the chunks are read before they are filled again
+      parity ^= 1;
+      begun = true;
+      fresh = true;
+    }
+    __syncwarp();
+    issue(stage);
+    stage = stage + 1 == kStages ? 0 : stage + 1;
+    advance<kTile>(a, cur, &fault);
+  }
+  cp_async_wait<0>();
+  if (fault) atomicOr(&g_page_fault, 1);
+}
+
+// ---------------------------------------------------------------------------
+// SIMT kernel: fp32, any head dim, any strides
+// ---------------------------------------------------------------------------
+
+// A warp takes 16 tokens, kKeys at a time.  Lane holds dims lane + 32 i of q,
+// K, V and O.  The kRows * kKeys dot products of a step are summed over the
+// lanes by a butterfly that halves the number of values at each step, which
+// leaves each lane one product (31 shuffles for 32 products).
+template <int kRows>
+struct SimtCfg {
+  static constexpr int kKeys = kRows >= 4 ? 32 / kRows : 8;
+  static constexpr int kChunk = 16;
+  static constexpr int kTile = kWarps * kChunk;
+};
+
+template <typename T, int kPer, int kRows, bool kWeights>
+__global__ void __launch_bounds__(kThreads) attn_decode_simt_kernel(const __grid_constant__ DecodeArgs a) {
+  using C = SimtCfg<kRows>;
+  constexpr int kKeys = C::kKeys, kTile = C::kTile, kChunk = C::kChunk;
+  constexpr int kVals = kRows * kKeys;
+  constexpr int kSame = 32 / kVals;    // lanes that hold the same product
+  constexpr int kRowLanes = 32 / kRows;  // lanes of one row
+  __shared__ ScheduleSmem s_sched;
+  __shared__ float s_m[2][kWarps][kRows], s_l[2][kWarps][kRows];
+  __shared__ float s_o[kWarps][kRows][kPer * 32];
+
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int fault = 0;
+  if (threadIdx.x == 0) a.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
+  long long n, per;
+  Cursor cur = schedule<kTile>(a, s_sched, &n, &per, &fault);
+  launch_dependents();
+  zero_empty_rows<T>(a, &fault);
+  const T* kbase = static_cast<const T*>(a.c.k);
+  const T* vbase = static_cast<const T*>(a.c.v);
+
+  float q[kRows][kPer], o[kRows][kPer];
+  float m = -INFINITY, l = 0.f;  // of the row this lane's product belongs to
+  bool begun = cur.t == 0, fresh = true;
+  int parity = 0;
+  const int my_row = lane / kRowLanes, my_key = (lane / kSame) % kKeys;
+
+  for (long long i = 0; i < n; ++i) {
+    const int h = cur.hu / a.row_tiles, rt = cur.hu - h * a.row_tiles;
+    const int rows = min(a.rows, a.group - rt * a.rows);
+    const long long row0 = static_cast<long long>(cur.b) * a.Hq + h * a.group + rt * a.rows;
+    if (fresh) {
+      const T* qp = static_cast<const T*>(a.q) + cur.b * a.q_b + (static_cast<long long>(h) * a.group + rt * a.rows) * a.q_h;
+#pragma unroll
+      for (int r = 0; r < kRows; ++r)
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+          const int d = lane + 32 * e;
+          q[r][e] = (r < rows && d < a.c.D) ? to_f32(qp[r * a.q_h + d]) : 0.f;
+          o[r][e] = 0.f;
+        }
+      m = -INFINITY;
+      l = 0.f;
+      fresh = false;
+    }
+    int page = -1, row = 0;
+    const int pos0 = cur.t * kTile + warp * kChunk;
+    if (lane < kChunk) locate(a, cur.b, h, pos0 + lane, cur.len, &page, &row, &fault);
+    const uint32_t mask = __ballot_sync(0xffffffffu, page >= 0);
+    if (mask != 0 || kWeights) {
+      const long long kh = h * a.c.ks[1], vh = h * a.c.vs[1];
+#pragma unroll 1
+      for (int k0 = 0; k0 < kChunk; k0 += kKeys) {
+        float kv[kKeys][kPer], vv[kKeys][kPer];
+#pragma unroll
+        for (int k = 0; k < kKeys; ++k) {
+          const int pg = __shfl_sync(0xffffffffu, page, k0 + k), in = __shfl_sync(0xffffffffu, row, k0 + k);
+          const T* kp = kbase + (pg >= 0 ? pg * a.c.ks[0] + kh + in * a.c.ks[2] : 0);
+          const T* vp = vbase + (pg >= 0 ? pg * a.c.vs[0] + vh + in * a.c.vs[2] : 0);
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) {
+            const int d = lane + 32 * e;
+            const bool ok = pg >= 0 && d < a.c.D;
+            kv[k][e] = ok ? to_f32(kp[d]) : 0.f;
+            vv[k][e] = ok ? to_f32(vp[d]) : 0.f;
+          }
+        }
+        float s[kVals];
+#pragma unroll
+        for (int r = 0; r < kRows; ++r)
+#pragma unroll
+          for (int k = 0; k < kKeys; ++k) {
+            float x = 0.f;
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) x = fmaf(q[r][e], kv[k][e], x);
+            s[r * kKeys + k] = x;
+          }
+        int off = 16;
+#pragma unroll
+        for (int left = kVals; left > 1; left >>= 1) {
+          const bool up = lane & off;
+#pragma unroll
+          for (int j = 0; j < left / 2; ++j) {
+            const float keep = up ? s[j + left / 2] : s[j], give = up ? s[j] : s[j + left / 2];
+            s[j] = keep + __shfl_xor_sync(0xffffffffu, give, off);
+          }
+          off >>= 1;
+        }
+#pragma unroll
+        for (int rest = kSame / 2; rest > 0; rest >>= 1) s[0] += __shfl_xor_sync(0xffffffffu, s[0], rest);
+        const float x = (mask >> (k0 + my_key) & 1u) ? s[0] * a.scale_log2 : -INFINITY;
+        if (kWeights && my_row < rows && lane % kSame == 0)
+          a.x[(row0 + my_row) * a.x_stride + pos0 + k0 + my_key] = x;
+        float mx = x;
+#pragma unroll
+        for (int w = kSame; w < kRowLanes; w <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+        const float mn = fmaxf(m, mx);
+        const float f = ex2_approx(m - finite_max(mn));
+        m = mn;
+        const float pr = ex2_approx(x - finite_max(mn));
+        float sum = pr;
+#pragma unroll
+        for (int w = kSame; w < kRowLanes; w <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+        l = l * f + sum;
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+          const float fr = __shfl_sync(0xffffffffu, f, r * kRowLanes);
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) o[r][e] *= fr;
+#pragma unroll
+          for (int k = 0; k < kKeys; ++k) {
+            const float w = __shfl_sync(0xffffffffu, pr, (r * kKeys + k) * kSame);
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) o[r][e] = fmaf(w, vv[k][e], o[r][e]);
+          }
+        }
+      }
+    }
+    if (cur.t + 1 == cur.T || i + 1 == n) {
+      const Place p = place_of(a, cur, begun, per);
+      if (lane % kRowLanes == 0) {
+        s_m[parity][warp][my_row] = m;
+        s_l[parity][warp][my_row] = l;
+      }
+#pragma unroll
+      for (int r = 0; r < kRows; ++r)
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) s_o[warp][r][lane + 32 * e] = o[r][e];
+      __syncthreads();
+      for (int e = threadIdx.x; e < p.rows * (kPer * 32); e += kThreads) {
+        const int r = e / (kPer * 32), d = e % (kPer * 32);
+        if (d >= a.c.D) continue;
+        float M = s_m[parity][0][r], L = 0.f, sum = 0.f;
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) M = fmaxf(M, s_m[parity][w][r]);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float f = ex2_approx(s_m[parity][w][r] - finite_max(M));
+          L += s_l[parity][w][r] * f;
+          sum += s_o[w][r][d] * f;
+        }
+        if (p.whole) {
+          static_cast<T*>(a.out)[(p.row0 + r) * a.c.D + d] = from_f32<T>(L == 0.f ? 0.f : sum / L);
+          if (kWeights && d == 0) a.lse2[p.row0 + r] = L == 0.f ? INFINITY : M + log2f(L);
+        } else {
+          const long long at = static_cast<long long>(p.slot) * a.rows + r;
+          a.part_o[at * a.D4 + d] = sum;
+          if (d == 0) a.part_ml[at] = make_float2(M, L);
+        }
+      }
+      __syncthreads();  // s_o is read before it is written again
+      parity ^= 1;
+      begun = true;
+      fresh = true;
+    }
+    advance<kTile>(a, cur, &fault);
+  }
+  if (fault) atomicOr(&g_page_fault, 1);
+}
+
+// ---------------------------------------------------------------------------
+// Join of units cut between CTAs, and the weights
+// ---------------------------------------------------------------------------
+
+// CTA (c, r): row r of the unit that CTA c of the grid before began and did
+// not finish, one thread per column.
+template <typename T>
+__global__ void attn_decode_join_kernel(const __grid_constant__ DecodeArgs a) {
+  grid_dependency_wait();
+  const int c = blockIdx.x, r = blockIdx.y;
+  const int4 meta = a.meta[c];
+  if (meta.z == 0 || r >= meta.y) return;
+  auto slot = [&](int i) { return static_cast<long long>(i == 0 ? 2 * c + 1 : 2 * (c + i)) * a.rows + r; };
+  float M = -INFINITY;
+  for (int i = 0; i <= meta.z; ++i) M = fmaxf(M, a.part_ml[slot(i)].x);
+  const int d = threadIdx.x;
+  float L = 0.f, sum = 0.f;
+  for (int i = 0; i <= meta.z; ++i) {
+    const float2 ml = a.part_ml[slot(i)];
+    const float f = ex2_approx(ml.x - finite_max(M));
+    L += ml.y * f;
+    if (d < a.c.D) sum += a.part_o[slot(i) * a.D4 + d] * f;
+  }
+  const long long row = meta.x + r;
+  if (d < a.c.D) static_cast<T*>(a.out)[row * a.c.D + d] = from_f32<T>(L == 0.f ? 0.f : sum / L);
+  if (a.lse2 && d == 0) a.lse2[row] = L == 0.f ? INFINITY : M + log2f(L);
+}
+
+// weights[b, h, t] += sum over the group of 2^(x_t - lse2), one thread per
+// token: reads the scores the kernel before kept.
+__global__ void __launch_bounds__(256) attn_decode_weights_kernel(const __grid_constant__ DecodeArgs a, float* weights,
+                                                                  long long w_b, long long w_h) {
+  grid_dependency_wait();
+  const int b = blockIdx.z, h = blockIdx.y;
+  int fault = 0;  // recorded by the first kernel
+  const int len = paged_len(a.c, b, &fault);
+  const int t = blockIdx.x * 256 + threadIdx.x;
+  if (t >= len) return;
+  const long long r0 = static_cast<long long>(b) * a.Hq + static_cast<long long>(h) * a.group;
+  float sum = 0.f;
+  for (int g = 0; g < a.group; ++g) sum += ex2_approx(a.x[(r0 + g) * a.x_stride + t] - a.lse2[r0 + g]);
+  float* w = weights + b * w_b + h * w_h + t;
+  *w += sum;
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+
+struct Plan {
+  bool mma;
+  int kd;  // head dim the kernel is compiled for (mma), or dims per lane (simt)
+  int rows, row_tiles, tile;
+  int grid;
+  long long x_stride;
+  size_t meta_at, ml_at, o_at, lse_at, x_at, bytes;
+};
+
+bool mma_takes(const AttnPagedCache* c) {
+  if (c->dtype == ATTN_F32 || c->D % 8 != 0) return false;
+  for (int i = 0; i < 3; ++i)
+    if (c->k_strides[i] % 8 != 0 || c->v_strides[i] % 8 != 0) return false;
+  return aligned_to(c->k, 16) && aligned_to(c->v, 16);
+}
+
+// `fast`: q and out allow the tensor-core kernel too.
+Plan make_plan(const AttnPagedCache* c, bool fast, int Hq, int n_pages, bool listed, bool weights, int sms) {
+  Plan p;
+  const int group = Hq / c->heads;
+  const int D = c->D;
+  int per_sm;
+  p.mma = fast && mma_takes(c);
+  if (p.mma) {
+    p.kd = D <= 64 ? 64 : D <= 128 ? 128 : 256;
+    p.rows = group < kMmaRows ? group : kMmaRows;
+    p.tile = p.kd == 64 ? MmaCfg<64>::kTile : p.kd == 128 ? MmaCfg<128>::kTile : MmaCfg<256>::kTile;
+    per_sm = p.kd == 64 ? MmaCfg<64>::kCtas : p.kd == 128 ? MmaCfg<128>::kCtas : MmaCfg<256>::kCtas;
+  } else {
+    p.kd = D <= 32 ? 1 : D <= 64 ? 2 : D <= 128 ? 4 : 8;
+    p.rows = group == 1 ? 1 : group <= 2 ? 2 : group <= 4 ? 4 : kSimtRows;
+    if (p.rows > group) p.rows = group;
+    p.tile = SimtCfg<8>::kTile;
+    per_sm = 4;
+  }
+  p.row_tiles = (group + p.rows - 1) / p.rows;
+  const long long capacity = static_cast<long long>(listed ? n_pages : c->table_width) * c->page_size;
+  const long long tiles = (capacity + p.tile - 1) / p.tile * c->B * c->heads * p.row_tiles;
+  long long grid = static_cast<long long>(sms) * per_sm;
+  if (grid > tiles) grid = tiles;
+  if (grid < 1) grid = 1;
+  p.grid = static_cast<int>(grid);
+  auto up = [](size_t x) { return (x + 255) & ~static_cast<size_t>(255); };
+  const size_t D4 = (D + 3) / 4 * 4;
+  p.meta_at = 0;
+  p.ml_at = up(sizeof(int4) * grid);
+  p.o_at = p.ml_at + up(sizeof(float2) * 2 * grid * p.rows);
+  p.lse_at = p.o_at + up(sizeof(float) * 2 * grid * p.rows * D4);
+  p.x_at = p.lse_at;
+  p.bytes = p.x_at;
+  p.x_stride = (capacity + p.tile - 1) / p.tile * p.tile;
+  if (weights) {
+    p.x_at += up(sizeof(float) * static_cast<size_t>(c->B) * Hq);
+    p.bytes = p.x_at + up(sizeof(float) * static_cast<size_t>(c->B) * Hq * p.x_stride);
+  }
+  return p;
+}
+
+// The checks of a call that need no device.  Returns ATTN_OK or a status.
+int check_decode(const AttnPagedCache* c, int Hq, const void* pages, int n_pages, bool weights, PagedView* view) {
+  const int st = check_paged_cache(c, kCacheK | kCacheV, view);
+  if (st != ATTN_OK) return st;
+  if (Hq < 0 || n_pages < 0) return ATTN_ERR_INVALID_ARGUMENT;
+  if (c->heads == 0 ? Hq != 0 : Hq % c->heads != 0) return ATTN_ERR_INVALID_ARGUMENT;
+  if (static_cast<long long>(c->B) * Hq > 0x7fffffffLL) return ATTN_ERR_INVALID_ARGUMENT;
+  if (static_cast<long long>(n_pages) * c->page_size > kMaxCapacity) return ATTN_ERR_INVALID_ARGUMENT;
+  if (pages && weights) return ATTN_ERR_UNSUPPORTED;
+  if (weights && (c->B > 65535 || c->heads > 65535)) return ATTN_ERR_UNSUPPORTED;
+  return ATTN_OK;
+}
+
+// The first launch on a device opts the kernel in to its shared memory and to
+// the largest shared-memory share of the SM, so that two CTAs fit.
+template <bool kBf16, int kD, bool kWeights>
+bool launch_mma(const DecodeArgs& a, int grid, cudaStream_t stream) {
+  auto kern = attn_decode_mma_kernel<kBf16, kD, kWeights>;
+  static bool done[64] = {};
+  static std::mutex mu;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+  {
+    std::lock_guard<std::mutex> g(mu);
+    if (!done[dev]) {
+      if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, MmaCfg<kD>::kRingBytes) !=
+              cudaSuccess ||
+          cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout,
+                               static_cast<int>(cudaSharedmemCarveoutMaxShared)) != cudaSuccess)
+        return false;
+      done[dev] = true;
+    }
+  }
+  kern<<<grid, kThreads, MmaCfg<kD>::kRingBytes, stream>>>(a);
+  return cudaGetLastError() == cudaSuccess;
+}
+
+template <bool kBf16, bool kWeights>
+bool launch_mma_d(const DecodeArgs& a, int kd, int grid, cudaStream_t stream) {
+  switch (kd) {
+    case 64: return launch_mma<kBf16, 64, kWeights>(a, grid, stream);
+    case 128: return launch_mma<kBf16, 128, kWeights>(a, grid, stream);
+    default: return launch_mma<kBf16, 256, kWeights>(a, grid, stream);
+  }
+}
+
+template <typename T, int kPer, bool kWeights>
+bool launch_simt_rows(const DecodeArgs& a, int grid, cudaStream_t stream) {
+  if (a.rows <= 1)
+    attn_decode_simt_kernel<T, kPer, 1, kWeights><<<grid, kThreads, 0, stream>>>(a);
+  else if (a.rows <= 2)
+    attn_decode_simt_kernel<T, kPer, 2, kWeights><<<grid, kThreads, 0, stream>>>(a);
+  else if (a.rows <= 4)
+    attn_decode_simt_kernel<T, kPer, 4, kWeights><<<grid, kThreads, 0, stream>>>(a);
+  else
+    attn_decode_simt_kernel<T, kPer, 8, kWeights><<<grid, kThreads, 0, stream>>>(a);
+  return cudaGetLastError() == cudaSuccess;
+}
+
+template <typename T, bool kWeights>
+bool launch_simt(const DecodeArgs& a, int per, int grid, cudaStream_t stream) {
+  switch (per) {
+    case 1: return launch_simt_rows<T, 1, kWeights>(a, grid, stream);
+    case 2: return launch_simt_rows<T, 2, kWeights>(a, grid, stream);
+    case 4: return launch_simt_rows<T, 4, kWeights>(a, grid, stream);
+    default: return launch_simt_rows<T, 8, kWeights>(a, grid, stream);
+  }
+}
+
+template <bool kWeights>
+bool launch_first(const DecodeArgs& a, const Plan& p, AttnDType dtype, cudaStream_t stream) {
+  if (p.mma)
+    return dtype == ATTN_BF16 ? launch_mma_d<true, kWeights>(a, p.kd, p.grid, stream)
+                              : launch_mma_d<false, kWeights>(a, p.kd, p.grid, stream);
+  switch (dtype) {
+    case ATTN_F16: return launch_simt<__half, kWeights>(a, p.kd, p.grid, stream);
+    case ATTN_BF16: return launch_simt<__nv_bfloat16, kWeights>(a, p.kd, p.grid, stream);
+    default: return launch_simt<float, kWeights>(a, p.kd, p.grid, stream);
+  }
+}
+
+}  // namespace
+
+int page_word_read_clear_decode(cudaStream_t stream, int* host) {
+  static const int zero = 0;
+  return cudaMemcpyFromSymbolAsync(host, g_page_fault, sizeof(int), 0, cudaMemcpyDeviceToHost, stream) ==
+                     cudaSuccess &&
+                 cudaMemcpyToSymbolAsync(g_page_fault, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, stream) ==
+                     cudaSuccess
+             ? 0
+             : -1;
+}
+
+}  // namespace ra
+
+extern "C" int attn_decode_workspace_bytes(const AttnPagedCache* cache, int Hq, bool listed, int n_pages, bool weights,
+                                           size_t* bytes) {
+  using namespace ra;
+  if (!bytes) return ATTN_ERR_INVALID_ARGUMENT;
+  PagedView view;
+  int st = check_decode(cache, Hq, nullptr, n_pages, weights, &view);
+  if (st != ATTN_OK) return st;
+  *bytes = 0;
+  if (cache->B == 0 || Hq == 0) return ATTN_OK;
+  st = check_device();
+  if (st != ATTN_OK) return st;
+  const int sms = sm_count();
+  // q or out may turn out to need the other kernel: room for either
+  const Plan fast = make_plan(cache, true, Hq, n_pages, listed, weights, sms);
+  const Plan other = make_plan(cache, false, Hq, n_pages, listed, weights, sms);
+  *bytes = fast.bytes > other.bytes ? fast.bytes : other.bytes;
+  return ATTN_OK;
+}
+
+extern "C" int launch_attn_decode(const AttnPagedCache* cache, const void* q, const long long* q_strides, void* out,
+                                  int Hq, float softmax_scale, const int* pages, int n_pages, float* weights,
+                                  const long long* weights_strides, void* workspace, size_t workspace_bytes,
+                                  cudaStream_t stream) {
+  using namespace ra;
+  PagedView view;
+  int st = check_decode(cache, Hq, pages, n_pages, weights != nullptr, &view);
+  if (st != ATTN_OK) return st;
+  if (cache->B == 0 || Hq == 0) return ATTN_OK;
+  if (!q || !out || !workspace || (weights && !weights_strides)) return ATTN_ERR_INVALID_ARGUMENT;
+  const int D = cache->D;
+  const long long contiguous[2] = {static_cast<long long>(Hq) * D, D};
+  const long long* qs = q_strides ? q_strides : contiguous;
+  if (qs[0] < 0 || qs[1] < 0) return ATTN_ERR_INVALID_ARGUMENT;
+  if (weights && (weights_strides[0] < 0 || weights_strides[1] < 0)) return ATTN_ERR_INVALID_ARGUMENT;
+  const size_t elem = cache->dtype == ATTN_F32 ? 4 : 2;
+  if (!aligned_to(q, elem) || !aligned_to(out, elem) || !aligned_to(pages, 4) || !aligned_to(weights, 4) ||
+      !aligned_to(workspace, 16))
+    return ATTN_ERR_MISALIGNED;
+  st = check_device();
+  if (st != ATTN_OK) return st;
+  const bool fast = aligned_to(q, 16) && aligned_to(out, 16) && qs[0] % 8 == 0 && qs[1] % 8 == 0;
+  const Plan p = make_plan(cache, fast, Hq, n_pages, pages != nullptr, weights != nullptr, sm_count());
+  if (workspace_bytes < p.bytes) return ATTN_ERR_INVALID_ARGUMENT;
+
+  float scale = softmax_scale;
+  if (!(scale > 0.f) || !isfinite(scale)) scale = 1.0f / sqrtf(static_cast<float>(D));
+  char* ws = static_cast<char*>(workspace);
+  DecodeArgs a;
+  a.c = view;
+  a.q = q;
+  a.q_b = qs[0];
+  a.q_h = qs[1];
+  a.out = out;
+  a.Hq = Hq;
+  a.group = Hq / cache->heads;
+  a.rows = p.rows;
+  a.row_tiles = p.row_tiles;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.pages = pages;
+  a.n_pages = n_pages;
+  a.x = weights ? reinterpret_cast<float*>(ws + p.x_at) : nullptr;
+  a.x_stride = p.x_stride;
+  a.lse2 = weights ? reinterpret_cast<float*>(ws + p.lse_at) : nullptr;
+  a.meta = reinterpret_cast<int4*>(ws + p.meta_at);
+  a.part_ml = reinterpret_cast<float2*>(ws + p.ml_at);
+  a.part_o = reinterpret_cast<float*>(ws + p.o_at);
+  a.D4 = (D + 3) / 4 * 4;
+
+  if (!(weights ? launch_first<true>(a, p, cache->dtype, stream) : launch_first<false>(a, p, cache->dtype, stream)))
+    return ATTN_ERR_LAUNCH;
+  const dim3 grid(p.grid, p.rows), block((D + 31) / 32 * 32);
+  bool ok;
+  switch (cache->dtype) {
+    case ATTN_F16: ok = launch_after(attn_decode_join_kernel<__half>, grid, block, stream, a); break;
+    case ATTN_BF16: ok = launch_after(attn_decode_join_kernel<__nv_bfloat16>, grid, block, stream, a); break;
+    default: ok = launch_after(attn_decode_join_kernel<float>, grid, block, stream, a); break;
+  }
+  if (ok && weights) {
+    const dim3 wgrid((view.capacity() + 255) / 256, cache->heads, cache->B);
+    ok = wgrid.x == 0 || launch_after(attn_decode_weights_kernel, wgrid, dim3(256), stream, a, weights,
+                                      weights_strides[0], weights_strides[1]);
+  }
+  return ok ? ATTN_OK : ATTN_ERR_LAUNCH;
+}

@@ -13,6 +13,7 @@
 
 #include "attn_fwd.cuh"
 #include "attn_general.h"
+#include "paged_cache.h"
 
 #include <atomic>
 #include <vector>
@@ -45,7 +46,7 @@ static int launch_impl(const FwdProblem& d, cudaStream_t stream) {
 
 // Multiprocessor count of the current device, cached per device (0 if it
 // cannot be read).
-static int sm_count() {
+int sm_count() {
   static std::atomic<int> cached[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
@@ -65,7 +66,7 @@ static int sm_count() {
 static bool d64_use_64_key_blocks(long long ctas) { return ctas >= 2LL * sm_count(); }
 
 // Compute capability 10.x check, cached per device.
-static int check_device() {
+int check_device() {
   static std::atomic<int> cached[64];  // 0 unknown, 1 ok, 2 not sm_100
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return ATTN_ERR_DEVICE;
@@ -347,11 +348,16 @@ int status_word_read_clear_single(cudaStream_t stream, int* host) {
 
 extern "C" int attn_get_status(cudaStream_t stream, int* status) {
   if (!status) return ATTN_ERR_INVALID_ARGUMENT;
-  int single = 0, grouped = 0;
+  int single = 0, grouped = 0, decode = 0, cache = 0;
   if (ra::status_word_read_clear_single(stream, &single) != 0 ||
-      ra::status_word_read_clear_grouped(stream, &grouped) != 0 || cudaStreamSynchronize(stream) != cudaSuccess)
+      ra::status_word_read_clear_grouped(stream, &grouped) != 0 ||
+      ra::page_word_read_clear_decode(stream, &decode) != 0 ||
+      ra::page_word_read_clear_cache(stream, &cache) != 0 || cudaStreamSynchronize(stream) != cudaSuccess)
     return ATTN_ERR_LAUNCH;
-  *status = (single == 0 && grouped == 0) ? ATTN_OK : ATTN_ERR_WATCHDOG;
+  if (single != 0 || grouped != 0)
+    *status = ATTN_ERR_WATCHDOG;
+  else
+    *status = (decode == 0 && cache == 0) ? ATTN_OK : ATTN_ERR_BAD_PAGE;
   return ATTN_OK;
 }
 

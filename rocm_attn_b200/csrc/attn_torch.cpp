@@ -17,7 +17,10 @@
 
 namespace py = pybind11;
 
-static const char* status_text(int s) {
+// The paged key-value cache's part of the module (paged_torch.cpp).
+void bind_paged(py::module& m);
+
+const char* status_text(int s) {
   switch (s) {
     case ATTN_OK: return "ok";
     case ATTN_ERR_INVALID_ARGUMENT: return "invalid argument";
@@ -27,6 +30,7 @@ static const char* status_text(int s) {
     case ATTN_ERR_LAUNCH: return "CUDA launch failed";
     case ATTN_ERR_DEVICE: return "the current device is not an sm_100 (B200-class) GPU";
     case ATTN_ERR_WATCHDOG: return "a kernel wait timed out; the output is invalid";
+    case ATTN_ERR_BAD_PAGE: return "a block table entry or a length was out of range";
     default: return "unknown error";
   }
 }
@@ -137,7 +141,8 @@ static std::vector<torch::Tensor> attn_forward_batch(std::vector<torch::Tensor> 
 }
 
 // Synchronises the current stream of `device` and returns (and clears) the
-// kernel watchdog status: 0 when every earlier launch completed its waits.
+// kernel status: 0 when every earlier launch completed its waits and met only
+// valid pages and lengths.
 static int check_status(int64_t device) {
   const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));
   cudaStream_t stream = at::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(device)).stream();
@@ -155,6 +160,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("ks"), py::arg("vs"), py::arg("causal") = false, py::arg("scale") = -1.0);
   m.def("check_status", &check_status, "Read and clear the kernel watchdog status", py::arg("device") = 0);
   m.def("library_version", &attn_library_version);
+  bind_paged(m);
   m.def("set_wait_limit_ns", [](uint64_t ns) { return static_cast<uint64_t>(attn_set_wait_limit_ns(ns)); },
         "Limit of each pipeline wait of the tensor-core kernel for later launches (0: default 2 s); returns the "
         "previous value. For tests of the watchdog path.",

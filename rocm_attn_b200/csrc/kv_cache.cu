@@ -1,0 +1,872 @@
+// What keeps a paged key-value cache: its writer (launch_kv_append), the page
+// bounds (launch_kv_page_bounds), the choice of pages a new token should read
+// (launch_kv_select_pages) and eviction by accumulated attention weight
+// (launch_kv_evict).  The attention that reads the cache is in attn_decode.cu.
+//
+// All of these move bytes: each row or bound is read once and written once,
+// by 16-byte accesses where D and the strides allow (element by element
+// otherwise), and the time is that of the bytes once there are enough of them.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+#include <string.h>
+
+#include <type_traits>
+
+#include "paged_cache.h"
+
+namespace ra {
+
+namespace {
+
+__device__ int g_page_fault = 0;
+
+// ---------------------------------------------------------------------------
+// Vectors of kVec elements and their elementwise minimum and maximum, NaN
+// where either is NaN
+// ---------------------------------------------------------------------------
+
+template <typename T, int kVec>
+struct alignas(sizeof(T) * kVec) Vec {
+  T v[kVec];
+};
+
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ __half min_nan(__half a, __half b) { return __hmin_nan(a, b); }
+__device__ __forceinline__ __half max_nan(__half a, __half b) { return __hmax_nan(a, b); }
+__device__ __forceinline__ __nv_bfloat16 min_nan(__nv_bfloat16 a, __nv_bfloat16 b) { return __hmin_nan(a, b); }
+__device__ __forceinline__ __nv_bfloat16 max_nan(__nv_bfloat16 a, __nv_bfloat16 b) { return __hmax_nan(a, b); }
+
+template <typename T, int kVec>
+__device__ __forceinline__ void fold(Vec<T, kVec>& lo, Vec<T, kVec>& hi, const Vec<T, kVec>& a, const Vec<T, kVec>& b) {
+  if constexpr (kVec % 2 == 0 && sizeof(T) == 2) {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+#pragma unroll
+    for (int i = 0; i < kVec / 2; ++i) {
+      T2 l, h, x, y;
+      memcpy(&l, &lo.v[2 * i], 4);
+      memcpy(&h, &hi.v[2 * i], 4);
+      memcpy(&x, &a.v[2 * i], 4);
+      memcpy(&y, &b.v[2 * i], 4);
+      l = __hmin2_nan(l, x);
+      h = __hmax2_nan(h, y);
+      memcpy(&lo.v[2 * i], &l, 4);
+      memcpy(&hi.v[2 * i], &h, 4);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      lo.v[i] = min_nan(lo.v[i], a.v[i]);
+      hi.v[i] = max_nan(hi.v[i], b.v[i]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Append and page bounds
+// ---------------------------------------------------------------------------
+
+struct RowsArgs {
+  PagedView c;
+  const void *k, *v;           // new rows (append)
+  long long k_b, k_h, k_s, v_b, v_h, v_s;
+  int S;
+  const int* new_lens;
+  void* bounds;
+  long long b_p, b_h, b_m;     // bounds strides over (page, head, min/max)
+  int runs;                    // pages a sequence may touch
+  int cols, heads_per_cta, row_lanes;
+};
+
+// CTA (b, run; heads): the rows of one page that are new (kAppend), or that
+// the sequence has there.  Thread (row lane, head, column): every
+// row_lanes-th row of one 16-byte column, four rows in flight; the row lanes'
+// minima and maxima meet in shared memory.
+template <typename T, int kVec, bool kAppend, bool kBounds>
+__global__ void __launch_bounds__(256) kv_rows_kernel(const __grid_constant__ RowsArgs a) {
+  using V = Vec<T, kVec>;
+  __shared__ V s_lo[256], s_hi[256];
+  const int b = static_cast<int>(blockIdx.x / a.runs), run = static_cast<int>(blockIdx.x - static_cast<unsigned>(b) * a.runs);
+  const int ps = a.c.page_size, cap = a.c.capacity();
+  int fault = 0;
+  long long len = __ldg(a.c.lens + b), first = 0;  // positions [first, len) are taken
+  long long start = 0;                             // position of token 0 of the new ones
+  if (kAppend) {
+    int n = a.S;
+    if (a.new_lens) {
+      n = __ldg(a.new_lens + b);
+      if (n > a.S) {
+        fault = 1;
+        n = a.S;
+      }
+      if (n < 0) n = 0;
+    }
+    start = len - n;
+    first = start > 0 ? start : 0;
+  }
+  if (len > cap) {
+    fault = 1;
+    len = cap;
+  }
+  const int lp = static_cast<int>(first / ps) + run;
+  const long long base = static_cast<long long>(lp) * ps;
+  int page = -1;
+  if (first < len && base < len) page = paged_page(a.c, b, lp, &fault);
+  if (fault && threadIdx.x == 0) atomicOr(&g_page_fault, 1);
+  if (page < 0) return;
+  const int r0 = first > base ? static_cast<int>(first - base) : 0;
+  const int r1 = len - base < ps ? static_cast<int>(len - base) : ps;
+
+  const int col = threadIdx.x % a.cols, rest = threadIdx.x / a.cols;
+  const int in_cta = rest % a.heads_per_cta, lane = rest / a.heads_per_cta;
+  const int h = blockIdx.y * a.heads_per_cta + in_cta;
+  const bool live = h < a.c.heads;
+  V lo, hi;
+  bool any = false;
+  if (live) {
+    const long long d = static_cast<long long>(col) * kVec;
+    T* ck = static_cast<T*>(a.c.k) + page * a.c.ks[0] + h * a.c.ks[1] + d;
+    T* cv = kAppend ? static_cast<T*>(a.c.v) + page * a.c.vs[0] + h * a.c.vs[1] + d : nullptr;
+    // row r of the page is new token base + r - start
+    const T* nk = kAppend ? static_cast<const T*>(a.k) + b * a.k_b + h * a.k_h + (base - start) * a.k_s + d : ck;
+    const T* nv = kAppend ? static_cast<const T*>(a.v) + b * a.v_b + h * a.v_h + (base - start) * a.v_s + d : nullptr;
+    const long long k_s = kAppend ? a.k_s : a.c.ks[2];
+    constexpr int kAhead = 4;
+    for (int r = r0 + lane; r < r1; r += kAhead * a.row_lanes) {
+      V x[kAhead], y[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int at = r + i * a.row_lanes;
+        if (at < r1) {
+          x[i] = *reinterpret_cast<const V*>(nk + at * k_s);
+          if (kAppend) y[i] = *reinterpret_cast<const V*>(nv + at * a.v_s);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int at = r + i * a.row_lanes;
+        if (at < r1) {
+          if (kAppend) {
+            *reinterpret_cast<V*>(ck + at * a.c.ks[2]) = x[i];
+            *reinterpret_cast<V*>(cv + at * a.c.vs[2]) = y[i];
+          }
+          if (kBounds) {
+            if (!any) {
+              lo = hi = x[i];
+              any = true;
+            } else {
+              fold(lo, hi, x[i], x[i]);
+            }
+          }
+        }
+      }
+    }
+  }
+  if constexpr (kBounds) {
+    if (a.row_lanes > 1) {
+      s_lo[threadIdx.x] = lo;
+      s_hi[threadIdx.x] = hi;
+      __syncthreads();
+    }
+    if (live && lane == 0) {
+      // row lane i has rows if r0 + i < r1; lane 0 always does
+      const int lanes = min(a.row_lanes, r1 - r0), step = a.cols * a.heads_per_cta;
+      for (int i = 1; i < lanes; ++i) fold(lo, hi, s_lo[threadIdx.x + i * step], s_hi[threadIdx.x + i * step]);
+      T* out = static_cast<T*>(a.bounds) + page * a.b_p + h * a.b_h + static_cast<long long>(col) * kVec;
+      V* out_lo = reinterpret_cast<V*>(out);
+      V* out_hi = reinterpret_cast<V*>(out + a.b_m);
+      if (kAppend && r0 > 0) fold(lo, hi, *out_lo, *out_hi);
+      *out_lo = lo;
+      *out_hi = hi;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Page scores
+// ---------------------------------------------------------------------------
+
+// Keys that order as unsigned integers as the values do, NaN above all, the
+// two zeros alike.
+__device__ __forceinline__ unsigned long long order_key(double x) {
+  if (x != x) return ~0ull;
+  const unsigned long long u = static_cast<unsigned long long>(__double_as_longlong(x + 0.0));
+  return (u >> 63) ? ~u : u | (1ull << 63);
+}
+__device__ __forceinline__ unsigned order_key(float x) {
+  if (x != x) return ~0u;
+  const unsigned u = __float_as_uint(x + 0.f);
+  return (u >> 31) ? ~u : u | (1u << 31);
+}
+
+template <typename T> __device__ __forceinline__ float to_f32(T x);
+template <> __device__ __forceinline__ float to_f32<float>(float x) { return x; }
+template <> __device__ __forceinline__ float to_f32<__half>(__half x) { return __half2float(x); }
+template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+struct ScoreArgs {
+  PagedView c;
+  const void* q;
+  long long q_b, q_h;
+  int group;
+  const void* bounds;
+  long long b_p, b_h, b_m;
+  unsigned long long* keys;  // [B, heads, table_width]
+  int chunks;                // CTAs per (sequence, head)
+};
+
+constexpr int kScorePages = 128;  // pages per CTA
+constexpr int kScoreLanes = 16;   // lanes per page
+
+// max(q min, q max) is q max where q >= 0 and q min where q < 0, so the sum
+// over the query heads needs only their summed positive and negative parts:
+// one fused multiply-add per bound whatever the group.  Products of 16-bit
+// values are exact in 64 bits and their sums as good as exact, so the choice
+// of pages does not depend on the order of the sum.
+template <typename T, int kVec, int kPer>
+__global__ void __launch_bounds__(256) kv_page_score_kernel(const __grid_constant__ ScoreArgs a) {
+  using V = Vec<T, kVec>;
+  __shared__ double s_up[256], s_down[256];
+  launch_dependents();
+  const int b = static_cast<int>(blockIdx.x / a.chunks), chunk = static_cast<int>(blockIdx.x - static_cast<unsigned>(b) * a.chunks);
+  const int h = blockIdx.y;
+  int fault = 0;
+  const int len = paged_len(a.c, b, &fault);
+  const int pages = static_cast<int>((static_cast<long long>(len) + a.c.page_size - 1) / a.c.page_size);
+  const int first = chunk * kScorePages, last = min(pages, first + kScorePages);
+  if (fault && threadIdx.x == 0) atomicOr(&g_page_fault, 1);
+  if (first >= last) return;
+  {
+    const int d = threadIdx.x;
+    double up = 0.0, down = 0.0;
+    if (d < a.c.D) {
+      const T* q = static_cast<const T*>(a.q) + b * a.q_b + static_cast<long long>(h) * a.group * a.q_h + d;
+      for (int g = 0; g < a.group; ++g) {
+        const double x = to_f32(q[g * a.q_h]);
+        // a NaN goes to both
+        if (!(x < 0.0)) up += x;
+        if (!(x >= 0.0)) down += x;
+      }
+    }
+    s_up[d] = up;
+    s_down[d] = down;
+  }
+  __syncthreads();
+  const int sub = threadIdx.x % kScoreLanes, slot = threadIdx.x / kScoreLanes;
+  double up[kPer][kVec], down[kPer][kVec];
+#pragma unroll
+  for (int j = 0; j < kPer; ++j)
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) {
+      const int d = (j * kScoreLanes + sub) * kVec + e;
+      up[j][e] = s_up[d & 255];
+      down[j][e] = s_down[d & 255];
+    }
+  const T* base = static_cast<const T*>(a.bounds) + h * a.b_h;
+  unsigned long long* keys = a.keys + (static_cast<long long>(b) * a.c.heads + h) * a.c.table_width;
+  constexpr int kSlots = 256 / kScoreLanes;
+#pragma unroll 4
+  for (int p0 = first; p0 < last; p0 += kSlots) {
+    const int p = p0 + slot;
+    int page = -1;
+    if (p < last) page = paged_page(a.c, b, p, &fault);
+    double sum = 0.0;
+    if (page >= 0) {
+      const T* at = base + page * a.b_p;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        const int d = (j * kScoreLanes + sub) * kVec;
+        if (d < a.c.D) {
+          const V lo = *reinterpret_cast<const V*>(at + d);
+          const V hi = *reinterpret_cast<const V*>(at + a.b_m + d);
+#pragma unroll
+          for (int e = 0; e < kVec; ++e) {
+            sum = fma(up[j][e], static_cast<double>(to_f32(hi.v[e])), sum);
+            sum = fma(down[j][e], static_cast<double>(to_f32(lo.v[e])), sum);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int o = kScoreLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    // a page the table does not name ranks last
+    if (p < last && sub == 0) keys[p] = page >= 0 ? order_key(sum) : 0ull;
+  }
+  if (fault) atomicOr(&g_page_fault, 1);
+}
+
+// ---------------------------------------------------------------------------
+// The largest `pick` of n values, in the order of their places
+// ---------------------------------------------------------------------------
+
+constexpr int kPickThreads = 512;
+constexpr int kPickItems = 8;  // consecutive places per thread and step
+
+struct PickSmem {
+  unsigned count[256];
+  unsigned scan[kPickThreads / 32][2];
+  unsigned digit, above;
+};
+
+// Threshold of the `pick` largest of key(0..n-1), 0 < pick < n: a place is
+// taken if key & mask > prefix, and the first `ties` of those that are equal.
+// Eight bits a pass from the top; a pass whose bucket is taken whole is the last.
+template <typename Key, typename Get>
+__device__ void pick_threshold(PickSmem& s, Get key, int n, int pick, Key* prefix_out, Key* mask_out, int* ties_out) {
+  const int tid = threadIdx.x;
+  Key prefix = 0, mask = 0;
+  int need = pick;
+  for (int shift = sizeof(Key) * 8 - 8; shift >= 0; shift -= 8) {
+    if (tid < 256) s.count[tid] = 0;
+    __syncthreads();
+    for (int i = tid; i < n; i += kPickThreads) {
+      const Key x = key(i);
+      if ((x & mask) == prefix) atomicAdd(&s.count[static_cast<unsigned>(x >> shift) & 255u], 1u);
+    }
+    __syncthreads();
+    if (tid < 32) {
+      // Lane 0 holds the eight largest digits.
+      unsigned c[8], sum = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum += c[j] = s.count[255 - (tid * 8 + j)];
+      unsigned upto = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (tid >= o) upto += y;
+      }
+      unsigned above = upto - sum;
+      if (above < static_cast<unsigned>(need) && upto >= static_cast<unsigned>(need)) {
+        int j = 0;
+#pragma unroll
+        for (; j < 7; ++j) {
+          if (above + c[j] >= static_cast<unsigned>(need)) break;
+          above += c[j];
+        }
+        s.digit = 255 - (tid * 8 + j);
+        s.above = above;
+      }
+    }
+    __syncthreads();
+    const unsigned digit = s.digit;
+    need -= static_cast<int>(s.above);
+    prefix |= static_cast<Key>(digit) << shift;
+    mask |= static_cast<Key>(255) << shift;
+    const bool whole = s.count[digit] == static_cast<unsigned>(need);
+    __syncthreads();
+    if (whole) break;
+  }
+  *prefix_out = prefix;
+  *mask_out = mask;
+  *ties_out = need;
+}
+
+// Calls emit(rank, place) for the taken places of [0, n) in their order.
+template <typename Key, typename Get, typename Emit>
+__device__ void pick_emit(PickSmem& s, Get key, int n, Key prefix, Key mask, int ties, Emit emit) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  unsigned gt_before = 0, eq_before = 0;
+  for (int base = 0; base < n; base += kPickThreads * kPickItems) {
+    Key x[kPickItems];
+    unsigned gt = 0, eq = 0;
+#pragma unroll
+    for (int j = 0; j < kPickItems; ++j) {
+      const int i = base + tid * kPickItems + j;
+      x[j] = i < n ? key(i) & mask : 0;
+      if (i < n) {
+        gt += x[j] > prefix;
+        eq += x[j] == prefix;
+      }
+    }
+    unsigned g = gt, e = eq;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned y = __shfl_up_sync(0xffffffffu, g, o), z = __shfl_up_sync(0xffffffffu, e, o);
+      if (lane >= o) {
+        g += y;
+        e += z;
+      }
+    }
+    if (lane == 31) {
+      s.scan[warp][0] = g;
+      s.scan[warp][1] = e;
+    }
+    __syncthreads();
+    unsigned gs = gt_before + g - gt, es = eq_before + e - eq;
+#pragma unroll
+    for (int w = 0; w < kPickThreads / 32; ++w) {
+      if (w < warp) {
+        gs += s.scan[w][0];
+        es += s.scan[w][1];
+      }
+      gt_before += s.scan[w][0];
+      eq_before += s.scan[w][1];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kPickItems; ++j) {
+      const int i = base + tid * kPickItems + j;
+      if (i >= n) break;
+      const bool is_gt = x[j] > prefix, is_eq = x[j] == prefix;
+      if (is_gt || (is_eq && es < static_cast<unsigned>(ties)))
+        emit(static_cast<int>(gs + min(es, static_cast<unsigned>(ties))), i);
+      gs += is_gt;
+      es += is_eq;
+    }
+  }
+}
+
+// CTA (head, b): the last place, and the pick - 1 largest of the others.
+__global__ void __launch_bounds__(kPickThreads) kv_pick_pages_kernel(PagedView c, const unsigned long long* keys, int top,
+                                                                     int* pages) {
+  __shared__ PickSmem s;
+  grid_dependency_wait();
+  const int h = blockIdx.x % c.heads, b = blockIdx.x / c.heads;
+  int fault = 0;  // recorded by the kernel before
+  const int len = paged_len(c, b, &fault);
+  const int n = static_cast<int>((static_cast<long long>(len) + c.page_size - 1) / c.page_size);
+  const unsigned long long* k = keys + (static_cast<long long>(b) * c.heads + h) * c.table_width;
+  int* out = pages + (static_cast<long long>(b) * c.heads + h) * top;
+  if (n <= top) {
+    for (int i = threadIdx.x; i < top; i += kPickThreads) out[i] = i < n ? i : -1;
+    return;
+  }
+  if (threadIdx.x == 0) out[top - 1] = n - 1;
+  if (top == 1) return;
+  auto key = [&](int i) { return k[i]; };
+  unsigned long long prefix, mask;
+  int ties;
+  pick_threshold<unsigned long long>(s, key, n - 1, top - 1, &prefix, &mask, &ties);
+  pick_emit<unsigned long long>(s, key, n - 1, prefix, mask, ties, [&](int rank, int i) { out[rank] = i; });
+}
+
+// ---------------------------------------------------------------------------
+// Eviction
+// ---------------------------------------------------------------------------
+
+struct EvictArgs {
+  PagedView c;
+  const float* w;
+  long long w_b, w_h;
+  const int* new_table;
+  long long new_stride;
+  int new_width, budget, recent;
+  float* new_w;
+  int* kept;
+  int* new_lens;
+  int cols, rows_per_cta, chunks;
+};
+
+// CTA (head, b): the kept positions and their weights.
+__global__ void __launch_bounds__(kPickThreads) kv_evict_pick_kernel(const __grid_constant__ EvictArgs a) {
+  __shared__ PickSmem s;
+  launch_dependents();
+  const int h = blockIdx.x % a.c.heads, b = blockIdx.x / a.c.heads;
+  int fault = 0;
+  const int n = paged_len(a.c, b, &fault);
+  if (fault && threadIdx.x == 0) atomicOr(&g_page_fault, 1);
+  const float* w = a.w + b * a.w_b + h * a.w_h;
+  const long long unit = static_cast<long long>(b) * a.c.heads + h;
+  int* kept = a.kept + unit * a.budget;
+  const int new_cap = a.new_width * a.c.page_size;
+  float* new_w = a.new_w + unit * new_cap;
+  const int m = min(n, a.budget);
+  if (h == 0 && threadIdx.x == 0) a.new_lens[b] = m;
+  for (int i = m + threadIdx.x; i < new_cap; i += kPickThreads) new_w[i] = 0.f;
+  for (int i = m + threadIdx.x; i < a.budget; i += kPickThreads) kept[i] = -1;
+  auto emit = [&](int rank, int i) {
+    kept[rank] = i;
+    new_w[rank] = w[i];
+  };
+  // positions [0, sure) compete for `pick` places, those behind are kept
+  const int pick = n <= a.budget ? 0 : a.budget - a.recent;
+  const int sure = n <= a.budget ? 0 : n - a.recent;
+  for (int i = sure + threadIdx.x; i < n; i += kPickThreads) emit(pick + i - sure, i);
+  if (pick == 0) return;
+  auto key = [&](int i) { return order_key(w[i]); };
+  unsigned prefix, mask;
+  int ties;
+  pick_threshold<unsigned>(s, key, sure, pick, &prefix, &mask, &ties);
+  pick_emit<unsigned>(s, key, sure, prefix, mask, ties, emit);
+}
+
+// CTA (b, chunk of rows; head): copies kept rows to the new pages, a column
+// of kVec elements of four rows per thread, K and V.
+template <typename T, int kVec>
+__global__ void __launch_bounds__(256) kv_evict_copy_kernel(const __grid_constant__ EvictArgs a) {
+  using V = Vec<T, kVec>;
+  constexpr int kAhead = 4;
+  grid_dependency_wait();
+  const int b = static_cast<int>(blockIdx.x / a.chunks), chunk = static_cast<int>(blockIdx.x - static_cast<unsigned>(b) * a.chunks);
+  const int h = blockIdx.y, ps = a.c.page_size;
+  int fault = 0;
+  const int m = min(paged_len(a.c, b, &fault), a.budget);
+  fault = 0;  // recorded by the kernel before
+  const int col = threadIdx.x % a.cols, lane = threadIdx.x / a.cols;
+  if (lane >= a.rows_per_cta) return;
+  const int* kept = a.kept + (static_cast<long long>(b) * a.c.heads + h) * a.budget;
+  const long long d = static_cast<long long>(col) * kVec;
+  T* ck = static_cast<T*>(a.c.k) + h * a.c.ks[1] + d;
+  T* cv = static_cast<T*>(a.c.v) + h * a.c.vs[1] + d;
+  V x[kAhead], y[kAhead];
+  int to[kAhead], row[kAhead];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) {
+    const long long place = static_cast<long long>(chunk) * (kAhead * a.rows_per_cta) + i * a.rows_per_cta + lane;
+    to[i] = -1;
+    if (place < m) {
+      const int src = kept[place];
+      const int lp = src / ps, page = paged_page(a.c, b, lp, &fault);
+      const int np = static_cast<int>(place) / ps;
+      row[i] = static_cast<int>(place) - np * ps;
+      const int t = __ldg(a.new_table + b * a.new_stride + np);
+      const bool good = static_cast<unsigned>(t) < static_cast<unsigned>(a.c.num_pages);
+      if (!good) fault = 1;
+      if (good && page >= 0) {
+        to[i] = t;
+        x[i] = *reinterpret_cast<const V*>(ck + page * a.c.ks[0] + (src - lp * ps) * a.c.ks[2]);
+        y[i] = *reinterpret_cast<const V*>(cv + page * a.c.vs[0] + (src - lp * ps) * a.c.vs[2]);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i)
+    if (to[i] >= 0) {
+      *reinterpret_cast<V*>(ck + to[i] * a.c.ks[0] + row[i] * a.c.ks[2]) = x[i];
+      *reinterpret_cast<V*>(cv + to[i] * a.c.vs[0] + row[i] * a.c.vs[2]) = y[i];
+    }
+  if (fault) atomicOr(&g_page_fault, 1);
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+
+bool all_multiples(const long long* s, int n, int of) {
+  for (int i = 0; i < n; ++i)
+    if (s[i] % of != 0) return false;
+  return true;
+}
+
+// Elements per 16-byte access when D, the given strides and pointers allow
+// them, else 1.
+struct Width {
+  int vec;
+  explicit Width(const AttnPagedCache* c) : vec(c->dtype == ATTN_F32 ? 4 : 8) {
+    if (c->D % vec != 0) vec = 1;
+  }
+  void need(const void* p, const long long* strides, int n) {
+    if (!aligned_to(p, 16) || !all_multiples(strides, n, vec)) vec = 1;
+  }
+};
+
+size_t elem_size(AttnDType t) { return t == ATTN_F32 ? 4 : 2; }
+
+template <typename T, int kVec>
+bool launch_rows_typed(const RowsArgs& a, bool append, dim3 grid, int threads, cudaStream_t stream) {
+  if (!append)
+    kv_rows_kernel<T, kVec, false, true><<<grid, threads, 0, stream>>>(a);
+  else if (a.bounds)
+    kv_rows_kernel<T, kVec, true, true><<<grid, threads, 0, stream>>>(a);
+  else
+    kv_rows_kernel<T, kVec, true, false><<<grid, threads, 0, stream>>>(a);
+  return cudaGetLastError() == cudaSuccess;
+}
+
+// rows: rows of one page that a CTA may find to do.
+int launch_rows(RowsArgs& a, AttnDType dtype, int vec, bool append, int rows, cudaStream_t stream) {
+  a.cols = a.c.D / vec;
+  a.row_lanes = 1;
+  while (a.row_lanes * 2 * a.cols <= 256 && a.row_lanes * 4 < rows) a.row_lanes *= 2;
+  a.heads_per_cta = 256 / (a.cols * a.row_lanes);
+  if (a.heads_per_cta > a.c.heads) a.heads_per_cta = a.c.heads;
+  const long long x = static_cast<long long>(a.c.B) * a.runs;
+  const int y = (a.c.heads + a.heads_per_cta - 1) / a.heads_per_cta;
+  if (x == 0) return ATTN_OK;
+  if (x > 0x7fffffffLL || y > 65535) return ATTN_ERR_INVALID_ARGUMENT;
+  const dim3 grid(static_cast<unsigned>(x), y);
+  const int threads = a.cols * a.heads_per_cta * a.row_lanes;
+  bool ok;
+  switch (dtype) {
+    case ATTN_F16:
+      ok = vec == 8 ? launch_rows_typed<__half, 8>(a, append, grid, threads, stream)
+                    : launch_rows_typed<__half, 1>(a, append, grid, threads, stream);
+      break;
+    case ATTN_BF16:
+      ok = vec == 8 ? launch_rows_typed<__nv_bfloat16, 8>(a, append, grid, threads, stream)
+                    : launch_rows_typed<__nv_bfloat16, 1>(a, append, grid, threads, stream);
+      break;
+    default:
+      ok = vec == 4 ? launch_rows_typed<float, 4>(a, append, grid, threads, stream)
+                    : launch_rows_typed<float, 1>(a, append, grid, threads, stream);
+      break;
+  }
+  return ok ? ATTN_OK : ATTN_ERR_LAUNCH;
+}
+
+bool negative(const long long* s, int n) {
+  for (int i = 0; i < n; ++i)
+    if (s[i] < 0) return true;
+  return false;
+}
+
+template <typename T, int kVec, int kPer>
+bool launch_score(const ScoreArgs& a, dim3 grid, cudaStream_t stream) {
+  kv_page_score_kernel<T, kVec, kPer><<<grid, 256, 0, stream>>>(a);
+  return cudaGetLastError() == cudaSuccess;
+}
+
+template <typename T>
+bool launch_score_typed(const ScoreArgs& a, int vec, dim3 grid, cudaStream_t stream) {
+  if (vec == 1) return launch_score<T, 1, 16>(a, grid, stream);
+  constexpr int kVec = sizeof(T) == 2 ? 8 : 4;
+  const int per = (a.c.D + kScoreLanes * kVec - 1) / (kScoreLanes * kVec);
+  if (per == 1) return launch_score<T, kVec, 1>(a, grid, stream);
+  if (per == 2) return launch_score<T, kVec, 2>(a, grid, stream);
+  return launch_score<T, kVec, 256 / (kScoreLanes * kVec)>(a, grid, stream);
+}
+
+}  // namespace
+
+int check_paged_cache(const AttnPagedCache* c, int tensors, PagedView* view) {
+  if (!c) return ATTN_ERR_INVALID_ARGUMENT;
+  if (c->dtype != ATTN_F16 && c->dtype != ATTN_BF16 && c->dtype != ATTN_F32) return ATTN_ERR_UNSUPPORTED;
+  if (c->B < 0 || c->heads < 1 || c->page_size < 1 || c->num_pages < 0 || c->table_width < 0 || c->table_stride < 0 ||
+      c->D < 1)
+    return ATTN_ERR_INVALID_ARGUMENT;
+  if (c->D > 256) return ATTN_ERR_UNSUPPORTED;
+  if (static_cast<long long>(c->table_width) * c->page_size > kMaxCapacity) return ATTN_ERR_INVALID_ARGUMENT;
+  if (c->B > 0 && (!c->seq_lens || (c->table_width > 0 && !c->block_table))) return ATTN_ERR_INVALID_ARGUMENT;
+  if (!aligned_to(c->seq_lens, 4) || !aligned_to(c->block_table, 4)) return ATTN_ERR_MISALIGNED;
+  const void* ptr[2] = {c->k, c->v};
+  const long long* st[2] = {c->k_strides, c->v_strides};
+  for (int i = 0; i < 2; ++i) {
+    if (!(tensors >> i & 1)) continue;
+    if ((c->num_pages > 0 && !ptr[i]) || negative(st[i], 3)) return ATTN_ERR_INVALID_ARGUMENT;
+    if (!aligned_to(ptr[i], elem_size(c->dtype))) return ATTN_ERR_MISALIGNED;
+  }
+  *view = PagedView{c->k,
+                    c->v,
+                    {c->k_strides[0], c->k_strides[1], c->k_strides[2]},
+                    {c->v_strides[0], c->v_strides[1], c->v_strides[2]},
+                    c->block_table,
+                    c->table_stride,
+                    c->seq_lens,
+                    c->table_width,
+                    c->num_pages,
+                    c->heads,
+                    c->page_size,
+                    c->D,
+                    c->B};
+  return ATTN_OK;
+}
+
+int page_word_read_clear_cache(cudaStream_t stream, int* host) {
+  static const int zero = 0;
+  return cudaMemcpyFromSymbolAsync(host, g_page_fault, sizeof(int), 0, cudaMemcpyDeviceToHost, stream) ==
+                     cudaSuccess &&
+                 cudaMemcpyToSymbolAsync(g_page_fault, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, stream) ==
+                     cudaSuccess
+             ? 0
+             : -1;
+}
+
+}  // namespace ra
+
+extern "C" int launch_kv_append(const AttnPagedCache* cache, const void* k, const long long* k_strides, const void* v,
+                                const long long* v_strides, int S, const int* new_lens, void* bounds,
+                                const long long* bounds_strides, cudaStream_t stream) {
+  using namespace ra;
+  PagedView view;
+  int st = check_paged_cache(cache, kCacheK | kCacheV, &view);
+  if (st != ATTN_OK) return st;
+  if (S < 0) return ATTN_ERR_INVALID_ARGUMENT;
+  if (cache->B == 0 || S == 0) return ATTN_OK;
+  if (!k || !v || !k_strides || !v_strides || negative(k_strides, 3) || negative(v_strides, 3) ||
+      (bounds && (!bounds_strides || negative(bounds_strides, 3))))
+    return ATTN_ERR_INVALID_ARGUMENT;
+  const size_t elem = elem_size(cache->dtype);
+  if (!aligned_to(k, elem) || !aligned_to(v, elem) || !aligned_to(bounds, elem) || !aligned_to(new_lens, 4))
+    return ATTN_ERR_MISALIGNED;
+  st = check_device();
+  if (st != ATTN_OK) return st;
+  Width w(cache);
+  w.need(cache->k, cache->k_strides, 3);
+  w.need(cache->v, cache->v_strides, 3);
+  w.need(k, k_strides, 3);
+  w.need(v, v_strides, 3);
+  if (bounds) w.need(bounds, bounds_strides, 3);
+  RowsArgs a = {};
+  a.c = view;
+  a.k = k;
+  a.v = v;
+  a.k_b = k_strides[0], a.k_h = k_strides[1], a.k_s = k_strides[2];
+  a.v_b = v_strides[0], a.v_h = v_strides[1], a.v_s = v_strides[2];
+  a.S = S;
+  a.new_lens = new_lens;
+  a.bounds = bounds;
+  if (bounds) a.b_p = bounds_strides[0], a.b_h = bounds_strides[1], a.b_m = bounds_strides[2];
+  // S tokens touch at most this many pages of the table
+  const long long runs = (static_cast<long long>(S) - 1 + cache->page_size - 1) / cache->page_size + 1;
+  a.runs = static_cast<int>(runs < cache->table_width ? runs : cache->table_width > 0 ? cache->table_width : 1);
+  return launch_rows(a, cache->dtype, w.vec, true, S < cache->page_size ? S : cache->page_size, stream);
+}
+
+extern "C" int launch_kv_page_bounds(const AttnPagedCache* cache, void* bounds, const long long* bounds_strides,
+                                     cudaStream_t stream) {
+  using namespace ra;
+  PagedView view;
+  int st = check_paged_cache(cache, kCacheK, &view);
+  if (st != ATTN_OK) return st;
+  if (cache->B == 0) return ATTN_OK;
+  if ((cache->num_pages > 0 && !bounds) || !bounds_strides || negative(bounds_strides, 3))
+    return ATTN_ERR_INVALID_ARGUMENT;
+  if (!aligned_to(bounds, elem_size(cache->dtype))) return ATTN_ERR_MISALIGNED;
+  st = check_device();
+  if (st != ATTN_OK) return st;
+  Width w(cache);
+  w.need(cache->k, cache->k_strides, 3);
+  w.need(bounds, bounds_strides, 3);
+  RowsArgs a = {};
+  a.c = view;
+  a.bounds = bounds;
+  a.b_p = bounds_strides[0], a.b_h = bounds_strides[1], a.b_m = bounds_strides[2];
+  a.runs = cache->table_width > 0 ? cache->table_width : 1;
+  return launch_rows(a, cache->dtype, w.vec, false, cache->page_size, stream);
+}
+
+extern "C" int kv_select_pages_workspace_bytes(const AttnPagedCache* cache, size_t* bytes) {
+  using namespace ra;
+  if (!bytes) return ATTN_ERR_INVALID_ARGUMENT;
+  PagedView view;
+  const int st = check_paged_cache(cache, 0, &view);
+  if (st != ATTN_OK) return st;
+  *bytes = sizeof(unsigned long long) * static_cast<size_t>(cache->B) * cache->heads * cache->table_width;
+  return ATTN_OK;
+}
+
+extern "C" int launch_kv_select_pages(const AttnPagedCache* cache, const void* q, const long long* q_strides, int Hq,
+                                      const void* bounds, const long long* bounds_strides, int top, int* pages,
+                                      void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+  using namespace ra;
+  PagedView view;
+  int st = check_paged_cache(cache, 0, &view);
+  if (st != ATTN_OK) return st;
+  if (top < 1 || Hq < 0 || Hq % cache->heads != 0 || cache->heads > 65535) return ATTN_ERR_INVALID_ARGUMENT;
+  if (cache->B == 0) return ATTN_OK;
+  const long long units = static_cast<long long>(cache->B) * cache->heads;
+  const int chunks = (cache->table_width + kScorePages - 1) / kScorePages;
+  if (units > 0x7fffffffLL || static_cast<long long>(cache->B) * chunks > 0x7fffffffLL)
+    return ATTN_ERR_INVALID_ARGUMENT;
+  const long long contiguous[2] = {static_cast<long long>(Hq) * cache->D, cache->D};
+  const long long* qs = q_strides ? q_strides : contiguous;
+  if ((Hq > 0 && !q) || !pages || (cache->num_pages > 0 && !bounds) || !bounds_strides || negative(bounds_strides, 3) ||
+      negative(qs, 2) || (cache->table_width > 0 && !workspace))
+    return ATTN_ERR_INVALID_ARGUMENT;
+  const size_t elem = elem_size(cache->dtype);
+  if (!aligned_to(q, elem) || !aligned_to(bounds, elem) || !aligned_to(pages, 4) || !aligned_to(workspace, 16))
+    return ATTN_ERR_MISALIGNED;
+  if (workspace_bytes < sizeof(unsigned long long) * static_cast<size_t>(units) * cache->table_width)
+    return ATTN_ERR_INVALID_ARGUMENT;
+  st = check_device();
+  if (st != ATTN_OK) return st;
+  Width w(cache);
+  w.need(bounds, bounds_strides, 3);
+  ScoreArgs a;
+  a.c = view;
+  a.q = q;
+  a.q_b = qs[0];
+  a.q_h = qs[1];
+  a.group = Hq / cache->heads;
+  a.bounds = bounds;
+  a.b_p = bounds_strides[0], a.b_h = bounds_strides[1], a.b_m = bounds_strides[2];
+  a.keys = static_cast<unsigned long long*>(workspace);
+  a.chunks = chunks;
+  if (chunks > 0) {
+    const dim3 grid(static_cast<unsigned>(cache->B) * chunks, cache->heads);
+    bool ok;
+    switch (cache->dtype) {
+      case ATTN_F16: ok = launch_score_typed<__half>(a, w.vec, grid, stream); break;
+      case ATTN_BF16: ok = launch_score_typed<__nv_bfloat16>(a, w.vec, grid, stream); break;
+      default: ok = launch_score_typed<float>(a, w.vec, grid, stream); break;
+    }
+    if (!ok) return ATTN_ERR_LAUNCH;
+  }
+  return launch_after(kv_pick_pages_kernel, dim3(static_cast<unsigned>(units)), dim3(kPickThreads), stream, view,
+                      static_cast<const unsigned long long*>(a.keys), top, pages)
+             ? ATTN_OK
+             : ATTN_ERR_LAUNCH;
+}
+
+extern "C" int launch_kv_evict(const AttnPagedCache* cache, const float* weights, const long long* weights_strides,
+                               const int* new_table, long long new_stride, int new_width, int budget, int recent,
+                               float* new_weights, int* kept, int* new_lens, cudaStream_t stream) {
+  using namespace ra;
+  PagedView view;
+  int st = check_paged_cache(cache, kCacheK | kCacheV, &view);
+  if (st != ATTN_OK) return st;
+  if (budget < 1 || recent < 0 || recent > budget || new_width < 0 || new_stride < 0 || cache->heads > 65535 ||
+      static_cast<long long>(new_width) * cache->page_size > kMaxCapacity ||
+      budget > static_cast<long long>(new_width) * cache->page_size)
+    return ATTN_ERR_INVALID_ARGUMENT;
+  if (cache->B == 0) return ATTN_OK;
+  if (!weights || !weights_strides || negative(weights_strides, 2) || !new_table || !new_weights || !kept || !new_lens)
+    return ATTN_ERR_INVALID_ARGUMENT;
+  if (!aligned_to(weights, 4) || !aligned_to(new_table, 4) || !aligned_to(new_weights, 4) || !aligned_to(kept, 4) ||
+      !aligned_to(new_lens, 4))
+    return ATTN_ERR_MISALIGNED;
+  Width w(cache);
+  w.need(cache->k, cache->k_strides, 3);
+  w.need(cache->v, cache->v_strides, 3);
+  EvictArgs a;
+  a.c = view;
+  a.w = weights;
+  a.w_b = weights_strides[0];
+  a.w_h = weights_strides[1];
+  a.new_table = new_table;
+  a.new_stride = new_stride;
+  a.new_width = new_width;
+  a.budget = budget;
+  a.recent = recent;
+  a.new_w = new_weights;
+  a.kept = kept;
+  a.new_lens = new_lens;
+  a.cols = cache->D / w.vec;
+  a.rows_per_cta = 256 / a.cols;
+  const long long units = static_cast<long long>(cache->B) * cache->heads;
+  a.chunks = (budget + 4 * a.rows_per_cta - 1) / (4 * a.rows_per_cta);
+  const long long x = static_cast<long long>(cache->B) * a.chunks;
+  if (units > 0x7fffffffLL || x > 0x7fffffffLL) return ATTN_ERR_INVALID_ARGUMENT;
+  st = check_device();
+  if (st != ATTN_OK) return st;
+  kv_evict_pick_kernel<<<static_cast<unsigned>(units), kPickThreads, 0, stream>>>(a);
+  if (cudaGetLastError() != cudaSuccess) return ATTN_ERR_LAUNCH;
+  const dim3 grid(static_cast<unsigned>(x), cache->heads), block(256);
+  bool ok;
+  switch (cache->dtype) {
+    case ATTN_F16:
+      ok = w.vec == 8 ? launch_after(kv_evict_copy_kernel<__half, 8>, grid, block, stream, a)
+                      : launch_after(kv_evict_copy_kernel<__half, 1>, grid, block, stream, a);
+      break;
+    case ATTN_BF16:
+      ok = w.vec == 8 ? launch_after(kv_evict_copy_kernel<__nv_bfloat16, 8>, grid, block, stream, a)
+                      : launch_after(kv_evict_copy_kernel<__nv_bfloat16, 1>, grid, block, stream, a);
+      break;
+    default:
+      ok = w.vec == 4 ? launch_after(kv_evict_copy_kernel<float, 4>, grid, block, stream, a)
+                      : launch_after(kv_evict_copy_kernel<float, 1>, grid, block, stream, a);
+      break;
+  }
+  return ok ? ATTN_OK : ATTN_ERR_LAUNCH;
+}

@@ -1,0 +1,91 @@
+// Internal view of a paged key-value cache, shared by the kernels that read
+// and write it (attn_decode.cu, kv_cache.cu) and by their host-side checks.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "attn_kernel.h"
+
+namespace ra {
+
+// What a kernel needs of an AttnPagedCache.  Strides are elements over (page,
+// head, row); the head dim is contiguous.
+struct PagedView {
+  void *k, *v;
+  long long ks[3], vs[3];
+  const int* table;
+  long long table_stride;
+  const int* lens;
+  int table_width, num_pages, heads, page_size, D, B;
+
+  // Token positions the block table can name; the host checks that it fits an
+  // int with room for one tile behind it.
+  __host__ __device__ int capacity() const { return table_width * page_size; }
+};
+
+// Largest capacity (table_width * page_size) the kernels take: positions,
+// rounded up by a tile, stay within an int.
+constexpr long long kMaxCapacity = 0x7fffffffLL - 65536;
+
+// Checks an AttnPagedCache (everything but the device) and fills *view.
+// tensors: which of k and v the call uses.  Returns ATTN_OK or the status the
+// entry point reports.
+constexpr int kCacheK = 1, kCacheV = 2;
+int check_paged_cache(const AttnPagedCache* c, int tensors, PagedView* view);
+
+// Compute capability 10.0 check of the current device (attn_kernel.cu), and
+// its multiprocessor count (0 if it cannot be read).
+int check_device();
+int sm_count();
+
+// Copies of the page-fault words of the two translation units into *host and
+// resets, queued on `stream` (see attn_get_status).
+int page_word_read_clear_decode(cudaStream_t stream, int* host);
+int page_word_read_clear_cache(cudaStream_t stream, int* host);
+
+inline bool aligned_to(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+#ifdef __CUDACC__
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// Launches a kernel that waits on the grid before it itself
+// (grid_dependency_wait), so that its launch overlaps that grid.
+template <typename... Params, typename... Args>
+bool launch_after(void (*kern)(Params...), dim3 grid, dim3 block, cudaStream_t stream, Args&&... args) {
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, static_cast<Args&&>(args)...) == cudaSuccess;
+}
+
+// The length of sequence b as the kernels use it: negative lengths are empty,
+// and lengths beyond the block table's capacity end there, with the fault
+// recorded.
+__device__ __forceinline__ int paged_len(const PagedView& c, int b, int* fault) {
+  const int n = __ldg(c.lens + b);
+  if (n > c.capacity()) {
+    *fault = 1;
+    return c.capacity();
+  }
+  return n > 0 ? n : 0;
+}
+
+// The physical page of logical page lp of sequence b, or -1, with the fault
+// recorded, when the table names a page outside the cache.
+__device__ __forceinline__ int paged_page(const PagedView& c, int b, int lp, int* fault) {
+  const int p = __ldg(c.table + static_cast<long long>(b) * c.table_stride + lp);
+  if (static_cast<unsigned>(p) < static_cast<unsigned>(c.num_pages)) return p;
+  *fault = 1;
+  return -1;
+}
+#endif
+
+}  // namespace ra
