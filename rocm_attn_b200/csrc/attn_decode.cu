@@ -49,8 +49,7 @@ __device__ int g_page_fault = 0;
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kMmaRows = 16;  // query heads per unit of the tensor-core kernel
-constexpr int kSimtRows = 8;  // ... at most, of the other one
+constexpr int kSimtRows = 8;  // query heads per unit of the SIMT kernel, at most
 
 struct DecodeArgs {
   PagedView c;
@@ -259,10 +258,18 @@ __device__ __forceinline__ Place place_of(const DecodeArgs& a, const Cursor& c, 
 // Tensor-core kernel
 // ---------------------------------------------------------------------------
 
+// Products are taken with the tokens (then the head dim) as the rows of the
+// m16n8k16 product and eight query heads as its columns: S^T = K Q^T and O^T =
+// V^T P^T.  A group of up to eight heads then fills a product that the other
+// way round it would half waste, with half the registers for O and Q; groups
+// of up to 32 heads take two or four column tiles over the same K and V
+// fragments.  P^T comes out of S^T's accumulators transposed against what the
+// second product reads, which one 8x8 transpose (movmatrix) per 8 tokens mends.
+//
 // A warp's chunk is kKeys tokens: K rows, then V rows, of kD 16-bit elements,
 // 16-byte columns XOR-swizzled by the row so that ldmatrix reads every bank
-// once.  Its size, 4 kKeys kD bytes, is at least that of the 16 x kD fp32
-// output tile, which is what the freed chunk holds where a unit ends.
+// once.  Its size, 4 kKeys kD bytes, is that of 16 rows of O in fp32 or more,
+// which is what the freed chunk holds where a unit ends.
 template <int kD>
 struct MmaCfg {
   static constexpr int kKeys = kD <= 64 ? 32 : 16;
@@ -271,23 +278,28 @@ struct MmaCfg {
   static constexpr int kStageBytes = kKeys * kD * 4;
   static constexpr int kStages = 3;
   static constexpr int kRingBytes = kWarps * kStages * kStageBytes;
+  static constexpr int kMaxHeads = kD <= 128 ? 32 : 16;  // query heads per unit
 };
 
-template <bool kBf16, int kD, bool kWeights>
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+template <bool kBf16, int kD, int kNT, bool kWeights>
 __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas) attn_decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
   using C = MmaCfg<kD>;
   using T = typename std::conditional<kBf16, __nv_bfloat16, __half>::type;
   constexpr int kKeys = C::kKeys, kTile = C::kTile, kStages = C::kStages;
-  constexpr int kCols = kD / 8;           // 16-byte columns of a row
-  constexpr int kSteps = kD / 16;         // 16-wide steps of the head dim
+  constexpr int kCols = kD / 8;                // 16-byte columns of a row
+  constexpr int kSteps = kD / 16;              // 16-wide steps of the head dim
   constexpr int kCopies = kKeys * kCols / 32;  // 16-byte copies per lane for K, and for V
-  constexpr bool kQInRegs = kD <= 128;
 
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ ScheduleSmem s_sched;
-  __shared__ float s_m[2][kWarps][kMmaRows], s_l[2][kWarps][kMmaRows];
+  __shared__ float s_m[2][kWarps][8 * kNT], s_l[2][kWarps][8 * kNT];
   __shared__ uint32_t s_mask[kWarps][kStages];
-  __shared__ __align__(16) uint16_t s_q[kQInRegs ? 1 : kMmaRows * kD];
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int fault = 0;
@@ -301,6 +313,8 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas) attn_decode_mma_k
   const uint32_t ring_addr = smem_addr(ring);
   const T* kbase = static_cast<const T*>(a.c.k);
   const T* vbase = static_cast<const T*>(a.c.v);
+  // Where 16 divides the page size, 16 tokens in a row are rows of one page.
+  const bool one_page = a.c.page_size % 16 == 0;
 
   // The chunk whose copies go out next: its head, and (lane = token) the
   // page and row of each token, looked up when the one before was issued.
@@ -322,17 +336,36 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas) attn_decode_mma_k
     if (mask != 0) {
       const uint32_t dst = ring_addr + stage * C::kStageBytes;
       const long long kh = head * a.c.ks[1], vh = head * a.c.vs[1];
+      if (one_page) {
+        // The first of 16 tokens has a page if any has.
 #pragma unroll
-      for (int i = 0; i < kCopies; ++i) {
-        const int e = i * 32 + lane;
-        const int r = e / kCols, col = e % kCols;
-        const int pg = __shfl_sync(0xffffffffu, page, r), in = __shfl_sync(0xffffffffu, row, r);
-        const bool ok = pg >= 0 && col * 8 < a.c.D;
-        const long long ko = ok ? pg * a.c.ks[0] + kh + in * a.c.ks[2] + col * 8 : 0;
-        const long long vo = ok ? pg * a.c.vs[0] + vh + in * a.c.vs[2] + col * 8 : 0;
-        const uint32_t at = dst + r * (kD * 2) + ((col ^ (r & 7)) << 4);
-        cp_async16(at, kbase + ko, ok);
-        cp_async16(at + kKeys * kD * 2, vbase + vo, ok);
+        for (int g = 0; g < kKeys / 16; ++g) {
+          const int pg = __shfl_sync(0xffffffffu, page, g * 16), in = __shfl_sync(0xffffffffu, row, g * 16);
+          const T* kp = kbase + pg * a.c.ks[0] + kh + in * a.c.ks[2];
+          const T* vp = vbase + pg * a.c.vs[0] + vh + in * a.c.vs[2];
+#pragma unroll
+          for (int i = 0; i < kCols / 2; ++i) {
+            const int e = i * 32 + lane;
+            const int r = e / kCols, col = e % kCols, tok = g * 16 + r;
+            const bool ok = (mask >> tok & 1u) && col * 8 < a.c.D;
+            const uint32_t at = dst + tok * (kD * 2) + ((col ^ (r & 7)) << 4);
+            cp_async16(at, ok ? kp + r * a.c.ks[2] + col * 8 : kbase, ok);
+            cp_async16(at + kKeys * kD * 2, ok ? vp + r * a.c.vs[2] + col * 8 : vbase, ok);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+          const int e = i * 32 + lane;
+          const int r = e / kCols, col = e % kCols;
+          const int pg = __shfl_sync(0xffffffffu, page, r), in = __shfl_sync(0xffffffffu, row, r);
+          const bool ok = pg >= 0 && col * 8 < a.c.D;
+          const long long ko = ok ? pg * a.c.ks[0] + kh + in * a.c.ks[2] + col * 8 : 0;
+          const long long vo = ok ? pg * a.c.vs[0] + vh + in * a.c.vs[2] + col * 8 : 0;
+          const uint32_t at = dst + r * (kD * 2) + ((col ^ (r & 7)) << 4);
+          cp_async16(at, kbase + ko, ok);
+          cp_async16(at + kKeys * kD * 2, vbase + vo, ok);
+        }
       }
     }
     cp_async_commit();
@@ -344,40 +377,33 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas) attn_decode_mma_k
 #pragma unroll
   for (int s = 0; s < kStages; ++s) issue(s);
 
-  uint32_t qf[kQInRegs ? kSteps : 1][4];
-  float o[kD / 8][4];
-  float m[2], l[2];
+  uint32_t qf[kNT][kSteps][2];
+  float o[kNT][kSteps][4];
+  float m[kNT][2], l[kNT][2];  // of query heads 8 t + 2 (lane % 4) + {0, 1}
   bool begun = cur.t == 0, fresh = true;
   int parity = 0, stage = 0;
 
   for (long long i = 0; i < n; ++i) {
     if (fresh) {
-      // A new unit: its query rows as A fragments (rows behind the last are zero).
+      // A new unit: its query heads as B fragments (heads behind the last are zero).
       const int h = cur.hu / a.row_tiles, rt = cur.hu - h * a.row_tiles;
       const int rows = min(a.rows, a.group - rt * a.rows);
       const T* q = static_cast<const T*>(a.q) + cur.b * a.q_b + (static_cast<long long>(h) * a.group + rt * a.rows) * a.q_h;
-      if constexpr (kQInRegs) {
 #pragma unroll
-        for (int ks = 0; ks < kSteps; ++ks)
+      for (int t = 0; t < kNT; ++t) {
+        const int r = t * 8 + (lane >> 2);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int r = (lane >> 2) + (j & 1) * 8, d = ks * 16 + (j >> 1) * 8 + (lane & 3) * 2;
-            qf[ks][j] = (r < rows && d < a.c.D) ? __ldg(reinterpret_cast<const uint32_t*>(q + r * a.q_h + d)) : 0u;
+        for (int ks = 0; ks < kSteps; ++ks) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int d = ks * 16 + j * 8 + (lane & 3) * 2;
+            qf[t][ks][j] = (r < rows && d < a.c.D) ? __ldg(reinterpret_cast<const uint32_t*>(q + r * a.q_h + d)) : 0u;
           }
-      } else {
-        __syncthreads();
-        for (int e = threadIdx.x; e < kMmaRows * kCols; e += kThreads) {
-          const int r = e / kCols, col = e % kCols;
-          uint4 w = make_uint4(0, 0, 0, 0);
-          if (r < rows && col * 8 < a.c.D) w = __ldg(reinterpret_cast<const uint4*>(q + r * a.q_h + col * 8));
-          *reinterpret_cast<uint4*>(s_q + r * kD + ((col ^ (r & 7)) << 3)) = w;
+          o[t][ks][0] = o[t][ks][1] = o[t][ks][2] = o[t][ks][3] = 0.f;
         }
-        __syncthreads();
+        m[t][0] = m[t][1] = -INFINITY;
+        l[t][0] = l[t][1] = 0.f;
       }
-#pragma unroll
-      for (int j = 0; j < kD / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-      m[0] = m[1] = -INFINITY;
-      l[0] = l[1] = 0.f;
       fresh = false;
     }
     cp_async_wait<kStages - 1>();
@@ -386,167 +412,158 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas) attn_decode_mma_k
     const uint32_t kaddr = ring_addr + stage * C::kStageBytes;
     const uint32_t vaddr = kaddr + kKeys * kD * 2;
     if (mask != 0 || kWeights) {
-      float s[kKeys / 8][4];
 #pragma unroll
-      for (int j = 0; j < kKeys / 8; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
-      if (mask != 0) {
+      for (int g = 0; g < kKeys / 16; ++g) {
+        // Scores of 16 tokens: thread has tokens lane / 4 + {0, 8} of its two
+        // heads.  Even and odd steps of the head dim in two accumulators.
+        float s[kNT][4], s2[kNT][4];
+#pragma unroll
+        for (int t = 0; t < kNT; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[t][e] = s2[t][e] = 0.f;
 #pragma unroll
         for (int ks = 0; ks < kSteps; ++ks) {
-          uint32_t af[4];
-          if constexpr (kQInRegs) {
+          uint32_t kf[4];
+          const int r = g * 16 + (lane & 15), col = ks * 2 + (lane >> 4);
+          ldsm_x4(kaddr + r * (kD * 2) + ((col ^ (r & 7)) << 4), kf);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) af[j] = qf[ks][j];
-          } else {
-            const int r = (lane & 7) + ((lane >> 3) & 1) * 8, col = ks * 2 + (lane >> 4);
-            ldsm_x4(smem_addr(s_q) + r * (kD * 2) + ((col ^ (r & 7)) << 4), af);
-          }
-#pragma unroll
-          for (int g = 0; g < kKeys / 16; ++g) {
-            uint32_t kf[4];
-            const int r = g * 16 + (lane >> 4) * 8 + (lane & 7), col = ks * 2 + ((lane >> 3) & 1);
-            ldsm_x4(kaddr + r * (kD * 2) + ((col ^ (r & 7)) << 4), kf);
-            mma16816<kBf16>(s[2 * g], af, kf[0], kf[1]);
-            mma16816<kBf16>(s[2 * g + 1], af, kf[2], kf[3]);
-          }
+          for (int t = 0; t < kNT; ++t)
+            mma16816<kBf16>(ks % 2 ? s2[t] : s[t], kf, qf[t][ks][0], qf[t][ks][1]);
         }
-      }
-      // Thread: rows lane / 4 and lane / 4 + 8, tokens 8 j + 2 (lane % 4) + {0, 1}.
-      float mx[2] = {-INFINITY, -INFINITY};
+        const bool live[2] = {(mask >> (g * 16 + (lane >> 2)) & 1u) != 0, (mask >> (g * 16 + 8 + (lane >> 2)) & 1u) != 0};
+        uint32_t pf[kNT][2];
 #pragma unroll
-      for (int j = 0; j < kKeys / 8; ++j)
+        for (int t = 0; t < kNT; ++t) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int tok = j * 8 + (lane & 3) * 2 + (e & 1);
-          s[j][e] = (mask >> tok & 1u) ? s[j][e] * a.scale_log2 : -INFINITY;
-          mx[e >> 1] = fmaxf(mx[e >> 1], s[j][e]);
-        }
-      if constexpr (kWeights) {
-        const int h = cur.hu / a.row_tiles, rt = cur.hu - h * a.row_tiles;
-        const int rows = min(a.rows, a.group - rt * a.rows);
-        const long long r0 = static_cast<long long>(cur.b) * a.Hq + h * a.group + rt * a.rows;
-        float* x = a.x + r0 * a.x_stride + cur.t * kTile + warp * kKeys + (lane & 3) * 2;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int r = (lane >> 2) + half * 8;
-          if (r < rows)
-#pragma unroll
-            for (int j = 0; j < kKeys / 8; ++j)
-              *reinterpret_cast<float2*>(x + r * a.x_stride + j * 8) = make_float2(s[j][2 * half], s[j][2 * half + 1]);
-        }
-      }
-      if (mask != 0) {
-        float f[2];
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 1));
-          mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 2));
-          const float mn = fmaxf(m[half], mx[half]);
-          f[half] = ex2_approx(m[half] - finite_max(mn));
-          m[half] = mn;
-          l[half] *= f[half];
-        }
-        if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
-#pragma unroll
-          for (int j = 0; j < kD / 8; ++j) {
-            o[j][0] *= f[0];
-            o[j][1] *= f[0];
-            o[j][2] *= f[1];
-            o[j][3] *= f[1];
+          for (int e = 0; e < 4; ++e) s[t][e] = live[e >> 1] ? (s[t][e] + s2[t][e]) * a.scale_log2 : -INFINITY;
+          if constexpr (kWeights) {
+            const int h = cur.hu / a.row_tiles, rt = cur.hu - h * a.row_tiles;
+            const int rows = min(a.rows, a.group - rt * a.rows);
+            const long long r0 = static_cast<long long>(cur.b) * a.Hq + h * a.group + rt * a.rows;
+            const int r = t * 8 + (lane & 3) * 2;
+            float* x = a.x + (r0 + r) * a.x_stride + cur.t * kTile + warp * kKeys + g * 16 + (lane >> 2);
+            if (r < rows) x[0] = s[t][0], x[8] = s[t][2];
+            if (r + 1 < rows) x[a.x_stride] = s[t][1], x[a.x_stride + 8] = s[t][3];
           }
+          float f[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float mx = fmaxf(s[t][e], s[t][e + 2]);
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            const float mn = fmaxf(m[t][e], mx);
+            f[e] = ex2_approx(m[t][e] - finite_max(mn));
+            m[t][e] = mn;
+          }
+          if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
+            l[t][0] *= f[0];
+            l[t][1] *= f[1];
+#pragma unroll
+            for (int j = 0; j < kSteps; ++j) {
+              o[t][j][0] *= f[0];
+              o[t][j][1] *= f[1];
+              o[t][j][2] *= f[0];
+              o[t][j][3] *= f[1];
+            }
+          }
+          const float m0 = finite_max(m[t][0]), m1 = finite_max(m[t][1]);
+          // P is rounded to the input type for P V (half a step, 2^-9 or 2^-12
+          // of each weight); its sum is taken before the rounding.
+          s[t][0] = ex2_approx(s[t][0] - m0);
+          s[t][1] = ex2_approx(s[t][1] - m1);
+          s[t][2] = ex2_approx(s[t][2] - m0);
+          s[t][3] = ex2_approx(s[t][3] - m1);
+          l[t][0] += s[t][0] + s[t][2];
+          l[t][1] += s[t][1] + s[t][3];
+          pf[t][0] = transpose_8x8(pack2<kBf16>(s[t][0], s[t][1]));
+          pf[t][1] = transpose_8x8(pack2<kBf16>(s[t][2], s[t][3]));
         }
-        const float m0 = finite_max(m[0]), m1 = finite_max(m[1]);
-        // P is rounded to the input type for P V (half a step, 2^-9 or 2^-12
-        // of each weight); its sum is taken before the rounding.
 #pragma unroll
-        for (int g = 0; g < kKeys / 16; ++g) {
-          uint32_t pf[4];
+        for (int j = 0; j < kSteps; ++j) {
+          uint32_t vf[4];
+          const int r = g * 16 + (lane >> 4) * 8 + (lane & 7), col = j * 2 + ((lane >> 3) & 1);
+          ldsm_x4_trans(vaddr + r * (kD * 2) + ((col ^ (r & 7)) << 4), vf);
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            float(&sj)[4] = s[2 * g + j];
-            sj[0] = ex2_approx(sj[0] - m0);
-            sj[1] = ex2_approx(sj[1] - m0);
-            sj[2] = ex2_approx(sj[2] - m1);
-            sj[3] = ex2_approx(sj[3] - m1);
-            l[0] += sj[0] + sj[1];
-            l[1] += sj[2] + sj[3];
-            pf[2 * j] = pack2<kBf16>(sj[0], sj[1]);
-            pf[2 * j + 1] = pack2<kBf16>(sj[2], sj[3]);
-          }
-#pragma unroll
-          for (int dt = 0; dt < kSteps; ++dt) {
-            uint32_t vf[4];
-            const int r = g * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), col = dt * 2 + (lane >> 4);
-            ldsm_x4_trans(vaddr + r * (kD * 2) + ((col ^ (r & 7)) << 4), vf);
-            mma16816<kBf16>(o[2 * dt], pf, vf[0], vf[1]);
-            mma16816<kBf16>(o[2 * dt + 1], pf, vf[2], vf[3]);
-          }
+          for (int t = 0; t < kNT; ++t) mma16816<kBf16>(o[t][j], vf, pf[t][0], pf[t][1]);
         }
       }
     }
 
     if (cur.t + 1 == cur.T || i + 1 == n) {
       // The unit, or this CTA's part of it, ends: the warps' parts are scaled
-      // to their common maximum and summed over the chunks just freed.
+      // to their common maximum and summed over the chunks just freed, 16 heads
+      // at a time.
       const Place p = place_of(a, cur, begun, per);
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
-        l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
-        if ((lane & 3) == 0) {
-          s_m[parity][warp][(lane >> 2) + half * 8] = m[half];
-          s_l[parity][warp][(lane >> 2) + half * 8] = l[half];
+      for (int t = 0; t < kNT; ++t)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], 4);
+          l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], 8);
+          l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], 16);
+          if (lane < 4) {
+            s_m[parity][warp][t * 8 + lane * 2 + e] = m[t][e];
+            s_l[parity][warp][t * 8 + lane * 2 + e] = l[t][e];
+          }
         }
-      }
       __syncthreads();
       float* ot = reinterpret_cast<float*>(ring + stage * C::kStageBytes);
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int r = (lane >> 2) + half * 8;
-        if (r < p.rows) {
-          float M = s_m[parity][0][r];
+      for (int t0 = 0; t0 < kNT; t0 += 2) {
+#pragma unroll
+        for (int t = t0; t < (t0 + 2 < kNT ? t0 + 2 : kNT); ++t)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int r = t * 8 + (lane & 3) * 2 + e, at = r - t0 * 8;
+            if (r < p.rows) {
+              float M = s_m[parity][0][r];
+#pragma unroll
+              for (int w = 1; w < kWarps; ++w) M = fmaxf(M, s_m[parity][w][r]);
+              const float f = ex2_approx(m[t][e] - finite_max(M));
+#pragma unroll
+              for (int j = 0; j < kSteps; ++j)
+#pragma unroll
+                for (int up = 0; up < 2; ++up) {
+                  const int d = j * 16 + up * 8 + (lane >> 2);
+                  ot[at * kD + (((d >> 2) ^ ((lane & 3) << 1)) << 2) + (d & 3)] = o[t][j][2 * up + e] * f;
+                }
+            }
+          }
+        __syncthreads();
+        const int here = min(p.rows - t0 * 8, 16);
+        for (int e = threadIdx.x; e < here * (kD / 4); e += kThreads) {
+          const int at = e / (kD / 4), c4 = e % (kD / 4), r = t0 * 8 + at;
+          if (c4 * 4 >= a.c.D) continue;
+          float M = s_m[parity][0][r], L = 0.f;
 #pragma unroll
           for (int w = 1; w < kWarps; ++w) M = fmaxf(M, s_m[parity][w][r]);
-          const float f = ex2_approx(m[half] - finite_max(M));
+          float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-          for (int j = 0; j < kD / 8; ++j) {
-            const int c4 = (2 * j + ((lane & 3) >> 1)) ^ ((r & 7) << 1);
-            *reinterpret_cast<float2*>(ot + r * kD + c4 * 4 + (lane & 1) * 2) =
-                make_float2(o[j][2 * half] * f, o[j][2 * half + 1] * f);
+          for (int w = 0; w < kWarps; ++w) {
+            L += s_l[parity][w][r] * ex2_approx(s_m[parity][w][r] - finite_max(M));
+            const float4 y = *reinterpret_cast<const float4*>(
+                reinterpret_cast<const float*>(smem + (w * kStages + stage) * C::kStageBytes) + at * kD +
+                ((c4 ^ ((at >> 1 & 3) << 1)) << 2));
+            sum.x += y.x;
+            sum.y += y.y;
+            sum.z += y.z;
+            sum.w += y.w;
+          }
+          if (p.whole) {
+            const float inv = L == 0.f ? 0.f : 1.f / L;
+            T* out = static_cast<T*>(a.out) + (p.row0 + r) * a.c.D + c4 * 4;
+            *reinterpret_cast<uint2*>(out) =
+                make_uint2(pack2<kBf16>(sum.x * inv, sum.y * inv), pack2<kBf16>(sum.z * inv, sum.w * inv));
+            if (kWeights && c4 == 0) a.lse2[p.row0 + r] = L == 0.f ? INFINITY : M + log2f(L);
+          } else {
+            const long long slot = static_cast<long long>(p.slot) * a.rows + r;
+            *reinterpret_cast<float4*>(a.part_o + slot * a.D4 + c4 * 4) = sum;
+            if (c4 == 0) a.part_ml[slot] = make_float2(M, L);
           }
         }
+        __syncthreads();  // the chunks are read before they are filled again
       }
-      __syncthreads();
-      for (int e = threadIdx.x; e < p.rows * (kD / 4); e += kThreads) {
-        const int r = e / (kD / 4), c4 = e % (kD / 4);
-        if (c4 * 4 >= a.c.D) continue;
-        float M = s_m[parity][0][r], L = 0.f;
-#pragma unroll
-        for (int w = 1; w < kWarps; ++w) M = fmaxf(M, s_m[parity][w][r]);
-        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          L += s_l[parity][w][r] * ex2_approx(s_m[parity][w][r] - finite_max(M));
-          const float4 y = *reinterpret_cast<const float4*>(
-              reinterpret_cast<const float*>(smem + (w * kStages + stage) * C::kStageBytes) + r * kD +
-              ((c4 ^ ((r & 7) << 1)) << 2));
-          sum.x += y.x;
-          sum.y += y.y;
-          sum.z += y.z;
-          sum.w += y.w;
-        }
-        if (p.whole) {
-          const float inv = L == 0.f ? 0.f : 1.f / L;
-          T* out = static_cast<T*>(a.out) + (p.row0 + r) * a.c.D + c4 * 4;
-          *reinterpret_cast<uint2*>(out) =
-              make_uint2(pack2<kBf16>(sum.x * inv, sum.y * inv), pack2<kBf16>(sum.z * inv, sum.w * inv));
-          if (kWeights && c4 == 0) a.lse2[p.row0 + r] = L == 0.f ? INFINITY : M + log2f(L);
-        } else {
-          const long long at = static_cast<long long>(p.slot) * a.rows + r;
-          *reinterpret_cast<float4*>(a.part_o + at * a.D4 + c4 * 4) = sum;
-          if (c4 == 0) a.part_ml[at] = make_float2(M, L);
-        }
-      }
-      __syncthreads();  // the chunks are read before they are filled again
       parity ^= 1;
       begun = true;
       fresh = true;
@@ -809,7 +826,8 @@ Plan make_plan(const AttnPagedCache* c, bool fast, int Hq, int n_pages, bool lis
   p.mma = fast && mma_takes(c);
   if (p.mma) {
     p.kd = D <= 64 ? 64 : D <= 128 ? 128 : 256;
-    p.rows = group < kMmaRows ? group : kMmaRows;
+    const int most = p.kd == 256 ? MmaCfg<256>::kMaxHeads : MmaCfg<128>::kMaxHeads;
+    p.rows = group < most ? group : most;
     p.tile = p.kd == 64 ? MmaCfg<64>::kTile : p.kd == 128 ? MmaCfg<128>::kTile : MmaCfg<256>::kTile;
     per_sm = p.kd == 64 ? MmaCfg<64>::kCtas : p.kd == 128 ? MmaCfg<128>::kCtas : MmaCfg<256>::kCtas;
   } else {
@@ -857,9 +875,9 @@ int check_decode(const AttnPagedCache* c, int Hq, const void* pages, int n_pages
 
 // The first launch on a device opts the kernel in to its shared memory and to
 // the largest shared-memory share of the SM, so that two CTAs fit.
-template <bool kBf16, int kD, bool kWeights>
+template <bool kBf16, int kD, int kNT, bool kWeights>
 bool launch_mma(const DecodeArgs& a, int grid, cudaStream_t stream) {
-  auto kern = attn_decode_mma_kernel<kBf16, kD, kWeights>;
+  auto kern = attn_decode_mma_kernel<kBf16, kD, kNT, kWeights>;
   static bool done[64] = {};
   static std::mutex mu;
   int dev = 0;
@@ -879,12 +897,21 @@ bool launch_mma(const DecodeArgs& a, int grid, cudaStream_t stream) {
   return cudaGetLastError() == cudaSuccess;
 }
 
+// Column tiles of eight query heads: 1, 2 or 4.
+template <bool kBf16, int kD, bool kWeights>
+bool launch_mma_tiles(const DecodeArgs& a, int grid, cudaStream_t stream) {
+  if (a.rows <= 8) return launch_mma<kBf16, kD, 1, kWeights>(a, grid, stream);
+  if (a.rows <= 16) return launch_mma<kBf16, kD, 2, kWeights>(a, grid, stream);
+  if constexpr (MmaCfg<kD>::kMaxHeads > 16) return launch_mma<kBf16, kD, 4, kWeights>(a, grid, stream);
+  return false;
+}
+
 template <bool kBf16, bool kWeights>
 bool launch_mma_d(const DecodeArgs& a, int kd, int grid, cudaStream_t stream) {
   switch (kd) {
-    case 64: return launch_mma<kBf16, 64, kWeights>(a, grid, stream);
-    case 128: return launch_mma<kBf16, 128, kWeights>(a, grid, stream);
-    default: return launch_mma<kBf16, 256, kWeights>(a, grid, stream);
+    case 64: return launch_mma_tiles<kBf16, 64, kWeights>(a, grid, stream);
+    case 128: return launch_mma_tiles<kBf16, 128, kWeights>(a, grid, stream);
+    default: return launch_mma_tiles<kBf16, 256, kWeights>(a, grid, stream);
   }
 }
 
