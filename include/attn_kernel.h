@@ -245,7 +245,9 @@ ATTN_API int launch_kv_append(const AttnPagedCache* cache, const void* k, const 
  * Bounds of the pages of every sequence: bounds[page, h, 0, :] and
  * bounds[page, h, 1, :] are the elementwise minimum and maximum of the keys of
  * the sequence's tokens in the page (NaN where one is NaN), in the cache's
- * type.  Pages of no sequence are left as they are.  cache->v is not used.
+ * type.  Pages of no sequence are left as they are; a page that sequences
+ * share should hold the same tokens of each (a full page of a common prefix),
+ * otherwise it gets the bounds of one of them.  cache->v is not used.
  */
 ATTN_API int launch_kv_page_bounds(const AttnPagedCache* cache, void* bounds, const long long* bounds_strides,
                                    cudaStream_t stream);

@@ -67,6 +67,11 @@ struct DecodeArgs {
   float2* part_ml;  // [2 gridDim.x][rows]
   float* part_o;    // [2 gridDim.x][rows][D4]
   int D4;           // D rounded up to 4
+  // pos / page_size for pos < 2^31 as (umulhi(pos, ps_mul) + pos) >> ps_shift:
+  // Granlund and Montgomery, Division by Invariant Integers using
+  // Multiplication (1994), figure 4.1.
+  unsigned ps_mul;
+  int ps_shift;
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
@@ -123,10 +128,10 @@ __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0
 // The run of tiles of one CTA
 // ---------------------------------------------------------------------------
 
-// A place in the row of tiles: tile t of the T tiles of unit `hu` (kv head *
-// row_tiles + row tile) of sequence b.
+// A place in the row of tiles: tile t of the T tiles of the unit (sequence b,
+// kv head h, tile rt of its query heads).
 struct Cursor {
-  int b, hu, t, T, len;
+  int b, h, rt, t, T, len;
 };
 
 template <int kTile>
@@ -139,8 +144,10 @@ template <int kTile>
 __device__ __forceinline__ void advance(const DecodeArgs& a, Cursor& c, int* fault) {
   if (++c.t < c.T) return;
   c.t = 0;
-  if (++c.hu < a.c.heads * a.row_tiles) return;
-  c.hu = 0;
+  if (++c.rt < a.row_tiles) return;
+  c.rt = 0;
+  if (++c.h < a.c.heads) return;
+  c.h = 0;
   c.T = 0;
   while (c.T == 0 && ++c.b < a.c.B) {
     c.len = paged_len(a.c, c.b, fault);
@@ -156,8 +163,7 @@ struct ScheduleSmem {
 // Works out this CTA's run: its first tile (returned), the number of its
 // tiles *n and the run length of the grid *per.
 template <int kTile>
-__device__ __forceinline__ Cursor schedule(const DecodeArgs& a, ScheduleSmem& s, long long* n, long long* per,
-                                           int* fault) {
+__device__ __forceinline__ Cursor schedule(const DecodeArgs& a, ScheduleSmem& s, int* n, long long* per, int* fault) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int seg = (a.c.B + kThreads - 1) / kThreads;
   const int b0 = min(a.c.B, tid * seg), b1 = min(a.c.B, b0 + seg);
@@ -178,9 +184,12 @@ __device__ __forceinline__ Cursor schedule(const DecodeArgs& a, ScheduleSmem& s,
     total += s.warp_sum[w];
   }
   const int units = a.c.heads * a.row_tiles;
-  *per = (total * units + gridDim.x - 1) / gridDim.x;
+  // 64-bit division takes about half a microsecond
+  total *= units;
+  *per = total <= 0x7fffffffLL - gridDim.x ? (static_cast<unsigned>(total) + gridDim.x - 1) / gridDim.x
+                                           : (total + gridDim.x - 1) / gridDim.x;
   const long long f0 = *per * blockIdx.x;
-  *n = max(0LL, min(*per, total * units - f0));
+  *n = static_cast<int>(max(0LL, min(*per, total - f0)));  // the host checks that it fits
   before += upto - mine;
   if (*n > 0 && f0 >= before * units && f0 < (before + mine) * units) {
     for (int b = b0; b < b1; ++b) {
@@ -188,8 +197,9 @@ __device__ __forceinline__ Cursor schedule(const DecodeArgs& a, ScheduleSmem& s,
       const int T = tiles_of<kTile>(a, len);
       if (f0 < (before + T) * units) {
         const long long in = f0 - before * units;
-        const int hu = static_cast<int>(in / T);
-        s.first = Cursor{b, hu, static_cast<int>(in - static_cast<long long>(hu) * T), T, len};
+        const int hu = in <= 0x7fffffffLL ? static_cast<int>(in) / T : static_cast<int>(in / T);
+        const int h = hu / a.row_tiles;
+        s.first = Cursor{b, h, hu - h * a.row_tiles, static_cast<int>(in - static_cast<long long>(hu) * T), T, len};
         break;
       }
       before += T;
@@ -211,22 +221,33 @@ __device__ __forceinline__ void zero_empty_rows(const DecodeArgs& a, int* fault)
 }
 
 // Where token `pos` of (sequence b, kv head h) lies, pos counting the tokens
-// of the listed pages when there is a list: its page (-1: no such token, or
-// no such page) and its row in that page.
-__device__ __forceinline__ void locate(const DecodeArgs& a, int b, int h, int pos, int len, int* page, int* row,
-                                       int* fault) {
-  const int ps = a.c.page_size;
-  int lp = static_cast<int>(static_cast<unsigned>(pos) / static_cast<unsigned>(ps));
-  *row = pos - lp * ps;
-  *page = -1;
+// of the listed pages when there is a list.  In two steps, each a load whose
+// value only the next needs, so that the loads of several tokens overlap: its
+// logical page (row < 0: no such token), then its physical page.
+__device__ __forceinline__ void locate_logical(const DecodeArgs& a, int b, int h, int pos, int len, int* lp, int* row) {
+  const int j = static_cast<int>((__umulhi(static_cast<unsigned>(pos), a.ps_mul) + static_cast<unsigned>(pos)) >> a.ps_shift);
+  *row = pos - j * a.c.page_size;
+  *lp = j;
   if (a.pages) {
-    if (lp >= a.n_pages) return;
-    lp = __ldg(a.pages + (static_cast<long long>(b) * a.c.heads + h) * a.n_pages + lp);
-    // An entry that names no page of the sequence adds nothing.
-    if (lp < 0 || lp >= a.c.table_width) return;
-    pos = lp * ps + *row;
+    if (j < a.n_pages)
+      *lp = __ldg(a.pages + (static_cast<long long>(b) * a.c.heads + h) * a.n_pages + j);
+    else
+      *row = -1;
+  } else if (pos >= len) {
+    *row = -1;
   }
-  if (pos < len) *page = paged_page(a.c, b, lp, fault);
+}
+__device__ __forceinline__ void locate_physical(const DecodeArgs& a, int b, int len, int* page, int* row) {
+  const int lp = *page;
+  // A list's entry that names no page of the sequence adds nothing.
+  if (a.pages && (lp < 0 || lp >= a.c.table_width || lp * a.c.page_size + *row >= len)) *row = -1;
+  if (*row >= 0) *page = __ldg(a.c.table + static_cast<long long>(b) * a.c.table_stride + lp);
+}
+// After both: whether there is such a token, in a page of the cache.
+__device__ __forceinline__ bool located(const DecodeArgs& a, int page, int row, int* fault) {
+  const bool in = static_cast<unsigned>(page) < static_cast<unsigned>(a.c.num_pages);
+  if (row >= 0 && !in) *fault = 1;
+  return row >= 0 && in;
 }
 
 // Where a unit's result goes: the output when the whole unit was in this
@@ -239,15 +260,16 @@ struct Place {
 };
 
 __device__ __forceinline__ Place place_of(const DecodeArgs& a, const Cursor& c, bool begun, long long per) {
-  const int h = c.hu / a.row_tiles, rt = c.hu - h * a.row_tiles;
   Place p;
-  p.rows = min(a.rows, a.group - rt * a.rows);
-  p.row0 = static_cast<long long>(c.b) * a.Hq + h * a.group + rt * a.rows;
+  p.rows = min(a.rows, a.group - c.rt * a.rows);
+  p.row0 = static_cast<long long>(c.b) * a.Hq + c.h * a.group + c.rt * a.rows;
   const bool ends = c.t + 1 == c.T;
   p.whole = begun && ends;
   p.slot = 2 * blockIdx.x + (begun ? 1 : 0);
   if (begun && !ends && threadIdx.x == 0) {
-    const int later = static_cast<int>((c.T - (c.t + 1) + per - 1) / per);
+    const int rest = c.T - (c.t + 1);
+    const int later = per <= 0x3fffffffLL ? (rest + static_cast<int>(per) - 1) / static_cast<int>(per)
+                                          : static_cast<int>((rest + per - 1) / per);
     // row0 < B * Hq, which the host keeps below 2^31
     a.meta[blockIdx.x] = make_int4(static_cast<int>(p.row0), p.rows, later, 0);
   }
@@ -294,9 +316,9 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas) attn_decode_mma_k
   constexpr int kKeys = C::kKeys, kTile = C::kTile, kStages = C::kStages;
   constexpr int kCols = kD / 8;                // 16-byte columns of a row
   constexpr int kSteps = kD / 16;              // 16-wide steps of the head dim
-  constexpr int kCopies = kKeys * kCols / 32;  // 16-byte copies per lane for K, and for V
+  constexpr int kRowsPerCopy = 32 / kCols;     // rows of one 16-byte copy of the warp
 
-  extern __shared__ __align__(128) unsigned char smem[];
+  extern __shared__ __align__(1024) unsigned char smem[];
   __shared__ ScheduleSmem s_sched;
   __shared__ float s_m[2][kWarps][8 * kNT], s_l[2][kWarps][8 * kNT];
   __shared__ uint32_t s_mask[kWarps][kStages];
@@ -304,78 +326,109 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas) attn_decode_mma_k
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int fault = 0;
   if (threadIdx.x == 0) a.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
-  long long n, per;
+  int n;
+  long long per;
   Cursor cur = schedule<kTile>(a, s_sched, &n, &per, &fault);
   launch_dependents();
   zero_empty_rows<T>(a, &fault);
 
   unsigned char* ring = smem + warp * (kStages * C::kStageBytes);
   const uint32_t ring_addr = smem_addr(ring);
-  const T* kbase = static_cast<const T*>(a.c.k);
-  const T* vbase = static_cast<const T*>(a.c.v);
+  // A lane copies one 16-byte column (zeros behind D) of every kRowsPerCopy-th
+  // row; with the rows of a chunk 2 kD bytes apart and the chunk aligned to
+  // that, the swizzle of later rows is an XOR of the address with a constant.
+  const int my_row = lane / kCols;
+  const bool my_col_ok = (lane % kCols) * 8 < a.c.D;
+  const int my_col = my_col_ok ? (lane % kCols) * 8 : 0;
+  const uint32_t my_dst = my_row * (kD * 2) + (((lane % kCols) ^ my_row) << 4);
+  const T* kbase = static_cast<const T*>(a.c.k) + my_col;
+  const T* vbase = static_cast<const T*>(a.c.v) + my_col;
   // Where 16 divides the page size, 16 tokens in a row are rows of one page.
   const bool one_page = a.c.page_size % 16 == 0;
 
-  // The chunk whose copies go out next: its head, and (lane = token) the
-  // page and row of each token, looked up when the one before was issued.
+  // The chunks whose copies go out next, with the page and row of each token
+  // (lane = token): logical pages are looked up kStages + 1 chunks ahead of
+  // the copies and physical pages kStages ahead, so that no copy waits for a
+  // look-up and the first ones wait for one together.
+  int page[kStages + 1], row[kStages + 1], head[kStages + 1];
   Cursor ahead = cur;
-  long long issued = 0;
-  int page = -1, row = 0, head = 0;
-  auto look_up = [&]() {
-    page = -1;
-    if (issued < n) {
-      head = ahead.hu / a.row_tiles;
-      if (lane < kKeys)
-        locate(a, ahead.b, head, ahead.t * kTile + warp * kKeys + lane, ahead.len, &page, &row, &fault);
+  int looked = 0, last_b = 0, last_len = 0;
+  auto logical = [&](int s) {
+    row[s] = -1;
+    if (looked < n) {
+      last_b = ahead.b;
+      last_len = ahead.len;
+      head[s] = ahead.h;
+      if (kKeys == 32 || lane < kKeys)
+        locate_logical(a, last_b, ahead.h, ahead.t * kTile + warp * kKeys + lane, last_len, &page[s], &row[s]);
       advance<kTile>(a, ahead, &fault);
+      ++looked;
     }
   };
+  auto physical = [&](int s) { locate_physical(a, last_b, last_len, &page[s], &row[s]); };
   auto issue = [&](int stage) {
-    const uint32_t mask = __ballot_sync(0xffffffffu, page >= 0);
+    const uint32_t mask = __ballot_sync(0xffffffffu, located(a, page[0], row[0], &fault));
     if (lane == 0) s_mask[warp][stage] = mask;
     if (mask != 0) {
-      const uint32_t dst = ring_addr + stage * C::kStageBytes;
-      const long long kh = head * a.c.ks[1], vh = head * a.c.vs[1];
-      if (one_page) {
-        // The first of 16 tokens has a page if any has.
+      const uint32_t dst = ring_addr + stage * C::kStageBytes + my_dst;
+      const T* kh = kbase + head[0] * a.c.ks[1];
+      const T* vh = vbase + head[0] * a.c.vs[1];
 #pragma unroll
-        for (int g = 0; g < kKeys / 16; ++g) {
-          const int pg = __shfl_sync(0xffffffffu, page, g * 16), in = __shfl_sync(0xffffffffu, row, g * 16);
-          const T* kp = kbase + pg * a.c.ks[0] + kh + in * a.c.ks[2];
-          const T* vp = vbase + pg * a.c.vs[0] + vh + in * a.c.vs[2];
+      for (int g = 0; g < kKeys / 16; ++g) {
+        if (one_page) {
+          // All 16 rows lie in the page, whether they hold tokens or not; the
+          // first does if any does, and those that do come first.
+          const int pg = __shfl_sync(0xffffffffu, page[0], g * 16), in = __shfl_sync(0xffffffffu, row[0], g * 16);
+          const int live = __popc(mask >> (g * 16) & 0xffffu);
+          const T* kp = live ? kh + pg * a.c.ks[0] + (in + my_row) * a.c.ks[2] : kh;
+          const T* vp = live ? vh + pg * a.c.vs[0] + (in + my_row) * a.c.vs[2] : vh;
+          const long long k_step = live ? kRowsPerCopy * a.c.ks[2] : 0, v_step = live ? kRowsPerCopy * a.c.vs[2] : 0;
+          const int mine = my_col_ok ? live - my_row : 0;
 #pragma unroll
           for (int i = 0; i < kCols / 2; ++i) {
-            const int e = i * 32 + lane;
-            const int r = e / kCols, col = e % kCols, tok = g * 16 + r;
-            const bool ok = (mask >> tok & 1u) && col * 8 < a.c.D;
-            const uint32_t at = dst + tok * (kD * 2) + ((col ^ (r & 7)) << 4);
-            cp_async16(at, ok ? kp + r * a.c.ks[2] + col * 8 : kbase, ok);
-            cp_async16(at + kKeys * kD * 2, ok ? vp + r * a.c.vs[2] + col * 8 : vbase, ok);
+            const uint32_t at = (dst ^ ((i * kRowsPerCopy & 7) << 4)) + (g * 16 + i * kRowsPerCopy) * (kD * 2);
+            cp_async16(at, kp, mine > i * kRowsPerCopy);
+            cp_async16(at + kKeys * kD * 2, vp, mine > i * kRowsPerCopy);
+            kp += k_step;
+            vp += v_step;
           }
-        }
-      } else {
+        } else {
 #pragma unroll
-        for (int i = 0; i < kCopies; ++i) {
-          const int e = i * 32 + lane;
-          const int r = e / kCols, col = e % kCols;
-          const int pg = __shfl_sync(0xffffffffu, page, r), in = __shfl_sync(0xffffffffu, row, r);
-          const bool ok = pg >= 0 && col * 8 < a.c.D;
-          const long long ko = ok ? pg * a.c.ks[0] + kh + in * a.c.ks[2] + col * 8 : 0;
-          const long long vo = ok ? pg * a.c.vs[0] + vh + in * a.c.vs[2] + col * 8 : 0;
-          const uint32_t at = dst + r * (kD * 2) + ((col ^ (r & 7)) << 4);
-          cp_async16(at, kbase + ko, ok);
-          cp_async16(at + kKeys * kD * 2, vbase + vo, ok);
+          for (int i = 0; i < kCols / 2; ++i) {
+            const int tok = g * 16 + i * kRowsPerCopy + my_row;
+            const int pg = __shfl_sync(0xffffffffu, page[0], tok), in = __shfl_sync(0xffffffffu, row[0], tok);
+            const bool ok = (mask >> tok & 1u) && my_col_ok;
+            const uint32_t at = (dst ^ ((i * kRowsPerCopy & 7) << 4)) + (g * 16 + i * kRowsPerCopy) * (kD * 2);
+            cp_async16(at, kh + (ok ? pg * a.c.ks[0] + in * a.c.ks[2] : 0), ok);
+            cp_async16(at + kKeys * kD * 2, vh + (ok ? pg * a.c.vs[0] + in * a.c.vs[2] : 0), ok);
+          }
         }
       }
     }
     cp_async_commit();
-    ++issued;
-    look_up();
+#pragma unroll
+    for (int s = 0; s < kStages; ++s) {
+      page[s] = page[s + 1];
+      row[s] = row[s + 1];
+      head[s] = head[s + 1];
+    }
+    physical(kStages - 1);
+    logical(kStages);
   };
 
-  look_up();
+  // The first kStages physical look-ups overlap: each needs its own sequence,
+  // and only the first look-ups of a run can span several.
+  {
+    int bs[kStages], ls[kStages];
 #pragma unroll
-  for (int s = 0; s < kStages; ++s) issue(s);
+    for (int s = 0; s <= kStages; ++s) {
+      page[s] = head[s] = 0;
+      logical(s);
+      if (s < kStages) bs[s] = last_b, ls[s] = last_len;
+    }
+#pragma unroll
+    for (int s = 0; s < kStages; ++s) locate_physical(a, bs[s], ls[s], &page[s], &row[s]);
+  }
 
   uint32_t qf[kNT][kSteps][2];
   float o[kNT][kSteps][4];
@@ -383,195 +436,199 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas) attn_decode_mma_k
   bool begun = cur.t == 0, fresh = true;
   int parity = 0, stage = 0;
 
-  for (long long i = 0; i < n; ++i) {
-    if (fresh) {
-      // A new unit: its query heads as B fragments (heads behind the last are zero).
-      const int h = cur.hu / a.row_tiles, rt = cur.hu - h * a.row_tiles;
-      const int rows = min(a.rows, a.group - rt * a.rows);
-      const T* q = static_cast<const T*>(a.q) + cur.b * a.q_b + (static_cast<long long>(h) * a.group + rt * a.rows) * a.q_h;
+  // The first kStages turns only fill the ring (one copy of the code: a CTA's
+  // first pass over it comes from a cold instruction cache).
+  for (int i = -kStages; i < n; ++i) {
+    if (i >= 0) {
+      if (fresh) {
+        // A new unit: its query heads as B fragments (heads behind the last are zero).
+        const int rows = min(a.rows, a.group - cur.rt * a.rows);
+        const T* q = static_cast<const T*>(a.q) + cur.b * a.q_b + (static_cast<long long>(cur.h) * a.group + cur.rt * a.rows) * a.q_h;
 #pragma unroll
-      for (int t = 0; t < kNT; ++t) {
-        const int r = t * 8 + (lane >> 2);
+        for (int t = 0; t < kNT; ++t) {
+          const int r = t * 8 + (lane >> 2);
 #pragma unroll
-        for (int ks = 0; ks < kSteps; ++ks) {
+          for (int ks = 0; ks < kSteps; ++ks) {
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int d = ks * 16 + j * 8 + (lane & 3) * 2;
-            qf[t][ks][j] = (r < rows && d < a.c.D) ? __ldg(reinterpret_cast<const uint32_t*>(q + r * a.q_h + d)) : 0u;
+            for (int j = 0; j < 2; ++j) {
+              const int d = ks * 16 + j * 8 + (lane & 3) * 2;
+              qf[t][ks][j] = (r < rows && d < a.c.D) ? __ldg(reinterpret_cast<const uint32_t*>(q + r * a.q_h + d)) : 0u;
+            }
+            o[t][ks][0] = o[t][ks][1] = o[t][ks][2] = o[t][ks][3] = 0.f;
           }
-          o[t][ks][0] = o[t][ks][1] = o[t][ks][2] = o[t][ks][3] = 0.f;
+          m[t][0] = m[t][1] = -INFINITY;
+          l[t][0] = l[t][1] = 0.f;
         }
-        m[t][0] = m[t][1] = -INFINITY;
-        l[t][0] = l[t][1] = 0.f;
+        fresh = false;
       }
-      fresh = false;
-    }
-    cp_async_wait<kStages - 1>();
-    __syncwarp();
-    const uint32_t mask = s_mask[warp][stage];
-    const uint32_t kaddr = ring_addr + stage * C::kStageBytes;
-    const uint32_t vaddr = kaddr + kKeys * kD * 2;
-    if (mask != 0 || kWeights) {
+      cp_async_wait<kStages - 1>();
+      __syncwarp();
+      const uint32_t mask = s_mask[warp][stage];
+      if (mask != 0 || kWeights) {
+        const uint32_t chunk = ring_addr + stage * C::kStageBytes;
+        const uint32_t kaddr = chunk + (lane & 15) * (kD * 2) + (((lane >> 4) ^ (lane & 7)) << 4);
+        const uint32_t vaddr = chunk + (kKeys + (lane >> 4) * 8 + (lane & 7)) * (kD * 2) + (((lane >> 3 & 1) ^ (lane & 7)) << 4);
 #pragma unroll
-      for (int g = 0; g < kKeys / 16; ++g) {
-        // Scores of 16 tokens: thread has tokens lane / 4 + {0, 8} of its two
-        // heads.  Even and odd steps of the head dim in two accumulators.
-        float s[kNT][4], s2[kNT][4];
+        for (int g = 0; g < kKeys / 16; ++g) {
+          // Scores of 16 tokens: thread has tokens lane / 4 + {0, 8} of its two
+          // heads.  Even and odd steps of the head dim in two accumulators.
+          float s[kNT][4], s2[kNT][4];
+#pragma unroll
+          for (int t = 0; t < kNT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[t][e] = s2[t][e] = 0.f;
+#pragma unroll
+          for (int ks = 0; ks < kSteps; ++ks) {
+            uint32_t kf[4];
+            ldsm_x4((kaddr ^ (ks * 32)) + g * 16 * (kD * 2), kf);
+#pragma unroll
+            for (int t = 0; t < kNT; ++t)
+              mma16816<kBf16>(ks % 2 ? s2[t] : s[t], kf, qf[t][ks][0], qf[t][ks][1]);
+          }
+          uint32_t pf[kNT][2];
+          const uint32_t live = mask >> (g * 16);
+#pragma unroll
+          for (int t = 0; t < kNT; ++t) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[t][e] = (s[t][e] + s2[t][e]) * a.scale_log2;
+            if ((live & 0xffffu) != 0xffffu) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (!(live >> ((e >> 1) * 8 + (lane >> 2)) & 1u)) s[t][e] = -INFINITY;
+            }
+            if constexpr (kWeights) {
+              const int rows = min(a.rows, a.group - cur.rt * a.rows);
+              const long long r0 = static_cast<long long>(cur.b) * a.Hq + cur.h * a.group + cur.rt * a.rows;
+              const int r = t * 8 + (lane & 3) * 2;
+              float* x = a.x + (r0 + r) * a.x_stride + cur.t * kTile + warp * kKeys + g * 16 + (lane >> 2);
+              if (r < rows) x[0] = s[t][0], x[8] = s[t][2];
+              if (r + 1 < rows) x[a.x_stride] = s[t][1], x[a.x_stride + 8] = s[t][3];
+            }
+            float f[2], top[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float mx = fmaxf(s[t][e], s[t][e + 2]);
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+              const float mn = fmaxf(m[t][e], mx);
+              top[e] = finite_max(mn);
+              f[e] = ex2_approx(m[t][e] - top[e]);
+              m[t][e] = mn;
+            }
+            if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
+              l[t][0] *= f[0];
+              l[t][1] *= f[1];
+#pragma unroll
+              for (int j = 0; j < kSteps; ++j) {
+                o[t][j][0] *= f[0];
+                o[t][j][1] *= f[1];
+                o[t][j][2] *= f[0];
+                o[t][j][3] *= f[1];
+              }
+            }
+            // P is rounded to the input type for P V (half a step, 2^-9 or 2^-12
+            // of each weight); its sum is taken before the rounding.
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[t][e] = ex2_approx(s[t][e] - top[e & 1]);
+            l[t][0] += s[t][0] + s[t][2];
+            l[t][1] += s[t][1] + s[t][3];
+            pf[t][0] = transpose_8x8(pack2<kBf16>(s[t][0], s[t][1]));
+            pf[t][1] = transpose_8x8(pack2<kBf16>(s[t][2], s[t][3]));
+          }
+#pragma unroll
+          for (int j = 0; j < kSteps; ++j) {
+            uint32_t vf[4];
+            ldsm_x4_trans((vaddr ^ (j * 32)) + g * 16 * (kD * 2), vf);
+#pragma unroll
+            for (int t = 0; t < kNT; ++t) mma16816<kBf16>(o[t][j], vf, pf[t][0], pf[t][1]);
+          }
+        }
+      }
+
+      if (cur.t + 1 == cur.T || i + 1 == n) {
+        // The unit, or this CTA's part of it, ends: the warps' parts are scaled
+        // to their common maximum and summed over the chunks just freed, 16 heads
+        // at a time.
+        const Place p = place_of(a, cur, begun, per);
 #pragma unroll
         for (int t = 0; t < kNT; ++t)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[t][e] = s2[t][e] = 0.f;
-#pragma unroll
-        for (int ks = 0; ks < kSteps; ++ks) {
-          uint32_t kf[4];
-          const int r = g * 16 + (lane & 15), col = ks * 2 + (lane >> 4);
-          ldsm_x4(kaddr + r * (kD * 2) + ((col ^ (r & 7)) << 4), kf);
-#pragma unroll
-          for (int t = 0; t < kNT; ++t)
-            mma16816<kBf16>(ks % 2 ? s2[t] : s[t], kf, qf[t][ks][0], qf[t][ks][1]);
-        }
-        const bool live[2] = {(mask >> (g * 16 + (lane >> 2)) & 1u) != 0, (mask >> (g * 16 + 8 + (lane >> 2)) & 1u) != 0};
-        uint32_t pf[kNT][2];
-#pragma unroll
-        for (int t = 0; t < kNT; ++t) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[t][e] = live[e >> 1] ? (s[t][e] + s2[t][e]) * a.scale_log2 : -INFINITY;
-          if constexpr (kWeights) {
-            const int h = cur.hu / a.row_tiles, rt = cur.hu - h * a.row_tiles;
-            const int rows = min(a.rows, a.group - rt * a.rows);
-            const long long r0 = static_cast<long long>(cur.b) * a.Hq + h * a.group + rt * a.rows;
-            const int r = t * 8 + (lane & 3) * 2;
-            float* x = a.x + (r0 + r) * a.x_stride + cur.t * kTile + warp * kKeys + g * 16 + (lane >> 2);
-            if (r < rows) x[0] = s[t][0], x[8] = s[t][2];
-            if (r + 1 < rows) x[a.x_stride] = s[t][1], x[a.x_stride + 8] = s[t][3];
-          }
-          float f[2];
-#pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float mx = fmaxf(s[t][e], s[t][e + 2]);
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-            const float mn = fmaxf(m[t][e], mx);
-            f[e] = ex2_approx(m[t][e] - finite_max(mn));
-            m[t][e] = mn;
-          }
-          if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
-            l[t][0] *= f[0];
-            l[t][1] *= f[1];
-#pragma unroll
-            for (int j = 0; j < kSteps; ++j) {
-              o[t][j][0] *= f[0];
-              o[t][j][1] *= f[1];
-              o[t][j][2] *= f[0];
-              o[t][j][3] *= f[1];
-            }
-          }
-          const float m0 = finite_max(m[t][0]), m1 = finite_max(m[t][1]);
-          // P is rounded to the input type for P V (half a step, 2^-9 or 2^-12
-          // of each weight); its sum is taken before the rounding.
-          s[t][0] = ex2_approx(s[t][0] - m0);
-          s[t][1] = ex2_approx(s[t][1] - m1);
-          s[t][2] = ex2_approx(s[t][2] - m0);
-          s[t][3] = ex2_approx(s[t][3] - m1);
-          l[t][0] += s[t][0] + s[t][2];
-          l[t][1] += s[t][1] + s[t][3];
-          pf[t][0] = transpose_8x8(pack2<kBf16>(s[t][0], s[t][1]));
-          pf[t][1] = transpose_8x8(pack2<kBf16>(s[t][2], s[t][3]));
-        }
-#pragma unroll
-        for (int j = 0; j < kSteps; ++j) {
-          uint32_t vf[4];
-          const int r = g * 16 + (lane >> 4) * 8 + (lane & 7), col = j * 2 + ((lane >> 3) & 1);
-          ldsm_x4_trans(vaddr + r * (kD * 2) + ((col ^ (r & 7)) << 4), vf);
-#pragma unroll
-          for (int t = 0; t < kNT; ++t) mma16816<kBf16>(o[t][j], vf, pf[t][0], pf[t][1]);
-        }
-      }
-    }
-
-    if (cur.t + 1 == cur.T || i + 1 == n) {
-      // The unit, or this CTA's part of it, ends: the warps' parts are scaled
-      // to their common maximum and summed over the chunks just freed, 16 heads
-      // at a time.
-      const Place p = place_of(a, cur, begun, per);
-#pragma unroll
-      for (int t = 0; t < kNT; ++t)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], 4);
-          l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], 8);
-          l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], 16);
-          if (lane < 4) {
-            s_m[parity][warp][t * 8 + lane * 2 + e] = m[t][e];
-            s_l[parity][warp][t * 8 + lane * 2 + e] = l[t][e];
-          }
-        }
-      __syncthreads();
-      float* ot = reinterpret_cast<float*>(ring + stage * C::kStageBytes);
-#pragma unroll
-      for (int t0 = 0; t0 < kNT; t0 += 2) {
-#pragma unroll
-        for (int t = t0; t < (t0 + 2 < kNT ? t0 + 2 : kNT); ++t)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int r = t * 8 + (lane & 3) * 2 + e, at = r - t0 * 8;
-            if (r < p.rows) {
-              float M = s_m[parity][0][r];
-#pragma unroll
-              for (int w = 1; w < kWarps; ++w) M = fmaxf(M, s_m[parity][w][r]);
-              const float f = ex2_approx(m[t][e] - finite_max(M));
-#pragma unroll
-              for (int j = 0; j < kSteps; ++j)
-#pragma unroll
-                for (int up = 0; up < 2; ++up) {
-                  const int d = j * 16 + up * 8 + (lane >> 2);
-                  ot[at * kD + (((d >> 2) ^ ((lane & 3) << 1)) << 2) + (d & 3)] = o[t][j][2 * up + e] * f;
-                }
+            l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], 4);
+            l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], 8);
+            l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], 16);
+            if (lane < 4) {
+              s_m[parity][warp][t * 8 + lane * 2 + e] = m[t][e];
+              s_l[parity][warp][t * 8 + lane * 2 + e] = l[t][e];
             }
           }
         __syncthreads();
-        const int here = min(p.rows - t0 * 8, 16);
-        for (int e = threadIdx.x; e < here * (kD / 4); e += kThreads) {
-          const int at = e / (kD / 4), c4 = e % (kD / 4), r = t0 * 8 + at;
-          if (c4 * 4 >= a.c.D) continue;
-          float M = s_m[parity][0][r], L = 0.f;
+        float* ot = reinterpret_cast<float*>(ring + stage * C::kStageBytes);
 #pragma unroll
-          for (int w = 1; w < kWarps; ++w) M = fmaxf(M, s_m[parity][w][r]);
-          float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int t0 = 0; t0 < kNT; t0 += 2) {
 #pragma unroll
-          for (int w = 0; w < kWarps; ++w) {
-            L += s_l[parity][w][r] * ex2_approx(s_m[parity][w][r] - finite_max(M));
-            const float4 y = *reinterpret_cast<const float4*>(
-                reinterpret_cast<const float*>(smem + (w * kStages + stage) * C::kStageBytes) + at * kD +
-                ((c4 ^ ((at >> 1 & 3) << 1)) << 2));
-            sum.x += y.x;
-            sum.y += y.y;
-            sum.z += y.z;
-            sum.w += y.w;
+          for (int t = t0; t < (t0 + 2 < kNT ? t0 + 2 : kNT); ++t)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int r = t * 8 + (lane & 3) * 2 + e, at = r - t0 * 8;
+              if (r < p.rows) {
+                float M = s_m[parity][0][r];
+#pragma unroll
+                for (int w = 1; w < kWarps; ++w) M = fmaxf(M, s_m[parity][w][r]);
+                const float f = ex2_approx(m[t][e] - finite_max(M));
+#pragma unroll
+                for (int j = 0; j < kSteps; ++j)
+#pragma unroll
+                  for (int up = 0; up < 2; ++up) {
+                    const int d = j * 16 + up * 8 + (lane >> 2);
+                    ot[at * kD + (((d >> 2) ^ ((lane & 3) << 1)) << 2) + (d & 3)] = o[t][j][2 * up + e] * f;
+                  }
+              }
+            }
+          __syncthreads();
+          const int here = min(p.rows - t0 * 8, 16);
+          for (int e = threadIdx.x; e < here * (kD / 4); e += kThreads) {
+            const int at = e / (kD / 4), c4 = e % (kD / 4), r = t0 * 8 + at;
+            if (c4 * 4 >= a.c.D) continue;
+            float M = s_m[parity][0][r], L = 0.f;
+#pragma unroll
+            for (int w = 1; w < kWarps; ++w) M = fmaxf(M, s_m[parity][w][r]);
+            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+              L += s_l[parity][w][r] * ex2_approx(s_m[parity][w][r] - finite_max(M));
+              const float4 y = *reinterpret_cast<const float4*>(
+                  reinterpret_cast<const float*>(smem + (w * kStages + stage) * C::kStageBytes) + at * kD +
+                  ((c4 ^ ((at >> 1 & 3) << 1)) << 2));
+              sum.x += y.x;
+              sum.y += y.y;
+              sum.z += y.z;
+              sum.w += y.w;
+            }
+            if (p.whole) {
+              const float inv = L == 0.f ? 0.f : 1.f / L;
+              T* out = static_cast<T*>(a.out) + (p.row0 + r) * a.c.D + c4 * 4;
+              *reinterpret_cast<uint2*>(out) =
+                  make_uint2(pack2<kBf16>(sum.x * inv, sum.y * inv), pack2<kBf16>(sum.z * inv, sum.w * inv));
+              if (kWeights && c4 == 0) a.lse2[p.row0 + r] = L == 0.f ? INFINITY : M + log2f(L);
+            } else {
+              const long long slot = static_cast<long long>(p.slot) * a.rows + r;
+              *reinterpret_cast<float4*>(a.part_o + slot * a.D4 + c4 * 4) = sum;
+              if (c4 == 0) a.part_ml[slot] = make_float2(M, L);
+            }
           }
-          if (p.whole) {
-            const float inv = L == 0.f ? 0.f : 1.f / L;
-            T* out = static_cast<T*>(a.out) + (p.row0 + r) * a.c.D + c4 * 4;
-            *reinterpret_cast<uint2*>(out) =
-                make_uint2(pack2<kBf16>(sum.x * inv, sum.y * inv), pack2<kBf16>(sum.z * inv, sum.w * inv));
-            if (kWeights && c4 == 0) a.lse2[p.row0 + r] = L == 0.f ? INFINITY : M + log2f(L);
-          } else {
-            const long long slot = static_cast<long long>(p.slot) * a.rows + r;
-            *reinterpret_cast<float4*>(a.part_o + slot * a.D4 + c4 * 4) = sum;
-            if (c4 == 0) a.part_ml[slot] = make_float2(M, L);
-          }
+          __syncthreads();  // the chunks are read before they are filled again
         }
-        __syncthreads();  // the chunks are read before they are filled again
+        parity ^= 1;
+        begun = true;
+        fresh = true;
       }
-      parity ^= 1;
-      begun = true;
-      fresh = true;
     }
     __syncwarp();
     issue(stage);
     stage = stage + 1 == kStages ? 0 : stage + 1;
-    advance<kTile>(a, cur, &fault);
+    if (i >= 0) advance<kTile>(a, cur, &fault);
   }
   cp_async_wait<0>();
   if (fault) atomicOr(&g_page_fault, 1);
@@ -606,7 +663,8 @@ __global__ void __launch_bounds__(kThreads) attn_decode_simt_kernel(const __grid
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int fault = 0;
   if (threadIdx.x == 0) a.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
-  long long n, per;
+  int n;
+  long long per;
   Cursor cur = schedule<kTile>(a, s_sched, &n, &per, &fault);
   launch_dependents();
   zero_empty_rows<T>(a, &fault);
@@ -619,8 +677,8 @@ __global__ void __launch_bounds__(kThreads) attn_decode_simt_kernel(const __grid
   int parity = 0;
   const int my_row = lane / kRowLanes, my_key = (lane / kSame) % kKeys;
 
-  for (long long i = 0; i < n; ++i) {
-    const int h = cur.hu / a.row_tiles, rt = cur.hu - h * a.row_tiles;
+  for (int i = 0; i < n; ++i) {
+    const int h = cur.h, rt = cur.rt;
     const int rows = min(a.rows, a.group - rt * a.rows);
     const long long row0 = static_cast<long long>(cur.b) * a.Hq + h * a.group + rt * a.rows;
     if (fresh) {
@@ -639,8 +697,11 @@ __global__ void __launch_bounds__(kThreads) attn_decode_simt_kernel(const __grid
     }
     int page = -1, row = 0;
     const int pos0 = cur.t * kTile + warp * kChunk;
-    if (lane < kChunk) locate(a, cur.b, h, pos0 + lane, cur.len, &page, &row, &fault);
-    const uint32_t mask = __ballot_sync(0xffffffffu, page >= 0);
+    if (lane < kChunk) {
+      locate_logical(a, cur.b, h, pos0 + lane, cur.len, &page, &row);
+      locate_physical(a, cur.b, cur.len, &page, &row);
+    }
+    const uint32_t mask = __ballot_sync(0xffffffffu, lane < kChunk && located(a, page, row, &fault));
     if (mask != 0 || kWeights) {
       const long long kh = h * a.c.ks[1], vh = h * a.c.vs[1];
 #pragma unroll 1
@@ -649,12 +710,13 @@ __global__ void __launch_bounds__(kThreads) attn_decode_simt_kernel(const __grid
 #pragma unroll
         for (int k = 0; k < kKeys; ++k) {
           const int pg = __shfl_sync(0xffffffffu, page, k0 + k), in = __shfl_sync(0xffffffffu, row, k0 + k);
-          const T* kp = kbase + (pg >= 0 ? pg * a.c.ks[0] + kh + in * a.c.ks[2] : 0);
-          const T* vp = vbase + (pg >= 0 ? pg * a.c.vs[0] + vh + in * a.c.vs[2] : 0);
+          const bool live = mask >> (k0 + k) & 1u;
+          const T* kp = kbase + (live ? pg * a.c.ks[0] + kh + in * a.c.ks[2] : 0);
+          const T* vp = vbase + (live ? pg * a.c.vs[0] + vh + in * a.c.vs[2] : 0);
 #pragma unroll
           for (int e = 0; e < kPer; ++e) {
             const int d = lane + 32 * e;
-            const bool ok = pg >= 0 && d < a.c.D;
+            const bool ok = live && d < a.c.D;
             kv[k][e] = ok ? to_f32(kp[d]) : 0.f;
             vv[k][e] = ok ? to_f32(vp[d]) : 0.f;
           }
@@ -757,26 +819,62 @@ __global__ void __launch_bounds__(kThreads) attn_decode_simt_kernel(const __grid
 // ---------------------------------------------------------------------------
 
 // CTA (c, r): row r of the unit that CTA c of the grid before began and did
-// not finish, one thread per column.
+// not finish.  Warp w sums parts w, w + 8, ... (most units have no more than
+// eight, whose loads then all overlap), lane four columns of each 128; the
+// warps' sums meet in shared memory in their order.
+constexpr int kJoinWarps = 8;
+
 template <typename T>
-__global__ void attn_decode_join_kernel(const __grid_constant__ DecodeArgs a) {
+__global__ void __launch_bounds__(kJoinWarps * 32) attn_decode_join_kernel(const __grid_constant__ DecodeArgs a) {
+  __shared__ float4 s_o[kJoinWarps][2][32];
+  __shared__ float s_m[kJoinWarps], s_l[kJoinWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   grid_dependency_wait();
   const int c = blockIdx.x, r = blockIdx.y;
   const int4 meta = a.meta[c];
   if (meta.z == 0 || r >= meta.y) return;
-  auto slot = [&](int i) { return static_cast<long long>(i == 0 ? 2 * c + 1 : 2 * (c + i)) * a.rows + r; };
-  float M = -INFINITY;
-  for (int i = 0; i <= meta.z; ++i) M = fmaxf(M, a.part_ml[slot(i)].x);
+  float m = -INFINITY, l = 0.f;
+  float4 o[2] = {};
+#pragma unroll 4
+  for (int i = warp; i <= meta.z; i += kJoinWarps) {
+    const long long slot = static_cast<long long>(i == 0 ? 2 * c + 1 : 2 * (c + i)) * a.rows + r;
+    const float2 ml = a.part_ml[slot];
+    float4 y[2] = {};
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (k * 128 + lane * 4 < a.D4) y[k] = *reinterpret_cast<const float4*>(a.part_o + slot * a.D4 + k * 128 + lane * 4);
+    const float mn = fmaxf(m, ml.x);
+    const float f = ex2_approx(m - finite_max(mn)), g = ex2_approx(ml.x - finite_max(mn));
+    m = mn;
+    l = l * f + ml.y * g;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      o[k].x = o[k].x * f + y[k].x * g;
+      o[k].y = o[k].y * f + y[k].y * g;
+      o[k].z = o[k].z * f + y[k].z * g;
+      o[k].w = o[k].w * f + y[k].w * g;
+    }
+  }
+  if (lane == 0) {
+    s_m[warp] = m;
+    s_l[warp] = l;
+  }
+  s_o[warp][0][lane] = o[0];
+  s_o[warp][1][lane] = o[1];
+  __syncthreads();
   const int d = threadIdx.x;
-  float L = 0.f, sum = 0.f;
-  for (int i = 0; i <= meta.z; ++i) {
-    const float2 ml = a.part_ml[slot(i)];
-    const float f = ex2_approx(ml.x - finite_max(M));
-    L += ml.y * f;
-    if (d < a.c.D) sum += a.part_o[slot(i) * a.D4 + d] * f;
+  if (d >= a.c.D) return;
+  float M = s_m[0], L = 0.f, sum = 0.f;
+#pragma unroll
+  for (int w = 1; w < kJoinWarps; ++w) M = fmaxf(M, s_m[w]);
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) {
+    const float f = ex2_approx(s_m[w] - finite_max(M));
+    L += s_l[w] * f;
+    sum += reinterpret_cast<const float*>(s_o[w])[d] * f;
   }
   const long long row = meta.x + r;
-  if (d < a.c.D) static_cast<T*>(a.out)[row * a.c.D + d] = from_f32<T>(L == 0.f ? 0.f : sum / L);
+  static_cast<T*>(a.out)[row * a.c.D + d] = from_f32<T>(L == 0.f ? 0.f : sum / L);
   if (a.lse2 && d == 0) a.lse2[row] = L == 0.f ? INFINITY : M + log2f(L);
 }
 
@@ -806,6 +904,7 @@ struct Plan {
   int kd;  // head dim the kernel is compiled for (mma), or dims per lane (simt)
   int rows, row_tiles, tile;
   int grid;
+  long long per_cta;  // tiles, at most
   long long x_stride;
   size_t meta_at, ml_at, o_at, lse_at, x_at, bytes;
 };
@@ -844,6 +943,7 @@ Plan make_plan(const AttnPagedCache* c, bool fast, int Hq, int n_pages, bool lis
   if (grid > tiles) grid = tiles;
   if (grid < 1) grid = 1;
   p.grid = static_cast<int>(grid);
+  p.per_cta = (tiles + grid - 1) / grid;
   auto up = [](size_t x) { return (x + 255) & ~static_cast<size_t>(255); };
   const size_t D4 = (D + 3) / 4 * 4;
   p.meta_at = 0;
@@ -1006,7 +1106,7 @@ extern "C" int launch_attn_decode(const AttnPagedCache* cache, const void* q, co
   if (st != ATTN_OK) return st;
   const bool fast = aligned_to(q, 16) && aligned_to(out, 16) && qs[0] % 8 == 0 && qs[1] % 8 == 0;
   const Plan p = make_plan(cache, fast, Hq, n_pages, pages != nullptr, weights != nullptr, sm_count());
-  if (workspace_bytes < p.bytes) return ATTN_ERR_INVALID_ARGUMENT;
+  if (workspace_bytes < p.bytes || p.per_cta > 0x7fffff00LL) return ATTN_ERR_INVALID_ARGUMENT;
 
   float scale = softmax_scale;
   if (!(scale > 0.f) || !isfinite(scale)) scale = 1.0f / sqrtf(static_cast<float>(D));
@@ -1031,10 +1131,14 @@ extern "C" int launch_attn_decode(const AttnPagedCache* cache, const void* q, co
   a.part_ml = reinterpret_cast<float2*>(ws + p.ml_at);
   a.part_o = reinterpret_cast<float*>(ws + p.o_at);
   a.D4 = (D + 3) / 4 * 4;
+  const unsigned long long ps = static_cast<unsigned long long>(cache->page_size);
+  a.ps_shift = 0;
+  while ((1ull << a.ps_shift) < ps) ++a.ps_shift;
+  a.ps_mul = static_cast<unsigned>((((1ull << a.ps_shift) - ps) << 32) / ps + 1);
 
   if (!(weights ? launch_first<true>(a, p, cache->dtype, stream) : launch_first<false>(a, p, cache->dtype, stream)))
     return ATTN_ERR_LAUNCH;
-  const dim3 grid(p.grid, p.rows), block((D + 31) / 32 * 32);
+  const dim3 grid(p.grid, p.rows), block(kJoinWarps * 32);
   bool ok;
   switch (cache->dtype) {
     case ATTN_F16: ok = launch_after(attn_decode_join_kernel<__half>, grid, block, stream, a); break;

@@ -80,7 +80,9 @@ def kv_page_bounds(k_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: t
     ``bounds[page, h, 0 or 1]`` for the pages of the given sequences, over the
     sequence's tokens in the page.  ``[num_pages, Hkv, 2, D]`` in the cache's
     type; written to ``bounds`` if given (pages of no sequence keep their
-    values), else to a new tensor (where they are zero).  Returns it.
+    values), else to a new tensor (where they are zero).  A page that sequences
+    share should hold the same tokens of each, otherwise it gets the bounds of
+    one of them.  Returns it.
     """
     return rocm_attn_ext.kv_page_bounds(k_cache, block_table, seq_lens, bounds)
 

@@ -488,8 +488,9 @@ def test_evict_bad_pages(attn):
 
 def test_capture_follows_lengths_and_pages(attn):
     lens = [50, 0, 700, 3]
-    k, v, table, ln = make_cache(lens, 2, 128, 16, BF16, width=60, poison=False, spare=100)
-    table = torch.randint(0, k.shape[0], (4, 60), dtype=torch.int32)
+    # no page in two sequences: bounds of a page that two of them fill differently would be either's
+    k, v, table, ln = make_cache(lens, 2, 128, 16, BF16, width=60, poison=False, spare=240)
+    table = torch.randperm(k.shape[0])[:240].reshape(4, 60).to(torch.int32)
     q = _q(4, 8, 128, BF16)
     dk, dv, dt, dl, dq = (t.cuda() for t in (k, v, table, ln, q))
     w = torch.zeros(4, 2, 960, device="cuda")
@@ -507,7 +508,7 @@ def test_capture_follows_lengths_and_pages(attn):
     streams = [torch.cuda.Stream(), torch.cuda.Stream()]
     for new in ([50, 0, 700, 3], [1, 960, 5, 0], [300, 301, 302, 303]):
         dl.copy_(torch.tensor(new, dtype=torch.int32))
-        table = torch.randint(0, k.shape[0], (4, 60), dtype=torch.int32)
+        table = torch.randperm(k.shape[0])[:240].reshape(4, 60).to(torch.int32)
         dt.copy_(table)
         torch.cuda.synchronize()
         for _ in range(5):
