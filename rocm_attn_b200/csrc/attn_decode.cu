@@ -298,7 +298,7 @@ struct MmaCfg {
   static constexpr int kTile = kWarps * kKeys;
   static constexpr int kCtas = kD <= 128 ? 2 : 1;
   static constexpr int kStageBytes = kKeys * kD * 4;
-  static constexpr int kStages = 3;
+  static constexpr int kStages = 2;
   static constexpr int kRingBytes = kWarps * kStages * kStageBytes;
   static constexpr int kMaxHeads = kD <= 128 ? 32 : 16;  // query heads per unit
 };
