@@ -40,11 +40,13 @@
 
 #include "paged_cache.h"
 #include "sm100_ptx.cuh"
+#include "tensor_map.h"
 
 namespace ra {
 
 namespace {
 
+// What went wrong since the word was last read (kFault* bits).
 __device__ int g_page_fault = 0;
 
 constexpr int kWarps = 4;
@@ -246,7 +248,7 @@ __device__ __forceinline__ void locate_physical(const DecodeArgs& a, int b, int 
 // After both: whether there is such a token, in a page of the cache.
 __device__ __forceinline__ bool located(const DecodeArgs& a, int page, int row, int* fault) {
   const bool in = static_cast<unsigned>(page) < static_cast<unsigned>(a.c.num_pages);
-  if (row >= 0 && !in) *fault = 1;
+  if (row >= 0 && !in) *fault |= kFaultPage;
   return row >= 0 && in;
 }
 
@@ -309,8 +311,17 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
   return y;
 }
 
-template <bool kBf16, int kD, int kNT, bool kWeights>
-__global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas) attn_decode_mma_kernel(const __grid_constant__ DecodeArgs a) {
+// The two caches as [num_pages, heads, page_size, D] tensors read in boxes of
+// `rows` rows (16 or 8, a divisor of the page size) by 64 columns.
+struct TmaMaps {
+  CUtensorMap k, v;
+  int rows;
+  unsigned long long wait_ns;
+};
+
+template <bool kBf16, int kD, int kNT, bool kWeights, bool kTma>
+__global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
+    attn_decode_mma_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ TmaMaps maps) {
   using C = MmaCfg<kD>;
   using T = typename std::conditional<kBf16, __nv_bfloat16, __half>::type;
   constexpr int kKeys = C::kKeys, kTile = C::kTile, kStages = C::kStages;
@@ -322,29 +333,38 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas) attn_decode_mma_k
   __shared__ ScheduleSmem s_sched;
   __shared__ float s_m[2][kWarps][8 * kNT], s_l[2][kWarps][8 * kNT];
   __shared__ uint32_t s_mask[kWarps][kStages];
+  __shared__ uint64_t s_full[kWarps][kStages];
+  __shared__ int s_abort, s_code, s_late;
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int fault = 0;
   if (threadIdx.x == 0) a.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
+  if constexpr (kTma) {
+    if (lane == 0) {
+      tma_prefetch_desc(&maps.k);
+      tma_prefetch_desc(&maps.v);
+#pragma unroll
+      for (int s = 0; s < kStages; ++s) mbar_init(&s_full[warp][s], 1);
+      fence_mbar_init();
+    }
+    if (threadIdx.x == 0) s_abort = s_code = s_late = 0;
+  }
   int n;
   long long per;
-  Cursor cur = schedule<kTile>(a, s_sched, &n, &per, &fault);
+  Cursor cur = schedule<kTile>(a, s_sched, &n, &per, &fault);  // (its barriers cover the set-up above)
   launch_dependents();
   zero_empty_rows<T>(a, &fault);
 
   unsigned char* ring = smem + warp * (kStages * C::kStageBytes);
   const uint32_t ring_addr = smem_addr(ring);
-  // A lane copies one 16-byte column (zeros behind D) of every kRowsPerCopy-th
-  // row; with the rows of a chunk 2 kD bytes apart and the chunk aligned to
-  // that, the swizzle of later rows is an XOR of the address with a constant.
+  // Without TMA a lane copies one 16-byte column (zeros behind D) of every
+  // kRowsPerCopy-th row; the swizzle of later rows is an XOR with a constant.
   const int my_row = lane / kCols;
   const bool my_col_ok = (lane % kCols) * 8 < a.c.D;
   const int my_col = my_col_ok ? (lane % kCols) * 8 : 0;
-  const uint32_t my_dst = my_row * (kD * 2) + (((lane % kCols) ^ my_row) << 4);
+  const uint32_t my_dst = (lane % kCols) / 8 * (kKeys * 128) + my_row * 128 + (((lane % 8) ^ my_row) << 4);
   const T* kbase = static_cast<const T*>(a.c.k) + my_col;
   const T* vbase = static_cast<const T*>(a.c.v) + my_col;
-  // Where 16 divides the page size, 16 tokens in a row are rows of one page.
-  const bool one_page = a.c.page_size % 16 == 0;
 
   // The chunks whose copies go out next, with the page and row of each token
   // (lane = token): logical pages are looked up kStages + 1 chunks ahead of
@@ -366,46 +386,50 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas) attn_decode_mma_k
     }
   };
   auto physical = [&](int s) { locate_physical(a, last_b, last_len, &page[s], &row[s]); };
+  const uint64_t policy = l2_policy_evict_first();
   auto issue = [&](int stage) {
     const uint32_t mask = __ballot_sync(0xffffffffu, located(a, page[0], row[0], &fault));
     if (lane == 0) s_mask[warp][stage] = mask;
-    if (mask != 0) {
-      const uint32_t dst = ring_addr + stage * C::kStageBytes + my_dst;
-      const T* kh = kbase + head[0] * a.c.ks[1];
-      const T* vh = vbase + head[0] * a.c.vs[1];
+    if constexpr (kTma) {
+      // One lane asks for the boxes that hold tokens.  All rows of a box lie
+      // in one page; its first row holds a token if any does.
+      if (mask != 0) {
+        const int boxes = kKeys / maps.rows;
+        uint32_t first = 0;  // first rows of the boxes wanted
+        for (int j = 0; j < boxes; ++j) first |= mask & (1u << (j * maps.rows));
+        if (lane == 0) mbar_arrive_expect_tx(&s_full[warp][stage], __popc(first) * maps.rows * (kD * 4));
+        while (first != 0) {
+          const int at = __ffs(first) - 1;
+          first &= first - 1;
+          const int pg = __shfl_sync(0xffffffffu, page[0], at), in = __shfl_sync(0xffffffffu, row[0], at);
+          if (lane == 0) {
+            const uint32_t dst = ring_addr + stage * C::kStageBytes + at * 128;
 #pragma unroll
-      for (int g = 0; g < kKeys / 16; ++g) {
-        if (one_page) {
-          // All 16 rows lie in the page, whether they hold tokens or not; the
-          // first does if any does, and those that do come first.
-          const int pg = __shfl_sync(0xffffffffu, page[0], g * 16), in = __shfl_sync(0xffffffffu, row[0], g * 16);
-          const int live = __popc(mask >> (g * 16) & 0xffffu);
-          const T* kp = live ? kh + pg * a.c.ks[0] + (in + my_row) * a.c.ks[2] : kh;
-          const T* vp = live ? vh + pg * a.c.vs[0] + (in + my_row) * a.c.vs[2] : vh;
-          const long long k_step = live ? kRowsPerCopy * a.c.ks[2] : 0, v_step = live ? kRowsPerCopy * a.c.vs[2] : 0;
-          const int mine = my_col_ok ? live - my_row : 0;
-#pragma unroll
-          for (int i = 0; i < kCols / 2; ++i) {
-            const uint32_t at = (dst ^ ((i * kRowsPerCopy & 7) << 4)) + (g * 16 + i * kRowsPerCopy) * (kD * 2);
-            cp_async16(at, kp, mine > i * kRowsPerCopy);
-            cp_async16(at + kKeys * kD * 2, vp, mine > i * kRowsPerCopy);
-            kp += k_step;
-            vp += v_step;
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < kCols / 2; ++i) {
-            const int tok = g * 16 + i * kRowsPerCopy + my_row;
-            const int pg = __shfl_sync(0xffffffffu, page[0], tok), in = __shfl_sync(0xffffffffu, row[0], tok);
-            const bool ok = (mask >> tok & 1u) && my_col_ok;
-            const uint32_t at = (dst ^ ((i * kRowsPerCopy & 7) << 4)) + (g * 16 + i * kRowsPerCopy) * (kD * 2);
-            cp_async16(at, kh + (ok ? pg * a.c.ks[0] + in * a.c.ks[2] : 0), ok);
-            cp_async16(at + kKeys * kD * 2, vh + (ok ? pg * a.c.vs[0] + in * a.c.vs[2] : 0), ok);
+            for (int c = 0; c < kD / 64; ++c) {
+              tma_load_4d(dst + c * (kKeys * 128), &maps.k, &s_full[warp][stage], c * 64, in, head[0], pg, policy);
+              tma_load_4d(dst + c * (kKeys * 128) + kKeys * kD * 2, &maps.v, &s_full[warp][stage], c * 64, in, head[0],
+                          pg, policy);
+            }
           }
         }
       }
+    } else {
+      if (mask != 0) {
+        const uint32_t dst = ring_addr + stage * C::kStageBytes + my_dst;
+        const T* kh = kbase + head[0] * a.c.ks[1];
+        const T* vh = vbase + head[0] * a.c.vs[1];
+#pragma unroll
+        for (int i = 0; i < kKeys / kRowsPerCopy; ++i) {
+          const int tok = i * kRowsPerCopy + my_row;
+          const int pg = __shfl_sync(0xffffffffu, page[0], tok), in = __shfl_sync(0xffffffffu, row[0], tok);
+          const bool ok = (mask >> tok & 1u) && my_col_ok;
+          const uint32_t at = (dst ^ ((i * kRowsPerCopy & 7) << 4)) + i * kRowsPerCopy * 128;
+          cp_async16(at, kh + (ok ? pg * a.c.ks[0] + in * a.c.ks[2] : 0), ok);
+          cp_async16(at + kKeys * kD * 2, vh + (ok ? pg * a.c.vs[0] + in * a.c.vs[2] : 0), ok);
+        }
+      }
+      cp_async_commit();
     }
-    cp_async_commit();
 #pragma unroll
     for (int s = 0; s < kStages; ++s) {
       page[s] = page[s + 1];
@@ -435,6 +459,17 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas) attn_decode_mma_k
   float m[kNT][2], l[kNT][2];  // of query heads 8 t + 2 (lane % 4) + {0, 1}
   bool begun = cur.t == 0, fresh = true;
   int parity = 0, stage = 0;
+  uint32_t phase = 0;  // of each stage's barrier
+
+  // Scores of tokens lane / 4 + {0, 8} of the chunk's g-th 16 and of two heads
+  // of column tile t, for the weights.
+  auto keep_scores = [&](int t, int g, float x0, float x1, float y0, float y1) {
+    const int rows = min(a.rows, a.group - cur.rt * a.rows), r = t * 8 + (lane & 3) * 2;
+    const long long row0 = static_cast<long long>(cur.b) * a.Hq + cur.h * a.group + cur.rt * a.rows;
+    float* x = a.x + (row0 + r) * a.x_stride + cur.t * kTile + warp * kKeys + g * 16 + (lane >> 2);
+    if (r < rows) x[0] = x0, x[8] = y0;
+    if (r + 1 < rows) x[a.x_stride] = x1, x[a.x_stride + 8] = y1;
+  };
 
   // The first kStages turns only fill the ring (one copy of the code: a CTA's
   // first pass over it comes from a cold instruction cache).
@@ -461,15 +496,43 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas) attn_decode_mma_k
         }
         fresh = false;
       }
-      cp_async_wait<kStages - 1>();
+      if constexpr (!kTma) cp_async_wait<kStages - 1>();
       __syncwarp();
       const uint32_t mask = s_mask[warp][stage];
       if (mask != 0 || kWeights) {
         const uint32_t chunk = ring_addr + stage * C::kStageBytes;
-        const uint32_t kaddr = chunk + (lane & 15) * (kD * 2) + (((lane >> 4) ^ (lane & 7)) << 4);
-        const uint32_t vaddr = chunk + (kKeys + (lane >> 4) * 8 + (lane & 7)) * (kD * 2) + (((lane >> 3 & 1) ^ (lane & 7)) << 4);
+        const uint32_t kaddr = chunk + (lane & 15) * 128 + (((lane >> 4) ^ (lane & 7)) << 4);
+        const uint32_t vaddr = chunk + kKeys * kD * 2 + ((lane >> 4) * 8 + (lane & 7)) * 128 + (((lane >> 3 & 1) ^ (lane & 7)) << 4);
+        if constexpr (kTma) {
+          if (mask != 0) {
+            // A wait that runs out marks the launch; the CTA goes on, at once
+            // from then on, so that its warps still meet.
+            if (!mbar_wait(&s_full[warp][stage], phase >> stage & 1u, &s_abort, &s_code, 1, maps.wait_ns)) fault |= kFaultWait;
+            phase ^= 1u << stage;
+            if (mask != 0xffffffffu >> (32 - kKeys)) {
+              // Rows of a box that hold no token have come along; V's are
+              // cleared, as no weight, not even zero, may meet them.
+#pragma unroll 1
+              for (int e = lane; e < kKeys * kCols; e += 32) {
+                const int r = e % kKeys, c = e / kKeys;
+                if (!(mask >> r & 1u))
+                  *reinterpret_cast<uint4*>(ring + stage * C::kStageBytes + kKeys * kD * 2 + (c / 8) * (kKeys * 128) + r * 128 + (c % 8) * 16) = make_uint4(0, 0, 0, 0);
+              }
+              fence_proxy_async_smem();
+              __syncwarp();
+            }
+          }
+        }
 #pragma unroll
         for (int g = 0; g < kKeys / 16; ++g) {
+          const uint32_t live = mask >> (g * 16) & 0xffffu;
+          if (live == 0) {
+            if constexpr (kWeights) {
+#pragma unroll
+              for (int t = 0; t < kNT; ++t) keep_scores(t, g, -INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            }
+            continue;
+          }
           // Scores of 16 tokens: thread has tokens lane / 4 + {0, 8} of its two
           // heads.  Even and odd steps of the head dim in two accumulators.
           float s[kNT][4], s2[kNT][4];
@@ -480,30 +543,22 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas) attn_decode_mma_k
 #pragma unroll
           for (int ks = 0; ks < kSteps; ++ks) {
             uint32_t kf[4];
-            ldsm_x4((kaddr ^ (ks * 32)) + g * 16 * (kD * 2), kf);
+            ldsm_x4((kaddr ^ (ks % 4 * 32)) + (ks / 4 * kKeys + g * 16) * 128, kf);
 #pragma unroll
             for (int t = 0; t < kNT; ++t)
               mma16816<kBf16>(ks % 2 ? s2[t] : s[t], kf, qf[t][ks][0], qf[t][ks][1]);
           }
           uint32_t pf[kNT][2];
-          const uint32_t live = mask >> (g * 16);
 #pragma unroll
           for (int t = 0; t < kNT; ++t) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[t][e] = (s[t][e] + s2[t][e]) * a.scale_log2;
-            if ((live & 0xffffu) != 0xffffu) {
+            if (live != 0xffffu) {
 #pragma unroll
               for (int e = 0; e < 4; ++e)
                 if (!(live >> ((e >> 1) * 8 + (lane >> 2)) & 1u)) s[t][e] = -INFINITY;
             }
-            if constexpr (kWeights) {
-              const int rows = min(a.rows, a.group - cur.rt * a.rows);
-              const long long r0 = static_cast<long long>(cur.b) * a.Hq + cur.h * a.group + cur.rt * a.rows;
-              const int r = t * 8 + (lane & 3) * 2;
-              float* x = a.x + (r0 + r) * a.x_stride + cur.t * kTile + warp * kKeys + g * 16 + (lane >> 2);
-              if (r < rows) x[0] = s[t][0], x[8] = s[t][2];
-              if (r + 1 < rows) x[a.x_stride] = s[t][1], x[a.x_stride + 8] = s[t][3];
-            }
+            if constexpr (kWeights) keep_scores(t, g, s[t][0], s[t][1], s[t][2], s[t][3]);
             float f[2], top[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
@@ -539,7 +594,7 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas) attn_decode_mma_k
 #pragma unroll
           for (int j = 0; j < kSteps; ++j) {
             uint32_t vf[4];
-            ldsm_x4_trans((vaddr ^ (j * 32)) + g * 16 * (kD * 2), vf);
+            ldsm_x4_trans((vaddr ^ (j % 4 * 32)) + (j / 4 * kKeys + g * 16) * 128, vf);
 #pragma unroll
             for (int t = 0; t < kNT; ++t) mma16816<kBf16>(o[t][j], vf, pf[t][0], pf[t][1]);
           }
@@ -618,6 +673,7 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas) attn_decode_mma_k
               if (c4 == 0) a.part_ml[slot] = make_float2(M, L);
             }
           }
+          if constexpr (kTma) fence_proxy_async_smem();
           __syncthreads();  // the chunks are read before they are filled again
         }
         parity ^= 1;
@@ -630,8 +686,16 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas) attn_decode_mma_k
     stage = stage + 1 == kStages ? 0 : stage + 1;
     if (i >= 0) advance<kTile>(a, cur, &fault);
   }
-  cp_async_wait<0>();
-  if (fault) atomicOr(&g_page_fault, 1);
+  if constexpr (kTma) {
+    if (s_abort) {
+      // Copies still in flight must not outlive the CTA's shared memory.
+      for (int s = 0; s < kStages; ++s)
+        if (s_mask[warp][s] != 0) mbar_wait(&s_full[warp][s], phase >> s & 1u, &s_late, &s_code, 1);
+    }
+  } else {
+    cp_async_wait<0>();
+  }
+  if (fault) atomicOr(&g_page_fault, fault);
 }
 
 // ---------------------------------------------------------------------------
@@ -811,7 +875,7 @@ __global__ void __launch_bounds__(kThreads) attn_decode_simt_kernel(const __grid
     }
     advance<kTile>(a, cur, &fault);
   }
-  if (fault) atomicOr(&g_page_fault, 1);
+  if (fault) atomicOr(&g_page_fault, fault);
 }
 
 // ---------------------------------------------------------------------------
@@ -975,9 +1039,9 @@ int check_decode(const AttnPagedCache* c, int Hq, const void* pages, int n_pages
 
 // The first launch on a device opts the kernel in to its shared memory and to
 // the largest shared-memory share of the SM, so that two CTAs fit.
-template <bool kBf16, int kD, int kNT, bool kWeights>
-bool launch_mma(const DecodeArgs& a, int grid, cudaStream_t stream) {
-  auto kern = attn_decode_mma_kernel<kBf16, kD, kNT, kWeights>;
+template <bool kBf16, int kD, int kNT, bool kWeights, bool kTma>
+bool launch_mma(const DecodeArgs& a, const TmaMaps& maps, int grid, cudaStream_t stream) {
+  auto kern = attn_decode_mma_kernel<kBf16, kD, kNT, kWeights, kTma>;
   static bool done[64] = {};
   static std::mutex mu;
   int dev = 0;
@@ -993,26 +1057,43 @@ bool launch_mma(const DecodeArgs& a, int grid, cudaStream_t stream) {
       done[dev] = true;
     }
   }
-  kern<<<grid, kThreads, MmaCfg<kD>::kRingBytes, stream>>>(a);
+  kern<<<grid, kThreads, MmaCfg<kD>::kRingBytes, stream>>>(a, maps);
   return cudaGetLastError() == cudaSuccess;
 }
 
 // Column tiles of eight query heads: 1, 2 or 4.
-template <bool kBf16, int kD, bool kWeights>
-bool launch_mma_tiles(const DecodeArgs& a, int grid, cudaStream_t stream) {
-  if (a.rows <= 8) return launch_mma<kBf16, kD, 1, kWeights>(a, grid, stream);
-  if (a.rows <= 16) return launch_mma<kBf16, kD, 2, kWeights>(a, grid, stream);
-  if constexpr (MmaCfg<kD>::kMaxHeads > 16) return launch_mma<kBf16, kD, 4, kWeights>(a, grid, stream);
+template <bool kBf16, int kD, bool kWeights, bool kTma>
+bool launch_mma_tiles(const DecodeArgs& a, const TmaMaps& maps, int grid, cudaStream_t stream) {
+  if (a.rows <= 8) return launch_mma<kBf16, kD, 1, kWeights, kTma>(a, maps, grid, stream);
+  if (a.rows <= 16) return launch_mma<kBf16, kD, 2, kWeights, kTma>(a, maps, grid, stream);
+  if constexpr (MmaCfg<kD>::kMaxHeads > 16) return launch_mma<kBf16, kD, 4, kWeights, kTma>(a, maps, grid, stream);
   return false;
 }
 
-template <bool kBf16, bool kWeights>
-bool launch_mma_d(const DecodeArgs& a, int kd, int grid, cudaStream_t stream) {
+template <bool kBf16, bool kWeights, bool kTma>
+bool launch_mma_d(const DecodeArgs& a, const TmaMaps& maps, int kd, int grid, cudaStream_t stream) {
   switch (kd) {
-    case 64: return launch_mma_tiles<kBf16, 64, kWeights>(a, grid, stream);
-    case 128: return launch_mma_tiles<kBf16, 128, kWeights>(a, grid, stream);
-    default: return launch_mma_tiles<kBf16, 256, kWeights>(a, grid, stream);
+    case 64: return launch_mma_tiles<kBf16, 64, kWeights, kTma>(a, maps, grid, stream);
+    case 128: return launch_mma_tiles<kBf16, 128, kWeights, kTma>(a, maps, grid, stream);
+    default: return launch_mma_tiles<kBf16, 256, kWeights, kTma>(a, maps, grid, stream);
   }
+}
+
+// TMA where 8 divides the page size (a box is rows of one page) and the
+// strides suit it, else 16-byte copies.
+template <bool kBf16, bool kWeights>
+bool launch_mma_any(const DecodeArgs& a, const Plan& p, cudaStream_t stream) {
+  TmaMaps maps;
+  maps.rows = a.c.page_size % 16 == 0 ? 16 : 8;
+  const unsigned long long limit = wait_limit_ns();
+  maps.wait_ns = limit != 0 ? limit : kWaitTimeoutNs;
+  auto encode = [&](CUtensorMap* map, const void* base, const long long* st) {
+    return make_tensor_map_4d(map, base, kBf16, a.c.D, a.c.page_size, a.c.heads, a.c.num_pages, st[2], st[1], st[0], 64,
+                              maps.rows) == 0;
+  };
+  if (a.c.page_size % 8 == 0 && a.c.num_pages > 0 && encode(&maps.k, a.c.k, a.c.ks) && encode(&maps.v, a.c.v, a.c.vs))
+    return launch_mma_d<kBf16, kWeights, true>(a, maps, p.kd, p.grid, stream);
+  return launch_mma_d<kBf16, kWeights, false>(a, maps, p.kd, p.grid, stream);
 }
 
 template <typename T, int kPer, bool kWeights>
@@ -1041,8 +1122,8 @@ bool launch_simt(const DecodeArgs& a, int per, int grid, cudaStream_t stream) {
 template <bool kWeights>
 bool launch_first(const DecodeArgs& a, const Plan& p, AttnDType dtype, cudaStream_t stream) {
   if (p.mma)
-    return dtype == ATTN_BF16 ? launch_mma_d<true, kWeights>(a, p.kd, p.grid, stream)
-                              : launch_mma_d<false, kWeights>(a, p.kd, p.grid, stream);
+    return dtype == ATTN_BF16 ? launch_mma_any<true, kWeights>(a, p, stream)
+                              : launch_mma_any<false, kWeights>(a, p, stream);
   switch (dtype) {
     case ATTN_F16: return launch_simt<__half, kWeights>(a, p.kd, p.grid, stream);
     case ATTN_BF16: return launch_simt<__nv_bfloat16, kWeights>(a, p.kd, p.grid, stream);

@@ -354,7 +354,7 @@ extern "C" int attn_get_status(cudaStream_t stream, int* status) {
       ra::page_word_read_clear_decode(stream, &decode) != 0 ||
       ra::page_word_read_clear_cache(stream, &cache) != 0 || cudaStreamSynchronize(stream) != cudaSuccess)
     return ATTN_ERR_LAUNCH;
-  if (single != 0 || grouped != 0)
+  if (single != 0 || grouped != 0 || ((decode | cache) & ra::kFaultWait) != 0)
     *status = ATTN_ERR_WATCHDOG;
   else
     *status = (decode == 0 && cache == 0) ? ATTN_OK : ATTN_ERR_BAD_PAGE;

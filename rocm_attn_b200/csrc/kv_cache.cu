@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(256) kv_rows_kernel(const __grid_constant__ Ro
     if (a.new_lens) {
       n = __ldg(a.new_lens + b);
       if (n > a.S) {
-        fault = 1;
+        fault |= kFaultPage;
         n = a.S;
       }
       if (n < 0) n = 0;
@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(256) kv_rows_kernel(const __grid_constant__ Ro
     first = start > 0 ? start : 0;
   }
   if (len > cap) {
-    fault = 1;
+    fault |= kFaultPage;
     len = cap;
   }
   const int lp = static_cast<int>(first / ps) + run;
@@ -532,7 +532,7 @@ __global__ void __launch_bounds__(256) kv_evict_copy_kernel(const __grid_constan
       row[i] = static_cast<int>(place) - np * ps;
       const int t = __ldg(a.new_table + b * a.new_stride + np);
       const bool good = static_cast<unsigned>(t) < static_cast<unsigned>(a.c.num_pages);
-      if (!good) fault = 1;
+      if (!good) fault |= kFaultPage;
       if (good && page >= 0) {
         to[i] = t;
         x[i] = *reinterpret_cast<const V*>(ck + page * a.c.ks[0] + (src - lp * ps) * a.c.ks[2]);

@@ -38,8 +38,12 @@ int check_paged_cache(const AttnPagedCache* c, int tensors, PagedView* view);
 // its multiprocessor count (0 if it cannot be read).
 int check_device();
 int sm_count();
+unsigned long long wait_limit_ns();  // the setting of attn_set_wait_limit_ns
 
-// Copies of the page-fault words of the two translation units into *host and
+// Faults a kernel records: a page or length out of range, a wait that ran out.
+constexpr int kFaultPage = 1, kFaultWait = 2;
+
+// Copies of the fault words of the two translation units into *host and
 // resets, queued on `stream` (see attn_get_status).
 int page_word_read_clear_decode(cudaStream_t stream, int* host);
 int page_word_read_clear_cache(cudaStream_t stream, int* host);
@@ -72,7 +76,7 @@ bool launch_after(void (*kern)(Params...), dim3 grid, dim3 block, cudaStream_t s
 __device__ __forceinline__ int paged_len(const PagedView& c, int b, int* fault) {
   const int n = __ldg(c.lens + b);
   if (n > c.capacity()) {
-    *fault = 1;
+    *fault |= kFaultPage;
     return c.capacity();
   }
   return n > 0 ? n : 0;
@@ -83,7 +87,7 @@ __device__ __forceinline__ int paged_len(const PagedView& c, int b, int* fault) 
 __device__ __forceinline__ int paged_page(const PagedView& c, int b, int lp, int* fault) {
   const int p = __ldg(c.table + static_cast<long long>(b) * c.table_stride + lp);
   if (static_cast<unsigned>(p) < static_cast<unsigned>(c.num_pages)) return p;
-  *fault = 1;
+  *fault |= kFaultPage;
   return -1;
 }
 #endif
