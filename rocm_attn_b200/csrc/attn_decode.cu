@@ -51,6 +51,7 @@ __device__ int g_page_fault = 0;
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
+constexpr int kMaxCluster = 8;
 constexpr int kSimtRows = 8;  // query heads per unit of the SIMT kernel, at most
 
 struct DecodeArgs {
@@ -62,6 +63,7 @@ struct DecodeArgs {
   float scale_log2;
   const int* pages;  // [B, heads, n_pages] contiguous, or null
   int n_pages;
+  int cluster;      // CTAs per unit (a cluster), or 0: runs of tiles over the whole grid
   float* x;         // [B, Hq, x_stride] scores in the exp2 domain, or null
   long long x_stride;
   float* lse2;      // [B, Hq] M + log2 L, or null
@@ -144,7 +146,8 @@ __device__ __forceinline__ int tiles_of(const DecodeArgs& a, int len) {
 
 template <int kTile>
 __device__ __forceinline__ void advance(const DecodeArgs& a, Cursor& c, int* fault) {
-  if (++c.t < c.T) return;
+  c.t += max(a.cluster, 1);
+  if (c.t < c.T) return;
   c.t = 0;
   if (++c.rt < a.row_tiles) return;
   c.rt = 0;
@@ -158,54 +161,55 @@ __device__ __forceinline__ void advance(const DecodeArgs& a, Cursor& c, int* fau
 }
 
 struct ScheduleSmem {
-  long long warp_sum[kWarps];
+  int warp_sum[kWarps];
   Cursor first;
 };
 
 // Works out this CTA's run: its first tile (returned), the number of its
-// tiles *n and the run length of the grid *per.
+// tiles *n and the run length of the grid *per.  The host keeps the number of
+// tiles the block table can name below 2^31.
 template <int kTile>
-__device__ __forceinline__ Cursor schedule(const DecodeArgs& a, ScheduleSmem& s, int* n, long long* per, int* fault) {
+__device__ __forceinline__ Cursor schedule(const DecodeArgs& a, ScheduleSmem& s, int* n, int* per, int* fault) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int seg = (a.c.B + kThreads - 1) / kThreads;
   const int b0 = min(a.c.B, tid * seg), b1 = min(a.c.B, b0 + seg);
-  long long mine = 0;
-  for (int b = b0; b < b1; ++b) mine += tiles_of<kTile>(a, paged_len(a.c, b, fault));
-  long long upto = mine;
+  int mine = 0, len = 0, T = 0;
+  for (int b = b0; b < b1; ++b) {
+    len = paged_len(a.c, b, fault);
+    T = tiles_of<kTile>(a, len);
+    mine += T;
+  }
+  int upto = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long y = __shfl_up_sync(0xffffffffu, upto, o);
+    const int y = __shfl_up_sync(0xffffffffu, upto, o);
     if (lane >= o) upto += y;
   }
   if (lane == 31) s.warp_sum[warp] = upto;
   __syncthreads();
-  long long before = 0, total = 0;
+  int before = upto - mine, total = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
     if (w < warp) before += s.warp_sum[w];
     total += s.warp_sum[w];
   }
   const int units = a.c.heads * a.row_tiles;
-  // 64-bit division takes about half a microsecond
   total *= units;
-  *per = total <= 0x7fffffffLL - gridDim.x ? (static_cast<unsigned>(total) + gridDim.x - 1) / gridDim.x
-                                           : (total + gridDim.x - 1) / gridDim.x;
-  const long long f0 = *per * blockIdx.x;
-  *n = static_cast<int>(max(0LL, min(*per, total - f0)));  // the host checks that it fits
-  before += upto - mine;
+  *per = static_cast<int>((static_cast<unsigned>(total) + gridDim.x - 1) / gridDim.x);
+  const long long f0 = static_cast<long long>(*per) * blockIdx.x;
+  *n = static_cast<int>(max(0LL, min(static_cast<long long>(*per), total - f0)));
   if (*n > 0 && f0 >= before * units && f0 < (before + mine) * units) {
-    for (int b = b0; b < b1; ++b) {
-      const int len = paged_len(a.c, b, fault);
-      const int T = tiles_of<kTile>(a, len);
-      if (f0 < (before + T) * units) {
-        const long long in = f0 - before * units;
-        const int hu = in <= 0x7fffffffLL ? static_cast<int>(in) / T : static_cast<int>(in / T);
-        const int h = hu / a.row_tiles;
-        s.first = Cursor{b, h, hu - h * a.row_tiles, static_cast<int>(in - static_cast<long long>(hu) * T), T, len};
-        break;
+    int in = static_cast<int>(f0) - before * units, b = b0;
+    if (seg > 1) {
+      for (;; ++b) {
+        len = paged_len(a.c, b, fault);
+        T = tiles_of<kTile>(a, len);
+        if (in < T * units || b + 1 >= b1) break;
+        in -= T * units;
       }
-      before += T;
     }
+    const int hu = in / T, h = hu / a.row_tiles;
+    s.first = Cursor{b, h, hu - h * a.row_tiles, in - hu * T, T, len};
   }
   __syncthreads();
   return s.first;
@@ -261,17 +265,15 @@ struct Place {
   int rows, slot;
 };
 
-__device__ __forceinline__ Place place_of(const DecodeArgs& a, const Cursor& c, bool begun, long long per) {
+__device__ __forceinline__ Place place_of(const DecodeArgs& a, const Cursor& c, bool begun, int per) {
   Place p;
   p.rows = min(a.rows, a.group - c.rt * a.rows);
   p.row0 = static_cast<long long>(c.b) * a.Hq + c.h * a.group + c.rt * a.rows;
-  const bool ends = c.t + 1 == c.T;
-  p.whole = begun && ends;
+  const bool ends = a.cluster ? true : c.t + 1 == c.T;
+  p.whole = begun && ends && a.cluster <= 1;
   p.slot = 2 * blockIdx.x + (begun ? 1 : 0);
   if (begun && !ends && threadIdx.x == 0) {
-    const int rest = c.T - (c.t + 1);
-    const int later = per <= 0x3fffffffLL ? (rest + static_cast<int>(per) - 1) / static_cast<int>(per)
-                                          : static_cast<int>((rest + per - 1) / per);
+    const int later = (c.T - (c.t + 1) + per - 1) / per;
     // row0 < B * Hq, which the host keeps below 2^31
     a.meta[blockIdx.x] = make_int4(static_cast<int>(p.row0), p.rows, later, 0);
   }
@@ -311,6 +313,28 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
   return y;
 }
 
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// A value at the same place in the shared memory of CTA `rank` of the cluster.
+__device__ __forceinline__ float cluster_load(const float* p, int rank) {
+  uint32_t at;
+  float x;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_addr(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(at) : "memory");
+  return x;
+}
+__device__ __forceinline__ float4 cluster_load4(const float* p, int rank) {
+  uint32_t at;
+  float4 x;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_addr(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
+               : "r"(at)
+               : "memory");
+  return x;
+}
+
 // The two caches as [num_pages, heads, page_size, D] tensors read in boxes of
 // `rows` rows (16 or 8, a divisor of the page size) by 64 columns.
 struct TmaMaps {
@@ -335,10 +359,10 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
   __shared__ uint32_t s_mask[kWarps][kStages];
   __shared__ uint64_t s_full[kWarps][kStages];
   __shared__ int s_abort, s_code, s_late;
+  __shared__ float s_cm[8 * kNT], s_cl[8 * kNT];  // of this CTA's part of a cluster's unit
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int fault = 0;
-  if (threadIdx.x == 0) a.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
   if constexpr (kTma) {
     if (lane == 0) {
       tma_prefetch_desc(&maps.k);
@@ -349,11 +373,27 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
     }
     if (threadIdx.x == 0) s_abort = s_code = s_late = 0;
   }
-  int n;
-  long long per;
-  Cursor cur = schedule<kTile>(a, s_sched, &n, &per, &fault);  // (its barriers cover the set-up above)
   launch_dependents();
-  zero_empty_rows<T>(a, &fault);
+  grid_dependency_wait();
+  int n, per = 1;
+  Cursor cur;
+  if (a.cluster) {
+    // Tiles rank, rank + cluster, ... of one unit.  Which they are does not
+    // depend on the length, so the first look-ups need not wait for it.
+    const int unit = blockIdx.x / a.cluster, hu = unit % (a.c.heads * a.row_tiles);
+    cur.b = unit / (a.c.heads * a.row_tiles);
+    cur.h = hu / a.row_tiles;
+    cur.rt = hu - cur.h * a.row_tiles;
+    cur.t = blockIdx.x % a.cluster;
+    cur.len = a.pages ? paged_len(a.c, cur.b, &fault) : a.c.capacity();
+    cur.T = tiles_of<kTile>(a, cur.len);
+    n = (cur.T - cur.t + a.cluster - 1) / a.cluster;
+    if (threadIdx.x < 8 * kNT) s_cm[threadIdx.x] = -INFINITY, s_cl[threadIdx.x] = 0.f;
+  } else {
+    if (threadIdx.x == 0) a.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
+    cur = schedule<kTile>(a, s_sched, &n, &per, &fault);
+    zero_empty_rows<T>(a, &fault);
+  }
 
   unsigned char* ring = smem + warp * (kStages * C::kStageBytes);
   const uint32_t ring_addr = smem_addr(ring);
@@ -453,11 +493,25 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
 #pragma unroll
     for (int s = 0; s < kStages; ++s) locate_physical(a, bs[s], ls[s], &page[s], &row[s]);
   }
+  if (a.cluster) {
+    if (!a.pages) {
+      // The length: what was looked up behind it does not count.
+      cur.len = ahead.len = last_len = paged_len(a.c, cur.b, &fault);
+      cur.T = ahead.T = tiles_of<kTile>(a, cur.len);
+      n = max(0, (cur.T - cur.t + a.cluster - 1) / a.cluster);
+#pragma unroll
+      for (int s = 0; s <= kStages; ++s)
+        if ((cur.t + s * a.cluster) * kTile + warp * kKeys + lane >= cur.len) row[s] = -1;
+    }
+    __syncthreads();  // the set-up above
+  }
 
+  const int cur_rt = cur.rt, unit_T = cur.T;
+  const long long unit_row0 = static_cast<long long>(cur.b) * a.Hq + cur.h * a.group + cur.rt * a.rows;
   uint32_t qf[kNT][kSteps][2];
   float o[kNT][kSteps][4];
   float m[kNT][2], l[kNT][2];  // of query heads 8 t + 2 (lane % 4) + {0, 1}
-  bool begun = cur.t == 0, fresh = true;
+  bool begun = a.cluster ? true : cur.t == 0, fresh = true;
   int parity = 0, stage = 0;
   uint32_t phase = 0;  // of each stage's barrier
 
@@ -469,6 +523,14 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
     float* x = a.x + (row0 + r) * a.x_stride + cur.t * kTile + warp * kKeys + g * 16 + (lane >> 2);
     if (r < rows) x[0] = x0, x[8] = y0;
     if (r + 1 < rows) x[a.x_stride] = x1, x[a.x_stride + 8] = y1;
+  };
+
+  // Row r of this CTA's part of its cluster's unit: in the chunk of warp r / 16
+  // that the unit's end leaves free.
+  static_assert(kStages >= 2, "one chunk is scratch space, another holds the part");
+  auto cluster_part = [&](int r) {
+    const int other = n % kStages;  // the last chunk was n - 1
+    return reinterpret_cast<float*>(smem + ((r >> 4) * kStages + other) * C::kStageBytes) + (r & 15) * kD;
   };
 
   // The first kStages turns only fill the ring (one copy of the code: a CTA's
@@ -601,7 +663,7 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
         }
       }
 
-      if (cur.t + 1 == cur.T || i + 1 == n) {
+      if ((!a.cluster && cur.t + 1 == cur.T) || i + 1 == n) {
         // The unit, or this CTA's part of it, ends: the warps' parts are scaled
         // to their common maximum and summed over the chunks just freed, 16 heads
         // at a time.
@@ -667,6 +729,10 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
               *reinterpret_cast<uint2*>(out) =
                   make_uint2(pack2<kBf16>(sum.x * inv, sum.y * inv), pack2<kBf16>(sum.z * inv, sum.w * inv));
               if (kWeights && c4 == 0) a.lse2[p.row0 + r] = L == 0.f ? INFINITY : M + log2f(L);
+            } else if (a.cluster) {
+              // kept for the cluster in the other chunk of warp 0 (or 1), which is free: there are no more tiles
+              *reinterpret_cast<float4*>(cluster_part(r) + c4 * 4) = sum;
+              if (c4 == 0) s_cm[r] = M, s_cl[r] = L;
             } else {
               const long long slot = static_cast<long long>(p.slot) * a.rows + r;
               *reinterpret_cast<float4*>(a.part_o + slot * a.D4 + c4 * 4) = sum;
@@ -685,6 +751,55 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
     issue(stage);
     stage = stage + 1 == kStages ? 0 : stage + 1;
     if (i >= 0) advance<kTile>(a, cur, &fault);
+  }
+  if (a.cluster > 1) {
+    // The parts of the cluster's CTAs are joined in their order, each CTA
+    // taking its share of the columns; none leaves before all have read.
+    cluster_sync();
+    const int rank = blockIdx.x % a.cluster, rows = min(a.rows, a.group - cur_rt * a.rows);
+    for (int e = rank * kThreads + threadIdx.x; e < rows * (kD / 4); e += a.cluster * kThreads) {
+      const int r = e / (kD / 4), c4 = e % (kD / 4);
+      if (c4 * 4 >= a.c.D) continue;
+      // All loads first: each takes a good part of a microsecond.
+      float ms[kMaxCluster], ls[kMaxCluster];
+      float4 ys[kMaxCluster];
+#pragma unroll
+      for (int w = 0; w < kMaxCluster; ++w) {
+        if (w < a.cluster) {
+          const int n_w = (unit_T - w + a.cluster - 1) / a.cluster;
+          ms[w] = cluster_load(&s_cm[r], w);
+          ls[w] = cluster_load(&s_cl[r], w);
+          ys[w] = cluster_load4(reinterpret_cast<const float*>(smem + ((r >> 4) * kStages + n_w % kStages) * C::kStageBytes) +
+                                    (r & 15) * kD + c4 * 4,
+                                w);
+        }
+      }
+      float M = -INFINITY, L = 0.f;
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kMaxCluster; ++w)
+        if (w < a.cluster) M = fmaxf(M, ms[w]);
+#pragma unroll
+      for (int w = 0; w < kMaxCluster; ++w) {
+        if (w < a.cluster && ls[w] != 0.f) {  // 0: no token, and no part
+          const float f = ex2_approx(ms[w] - finite_max(M));
+          L += ls[w] * f;
+          sum.x += ys[w].x * f;
+          sum.y += ys[w].y * f;
+          sum.z += ys[w].z * f;
+          sum.w += ys[w].w * f;
+        }
+      }
+      const float inv = L == 0.f ? 0.f : 1.f / L;
+      T* out = static_cast<T*>(a.out) + (unit_row0 + r) * a.c.D + c4 * 4;
+      *reinterpret_cast<uint2*>(out) =
+          make_uint2(pack2<kBf16>(sum.x * inv, sum.y * inv), pack2<kBf16>(sum.z * inv, sum.w * inv));
+      if (kWeights && c4 == 0) a.lse2[unit_row0 + r] = L == 0.f ? INFINITY : M + log2f(L);
+    }
+    cluster_sync();
+  } else if (a.cluster == 1 && n == 0) {
+    const int rows = min(a.rows, a.group - cur_rt * a.rows);
+    for (int e = threadIdx.x; e < rows * a.c.D; e += kThreads) static_cast<T*>(a.out)[unit_row0 * a.c.D + e] = from_f32<T>(0.f);
   }
   if constexpr (kTma) {
     if (s_abort) {
@@ -726,11 +841,11 @@ __global__ void __launch_bounds__(kThreads) attn_decode_simt_kernel(const __grid
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int fault = 0;
-  if (threadIdx.x == 0) a.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
-  int n;
-  long long per;
-  Cursor cur = schedule<kTile>(a, s_sched, &n, &per, &fault);
   launch_dependents();
+  grid_dependency_wait();
+  if (threadIdx.x == 0) a.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
+  int n, per;
+  Cursor cur = schedule<kTile>(a, s_sched, &n, &per, &fault);
   zero_empty_rows<T>(a, &fault);
   const T* kbase = static_cast<const T*>(a.c.k);
   const T* vbase = static_cast<const T*>(a.c.v);
@@ -893,6 +1008,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_decode_join_kernel(const
   __shared__ float4 s_o[kJoinWarps][2][32];
   __shared__ float s_m[kJoinWarps], s_l[kJoinWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  launch_dependents();
   grid_dependency_wait();
   const int c = blockIdx.x, r = blockIdx.y;
   const int4 meta = a.meta[c];
@@ -946,6 +1062,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_decode_join_kernel(const
 // token: reads the scores the kernel before kept.
 __global__ void __launch_bounds__(256) attn_decode_weights_kernel(const __grid_constant__ DecodeArgs a, float* weights,
                                                                   long long w_b, long long w_h) {
+  launch_dependents();
   grid_dependency_wait();
   const int b = blockIdx.z, h = blockIdx.y;
   int fault = 0;  // recorded by the first kernel
@@ -967,8 +1084,8 @@ struct Plan {
   bool mma;
   int kd;  // head dim the kernel is compiled for (mma), or dims per lane (simt)
   int rows, row_tiles, tile;
-  int grid;
-  long long per_cta;  // tiles, at most
+  int grid, cluster;  // see DecodeArgs
+  long long tiles;      // the block table can name
   long long x_stride;
   size_t meta_at, ml_at, o_at, lse_at, x_at, bytes;
 };
@@ -1006,14 +1123,25 @@ Plan make_plan(const AttnPagedCache* c, bool fast, int Hq, int n_pages, bool lis
   long long grid = static_cast<long long>(sms) * per_sm;
   if (grid > tiles) grid = tiles;
   if (grid < 1) grid = 1;
+  p.cluster = 0;
+  if (p.mma) {
+    const long long unit_tiles = (capacity + p.tile - 1) / p.tile, units = static_cast<long long>(c->B) * c->heads * p.row_tiles;
+    int cl = 1;
+    while (cl < kMaxCluster && cl < unit_tiles && units * cl * 2 <= static_cast<long long>(sms) * per_sm) cl *= 2;
+    const long long slots = static_cast<long long>(sms) * per_sm, most = units * cl * 2 >= slots && units * cl <= slots ? 4 : 2;
+    if (unit_tiles <= cl * most && units * cl <= 2 * slots) {
+      p.cluster = cl;
+      grid = units * cl;
+    }
+  }
   p.grid = static_cast<int>(grid);
-  p.per_cta = (tiles + grid - 1) / grid;
+  p.tiles = tiles;
   auto up = [](size_t x) { return (x + 255) & ~static_cast<size_t>(255); };
-  const size_t D4 = (D + 3) / 4 * 4;
+  const size_t D4 = (D + 3) / 4 * 4, parts = p.cluster ? 0 : grid;
   p.meta_at = 0;
-  p.ml_at = up(sizeof(int4) * grid);
-  p.o_at = p.ml_at + up(sizeof(float2) * 2 * grid * p.rows);
-  p.lse_at = p.o_at + up(sizeof(float) * 2 * grid * p.rows * D4);
+  p.ml_at = up(sizeof(int4) * parts);
+  p.o_at = p.ml_at + up(sizeof(float2) * 2 * parts * p.rows);
+  p.lse_at = p.o_at + up(sizeof(float) * 2 * parts * p.rows * D4);
   p.x_at = p.lse_at;
   p.bytes = p.x_at;
   p.x_stride = (capacity + p.tile - 1) / p.tile * p.tile;
@@ -1057,8 +1185,7 @@ bool launch_mma(const DecodeArgs& a, const TmaMaps& maps, int grid, cudaStream_t
       done[dev] = true;
     }
   }
-  kern<<<grid, kThreads, MmaCfg<kD>::kRingBytes, stream>>>(a, maps);
-  return cudaGetLastError() == cudaSuccess;
+  return launch_after(kern, dim3(grid), dim3(kThreads), MmaCfg<kD>::kRingBytes, stream, a.cluster, a, maps);
 }
 
 // Column tiles of eight query heads: 1, 2 or 4.
@@ -1098,15 +1225,11 @@ bool launch_mma_any(const DecodeArgs& a, const Plan& p, cudaStream_t stream) {
 
 template <typename T, int kPer, bool kWeights>
 bool launch_simt_rows(const DecodeArgs& a, int grid, cudaStream_t stream) {
-  if (a.rows <= 1)
-    attn_decode_simt_kernel<T, kPer, 1, kWeights><<<grid, kThreads, 0, stream>>>(a);
-  else if (a.rows <= 2)
-    attn_decode_simt_kernel<T, kPer, 2, kWeights><<<grid, kThreads, 0, stream>>>(a);
-  else if (a.rows <= 4)
-    attn_decode_simt_kernel<T, kPer, 4, kWeights><<<grid, kThreads, 0, stream>>>(a);
-  else
-    attn_decode_simt_kernel<T, kPer, 8, kWeights><<<grid, kThreads, 0, stream>>>(a);
-  return cudaGetLastError() == cudaSuccess;
+  const auto kern = a.rows <= 1   ? attn_decode_simt_kernel<T, kPer, 1, kWeights>
+                    : a.rows <= 2 ? attn_decode_simt_kernel<T, kPer, 2, kWeights>
+                    : a.rows <= 4 ? attn_decode_simt_kernel<T, kPer, 4, kWeights>
+                                  : attn_decode_simt_kernel<T, kPer, 8, kWeights>;
+  return launch_after(kern, dim3(grid), dim3(kThreads), 0, stream, 1, a);
 }
 
 template <typename T, bool kWeights>
@@ -1187,7 +1310,7 @@ extern "C" int launch_attn_decode(const AttnPagedCache* cache, const void* q, co
   if (st != ATTN_OK) return st;
   const bool fast = aligned_to(q, 16) && aligned_to(out, 16) && qs[0] % 8 == 0 && qs[1] % 8 == 0;
   const Plan p = make_plan(cache, fast, Hq, n_pages, pages != nullptr, weights != nullptr, sm_count());
-  if (workspace_bytes < p.bytes || p.per_cta > 0x7fffff00LL) return ATTN_ERR_INVALID_ARGUMENT;
+  if (workspace_bytes < p.bytes || p.tiles > 0x7fffffffLL - 65536) return ATTN_ERR_INVALID_ARGUMENT;
 
   float scale = softmax_scale;
   if (!(scale > 0.f) || !isfinite(scale)) scale = 1.0f / sqrtf(static_cast<float>(D));
@@ -1205,6 +1328,7 @@ extern "C" int launch_attn_decode(const AttnPagedCache* cache, const void* q, co
   a.scale_log2 = scale * 1.4426950408889634f;
   a.pages = pages;
   a.n_pages = n_pages;
+  a.cluster = p.cluster;
   a.x = weights ? reinterpret_cast<float*>(ws + p.x_at) : nullptr;
   a.x_stride = p.x_stride;
   a.lse2 = weights ? reinterpret_cast<float*>(ws + p.lse_at) : nullptr;
@@ -1220,15 +1344,15 @@ extern "C" int launch_attn_decode(const AttnPagedCache* cache, const void* q, co
   if (!(weights ? launch_first<true>(a, p, cache->dtype, stream) : launch_first<false>(a, p, cache->dtype, stream)))
     return ATTN_ERR_LAUNCH;
   const dim3 grid(p.grid, p.rows), block(kJoinWarps * 32);
-  bool ok;
-  switch (cache->dtype) {
-    case ATTN_F16: ok = launch_after(attn_decode_join_kernel<__half>, grid, block, stream, a); break;
-    case ATTN_BF16: ok = launch_after(attn_decode_join_kernel<__nv_bfloat16>, grid, block, stream, a); break;
-    default: ok = launch_after(attn_decode_join_kernel<float>, grid, block, stream, a); break;
+  bool ok = true;
+  if (!p.cluster) switch (cache->dtype) {
+    case ATTN_F16: ok = launch_after(attn_decode_join_kernel<__half>, grid, block, 0, stream, 1, a); break;
+    case ATTN_BF16: ok = launch_after(attn_decode_join_kernel<__nv_bfloat16>, grid, block, 0, stream, 1, a); break;
+    default: ok = launch_after(attn_decode_join_kernel<float>, grid, block, 0, stream, 1, a); break;
   }
   if (ok && weights) {
     const dim3 wgrid((view.capacity() + 255) / 256, cache->heads, cache->B);
-    ok = wgrid.x == 0 || launch_after(attn_decode_weights_kernel, wgrid, dim3(256), stream, a, weights,
+    ok = wgrid.x == 0 || launch_after(attn_decode_weights_kernel, wgrid, dim3(256), 0, stream, 1, a, weights,
                                       weights_strides[0], weights_strides[1]);
   }
   return ok ? ATTN_OK : ATTN_ERR_LAUNCH;

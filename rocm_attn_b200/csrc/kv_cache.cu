@@ -97,6 +97,8 @@ template <typename T, int kVec, bool kAppend, bool kBounds>
 __global__ void __launch_bounds__(256) kv_rows_kernel(const __grid_constant__ RowsArgs a) {
   using V = Vec<T, kVec>;
   __shared__ V s_lo[256], s_hi[256];
+  launch_dependents();
+  grid_dependency_wait();
   const int b = static_cast<int>(blockIdx.x / a.runs), run = static_cast<int>(blockIdx.x - static_cast<unsigned>(b) * a.runs);
   const int ps = a.c.page_size, cap = a.c.capacity();
   int fault = 0;
@@ -239,6 +241,7 @@ __global__ void __launch_bounds__(256) kv_page_score_kernel(const __grid_constan
   using V = Vec<T, kVec>;
   __shared__ double s_up[256], s_down[256];
   launch_dependents();
+  grid_dependency_wait();
   const int b = static_cast<int>(blockIdx.x / a.chunks), chunk = static_cast<int>(blockIdx.x - static_cast<unsigned>(b) * a.chunks);
   const int h = blockIdx.y;
   int fault = 0;
@@ -431,6 +434,7 @@ __device__ void pick_emit(PickSmem& s, Get key, int n, Key prefix, Key mask, int
 __global__ void __launch_bounds__(kPickThreads) kv_pick_pages_kernel(PagedView c, const unsigned long long* keys, int top,
                                                                      int* pages) {
   __shared__ PickSmem s;
+  launch_dependents();
   grid_dependency_wait();
   const int h = blockIdx.x % c.heads, b = blockIdx.x / c.heads;
   int fault = 0;  // recorded by the kernel before
@@ -471,7 +475,7 @@ struct EvictArgs {
 // CTA (head, b): the kept positions and their weights.
 __global__ void __launch_bounds__(kPickThreads) kv_evict_pick_kernel(const __grid_constant__ EvictArgs a) {
   __shared__ PickSmem s;
-  launch_dependents();
+  grid_dependency_wait();
   const int h = blockIdx.x % a.c.heads, b = blockIdx.x / a.c.heads;
   int fault = 0;
   const int n = paged_len(a.c, b, &fault);
@@ -507,6 +511,7 @@ template <typename T, int kVec>
 __global__ void __launch_bounds__(256) kv_evict_copy_kernel(const __grid_constant__ EvictArgs a) {
   using V = Vec<T, kVec>;
   constexpr int kAhead = 4;
+  launch_dependents();
   grid_dependency_wait();
   const int b = static_cast<int>(blockIdx.x / a.chunks), chunk = static_cast<int>(blockIdx.x - static_cast<unsigned>(b) * a.chunks);
   const int h = blockIdx.y, ps = a.c.page_size;
@@ -575,13 +580,10 @@ size_t elem_size(AttnDType t) { return t == ATTN_F32 ? 4 : 2; }
 
 template <typename T, int kVec>
 bool launch_rows_typed(const RowsArgs& a, bool append, dim3 grid, int threads, cudaStream_t stream) {
-  if (!append)
-    kv_rows_kernel<T, kVec, false, true><<<grid, threads, 0, stream>>>(a);
-  else if (a.bounds)
-    kv_rows_kernel<T, kVec, true, true><<<grid, threads, 0, stream>>>(a);
-  else
-    kv_rows_kernel<T, kVec, true, false><<<grid, threads, 0, stream>>>(a);
-  return cudaGetLastError() == cudaSuccess;
+  const auto kern = !append    ? kv_rows_kernel<T, kVec, false, true>
+                    : a.bounds ? kv_rows_kernel<T, kVec, true, true>
+                               : kv_rows_kernel<T, kVec, true, false>;
+  return launch_after(kern, grid, dim3(threads), 0, stream, 1, a);
 }
 
 // rows: rows of one page that a CTA may find to do.
@@ -623,8 +625,7 @@ bool negative(const long long* s, int n) {
 
 template <typename T, int kVec, int kPer>
 bool launch_score(const ScoreArgs& a, dim3 grid, cudaStream_t stream) {
-  kv_page_score_kernel<T, kVec, kPer><<<grid, 256, 0, stream>>>(a);
-  return cudaGetLastError() == cudaSuccess;
+  return launch_after(kv_page_score_kernel<T, kVec, kPer>, grid, dim3(256), 0, stream, 1, a);
 }
 
 template <typename T>
@@ -803,7 +804,7 @@ extern "C" int launch_kv_select_pages(const AttnPagedCache* cache, const void* q
     }
     if (!ok) return ATTN_ERR_LAUNCH;
   }
-  return launch_after(kv_pick_pages_kernel, dim3(static_cast<unsigned>(units)), dim3(kPickThreads), stream, view,
+  return launch_after(kv_pick_pages_kernel, dim3(static_cast<unsigned>(units)), dim3(kPickThreads), 0, stream, 1, view,
                       static_cast<const unsigned long long*>(a.keys), top, pages)
              ? ATTN_OK
              : ATTN_ERR_LAUNCH;
@@ -850,22 +851,22 @@ extern "C" int launch_kv_evict(const AttnPagedCache* cache, const float* weights
   if (units > 0x7fffffffLL || x > 0x7fffffffLL) return ATTN_ERR_INVALID_ARGUMENT;
   st = check_device();
   if (st != ATTN_OK) return st;
-  kv_evict_pick_kernel<<<static_cast<unsigned>(units), kPickThreads, 0, stream>>>(a);
-  if (cudaGetLastError() != cudaSuccess) return ATTN_ERR_LAUNCH;
+  if (!launch_after(kv_evict_pick_kernel, dim3(static_cast<unsigned>(units)), dim3(kPickThreads), 0, stream, 1, a))
+    return ATTN_ERR_LAUNCH;
   const dim3 grid(static_cast<unsigned>(x), cache->heads), block(256);
   bool ok;
   switch (cache->dtype) {
     case ATTN_F16:
-      ok = w.vec == 8 ? launch_after(kv_evict_copy_kernel<__half, 8>, grid, block, stream, a)
-                      : launch_after(kv_evict_copy_kernel<__half, 1>, grid, block, stream, a);
+      ok = w.vec == 8 ? launch_after(kv_evict_copy_kernel<__half, 8>, grid, block, 0, stream, 1, a)
+                      : launch_after(kv_evict_copy_kernel<__half, 1>, grid, block, 0, stream, 1, a);
       break;
     case ATTN_BF16:
-      ok = w.vec == 8 ? launch_after(kv_evict_copy_kernel<__nv_bfloat16, 8>, grid, block, stream, a)
-                      : launch_after(kv_evict_copy_kernel<__nv_bfloat16, 1>, grid, block, stream, a);
+      ok = w.vec == 8 ? launch_after(kv_evict_copy_kernel<__nv_bfloat16, 8>, grid, block, 0, stream, 1, a)
+                      : launch_after(kv_evict_copy_kernel<__nv_bfloat16, 1>, grid, block, 0, stream, 1, a);
       break;
     default:
-      ok = w.vec == 4 ? launch_after(kv_evict_copy_kernel<float, 4>, grid, block, stream, a)
-                      : launch_after(kv_evict_copy_kernel<float, 1>, grid, block, stream, a);
+      ok = w.vec == 4 ? launch_after(kv_evict_copy_kernel<float, 4>, grid, block, 0, stream, 1, a)
+                      : launch_after(kv_evict_copy_kernel<float, 1>, grid, block, 0, stream, 1, a);
       break;
   }
   return ok ? ATTN_OK : ATTN_ERR_LAUNCH;

@@ -54,20 +54,34 @@ inline bool aligned_to(const void* p, size_t a) { return (reinterpret_cast<uintp
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-// Launches a kernel that waits on the grid before it itself
-// (grid_dependency_wait), so that its launch overlaps that grid.
+// Launches a kernel that waits itself for the work before it in the stream
+// (every thread calls grid_dependency_wait before it touches memory), so that
+// its launch overlaps that work.  The wait ends when the grid before has
+// completed, and so, as that grid waited too, everything before it.  Back to
+// back this hides about a microsecond per kernel.  `cluster` CTAs per cluster
+// (1 or 0: none); clusters are launched after the work before them, since
+// eight CTAs' room at once is hard to find beside it (32 units of 512 tokens:
+// 7.6 us against 9.6 us).
 template <typename... Params, typename... Args>
-bool launch_after(void (*kern)(Params...), dim3 grid, dim3 block, cudaStream_t stream, Args&&... args) {
+bool launch_after(void (*kern)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, int cluster,
+                  const Args&... args) {
   cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
+  if (cluster > 1) {
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = cluster;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  } else {
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, static_cast<Args&&>(args)...) == cudaSuccess;
+  return cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess;
 }
 
 // The length of sequence b as the kernels use it: negative lengths are empty,

@@ -185,7 +185,7 @@ Tensor attn_decode(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache
   size_t bytes = 0;
   check_launch(attn_decode_workspace_bytes(&c.c, Hq, pages.has_value(), n_pages, weights.has_value(), &bytes),
                "attn_decode_workspace_bytes");
-  const Tensor space = workspace(bytes, dev);
+  const Tensor space = bytes > 0 ? workspace(bytes, dev) : out;  // nothing is written to an empty workspace
   // an empty list has no data, but is a list all the same
   static const int none = 0;
   const int* list_ptr = !pages ? nullptr : n_pages > 0 ? list.data_ptr<int>() : &none;
