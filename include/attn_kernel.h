@@ -257,10 +257,11 @@ ATTN_API int launch_kv_page_bounds(const AttnPagedCache* cache, void* bounds, co
  * token: pages int32 [B, heads, top] receives ascending logical pages, -1
  * behind them where the sequence has fewer than `top`.  The newest page is
  * always in; of the others those with the largest
- *   score = sum over the query heads g of the kv head, and the dims d, of
- *           max(q[g, d] * min[d], q[g, d] * max[d]),
- * an upper bound of the summed scores of any token of the page; ties go to the
- * lower page, NaN counts as largest.  Sums are taken in 64 bits, since a score
+ *   score = sum over the dims d of max[d] * p[d] + min[d] * m[d],
+ * p and m being the sums of q's positive and negative parts over the query
+ * heads of the kv head: the sum of max(q * min, q * max), an upper bound of the
+ * summed scores of any token of the page.  Ties go to the lower page, NaN
+ * counts as largest.  Sums are taken in 64 bits, since a score
  * next to the border decides a page.  top >= 1; cache->k and v are not used.
  */
 ATTN_API int kv_select_pages_workspace_bytes(const AttnPagedCache* cache, size_t* bytes);

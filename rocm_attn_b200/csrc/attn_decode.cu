@@ -236,7 +236,7 @@ __device__ __forceinline__ void locate_logical(const DecodeArgs& a, int b, int h
   *lp = j;
   if (a.pages) {
     if (j < a.n_pages)
-      *lp = __ldg(a.pages + (static_cast<long long>(b) * a.c.heads + h) * a.n_pages + j);
+      *lp = *(a.pages + (static_cast<long long>(b) * a.c.heads + h) * a.n_pages + j);
     else
       *row = -1;
   } else if (pos >= len) {
@@ -247,7 +247,7 @@ __device__ __forceinline__ void locate_physical(const DecodeArgs& a, int b, int 
   const int lp = *page;
   // A list's entry that names no page of the sequence adds nothing.
   if (a.pages && (lp < 0 || lp >= a.c.table_width || lp * a.c.page_size + *row >= len)) *row = -1;
-  if (*row >= 0) *page = __ldg(a.c.table + static_cast<long long>(b) * a.c.table_stride + lp);
+  if (*row >= 0) *page = *(a.c.table + static_cast<long long>(b) * a.c.table_stride + lp);
 }
 // After both: whether there is such a token, in a page of the cache.
 __device__ __forceinline__ bool located(const DecodeArgs& a, int page, int row, int* fault) {
@@ -549,7 +549,7 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               const int d = ks * 16 + j * 8 + (lane & 3) * 2;
-              qf[t][ks][j] = (r < rows && d < a.c.D) ? __ldg(reinterpret_cast<const uint32_t*>(q + r * a.q_h + d)) : 0u;
+              qf[t][ks][j] = (r < rows && d < a.c.D) ? *reinterpret_cast<const uint32_t*>(q + r * a.q_h + d) : 0u;
             }
             o[t][ks][0] = o[t][ks][1] = o[t][ks][2] = o[t][ks][3] = 0.f;
           }

@@ -73,6 +73,25 @@ __device__ __forceinline__ void fold(Vec<T, kVec>& lo, Vec<T, kVec>& hi, const V
   }
 }
 
+// The vector of the lane `by` lanes up.
+template <typename T, int kVec>
+__device__ __forceinline__ Vec<T, kVec> shuffle_down(const Vec<T, kVec>& x, int by) {
+  Vec<T, kVec> y;
+  if constexpr (sizeof(y) >= 4) {
+    uint32_t w[sizeof(y) / 4];
+    memcpy(w, &x, sizeof(y));
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(y) / 4); ++i) w[i] = __shfl_down_sync(0xffffffffu, w[i], by);
+    memcpy(&y, w, sizeof(y));
+  } else {
+    uint16_t h;
+    memcpy(&h, &x, 2);
+    h = static_cast<uint16_t>(__shfl_down_sync(0xffffffffu, static_cast<unsigned>(h), by));
+    memcpy(&y, &h, 2);
+  }
+  return y;
+}
+
 // ---------------------------------------------------------------------------
 // Append and page bounds
 // ---------------------------------------------------------------------------
@@ -86,28 +105,35 @@ struct RowsArgs {
   void* bounds;
   long long b_p, b_h, b_m;     // bounds strides over (page, head, min/max)
   int runs;                    // pages a sequence may touch
-  int cols, heads_per_cta, row_lanes;
+  int cols, row_lanes;         // a warp's lanes: row_lanes rows of up to 32 columns
 };
 
-// CTA (b, run; heads): the rows of one page that are new (kAppend), or that
-// the sequence has there.  Thread (row lane, head, column): every
-// row_lanes-th row of one 16-byte column, four rows in flight; the row lanes'
-// minima and maxima meet in shared memory.
+constexpr int kRowsWarps = 8;
+
+// Warp (b, run, head): the rows of one page and head that are new (kAppend),
+// or that the sequence has there.  Lane (row lane, column): every
+// row_lanes-th row of one 16-byte column, kAhead rows in flight, so that a
+// page's rows are mostly on their way at once and nothing waits for other
+// warps; the row lanes' minima and maxima meet by shuffles.
 template <typename T, int kVec, bool kAppend, bool kBounds>
-__global__ void __launch_bounds__(256) kv_rows_kernel(const __grid_constant__ RowsArgs a) {
+__global__ void __launch_bounds__(kRowsWarps * 32) kv_rows_kernel(const __grid_constant__ RowsArgs a) {
   using V = Vec<T, kVec>;
-  __shared__ V s_lo[256], s_hi[256];
+  constexpr int kAhead = kAppend ? 4 : 8;
   launch_dependents();
   grid_dependency_wait();
-  const int b = static_cast<int>(blockIdx.x / a.runs), run = static_cast<int>(blockIdx.x - static_cast<unsigned>(b) * a.runs);
+  const int lane = threadIdx.x & 31;
+  const long long task = static_cast<long long>(blockIdx.x) * kRowsWarps + (threadIdx.x >> 5);
+  const int heads = a.c.heads, h = static_cast<int>(task % heads);
+  const int page_task = static_cast<int>(task / heads), b = page_task / a.runs, run = page_task - b * a.runs;
+  if (b >= a.c.B) return;
   const int ps = a.c.page_size, cap = a.c.capacity();
   int fault = 0;
-  long long len = __ldg(a.c.lens + b), first = 0;  // positions [first, len) are taken
+  long long len = *(a.c.lens + b), first = 0;  // positions [first, len) are taken
   long long start = 0;                             // position of token 0 of the new ones
   if (kAppend) {
     int n = a.S;
     if (a.new_lens) {
-      n = __ldg(a.new_lens + b);
+      n = *(a.new_lens + b);
       if (n > a.S) {
         fault |= kFaultPage;
         n = a.S;
@@ -121,76 +147,78 @@ __global__ void __launch_bounds__(256) kv_rows_kernel(const __grid_constant__ Ro
     fault |= kFaultPage;
     len = cap;
   }
-  const int lp = static_cast<int>(first / ps) + run;
-  const long long base = static_cast<long long>(lp) * ps;
-  int page = -1;
-  if (first < len && base < len) page = paged_page(a.c, b, lp, &fault);
-  if (fault && threadIdx.x == 0) atomicOr(&g_page_fault, 1);
+  int page = -1, lp = 0;
+  long long base = 0;
+  if (first < len) {
+    lp = static_cast<int>(first) / ps + run;
+    base = static_cast<long long>(lp) * ps;
+    if (base < len) page = paged_page(a.c, b, lp, &fault);
+  }
+  if (fault && lane == 0) atomicOr(&g_page_fault, fault);
   if (page < 0) return;
   const int r0 = first > base ? static_cast<int>(first - base) : 0;
   const int r1 = len - base < ps ? static_cast<int>(len - base) : ps;
 
-  const int col = threadIdx.x % a.cols, rest = threadIdx.x / a.cols;
-  const int in_cta = rest % a.heads_per_cta, lane = rest / a.heads_per_cta;
-  const int h = blockIdx.y * a.heads_per_cta + in_cta;
-  const bool live = h < a.c.heads;
-  V lo, hi;
-  bool any = false;
-  if (live) {
+  const int width = min(a.cols, 32);  // columns per turn
+  const int row_lane = lane / width, in_row = lane - row_lane * width;
+  for (int c0 = 0; c0 < a.cols; c0 += 32) {
+    const int col = c0 + in_row;
+    const bool live = row_lane < a.row_lanes && col < a.cols;
+    V lo = {}, hi = {};
+    bool any = false;
     const long long d = static_cast<long long>(col) * kVec;
-    T* ck = static_cast<T*>(a.c.k) + page * a.c.ks[0] + h * a.c.ks[1] + d;
-    T* cv = kAppend ? static_cast<T*>(a.c.v) + page * a.c.vs[0] + h * a.c.vs[1] + d : nullptr;
-    // row r of the page is new token base + r - start
-    const T* nk = kAppend ? static_cast<const T*>(a.k) + b * a.k_b + h * a.k_h + (base - start) * a.k_s + d : ck;
-    const T* nv = kAppend ? static_cast<const T*>(a.v) + b * a.v_b + h * a.v_h + (base - start) * a.v_s + d : nullptr;
-    const long long k_s = kAppend ? a.k_s : a.c.ks[2];
-    constexpr int kAhead = 4;
-    for (int r = r0 + lane; r < r1; r += kAhead * a.row_lanes) {
-      V x[kAhead], y[kAhead];
+    if (live) {
+      T* ck = static_cast<T*>(a.c.k) + page * a.c.ks[0] + h * a.c.ks[1] + d;
+      T* cv = kAppend ? static_cast<T*>(a.c.v) + page * a.c.vs[0] + h * a.c.vs[1] + d : nullptr;
+      // row r of the page is new token base + r - start
+      const T* nk = kAppend ? static_cast<const T*>(a.k) + b * a.k_b + h * a.k_h + (base - start) * a.k_s + d : ck;
+      const T* nv = kAppend ? static_cast<const T*>(a.v) + b * a.v_b + h * a.v_h + (base - start) * a.v_s + d : nullptr;
+      const long long k_s = kAppend ? a.k_s : a.c.ks[2];
+      for (int r = r0 + row_lane; r < r1; r += kAhead * a.row_lanes) {
+        V x[kAhead], y[kAhead];
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        const int at = r + i * a.row_lanes;
-        if (at < r1) {
-          x[i] = *reinterpret_cast<const V*>(nk + at * k_s);
-          if (kAppend) y[i] = *reinterpret_cast<const V*>(nv + at * a.v_s);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        const int at = r + i * a.row_lanes;
-        if (at < r1) {
-          if (kAppend) {
-            *reinterpret_cast<V*>(ck + at * a.c.ks[2]) = x[i];
-            *reinterpret_cast<V*>(cv + at * a.c.vs[2]) = y[i];
+        for (int i = 0; i < kAhead; ++i) {
+          const int at = r + i * a.row_lanes;
+          if (at < r1) {
+            x[i] = *reinterpret_cast<const V*>(nk + at * k_s);
+            if (kAppend) y[i] = *reinterpret_cast<const V*>(nv + at * a.v_s);
           }
-          if (kBounds) {
-            if (!any) {
-              lo = hi = x[i];
-              any = true;
-            } else {
-              fold(lo, hi, x[i], x[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          const int at = r + i * a.row_lanes;
+          if (at < r1) {
+            if (kAppend) {
+              *reinterpret_cast<V*>(ck + at * a.c.ks[2]) = x[i];
+              *reinterpret_cast<V*>(cv + at * a.c.vs[2]) = y[i];
+            }
+            if (kBounds) {
+              if (!any) {
+                lo = hi = x[i];
+                any = true;
+              } else {
+                fold(lo, hi, x[i], x[i]);
+              }
             }
           }
         }
       }
     }
-  }
-  if constexpr (kBounds) {
-    if (a.row_lanes > 1) {
-      s_lo[threadIdx.x] = lo;
-      s_hi[threadIdx.x] = hi;
-      __syncthreads();
-    }
-    if (live && lane == 0) {
-      // row lane i has rows if r0 + i < r1; lane 0 always does
-      const int lanes = min(a.row_lanes, r1 - r0), step = a.cols * a.heads_per_cta;
-      for (int i = 1; i < lanes; ++i) fold(lo, hi, s_lo[threadIdx.x + i * step], s_hi[threadIdx.x + i * step]);
-      T* out = static_cast<T*>(a.bounds) + page * a.b_p + h * a.b_h + static_cast<long long>(col) * kVec;
-      V* out_lo = reinterpret_cast<V*>(out);
-      V* out_hi = reinterpret_cast<V*>(out + a.b_m);
-      if (kAppend && r0 > 0) fold(lo, hi, *out_lo, *out_hi);
-      *out_lo = lo;
-      *out_hi = hi;
+    if constexpr (kBounds) {
+      // Row lane i has rows if r0 + i < r1; lane 0 always does.
+      const int lanes = min(a.row_lanes, r1 - r0);
+      for (int i = 1; i < lanes; ++i) {
+        const V l = shuffle_down(lo, i * width), x = shuffle_down(hi, i * width);
+        if (row_lane == 0) fold(lo, hi, l, x);
+      }
+      if (live && row_lane == 0) {
+        T* out = static_cast<T*>(a.bounds) + page * a.b_p + h * a.b_h + d;
+        V* out_lo = reinterpret_cast<V*>(out);
+        V* out_hi = reinterpret_cast<V*>(out + a.b_m);
+        if (kAppend && r0 > 0) fold(lo, hi, *out_lo, *out_hi);
+        *out_lo = lo;
+        *out_hi = hi;
+      }
     }
   }
 }
@@ -212,6 +240,10 @@ __device__ __forceinline__ unsigned order_key(float x) {
   return (u >> 31) ? ~u : u | (1u << 31);
 }
 
+__device__ __forceinline__ float key_value(unsigned key) {  // (a zero comes back as +0)
+  return __uint_as_float((key >> 31) ? key & 0x7fffffffu : ~key);
+}
+
 template <typename T> __device__ __forceinline__ float to_f32(T x);
 template <> __device__ __forceinline__ float to_f32<float>(float x) { return x; }
 template <> __device__ __forceinline__ float to_f32<__half>(__half x) { return __half2float(x); }
@@ -225,11 +257,11 @@ struct ScoreArgs {
   const void* bounds;
   long long b_p, b_h, b_m;
   unsigned long long* keys;  // [B, heads, table_width]
-  int chunks;                // CTAs per (sequence, head)
+  int chunks, pages;         // CTAs per (sequence, head), and pages of each
 };
 
-constexpr int kScorePages = 128;  // pages per CTA
-constexpr int kScoreLanes = 16;   // lanes per page
+constexpr int kScoreLanes = 16;                 // lanes per page
+constexpr int kScoreSlots = 256 / kScoreLanes;  // pages a CTA takes at a time
 
 // max(q min, q max) is q max where q >= 0 and q min where q < 0, so the sum
 // over the query heads needs only their summed positive and negative parts:
@@ -237,203 +269,314 @@ constexpr int kScoreLanes = 16;   // lanes per page
 // values are exact in 64 bits and their sums as good as exact, so the choice
 // of pages does not depend on the order of the sum.
 template <typename T, int kVec, int kPer>
-__global__ void __launch_bounds__(256) kv_page_score_kernel(const __grid_constant__ ScoreArgs a) {
+__global__ void __launch_bounds__(256, kPer == 1 ? 2 : 1) kv_page_score_kernel(const __grid_constant__ ScoreArgs a) {
   using V = Vec<T, kVec>;
   __shared__ double s_up[256], s_down[256];
   launch_dependents();
   grid_dependency_wait();
   const int b = static_cast<int>(blockIdx.x / a.chunks), chunk = static_cast<int>(blockIdx.x - static_cast<unsigned>(b) * a.chunks);
-  const int h = blockIdx.y;
+  const int h = blockIdx.y, lane = threadIdx.x & 31;
+  const int sub = threadIdx.x % kScoreLanes, slot = threadIdx.x / kScoreLanes;
   int fault = 0;
   const int len = paged_len(a.c, b, &fault);
   const int pages = static_cast<int>((static_cast<long long>(len) + a.c.page_size - 1) / a.c.page_size);
-  const int first = chunk * kScorePages, last = min(pages, first + kScorePages);
-  if (fault && threadIdx.x == 0) atomicOr(&g_page_fault, 1);
-  if (first >= last) return;
-  {
-    const int d = threadIdx.x;
-    double up = 0.0, down = 0.0;
-    if (d < a.c.D) {
-      const T* q = static_cast<const T*>(a.q) + b * a.q_b + static_cast<long long>(h) * a.group * a.q_h + d;
-      for (int g = 0; g < a.group; ++g) {
-        const double x = to_f32(q[g * a.q_h]);
-        // a NaN goes to both
-        if (!(x < 0.0)) up += x;
-        if (!(x >= 0.0)) down += x;
+  const int first = chunk * a.pages, last = min(pages, first + a.pages);
+  if (first < last) {
+    // Page ids of the next 16 turns, one per lane of the page's lanes.
+    auto look_up = [&](int p0) {
+      const int p = p0 + sub * kScoreSlots + slot;
+      return p < last ? paged_page(a.c, b, p, &fault) : -1;
+    };
+    int ids = look_up(first);
+    {
+      const int d = threadIdx.x;
+      double up = 0.0, down = 0.0;
+      if (d < a.c.D) {
+        const T* q = static_cast<const T*>(a.q) + b * a.q_b + static_cast<long long>(h) * a.group * a.q_h + d;
+#pragma unroll 8
+        for (int g = 0; g < a.group; ++g) {
+          const double x = to_f32(q[g * a.q_h]);
+          // a NaN goes to both
+          if (!(x < 0.0)) up += x;
+          if (!(x >= 0.0)) down += x;
+        }
       }
+      s_up[d] = up;
+      s_down[d] = down;
     }
-    s_up[d] = up;
-    s_down[d] = down;
-  }
-  __syncthreads();
-  const int sub = threadIdx.x % kScoreLanes, slot = threadIdx.x / kScoreLanes;
-  double up[kPer][kVec], down[kPer][kVec];
+    __syncthreads();
+    double up[kPer][kVec], down[kPer][kVec];
 #pragma unroll
-  for (int j = 0; j < kPer; ++j)
+    for (int j = 0; j < kPer; ++j)
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) {
-      const int d = (j * kScoreLanes + sub) * kVec + e;
-      up[j][e] = s_up[d & 255];
-      down[j][e] = s_down[d & 255];
-    }
-  const T* base = static_cast<const T*>(a.bounds) + h * a.b_h;
-  unsigned long long* keys = a.keys + (static_cast<long long>(b) * a.c.heads + h) * a.c.table_width;
-  constexpr int kSlots = 256 / kScoreLanes;
-#pragma unroll 4
-  for (int p0 = first; p0 < last; p0 += kSlots) {
-    const int p = p0 + slot;
-    int page = -1;
-    if (p < last) page = paged_page(a.c, b, p, &fault);
-    double sum = 0.0;
-    if (page >= 0) {
-      const T* at = base + page * a.b_p;
+      for (int e = 0; e < kVec; ++e) {
+        const int d = (j * kScoreLanes + sub) * kVec + e;
+        up[j][e] = s_up[d & 255];
+        down[j][e] = s_down[d & 255];
+      }
+    const T* base = static_cast<const T*>(a.bounds) + h * a.b_h;
+    unsigned long long* keys = a.keys + (static_cast<long long>(b) * a.c.heads + h) * a.c.table_width;
+    // kBatch turns at a time: the bounds of the next are on their way while
+    // these are summed.
+    constexpr int kBatch = kPer == 1 ? 4 : kPer == 2 ? 2 : 1;
+    V lo[kBatch][kPer], hi[kBatch][kPer];
+    int page[kBatch];
+    int turn = 0;
+    auto load = [&](int p0) {
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        const int d = (j * kScoreLanes + sub) * kVec;
-        if (d < a.c.D) {
-          const V lo = *reinterpret_cast<const V*>(at + d);
-          const V hi = *reinterpret_cast<const V*>(at + a.b_m + d);
+      for (int i = 0; i < kBatch; ++i) {
+        page[i] = __shfl_sync(0xffffffffu, ids, (lane & 16) + turn + i);
+        const T* at = base + page[i] * a.b_p;
 #pragma unroll
-          for (int e = 0; e < kVec; ++e) {
-            sum = fma(up[j][e], static_cast<double>(to_f32(hi.v[e])), sum);
-            sum = fma(down[j][e], static_cast<double>(to_f32(lo.v[e])), sum);
+        for (int j = 0; j < kPer; ++j) {
+          const int d = (j * kScoreLanes + sub) * kVec;
+          lo[i][j] = hi[i][j] = V{};
+          if (page[i] >= 0 && d < a.c.D) {
+            lo[i][j] = *reinterpret_cast<const V*>(at + d);
+            hi[i][j] = *reinterpret_cast<const V*>(at + a.b_m + d);
           }
         }
       }
-    }
+      turn += kBatch;
+      if (turn == kScoreLanes) {
+        turn = 0;
+        ids = look_up(p0 + kBatch * kScoreSlots);
+      }
+    };
+    load(first);
+    for (int p0 = first; p0 < last; p0 += kBatch * kScoreSlots) {
+      double sum[kBatch], sum2[kBatch];
+      bool named[kBatch];
+      {
+        V l[kBatch][kPer], x[kBatch][kPer];
 #pragma unroll
-    for (int o = kScoreLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    // a page the table does not name ranks last
-    if (p < last && sub == 0) keys[p] = page >= 0 ? order_key(sum) : 0ull;
+        for (int i = 0; i < kBatch; ++i) {
+          named[i] = page[i] >= 0;
+          sum[i] = sum2[i] = 0.0;
+#pragma unroll
+          for (int j = 0; j < kPer; ++j) l[i][j] = lo[i][j], x[i][j] = hi[i][j];
+        }
+        if (p0 + kBatch * kScoreSlots < last) load(p0 + kBatch * kScoreSlots);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j)
+#pragma unroll
+          for (int e = 0; e < kVec; ++e)
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+              sum[i] = fma(up[j][e], static_cast<double>(to_f32(x[i][j].v[e])), sum[i]);
+              sum2[i] = fma(down[j][e], static_cast<double>(to_f32(l[i][j].v[e])), sum2[i]);
+            }
+      }
+      // The turns' sums over the lanes: halves of the batch are exchanged until
+      // a lane has one turn, then that one is summed.
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) sum[i] += sum2[i];
+      int mine = 0, off = kScoreLanes / 2;
+#pragma unroll
+      for (int left = kBatch; left > 1; left /= 2) {
+        const bool up_half = lane & off;
+#pragma unroll
+        for (int i = 0; i < left / 2; ++i) {
+          const double keep = up_half ? sum[i + left / 2] : sum[i], give = up_half ? sum[i] : sum[i + left / 2];
+          sum[i] = keep + __shfl_xor_sync(0xffffffffu, give, off);
+        }
+        mine += up_half ? left / 2 : 0;
+        off /= 2;
+      }
+      for (; off > 0; off /= 2) sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], off);
+      bool is_named = false;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+        if (i == mine) is_named = named[i];
+      const int p = p0 + mine * kScoreSlots + slot;
+      // a page the table does not name ranks last
+      if (p < last && sub % (kScoreLanes / kBatch) == 0) keys[p] = is_named ? order_key(sum[0]) : 0ull;
+    }
   }
-  if (fault) atomicOr(&g_page_fault, 1);
+  if (fault) atomicOr(&g_page_fault, fault);
 }
 
 // ---------------------------------------------------------------------------
 // The largest `pick` of n values, in the order of their places
 // ---------------------------------------------------------------------------
 
-constexpr int kPickThreads = 512;
-constexpr int kPickItems = 8;  // consecutive places per thread and step
+// CTAs of 32 warps, or of 8 where there are few places (kPickFew): their
+// barriers are shorter.
+constexpr int kPickFew = 4096;
+constexpr int kPickBits = 11;
 
 struct PickSmem {
-  unsigned count[256];
-  unsigned scan[kPickThreads / 32][2];
-  unsigned digit, above;
+  unsigned count[1 << kPickBits];
+  unsigned scan[32][2];
+  unsigned long long low[32], high[32];
+  unsigned digit, above, whole;
 };
 
-// Threshold of the `pick` largest of key(0..n-1), 0 < pick < n: a place is
-// taken if key & mask > prefix, and the first `ties` of those that are equal.
-// Eight bits a pass from the top; a pass whose bucket is taken whole is the last.
-template <typename Key, typename Get>
-__device__ void pick_threshold(PickSmem& s, Get key, int n, int pick, Key* prefix_out, Key* mask_out, int* ties_out) {
-  const int tid = threadIdx.x;
-  Key prefix = 0, mask = 0;
-  int need = pick;
-  for (int shift = sizeof(Key) * 8 - 8; shift >= 0; shift -= 8) {
-    if (tid < 256) s.count[tid] = 0;
+// Calls emit(rank, place, key) for the places of the `pick` largest of key(0..n-1),
+// 0 < pick < n, in the order of their places; of equal keys at the border the
+// lower places.  Each warp has a run of n / 32 places, its lanes 32 in a row at
+// a time.  The first `room` keys are kept in shared memory (`kept`; all of
+// them up to kPickRoom, so that memory is read once), others are read again
+// each pass.
+//
+// The border is found from the top, eleven bits a pass, beginning at the
+// highest bit in which any two keys differ; a pass whose bucket is taken whole
+// is the last.  A place is then taken if key & mask > prefix, and the first
+// `need` of those that are equal.
+template <int kWarps, typename Key, typename Get, typename Emit>
+__device__ void pick_largest(PickSmem& s, Key* kept, int room, Get get, int n, int pick, Emit emit) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  constexpr int kPickThreads = kWarps * 32, kMine = (1 << kPickBits) / kPickThreads;
+  const int run = (n + kPickThreads - 1) / kPickThreads * 32;  // places per warp
+  const int begin = warp * run + lane, end = warp * run + run;
+  auto key = [&](int i) { return i < room ? kept[i] : get(i); };
+  Key low = ~Key(0), high = 0;
+  for (int i0 = begin; i0 < end; i0 += 8 * 32) {
+    Key x[8];  // eight loads on their way at a time
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = get(min(i0 + j * 32, n - 1));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int i = i0 + j * 32;
+      if (i < end && i < n) {
+        if (i < room) kept[i] = x[j];  // read by this lane only
+        low = x[j] < low ? x[j] : low;
+        high = x[j] > high ? x[j] : high;
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const Key l = __shfl_xor_sync(0xffffffffu, low, o), x = __shfl_xor_sync(0xffffffffu, high, o);
+    low = l < low ? l : low;
+    high = x > high ? x : high;
+  }
+  if (lane == 0) {
+    s.low[warp] = low;
+    s.high[warp] = high;
+  }
+  __syncthreads();
+  low = static_cast<Key>(s.low[lane % kWarps]);
+  high = static_cast<Key>(s.high[lane % kWarps]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const Key l = __shfl_xor_sync(0xffffffffu, low, o), x = __shfl_xor_sync(0xffffffffu, high, o);
+    low = l < low ? l : low;
+    high = x > high ? x : high;
+  }
+  const unsigned long long differ = static_cast<unsigned long long>(low ^ high);
+  int bit = differ == 0 ? 0 : 64 - __clzll(static_cast<long long>(differ));  // keys agree from this bit up
+  Key mask = bit >= static_cast<int>(sizeof(Key) * 8) ? Key(0) : static_cast<Key>(~Key(0) << bit);
+  Key prefix = low & mask;
+  unsigned need = pick;
+  while (bit > 0) {
+    const int shift = bit > kPickBits ? bit - kPickBits : 0;
+    const unsigned top = (1u << (bit - shift)) - 1;
+    for (int i = tid; i < (1 << kPickBits); i += kPickThreads) s.count[i] = 0;
     __syncthreads();
-    for (int i = tid; i < n; i += kPickThreads) {
-      const Key x = key(i);
-      if ((x & mask) == prefix) atomicAdd(&s.count[static_cast<unsigned>(x >> shift) & 255u], 1u);
+#pragma unroll 4
+    for (int i = begin; i < end; i += 32) {
+      if (i < n) {
+        const Key x = key(i);
+        if ((x & mask) == prefix) atomicAdd(&s.count[static_cast<unsigned>(x >> shift) & top], 1u);
+      }
     }
     __syncthreads();
-    if (tid < 32) {
-      // Lane 0 holds the eight largest digits.
-      unsigned c[8], sum = 0;
+    {
+      // Thread t has kMine buckets, those of thread 0 the highest.
+      unsigned c[kMine], upto = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sum += c[j] = s.count[255 - (tid * 8 + j)];
-      unsigned upto = sum;
+      for (int j = 0; j < kMine; ++j) upto += c[j] = s.count[(1 << kPickBits) - 1 - (kMine * tid + j)];
+      const unsigned mine = upto;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const unsigned y = __shfl_up_sync(0xffffffffu, upto, o);
-        if (tid >= o) upto += y;
+        if (lane >= o) upto += y;
       }
-      unsigned above = upto - sum;
-      if (above < static_cast<unsigned>(need) && upto >= static_cast<unsigned>(need)) {
-        int j = 0;
+      if (lane == 31) s.scan[warp][0] = upto;
+      __syncthreads();
+      unsigned before = lane < warp ? s.scan[lane][0] : 0;
 #pragma unroll
-        for (; j < 7; ++j) {
-          if (above + c[j] >= static_cast<unsigned>(need)) break;
-          above += c[j];
+      for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+      unsigned above = before + upto - mine;
+#pragma unroll
+      for (int j = 0; j < kMine; ++j) {
+        if (above < need && above + c[j] >= need) {
+          s.digit = (1 << kPickBits) - 1 - (kMine * tid + j);
+          s.above = above;
+          s.whole = above + c[j] == need;
         }
-        s.digit = 255 - (tid * 8 + j);
-        s.above = above;
+        above += c[j];
       }
     }
     __syncthreads();
-    const unsigned digit = s.digit;
-    need -= static_cast<int>(s.above);
-    prefix |= static_cast<Key>(digit) << shift;
-    mask |= static_cast<Key>(255) << shift;
-    const bool whole = s.count[digit] == static_cast<unsigned>(need);
-    __syncthreads();
-    if (whole) break;
+    need -= s.above;
+    prefix |= static_cast<Key>(s.digit) << shift;
+    mask |= static_cast<Key>(top) << shift;
+    bit = shift;
+    if (s.whole) break;
   }
-  *prefix_out = prefix;
-  *mask_out = mask;
-  *ties_out = need;
+  unsigned gt = 0, eq = 0;
+#pragma unroll 4
+  for (int i = begin; i < end; i += 32) {
+    if (i < n) {
+      const Key x = key(i) & mask;
+      gt += x > prefix;
+      eq += x == prefix;
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    gt += __shfl_xor_sync(0xffffffffu, gt, o);
+    eq += __shfl_xor_sync(0xffffffffu, eq, o);
+  }
+  __syncthreads();
+  if (lane == 0) {
+    s.scan[warp][0] = gt;
+    s.scan[warp][1] = eq;
+  }
+  __syncthreads();
+  gt = lane < warp ? s.scan[lane][0] : 0;
+  eq = lane < warp ? s.scan[lane][1] : 0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    gt += __shfl_xor_sync(0xffffffffu, gt, o);
+    eq += __shfl_xor_sync(0xffffffffu, eq, o);
+  }
+  const unsigned under = (1u << lane) - 1;
+#pragma unroll 4
+  for (int i = begin; i < end; i += 32) {
+    const Key full = i < n ? key(i) : Key(0), x = full & mask;
+    const bool is_gt = i < n && x > prefix, is_eq = i < n && x == prefix;
+    const unsigned g = __ballot_sync(0xffffffffu, is_gt), e = __ballot_sync(0xffffffffu, is_eq);
+    const unsigned eq_here = eq + __popc(e & under);
+    if (is_gt || (is_eq && eq_here < need)) emit(static_cast<int>(gt + __popc(g & under) + min(eq_here, need)), i, full);
+    gt += __popc(g);
+    eq += __popc(e);
+  }
 }
 
-// Calls emit(rank, place) for the taken places of [0, n) in their order.
-template <typename Key, typename Get, typename Emit>
-__device__ void pick_emit(PickSmem& s, Get key, int n, Key prefix, Key mask, int ties, Emit emit) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  unsigned gt_before = 0, eq_before = 0;
-  for (int base = 0; base < n; base += kPickThreads * kPickItems) {
-    Key x[kPickItems];
-    unsigned gt = 0, eq = 0;
-#pragma unroll
-    for (int j = 0; j < kPickItems; ++j) {
-      const int i = base + tid * kPickItems + j;
-      x[j] = i < n ? key(i) & mask : 0;
-      if (i < n) {
-        gt += x[j] > prefix;
-        eq += x[j] == prefix;
-      }
-    }
-    unsigned g = gt, e = eq;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const unsigned y = __shfl_up_sync(0xffffffffu, g, o), z = __shfl_up_sync(0xffffffffu, e, o);
-      if (lane >= o) {
-        g += y;
-        e += z;
-      }
-    }
-    if (lane == 31) {
-      s.scan[warp][0] = g;
-      s.scan[warp][1] = e;
-    }
-    __syncthreads();
-    unsigned gs = gt_before + g - gt, es = eq_before + e - eq;
-#pragma unroll
-    for (int w = 0; w < kPickThreads / 32; ++w) {
-      if (w < warp) {
-        gs += s.scan[w][0];
-        es += s.scan[w][1];
-      }
-      gt_before += s.scan[w][0];
-      eq_before += s.scan[w][1];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < kPickItems; ++j) {
-      const int i = base + tid * kPickItems + j;
-      if (i >= n) break;
-      const bool is_gt = x[j] > prefix, is_eq = x[j] == prefix;
-      if (is_gt || (is_eq && es < static_cast<unsigned>(ties)))
-        emit(static_cast<int>(gs + min(es, static_cast<unsigned>(ties))), i);
-      gs += is_gt;
-      es += is_eq;
-    }
-  }
+// Shared memory for the keys of up to `most` places.
+constexpr int kPickRoomBytes = 160 * 1024;
+int pick_room(long long most, int key_bytes) {
+  const long long room = kPickRoomBytes / key_bytes;
+  return static_cast<int>(most < room ? most : room);
+}
+
+template <typename... Params, typename... Args>
+bool launch_pick(void (*kern)(Params...), int warps, unsigned units, size_t smem, cudaStream_t stream, const Args&... args) {
+  if (smem > 32 * 1024 &&
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kPickRoomBytes) != cudaSuccess)
+    return false;
+  return launch_after(kern, dim3(units), dim3(warps * 32), smem, stream, 1, args...);
 }
 
 // CTA (head, b): the last place, and the pick - 1 largest of the others.
-__global__ void __launch_bounds__(kPickThreads) kv_pick_pages_kernel(PagedView c, const unsigned long long* keys, int top,
-                                                                     int* pages) {
+template <int kWarps>
+__global__ void __launch_bounds__(kWarps * 32) kv_pick_pages_kernel(PagedView c, const unsigned long long* keys, int top,
+                                                                     int* pages, int room) {
   __shared__ PickSmem s;
+  extern __shared__ __align__(16) unsigned char kept[];
   launch_dependents();
   grid_dependency_wait();
   const int h = blockIdx.x % c.heads, b = blockIdx.x / c.heads;
@@ -443,16 +586,14 @@ __global__ void __launch_bounds__(kPickThreads) kv_pick_pages_kernel(PagedView c
   const unsigned long long* k = keys + (static_cast<long long>(b) * c.heads + h) * c.table_width;
   int* out = pages + (static_cast<long long>(b) * c.heads + h) * top;
   if (n <= top) {
-    for (int i = threadIdx.x; i < top; i += kPickThreads) out[i] = i < n ? i : -1;
+    for (int i = threadIdx.x; i < top; i += kWarps * 32) out[i] = i < n ? i : -1;
     return;
   }
   if (threadIdx.x == 0) out[top - 1] = n - 1;
   if (top == 1) return;
-  auto key = [&](int i) { return k[i]; };
-  unsigned long long prefix, mask;
-  int ties;
-  pick_threshold<unsigned long long>(s, key, n - 1, top - 1, &prefix, &mask, &ties);
-  pick_emit<unsigned long long>(s, key, n - 1, prefix, mask, ties, [&](int rank, int i) { out[rank] = i; });
+  pick_largest<kWarps>(
+      s, reinterpret_cast<unsigned long long*>(kept), room, [&](int i) { return k[i]; }, n - 1, top - 1,
+      [&](int rank, int i, unsigned long long) { out[rank] = i; });
 }
 
 // ---------------------------------------------------------------------------
@@ -470,11 +611,14 @@ struct EvictArgs {
   int* kept;
   int* new_lens;
   int cols, rows_per_cta, chunks;
+  int room;  // keys in shared memory
 };
 
 // CTA (head, b): the kept positions and their weights.
-__global__ void __launch_bounds__(kPickThreads) kv_evict_pick_kernel(const __grid_constant__ EvictArgs a) {
+template <int kWarps>
+__global__ void __launch_bounds__(kWarps * 32) kv_evict_pick_kernel(const __grid_constant__ EvictArgs a) {
   __shared__ PickSmem s;
+  extern __shared__ __align__(16) unsigned char keys[];
   grid_dependency_wait();
   const int h = blockIdx.x % a.c.heads, b = blockIdx.x / a.c.heads;
   int fault = 0;
@@ -487,22 +631,22 @@ __global__ void __launch_bounds__(kPickThreads) kv_evict_pick_kernel(const __gri
   float* new_w = a.new_w + unit * new_cap;
   const int m = min(n, a.budget);
   if (h == 0 && threadIdx.x == 0) a.new_lens[b] = m;
-  for (int i = m + threadIdx.x; i < new_cap; i += kPickThreads) new_w[i] = 0.f;
-  for (int i = m + threadIdx.x; i < a.budget; i += kPickThreads) kept[i] = -1;
-  auto emit = [&](int rank, int i) {
-    kept[rank] = i;
-    new_w[rank] = w[i];
-  };
+  for (int i = m + threadIdx.x; i < new_cap; i += kWarps * 32) new_w[i] = 0.f;
+  for (int i = m + threadIdx.x; i < a.budget; i += kWarps * 32) kept[i] = -1;
   // positions [0, sure) compete for `pick` places, those behind are kept
   const int pick = n <= a.budget ? 0 : a.budget - a.recent;
   const int sure = n <= a.budget ? 0 : n - a.recent;
-  for (int i = sure + threadIdx.x; i < n; i += kPickThreads) emit(pick + i - sure, i);
+  for (int i = sure + threadIdx.x; i < n; i += kWarps * 32) {
+    kept[pick + i - sure] = i;
+    new_w[pick + i - sure] = w[i];
+  }
   if (pick == 0) return;
-  auto key = [&](int i) { return order_key(w[i]); };
-  unsigned prefix, mask;
-  int ties;
-  pick_threshold<unsigned>(s, key, sure, pick, &prefix, &mask, &ties);
-  pick_emit<unsigned>(s, key, sure, prefix, mask, ties, emit);
+  pick_largest<kWarps>(
+      s, reinterpret_cast<unsigned*>(keys), a.room, [&](int i) { return order_key(w[i]); }, sure, pick,
+      [&](int rank, int i, unsigned key) {
+        kept[rank] = i;
+        new_w[rank] = key_value(key);
+      });
 }
 
 // CTA (b, chunk of rows; head): copies kept rows to the new pages, a column
@@ -511,7 +655,6 @@ template <typename T, int kVec>
 __global__ void __launch_bounds__(256) kv_evict_copy_kernel(const __grid_constant__ EvictArgs a) {
   using V = Vec<T, kVec>;
   constexpr int kAhead = 4;
-  launch_dependents();
   grid_dependency_wait();
   const int b = static_cast<int>(blockIdx.x / a.chunks), chunk = static_cast<int>(blockIdx.x - static_cast<unsigned>(b) * a.chunks);
   const int h = blockIdx.y, ps = a.c.page_size;
@@ -535,7 +678,7 @@ __global__ void __launch_bounds__(256) kv_evict_copy_kernel(const __grid_constan
       const int lp = src / ps, page = paged_page(a.c, b, lp, &fault);
       const int np = static_cast<int>(place) / ps;
       row[i] = static_cast<int>(place) - np * ps;
-      const int t = __ldg(a.new_table + b * a.new_stride + np);
+      const int t = *(a.new_table + b * a.new_stride + np);
       const bool good = static_cast<unsigned>(t) < static_cast<unsigned>(a.c.num_pages);
       if (!good) fault |= kFaultPage;
       if (good && page >= 0) {
@@ -579,39 +722,34 @@ struct Width {
 size_t elem_size(AttnDType t) { return t == ATTN_F32 ? 4 : 2; }
 
 template <typename T, int kVec>
-bool launch_rows_typed(const RowsArgs& a, bool append, dim3 grid, int threads, cudaStream_t stream) {
+bool launch_rows_typed(const RowsArgs& a, bool append, dim3 grid, cudaStream_t stream) {
   const auto kern = !append    ? kv_rows_kernel<T, kVec, false, true>
                     : a.bounds ? kv_rows_kernel<T, kVec, true, true>
                                : kv_rows_kernel<T, kVec, true, false>;
-  return launch_after(kern, grid, dim3(threads), 0, stream, 1, a);
+  return launch_after(kern, grid, dim3(kRowsWarps * 32), 0, stream, 1, a);
 }
 
-// rows: rows of one page that a CTA may find to do.
-int launch_rows(RowsArgs& a, AttnDType dtype, int vec, bool append, int rows, cudaStream_t stream) {
+int launch_rows(RowsArgs& a, AttnDType dtype, int vec, bool append, cudaStream_t stream) {
   a.cols = a.c.D / vec;
-  a.row_lanes = 1;
-  while (a.row_lanes * 2 * a.cols <= 256 && a.row_lanes * 4 < rows) a.row_lanes *= 2;
-  a.heads_per_cta = 256 / (a.cols * a.row_lanes);
-  if (a.heads_per_cta > a.c.heads) a.heads_per_cta = a.c.heads;
-  const long long x = static_cast<long long>(a.c.B) * a.runs;
-  const int y = (a.c.heads + a.heads_per_cta - 1) / a.heads_per_cta;
-  if (x == 0) return ATTN_OK;
-  if (x > 0x7fffffffLL || y > 65535) return ATTN_ERR_INVALID_ARGUMENT;
-  const dim3 grid(static_cast<unsigned>(x), y);
-  const int threads = a.cols * a.heads_per_cta * a.row_lanes;
+  a.row_lanes = a.cols >= 32 ? 1 : 32 / a.cols;
+  const long long pages = static_cast<long long>(a.c.B) * a.runs;
+  if (pages == 0) return ATTN_OK;
+  if (pages > 0x7fffffffLL || (pages * a.c.heads + kRowsWarps - 1) / kRowsWarps > 0x7fffffffLL)
+    return ATTN_ERR_INVALID_ARGUMENT;
+  const dim3 grid(static_cast<unsigned>((pages * a.c.heads + kRowsWarps - 1) / kRowsWarps));
   bool ok;
   switch (dtype) {
     case ATTN_F16:
-      ok = vec == 8 ? launch_rows_typed<__half, 8>(a, append, grid, threads, stream)
-                    : launch_rows_typed<__half, 1>(a, append, grid, threads, stream);
+      ok = vec == 8 ? launch_rows_typed<__half, 8>(a, append, grid, stream)
+                    : launch_rows_typed<__half, 1>(a, append, grid, stream);
       break;
     case ATTN_BF16:
-      ok = vec == 8 ? launch_rows_typed<__nv_bfloat16, 8>(a, append, grid, threads, stream)
-                    : launch_rows_typed<__nv_bfloat16, 1>(a, append, grid, threads, stream);
+      ok = vec == 8 ? launch_rows_typed<__nv_bfloat16, 8>(a, append, grid, stream)
+                    : launch_rows_typed<__nv_bfloat16, 1>(a, append, grid, stream);
       break;
     default:
-      ok = vec == 4 ? launch_rows_typed<float, 4>(a, append, grid, threads, stream)
-                    : launch_rows_typed<float, 1>(a, append, grid, threads, stream);
+      ok = vec == 4 ? launch_rows_typed<float, 4>(a, append, grid, stream)
+                    : launch_rows_typed<float, 1>(a, append, grid, stream);
       break;
   }
   return ok ? ATTN_OK : ATTN_ERR_LAUNCH;
@@ -721,7 +859,7 @@ extern "C" int launch_kv_append(const AttnPagedCache* cache, const void* k, cons
   // S tokens touch at most this many pages of the table
   const long long runs = (static_cast<long long>(S) - 1 + cache->page_size - 1) / cache->page_size + 1;
   a.runs = static_cast<int>(runs < cache->table_width ? runs : cache->table_width > 0 ? cache->table_width : 1);
-  return launch_rows(a, cache->dtype, w.vec, true, S < cache->page_size ? S : cache->page_size, stream);
+  return launch_rows(a, cache->dtype, w.vec, true, stream);
 }
 
 extern "C" int launch_kv_page_bounds(const AttnPagedCache* cache, void* bounds, const long long* bounds_strides,
@@ -744,7 +882,7 @@ extern "C" int launch_kv_page_bounds(const AttnPagedCache* cache, void* bounds, 
   a.bounds = bounds;
   a.b_p = bounds_strides[0], a.b_h = bounds_strides[1], a.b_m = bounds_strides[2];
   a.runs = cache->table_width > 0 ? cache->table_width : 1;
-  return launch_rows(a, cache->dtype, w.vec, false, cache->page_size, stream);
+  return launch_rows(a, cache->dtype, w.vec, false, stream);
 }
 
 extern "C" int kv_select_pages_workspace_bytes(const AttnPagedCache* cache, size_t* bytes) {
@@ -767,7 +905,11 @@ extern "C" int launch_kv_select_pages(const AttnPagedCache* cache, const void* q
   if (top < 1 || Hq < 0 || Hq % cache->heads != 0 || cache->heads > 65535) return ATTN_ERR_INVALID_ARGUMENT;
   if (cache->B == 0) return ATTN_OK;
   const long long units = static_cast<long long>(cache->B) * cache->heads;
-  const int chunks = (cache->table_width + kScorePages - 1) / kScorePages;
+  // Pages per CTA: as many as leave eight CTAs per SM, two of which run at once
+  // (measured: 2 and 16 per SM 4 % slower on 32 contexts of 1024 pages).
+  int per = 4 * kScoreSlots;
+  while (per < cache->table_width && units * ((cache->table_width + per - 1) / per) > 148 * 8) per += 4 * kScoreSlots;
+  const int chunks = (cache->table_width + per - 1) / per;
   if (units > 0x7fffffffLL || static_cast<long long>(cache->B) * chunks > 0x7fffffffLL)
     return ATTN_ERR_INVALID_ARGUMENT;
   const long long contiguous[2] = {static_cast<long long>(Hq) * cache->D, cache->D};
@@ -794,6 +936,7 @@ extern "C" int launch_kv_select_pages(const AttnPagedCache* cache, const void* q
   a.b_p = bounds_strides[0], a.b_h = bounds_strides[1], a.b_m = bounds_strides[2];
   a.keys = static_cast<unsigned long long*>(workspace);
   a.chunks = chunks;
+  a.pages = per;
   if (chunks > 0) {
     const dim3 grid(static_cast<unsigned>(cache->B) * chunks, cache->heads);
     bool ok;
@@ -804,8 +947,11 @@ extern "C" int launch_kv_select_pages(const AttnPagedCache* cache, const void* q
     }
     if (!ok) return ATTN_ERR_LAUNCH;
   }
-  return launch_after(kv_pick_pages_kernel, dim3(static_cast<unsigned>(units)), dim3(kPickThreads), 0, stream, 1, view,
-                      static_cast<const unsigned long long*>(a.keys), top, pages)
+  const int room = pick_room(cache->table_width, sizeof(unsigned long long));
+  const bool few = cache->table_width <= kPickFew;
+  return launch_pick(few ? kv_pick_pages_kernel<8> : kv_pick_pages_kernel<32>, few ? 8 : 32, static_cast<unsigned>(units),
+                     room * sizeof(unsigned long long), stream, view, static_cast<const unsigned long long*>(a.keys),
+                     top, pages, room)
              ? ATTN_OK
              : ATTN_ERR_LAUNCH;
 }
@@ -851,7 +997,10 @@ extern "C" int launch_kv_evict(const AttnPagedCache* cache, const float* weights
   if (units > 0x7fffffffLL || x > 0x7fffffffLL) return ATTN_ERR_INVALID_ARGUMENT;
   st = check_device();
   if (st != ATTN_OK) return st;
-  if (!launch_after(kv_evict_pick_kernel, dim3(static_cast<unsigned>(units)), dim3(kPickThreads), 0, stream, 1, a))
+  a.room = pick_room(view.capacity(), sizeof(unsigned));
+  const bool few = view.capacity() <= kPickFew;
+  if (!launch_pick(few ? kv_evict_pick_kernel<8> : kv_evict_pick_kernel<32>, few ? 8 : 32, static_cast<unsigned>(units),
+                   a.room * sizeof(unsigned), stream, a))
     return ATTN_ERR_LAUNCH;
   const dim3 grid(static_cast<unsigned>(x), cache->heads), block(256);
   bool ok;

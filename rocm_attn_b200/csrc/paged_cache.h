@@ -84,11 +84,15 @@ bool launch_after(void (*kern)(Params...), dim3 grid, dim3 block, size_t smem, c
   return cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess;
 }
 
+// (Loads of what other kernels write, lengths and tables among it, are plain
+// ones throughout: a kernel launched ahead may not take the read-only path to
+// memory that is still being written when it starts.)
+
 // The length of sequence b as the kernels use it: negative lengths are empty,
 // and lengths beyond the block table's capacity end there, with the fault
 // recorded.
 __device__ __forceinline__ int paged_len(const PagedView& c, int b, int* fault) {
-  const int n = __ldg(c.lens + b);
+  const int n = *(c.lens + b);
   if (n > c.capacity()) {
     *fault |= kFaultPage;
     return c.capacity();
@@ -99,7 +103,7 @@ __device__ __forceinline__ int paged_len(const PagedView& c, int b, int* fault) 
 // The physical page of logical page lp of sequence b, or -1, with the fault
 // recorded, when the table names a page outside the cache.
 __device__ __forceinline__ int paged_page(const PagedView& c, int b, int lp, int* fault) {
-  const int p = __ldg(c.table + static_cast<long long>(b) * c.table_stride + lp);
+  const int p = *(c.table + static_cast<long long>(b) * c.table_stride + lp);
   if (static_cast<unsigned>(p) < static_cast<unsigned>(c.num_pages)) return p;
   *fault |= kFaultPage;
   return -1;

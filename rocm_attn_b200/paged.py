@@ -94,8 +94,10 @@ def kv_select_pages(q: torch.Tensor, bounds: torch.Tensor, block_table: torch.Te
     sequence has fewer than ``top``.
 
     The newest page is always in.  The others are those of largest score, the
-    sum over the kv head's query heads and over d of ``max(q * min, q * max)``:
-    an upper bound of the summed scores of any token of the page.  Ties go to
+    sum over d of ``max * p + min * m``, p and m being q's positive and negative
+    parts summed over the kv head's query heads.  That is the sum of ``max(q *
+    min, q * max)``, an upper bound of the summed scores of any token of the
+    page.  Ties go to
     the lower page and NaN counts as largest.  Scores are summed in 64 bits.
     """
     return rocm_attn_ext.kv_select_pages(q, bounds, block_table, seq_lens, int(page_size), int(top))
