@@ -160,19 +160,33 @@ __device__ __forceinline__ void advance(const DecodeArgs& a, Cursor& c, int* fau
   }
 }
 
+// This CTA's run of the grid's tiles: `n` of them from tile `first`, and how
+// to tell the CTA of a later tile.  The runs differ by one tile at most, the
+// longer ones first.
+struct Run {
+  int first, n;
+  int each, longer;  // tiles per CTA, and CTAs with one more
+  __device__ __forceinline__ int owner(int tile) const {
+    const int cut = longer * (each + 1);
+    return tile < cut ? tile / (each + 1) : longer + (tile - cut) / each;
+  }
+};
+
 struct ScheduleSmem {
   int warp_sum[kWarps];
   Cursor first;
 };
 
-// Works out this CTA's run: its first tile (returned), the number of its
-// tiles *n and the run length of the grid *per.  The host keeps the number of
-// tiles the block table can name below 2^31.
-template <int kTile>
-__device__ __forceinline__ Cursor schedule(const DecodeArgs& a, ScheduleSmem& s, int* n, int* per, int* fault) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int seg = (a.c.B + kThreads - 1) / kThreads;
-  const int b0 = min(a.c.B, tid * seg), b1 = min(a.c.B, b0 + seg);
+// Works out this CTA's run and its first tile.  The host keeps the number of
+// tiles the block table can name below 2^31.  kWhole: the threads of the CTA
+// share the batch; otherwise each warp looks at all of it by itself, without
+// barriers, which is quicker for batches that a few loads per lane cover.
+template <int kTile, bool kWhole>
+__device__ __forceinline__ Cursor schedule_by(const DecodeArgs& a, ScheduleSmem& s, Run* run, int* fault) {
+  constexpr int kShare = kWhole ? kThreads : 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, id = kWhole ? threadIdx.x : lane;
+  const int seg = (a.c.B + kShare - 1) / kShare;
+  const int b0 = min(a.c.B, id * seg), b1 = min(a.c.B, b0 + seg);
   int mine = 0, len = 0, T = 0;
   for (int b = b0; b < b1; ++b) {
     len = paged_len(a.c, b, fault);
@@ -185,21 +199,27 @@ __device__ __forceinline__ Cursor schedule(const DecodeArgs& a, ScheduleSmem& s,
     const int y = __shfl_up_sync(0xffffffffu, upto, o);
     if (lane >= o) upto += y;
   }
-  if (lane == 31) s.warp_sum[warp] = upto;
-  __syncthreads();
-  int before = upto - mine, total = 0;
+  int before = upto - mine, total = __shfl_sync(0xffffffffu, upto, 31);
+  if constexpr (kWhole) {
+    if (lane == 31) s.warp_sum[warp] = upto;
+    __syncthreads();
+    total = 0;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before += s.warp_sum[w];
-    total += s.warp_sum[w];
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += s.warp_sum[w];
+      total += s.warp_sum[w];
+    }
   }
-  const int units = a.c.heads * a.row_tiles;
+  const int units = a.c.heads * a.row_tiles, grid = gridDim.x, c = blockIdx.x;
   total *= units;
-  *per = static_cast<int>((static_cast<unsigned>(total) + gridDim.x - 1) / gridDim.x);
-  const long long f0 = static_cast<long long>(*per) * blockIdx.x;
-  *n = static_cast<int>(max(0LL, min(static_cast<long long>(*per), total - f0)));
-  if (*n > 0 && f0 >= before * units && f0 < (before + mine) * units) {
-    int in = static_cast<int>(f0) - before * units, b = b0;
+  run->each = static_cast<unsigned>(total) / static_cast<unsigned>(grid);
+  run->longer = total - run->each * grid;
+  run->first = c * run->each + min(c, run->longer);
+  run->n = run->each + (c < run->longer ? 1 : 0);
+  Cursor at = {};
+  const bool here = run->n > 0 && run->first >= before * units && run->first - before * units < mine * units;
+  if (here) {
+    int in = run->first - before * units, b = b0;
     if (seg > 1) {
       for (;; ++b) {
         len = paged_len(a.c, b, fault);
@@ -208,11 +228,25 @@ __device__ __forceinline__ Cursor schedule(const DecodeArgs& a, ScheduleSmem& s,
         in -= T * units;
       }
     }
-    const int hu = in / T, h = hu / a.row_tiles;
-    s.first = Cursor{b, h, hu - h * a.row_tiles, in - hu * T, T, len};
+    const int hu = static_cast<unsigned>(in) / static_cast<unsigned>(T), h = a.row_tiles == 1 ? hu : hu / a.row_tiles;
+    at = Cursor{b, h, hu - h * a.row_tiles, in - hu * T, T, len};
   }
-  __syncthreads();
-  return s.first;
+  if constexpr (kWhole) {
+    if (here) s.first = at;
+    __syncthreads();
+    return s.first;
+  } else {
+    const unsigned who = __ballot_sync(0xffffffffu, here);
+    const int from = who ? __ffs(who) - 1 : 0;
+    return Cursor{__shfl_sync(0xffffffffu, at.b, from), __shfl_sync(0xffffffffu, at.h, from),
+                  __shfl_sync(0xffffffffu, at.rt, from), __shfl_sync(0xffffffffu, at.t, from),
+                  __shfl_sync(0xffffffffu, at.T, from), __shfl_sync(0xffffffffu, at.len, from)};
+  }
+}
+
+template <int kTile>
+__device__ __forceinline__ Cursor schedule(const DecodeArgs& a, ScheduleSmem& s, Run* run, int* fault) {
+  return a.c.B <= 128 ? schedule_by<kTile, false>(a, s, run, fault) : schedule_by<kTile, true>(a, s, run, fault);
 }
 
 // Output rows of empty sequences are zeros.
@@ -265,7 +299,7 @@ struct Place {
   int rows, slot;
 };
 
-__device__ __forceinline__ Place place_of(const DecodeArgs& a, const Cursor& c, bool begun, int per) {
+__device__ __forceinline__ Place place_of(const DecodeArgs& a, const Cursor& c, bool begun, const Run& run, int tile) {
   Place p;
   p.rows = min(a.rows, a.group - c.rt * a.rows);
   p.row0 = static_cast<long long>(c.b) * a.Hq + c.h * a.group + c.rt * a.rows;
@@ -273,7 +307,7 @@ __device__ __forceinline__ Place place_of(const DecodeArgs& a, const Cursor& c, 
   p.whole = begun && ends && a.cluster <= 1;
   p.slot = 2 * blockIdx.x + (begun ? 1 : 0);
   if (begun && !ends && threadIdx.x == 0) {
-    const int later = (c.T - (c.t + 1) + per - 1) / per;
+    const int later = run.owner(tile + c.T - 1 - c.t) - static_cast<int>(blockIdx.x);  // `tile` is tile c.t of the unit
     // row0 < B * Hq, which the host keeps below 2^31
     a.meta[blockIdx.x] = make_int4(static_cast<int>(p.row0), p.rows, later, 0);
   }
@@ -375,7 +409,8 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
   }
   launch_dependents();
   grid_dependency_wait();
-  int n, per = 1;
+  int n;
+  Run run = {};
   Cursor cur;
   if (a.cluster) {
     // Tiles rank, rank + cluster, ... of one unit.  Which they are does not
@@ -391,8 +426,10 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
     if (threadIdx.x < 8 * kNT) s_cm[threadIdx.x] = -INFINITY, s_cl[threadIdx.x] = 0.f;
   } else {
     if (threadIdx.x == 0) a.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
-    cur = schedule<kTile>(a, s_sched, &n, &per, &fault);
+    cur = schedule<kTile>(a, s_sched, &run, &fault);
+    n = run.n;
     zero_empty_rows<T>(a, &fault);
+    __syncthreads();  // the set-up above
   }
 
   unsigned char* ring = smem + warp * (kStages * C::kStageBytes);
@@ -667,7 +704,7 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
         // The unit, or this CTA's part of it, ends: the warps' parts are scaled
         // to their common maximum and summed over the chunks just freed, 16 heads
         // at a time.
-        const Place p = place_of(a, cur, begun, per);
+        const Place p = place_of(a, cur, begun, run, run.first + i);
 #pragma unroll
         for (int t = 0; t < kNT; ++t)
 #pragma unroll
@@ -844,8 +881,9 @@ __global__ void __launch_bounds__(kThreads) attn_decode_simt_kernel(const __grid
   launch_dependents();
   grid_dependency_wait();
   if (threadIdx.x == 0) a.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
-  int n, per;
-  Cursor cur = schedule<kTile>(a, s_sched, &n, &per, &fault);
+  Run run;
+  Cursor cur = schedule<kTile>(a, s_sched, &run, &fault);
+  const int n = run.n;
   zero_empty_rows<T>(a, &fault);
   const T* kbase = static_cast<const T*>(a.c.k);
   const T* vbase = static_cast<const T*>(a.c.v);
@@ -952,7 +990,7 @@ __global__ void __launch_bounds__(kThreads) attn_decode_simt_kernel(const __grid
       }
     }
     if (cur.t + 1 == cur.T || i + 1 == n) {
-      const Place p = place_of(a, cur, begun, per);
+      const Place p = place_of(a, cur, begun, run, run.first + i);
       if (lane % kRowLanes == 0) {
         s_m[parity][warp][my_row] = m;
         s_l[parity][warp][my_row] = l;
@@ -998,61 +1036,102 @@ __global__ void __launch_bounds__(kThreads) attn_decode_simt_kernel(const __grid
 // ---------------------------------------------------------------------------
 
 // CTA (c, r): row r of the unit that CTA c of the grid before began and did
-// not finish.  Warp w sums parts w, w + 8, ... (most units have no more than
-// eight, whose loads then all overlap), lane four columns of each 128; the
-// warps' sums meet in shared memory in their order.
+// not finish.  First every part's maximum and sum at once, then the parts
+// themselves, warp w parts w, w + 8, ..., lane four columns of each 128, whose
+// loads depend on nothing; the warps' sums meet in shared memory in their order.
 constexpr int kJoinWarps = 8;
 
 template <typename T>
 __global__ void __launch_bounds__(kJoinWarps * 32) attn_decode_join_kernel(const __grid_constant__ DecodeArgs a) {
+  constexpr int kAtOnce = kJoinWarps * 32;  // parts
   __shared__ float4 s_o[kJoinWarps][2][32];
-  __shared__ float s_m[kJoinWarps], s_l[kJoinWarps];
+  __shared__ float s_f[kAtOnce], s_m[kJoinWarps], s_l[kJoinWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   launch_dependents();
   grid_dependency_wait();
   const int c = blockIdx.x, r = blockIdx.y;
+  auto slot = [&](int i) { return static_cast<long long>(i == 0 ? 2 * c + 1 : 2 * (c + i)) * a.rows + r; };
+  // Most units have few parts: the first eight are asked for before it is
+  // known that they are parts of it.
+  const bool ask = c + warp < gridDim.x;
+  float2 early_ml = make_float2(-INFINITY, 0.f);
+  float4 early[2] = {};
+  if (lane < kJoinWarps && c + lane < gridDim.x) early_ml = a.part_ml[slot(lane)];
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    if (ask && k * 128 + lane * 4 < a.D4) early[k] = *reinterpret_cast<const float4*>(a.part_o + slot(warp) * a.D4 + k * 128 + lane * 4);
   const int4 meta = a.meta[c];
   if (meta.z == 0 || r >= meta.y) return;
-  float m = -INFINITY, l = 0.f;
+  float M = -INFINITY, L = 0.f;
   float4 o[2] = {};
-#pragma unroll 4
-  for (int i = warp; i <= meta.z; i += kJoinWarps) {
-    const long long slot = static_cast<long long>(i == 0 ? 2 * c + 1 : 2 * (c + i)) * a.rows + r;
-    const float2 ml = a.part_ml[slot];
-    float4 y[2] = {};
+  if (meta.z < kJoinWarps) {
+    const bool part = lane <= meta.z;
+    float m = part ? early_ml.x : -INFINITY;
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
-      if (k * 128 + lane * 4 < a.D4) y[k] = *reinterpret_cast<const float4*>(a.part_o + slot * a.D4 + k * 128 + lane * 4);
-    const float mn = fmaxf(m, ml.x);
-    const float f = ex2_approx(m - finite_max(mn)), g = ex2_approx(ml.x - finite_max(mn));
-    m = mn;
-    l = l * f + ml.y * g;
+    for (int off = 4; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+    m = __shfl_sync(0xffffffffu, m, 0);
+    const float f = part ? ex2_approx(early_ml.x - finite_max(m)) : 0.f;
+    M = m;
+    L = part ? early_ml.y * f : 0.f;
+#pragma unroll
+    for (int off = 4; off > 0; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
+    L = __shfl_sync(0xffffffffu, L, 0);
+    const float g = __shfl_sync(0xffffffffu, f, warp);
+    if (warp <= meta.z) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        o[k] = make_float4(early[k].x * g, early[k].y * g, early[k].z * g, early[k].w * g);
+    }
+  } else
+  for (int i0 = 0; i0 <= meta.z; i0 += kAtOnce) {
+    const int here = min(kAtOnce, meta.z + 1 - i0);
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (threadIdx.x < here) ml = a.part_ml[slot(i0 + threadIdx.x)];
+    float m = ml.x;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+    if (i0 > 0) __syncthreads();  // the turn before has read s_f
+    if (lane == 0) s_m[warp] = m;
+    __syncthreads();
+    float mn = M;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) mn = fmaxf(mn, s_m[w]);
+    const float back = ex2_approx(M - finite_max(mn)), f = ex2_approx(ml.x - finite_max(mn));
+    M = mn;
+    s_f[threadIdx.x] = f;
+    float l = ml.y * f;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+    if (lane == 0) s_l[warp] = l;
+    __syncthreads();
+    L *= back;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) L += s_l[w];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) o[k].x *= back, o[k].y *= back, o[k].z *= back, o[k].w *= back;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      o[k].x = o[k].x * f + y[k].x * g;
-      o[k].y = o[k].y * f + y[k].y * g;
-      o[k].z = o[k].z * f + y[k].z * g;
-      o[k].w = o[k].w * f + y[k].w * g;
+      const int d = k * 128 + lane * 4;
+      if (d >= a.D4) break;
+#pragma unroll 8
+      for (int i = warp; i < here; i += kJoinWarps) {
+        const float4 y = *reinterpret_cast<const float4*>(a.part_o + slot(i0 + i) * a.D4 + d);
+        const float g = s_f[i];
+        o[k].x = fmaf(y.x, g, o[k].x);
+        o[k].y = fmaf(y.y, g, o[k].y);
+        o[k].z = fmaf(y.z, g, o[k].z);
+        o[k].w = fmaf(y.w, g, o[k].w);
+      }
     }
-  }
-  if (lane == 0) {
-    s_m[warp] = m;
-    s_l[warp] = l;
   }
   s_o[warp][0][lane] = o[0];
   s_o[warp][1][lane] = o[1];
   __syncthreads();
   const int d = threadIdx.x;
   if (d >= a.c.D) return;
-  float M = s_m[0], L = 0.f, sum = 0.f;
+  float sum = 0.f;
 #pragma unroll
-  for (int w = 1; w < kJoinWarps; ++w) M = fmaxf(M, s_m[w]);
-#pragma unroll
-  for (int w = 0; w < kJoinWarps; ++w) {
-    const float f = ex2_approx(s_m[w] - finite_max(M));
-    L += s_l[w] * f;
-    sum += reinterpret_cast<const float*>(s_o[w])[d] * f;
-  }
+  for (int w = 0; w < kJoinWarps; ++w) sum += reinterpret_cast<const float*>(s_o[w])[d];
   const long long row = meta.x + r;
   static_cast<T*>(a.out)[row * a.c.D + d] = from_f32<T>(L == 0.f ? 0.f : sum / L);
   if (a.lse2 && d == 0) a.lse2[row] = L == 0.f ? INFINITY : M + log2f(L);
