@@ -78,6 +78,8 @@ struct DecodeArgs {
   int ps_shift;
 };
 
+__device__ __forceinline__ void prefetch_l1(const void* p) { asm volatile("prefetch.global.L1 [%0];" ::"l"(p)); }
+
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0)
                : "memory");
@@ -370,10 +372,9 @@ __device__ __forceinline__ float4 cluster_load4(const float* p, int rank) {
 }
 
 // The two caches as [num_pages, heads, page_size, D] tensors read in boxes of
-// `rows` rows (16 or 8, a divisor of the page size) by 64 columns.
+// 16 rows by 64 columns.
 struct TmaMaps {
   CUtensorMap k, v;
-  int rows;
   unsigned long long wait_ns;
 };
 
@@ -389,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
 
   extern __shared__ __align__(1024) unsigned char smem[];
   __shared__ ScheduleSmem s_sched;
-  __shared__ float s_m[2][kWarps][8 * kNT], s_l[2][kWarps][8 * kNT];
+  __shared__ float s_m[kWarps][8 * kNT], s_l[kWarps][8 * kNT];
   __shared__ uint32_t s_mask[kWarps][kStages];
   __shared__ uint64_t s_full[kWarps][kStages];
   __shared__ int s_abort, s_code, s_late;
@@ -443,6 +444,14 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
   const T* kbase = static_cast<const T*>(a.c.k) + my_col;
   const T* vbase = static_cast<const T*>(a.c.v) + my_col;
 
+  auto prefetch_q = [&](const Cursor& c) {
+    constexpr int kLines = kD / 64;  // of 128 bytes in a row
+    const int rows = min(a.rows, a.group - c.rt * a.rows);
+    const T* q = static_cast<const T*>(a.q) + c.b * a.q_b + (static_cast<long long>(c.h) * a.group + c.rt * a.rows) * a.q_h;
+    for (int e = lane; e < rows * kLines; e += 32)
+      if (e % kLines * 64 < a.c.D) prefetch_l1(q + (e / kLines) * a.q_h + e % kLines * 64);
+  };
+
   // The chunks whose copies go out next, with the page and row of each token
   // (lane = token): logical pages are looked up kStages + 1 chunks ahead of
   // the copies and physical pages kStages ahead, so that no copy waits for a
@@ -456,6 +465,9 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
       last_b = ahead.b;
       last_len = ahead.len;
       head[s] = ahead.h;
+      // The query heads of a unit to come, so that its first product does not
+      // wait for them.
+      if (warp == 0 && ahead.t == 0) prefetch_q(ahead);
       if (kKeys == 32 || lane < kKeys)
         locate_logical(a, last_b, ahead.h, ahead.t * kTile + warp * kKeys + lane, last_len, &page[s], &row[s]);
       advance<kTile>(a, ahead, &fault);
@@ -468,19 +480,18 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
     const uint32_t mask = __ballot_sync(0xffffffffu, located(a, page[0], row[0], &fault));
     if (lane == 0) s_mask[warp][stage] = mask;
     if constexpr (kTma) {
-      // One lane asks for the boxes that hold tokens.  All rows of a box lie
-      // in one page; its first row holds a token if any does.
+      // One lane asks for the boxes, of 16 rows, that hold tokens.  All rows of
+      // a box lie in one page; its first row holds a token if any does.
       if (mask != 0) {
-        const int boxes = kKeys / maps.rows;
-        uint32_t first = 0;  // first rows of the boxes wanted
-        for (int j = 0; j < boxes; ++j) first |= mask & (1u << (j * maps.rows));
-        if (lane == 0) mbar_arrive_expect_tx(&s_full[warp][stage], __popc(first) * maps.rows * (kD * 4));
-        while (first != 0) {
-          const int at = __ffs(first) - 1;
-          first &= first - 1;
-          const int pg = __shfl_sync(0xffffffffu, page[0], at), in = __shfl_sync(0xffffffffu, row[0], at);
-          if (lane == 0) {
-            const uint32_t dst = ring_addr + stage * C::kStageBytes + at * 128;
+        int boxes = 0;
+#pragma unroll
+        for (int g = 0; g < kKeys / 16; ++g) boxes += mask >> (g * 16) & 1u;
+        if (lane == 0) mbar_arrive_expect_tx(&s_full[warp][stage], boxes * 16 * (kD * 4));
+#pragma unroll
+        for (int g = 0; g < kKeys / 16; ++g) {
+          const int pg = __shfl_sync(0xffffffffu, page[0], g * 16), in = __shfl_sync(0xffffffffu, row[0], g * 16);
+          if (lane == 0 && (mask >> (g * 16) & 1u)) {
+            const uint32_t dst = ring_addr + stage * C::kStageBytes + g * 16 * 128;
 #pragma unroll
             for (int c = 0; c < kD / 64; ++c) {
               tma_load_4d(dst + c * (kKeys * 128), &maps.k, &s_full[warp][stage], c * 64, in, head[0], pg, policy);
@@ -549,7 +560,7 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
   float o[kNT][kSteps][4];
   float m[kNT][2], l[kNT][2];  // of query heads 8 t + 2 (lane % 4) + {0, 1}
   bool begun = a.cluster ? true : cur.t == 0, fresh = true;
-  int parity = 0, stage = 0;
+  int stage = 0;
   uint32_t phase = 0;  // of each stage's barrier
 
   // Scores of tokens lane / 4 + {0, 8} of the chunk's g-th 16 and of two heads
@@ -701,9 +712,9 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
       }
 
       if ((!a.cluster && cur.t + 1 == cur.T) || i + 1 == n) {
-        // The unit, or this CTA's part of it, ends: the warps' parts are scaled
-        // to their common maximum and summed over the chunks just freed, 16 heads
-        // at a time.
+        // The unit, or this CTA's part of it, ends: the warps leave their parts
+        // in the chunks just freed, 16 heads at a time, and their sum is taken
+        // with each scaled to the common maximum.
         const Place p = place_of(a, cur, begun, run, run.first + i);
 #pragma unroll
         for (int t = 0; t < kNT; ++t)
@@ -713,11 +724,10 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
             l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], 8);
             l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], 16);
             if (lane < 4) {
-              s_m[parity][warp][t * 8 + lane * 2 + e] = m[t][e];
-              s_l[parity][warp][t * 8 + lane * 2 + e] = l[t][e];
+              s_m[warp][t * 8 + lane * 2 + e] = m[t][e];
+              s_l[warp][t * 8 + lane * 2 + e] = l[t][e];
             }
           }
-        __syncthreads();
         float* ot = reinterpret_cast<float*>(ring + stage * C::kStageBytes);
 #pragma unroll
         for (int t0 = 0; t0 < kNT; t0 += 2) {
@@ -727,16 +737,12 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
             for (int e = 0; e < 2; ++e) {
               const int r = t * 8 + (lane & 3) * 2 + e, at = r - t0 * 8;
               if (r < p.rows) {
-                float M = s_m[parity][0][r];
-#pragma unroll
-                for (int w = 1; w < kWarps; ++w) M = fmaxf(M, s_m[parity][w][r]);
-                const float f = ex2_approx(m[t][e] - finite_max(M));
 #pragma unroll
                 for (int j = 0; j < kSteps; ++j)
 #pragma unroll
                   for (int up = 0; up < 2; ++up) {
                     const int d = j * 16 + up * 8 + (lane >> 2);
-                    ot[at * kD + (((d >> 2) ^ ((lane & 3) << 1)) << 2) + (d & 3)] = o[t][j][2 * up + e] * f;
+                    ot[at * kD + (((d >> 2) ^ ((lane & 3) << 1)) << 2) + (d & 3)] = o[t][j][2 * up + e];
                   }
               }
             }
@@ -745,20 +751,21 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
           for (int e = threadIdx.x; e < here * (kD / 4); e += kThreads) {
             const int at = e / (kD / 4), c4 = e % (kD / 4), r = t0 * 8 + at;
             if (c4 * 4 >= a.c.D) continue;
-            float M = s_m[parity][0][r], L = 0.f;
+            float M = s_m[0][r], L = 0.f;
 #pragma unroll
-            for (int w = 1; w < kWarps; ++w) M = fmaxf(M, s_m[parity][w][r]);
+            for (int w = 1; w < kWarps; ++w) M = fmaxf(M, s_m[w][r]);
             float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
-              L += s_l[parity][w][r] * ex2_approx(s_m[parity][w][r] - finite_max(M));
+              const float f = ex2_approx(s_m[w][r] - finite_max(M));
               const float4 y = *reinterpret_cast<const float4*>(
                   reinterpret_cast<const float*>(smem + (w * kStages + stage) * C::kStageBytes) + at * kD +
                   ((c4 ^ ((at >> 1 & 3) << 1)) << 2));
-              sum.x += y.x;
-              sum.y += y.y;
-              sum.z += y.z;
-              sum.w += y.w;
+              L += s_l[w][r] * f;
+              sum.x += y.x * f;
+              sum.y += y.y * f;
+              sum.z += y.z * f;
+              sum.w += y.w * f;
             }
             if (p.whole) {
               const float inv = L == 0.f ? 0.f : 1.f / L;
@@ -777,9 +784,8 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
             }
           }
           if constexpr (kTma) fence_proxy_async_smem();
-          __syncthreads();  // the chunks are read before they are filled again
+          __syncthreads();  // all this is read before it is written again
         }
-        parity ^= 1;
         begun = true;
         fresh = true;
       }
@@ -1285,19 +1291,19 @@ bool launch_mma_d(const DecodeArgs& a, const TmaMaps& maps, int kd, int grid, cu
   }
 }
 
-// TMA where 8 divides the page size (a box is rows of one page) and the
-// strides suit it, else 16-byte copies.
+// TMA where 16 divides the page size (a box is rows of one page) and the
+// strides suit it, else 16-byte copies (pages of 24 rows of 128 bytes: boxes
+// of 8 rows 143 us, copies 135 us).
 template <bool kBf16, bool kWeights>
 bool launch_mma_any(const DecodeArgs& a, const Plan& p, cudaStream_t stream) {
   TmaMaps maps;
-  maps.rows = a.c.page_size % 16 == 0 ? 16 : 8;
   const unsigned long long limit = wait_limit_ns();
   maps.wait_ns = limit != 0 ? limit : kWaitTimeoutNs;
   auto encode = [&](CUtensorMap* map, const void* base, const long long* st) {
     return make_tensor_map_4d(map, base, kBf16, a.c.D, a.c.page_size, a.c.heads, a.c.num_pages, st[2], st[1], st[0], 64,
-                              maps.rows) == 0;
+                              16) == 0;
   };
-  if (a.c.page_size % 8 == 0 && a.c.num_pages > 0 && encode(&maps.k, a.c.k, a.c.ks) && encode(&maps.v, a.c.v, a.c.vs))
+  if (a.c.page_size % 16 == 0 && a.c.num_pages > 0 && encode(&maps.k, a.c.k, a.c.ks) && encode(&maps.v, a.c.v, a.c.vs))
     return launch_mma_d<kBf16, kWeights, true>(a, maps, p.kd, p.grid, stream);
   return launch_mma_d<kBf16, kWeights, false>(a, maps, p.kd, p.grid, stream);
 }
