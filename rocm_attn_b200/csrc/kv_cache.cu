@@ -404,42 +404,61 @@ __global__ void __launch_bounds__(256, kPer == 1 ? 2 : 1) kv_page_score_kernel(c
 // barriers are shorter.
 constexpr int kPickFew = 4096;
 constexpr int kPickBits = 11;
+constexpr int kPickList = 1024;
 
 struct PickSmem {
   unsigned count[1 << kPickBits];
-  unsigned scan[32][2];
-  unsigned long long low[32], high[32];
-  unsigned digit, above, whole;
+  unsigned scan[32][2], rank[32][2];
+  unsigned long long low[32], high[32], list[kPickList];
+  unsigned digit, above, in, listed;
 };
 
-// Calls emit(rank, place, key) for the places of the `pick` largest of key(0..n-1),
-// 0 < pick < n, in the order of their places; of equal keys at the border the
-// lower places.  Each warp has a run of n / 32 places, its lanes 32 in a row at
-// a time.  The first `room` keys are kept in shared memory (`kept`; all of
-// them up to kPickRoom, so that memory is read once), others are read again
-// each pass.
+// Calls emit(rank, place, key) for the places of the `pick` largest of
+// key(0..n-1), 0 < pick < n, in the order of their places; of equal keys at the
+// border the lower places.  Each warp has a run of n / 32 places, its lanes 32
+// in a row at a time.  Memory is read once if the keys fit `room` in shared
+// memory (`kept`), else once a pass.
 //
 // The border is found from the top, eleven bits a pass, beginning at the
 // highest bit in which any two keys differ; a pass whose bucket is taken whole
-// is the last.  A place is then taken if key & mask > prefix, and the first
-// `need` of those that are equal.
+// is the last.  Once the border's bucket holds few keys they are listed, and
+// the later passes look at the list alone.  A place is then taken if key &
+// mask > prefix, and the first `need` of those that are equal.
 template <int kWarps, typename Key, typename Get, typename Emit>
 __device__ void pick_largest(PickSmem& s, Key* kept, int room, Get get, int n, int pick, Emit emit) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   constexpr int kPickThreads = kWarps * 32, kMine = (1 << kPickBits) / kPickThreads;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int run = (n + kPickThreads - 1) / kPickThreads * 32;  // places per warp
-  const int begin = warp * run + lane, end = warp * run + run;
-  auto key = [&](int i) { return i < room ? kept[i] : get(i); };
+  const int begin = warp * run, have = min(max(n - begin, 0), run);
+  const bool near = n <= room;
+  // f(key, place, is) for 32 places in a row at a time, `is` false behind the
+  // end; a warp stays together.
+  auto each = [&](auto f) {
+    const int full = have & ~31;
+    if (near) {
+      const Key* at = kept + begin + lane;
+#pragma unroll 4
+      for (int j = 0; j < full; j += 32) f(at[j], begin + j + lane, true);
+    } else {
+#pragma unroll 4
+      for (int j = 0; j < full; j += 32) f(get(begin + j + lane), begin + j + lane, true);
+    }
+    if (full < have) {
+      const int i = begin + full + lane;
+      const bool is = i < begin + have;
+      f(is ? get(i) : Key(0), i, is);
+    }
+  };
   Key low = ~Key(0), high = 0;
-  for (int i0 = begin; i0 < end; i0 += 8 * 32) {
+  for (int j0 = 0; j0 < have; j0 += 8 * 32) {
     Key x[8];  // eight loads on their way at a time
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = get(min(i0 + j * 32, n - 1));
+    for (int j = 0; j < 8; ++j) x[j] = get(min(begin + j0 + j * 32 + lane, n - 1));
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int i = i0 + j * 32;
-      if (i < end && i < n) {
-        if (i < room) kept[i] = x[j];  // read by this lane only
+      const int i = j0 + j * 32 + lane;
+      if (i < have) {
+        if (near) kept[begin + i] = x[j];  // read by this warp only
         low = x[j] < low ? x[j] : low;
         high = x[j] > high ? x[j] : high;
       }
@@ -455,6 +474,8 @@ __device__ void pick_largest(PickSmem& s, Key* kept, int room, Get get, int n, i
     s.low[warp] = low;
     s.high[warp] = high;
   }
+  if (tid == 0) s.listed = 0;
+  for (int i = tid; i < (1 << kPickBits); i += kPickThreads) s.count[i] = 0;
   __syncthreads();
   low = static_cast<Key>(s.low[lane % kWarps]);
   high = static_cast<Key>(s.high[lane % kWarps]);
@@ -469,91 +490,97 @@ __device__ void pick_largest(PickSmem& s, Key* kept, int room, Get get, int n, i
   Key mask = bit >= static_cast<int>(sizeof(Key) * 8) ? Key(0) : static_cast<Key>(~Key(0) << bit);
   Key prefix = low & mask;
   unsigned need = pick;
+  bool listed = false;
   while (bit > 0) {
     const int shift = bit > kPickBits ? bit - kPickBits : 0;
     const unsigned top = (1u << (bit - shift)) - 1;
-    for (int i = tid; i < (1 << kPickBits); i += kPickThreads) s.count[i] = 0;
-    __syncthreads();
-#pragma unroll 4
-    for (int i = begin; i < end; i += 32) {
-      if (i < n) {
-        const Key x = key(i);
+    if (listed) {
+      const unsigned m = s.listed;
+      for (unsigned i = tid; i < m; i += kPickThreads) {
+        const Key x = static_cast<Key>(s.list[i]);
         if ((x & mask) == prefix) atomicAdd(&s.count[static_cast<unsigned>(x >> shift) & top], 1u);
       }
+    } else {
+      each([&](Key x, int, bool is) {
+        if (is && (x & mask) == prefix) atomicAdd(&s.count[static_cast<unsigned>(x >> shift) & top], 1u);
+      });
     }
     __syncthreads();
-    {
-      // Thread t has kMine buckets, those of thread 0 the highest.
-      unsigned c[kMine], upto = 0;
+    // Thread t has kMine buckets, those of thread 0 the highest.
+    unsigned c[kMine], upto = 0;
 #pragma unroll
-      for (int j = 0; j < kMine; ++j) upto += c[j] = s.count[(1 << kPickBits) - 1 - (kMine * tid + j)];
-      const unsigned mine = upto;
+    for (int j = 0; j < kMine; ++j) upto += c[j] = s.count[(1 << kPickBits) - 1 - (kMine * tid + j)];
+    const unsigned mine = upto;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const unsigned y = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += y;
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned y = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += y;
+    }
+    if (lane == 31) s.scan[warp][0] = upto;
+    __syncthreads();
+    unsigned before = lane < warp ? s.scan[lane][0] : 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+    unsigned above = before + upto - mine;
+#pragma unroll
+    for (int j = 0; j < kMine; ++j) {
+      const int at = (1 << kPickBits) - 1 - (kMine * tid + j);
+      if (above < need && above + c[j] >= need) {
+        s.digit = at;
+        s.above = above;
+        s.in = c[j];
       }
-      if (lane == 31) s.scan[warp][0] = upto;
-      __syncthreads();
-      unsigned before = lane < warp ? s.scan[lane][0] : 0;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
-      unsigned above = before + upto - mine;
-#pragma unroll
-      for (int j = 0; j < kMine; ++j) {
-        if (above < need && above + c[j] >= need) {
-          s.digit = (1 << kPickBits) - 1 - (kMine * tid + j);
-          s.above = above;
-          s.whole = above + c[j] == need;
-        }
-        above += c[j];
-      }
+      above += c[j];
+      s.count[at] = 0;  // for the next pass
     }
     __syncthreads();
     need -= s.above;
     prefix |= static_cast<Key>(s.digit) << shift;
     mask |= static_cast<Key>(top) << shift;
     bit = shift;
-    if (s.whole) break;
-  }
-  unsigned gt = 0, eq = 0;
-#pragma unroll 4
-  for (int i = begin; i < end; i += 32) {
-    if (i < n) {
-      const Key x = key(i) & mask;
-      gt += x > prefix;
-      eq += x == prefix;
+    const unsigned in = s.in;
+    if (in == need) break;
+    if (!listed && in <= kPickList && bit > 0) {
+      listed = true;
+      each([&](Key x, int, bool is) {
+        const bool hit = is && (x & mask) == prefix;
+        if (hit) s.list[atomicAdd(&s.listed, 1u)] = x;
+      });
+      __syncthreads();
     }
   }
+  unsigned gt = 0, eq = 0;
+  each([&](Key x, int, bool is) {
+    gt += is && (x & mask) > prefix;
+    eq += is && (x & mask) == prefix;
+  });
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     gt += __shfl_xor_sync(0xffffffffu, gt, o);
     eq += __shfl_xor_sync(0xffffffffu, eq, o);
   }
-  __syncthreads();
   if (lane == 0) {
-    s.scan[warp][0] = gt;
-    s.scan[warp][1] = eq;
+    s.rank[warp][0] = gt;
+    s.rank[warp][1] = eq;
   }
   __syncthreads();
-  gt = lane < warp ? s.scan[lane][0] : 0;
-  eq = lane < warp ? s.scan[lane][1] : 0;
+  gt = lane < warp ? s.rank[lane][0] : 0;
+  eq = lane < warp ? s.rank[lane][1] : 0;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     gt += __shfl_xor_sync(0xffffffffu, gt, o);
     eq += __shfl_xor_sync(0xffffffffu, eq, o);
   }
   const unsigned under = (1u << lane) - 1;
-#pragma unroll 4
-  for (int i = begin; i < end; i += 32) {
-    const Key full = i < n ? key(i) : Key(0), x = full & mask;
-    const bool is_gt = i < n && x > prefix, is_eq = i < n && x == prefix;
+  each([&](Key x, int i, bool is) {
+    const bool is_gt = is && (x & mask) > prefix, is_eq = is && (x & mask) == prefix;
     const unsigned g = __ballot_sync(0xffffffffu, is_gt), e = __ballot_sync(0xffffffffu, is_eq);
+    if ((g | e) == 0) return;
     const unsigned eq_here = eq + __popc(e & under);
-    if (is_gt || (is_eq && eq_here < need)) emit(static_cast<int>(gt + __popc(g & under) + min(eq_here, need)), i, full);
+    if (is_gt || (is_eq && eq_here < need)) emit(static_cast<int>(gt + __popc(g & under) + min(eq_here, need)), i, x);
     gt += __popc(g);
     eq += __popc(e);
-  }
+  });
 }
 
 // Shared memory for the keys of up to `most` places.
