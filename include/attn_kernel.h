@@ -165,7 +165,7 @@ ATTN_API int attn_library_version(void);
  *         strides.
  * Token t of sequence b lies in page block_table[b * table_stride + t /
  * page_size], row t % page_size.  block_table (int32) has table_width entries
- * per sequence; those behind a sequence's last page are not read.  seq_lens
+ * per sequence; those behind a sequence's last page do not matter.  seq_lens
  * (int32) holds the tokens of each sequence in the cache, the newest
  * included; a length of zero or less is an empty sequence (such as the unused
  * rows of a padded batch).  Both are device memory and read by the kernels
@@ -214,7 +214,9 @@ typedef struct AttnPagedCache {
  *        no two of which share memory: weights[b, h, t] += the sum of the
  *        softmax weights of token t over the query heads of kv head h.  Not
  *        together with `pages` (ATTN_ERR_UNSUPPORTED).
- * softmax_scale as in launch_attn_forward.  `listed` tells the workspace call
+ * softmax_scale as in launch_attn_forward.  With weights the workspace holds
+ * the scores, 4 * B * Hq * table_width * page_size bytes; without, it does not
+ * grow with the lengths (and may be empty: the pointer is then only checked). `listed` tells the workspace call
  * whether `pages` will be given, `weights` whether weights will be.
  */
 ATTN_API int attn_decode_workspace_bytes(const AttnPagedCache* cache, int Hq, bool listed, int n_pages, bool weights,
@@ -260,8 +262,9 @@ ATTN_API int launch_kv_page_bounds(const AttnPagedCache* cache, void* bounds, co
  *   score = sum over the dims d of max[d] * p[d] + min[d] * m[d],
  * p and m being the sums of q's positive and negative parts over the query
  * heads of the kv head: the sum of max(q * min, q * max), an upper bound of the
- * summed scores of any token of the page.  Ties go to the lower page, NaN
- * counts as largest.  Sums are taken in 64 bits, since a score
+ * summed scores of any token of the page (a part of q that is zero adds
+ * nothing, whatever the bound).  Ties go to the lower page, NaN counts as
+ * largest.  Sums are taken in 64 bits, since a score
  * next to the border decides a page.  top >= 1; cache->k and v are not used.
  */
 ATTN_API int kv_select_pages_workspace_bytes(const AttnPagedCache* cache, size_t* bytes);

@@ -860,21 +860,23 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
 // SIMT kernel: fp32, any head dim, any strides
 // ---------------------------------------------------------------------------
 
-// A warp takes 16 tokens, kKeys at a time.  Lane holds dims lane + 32 i of q,
-// K, V and O.  The kRows * kKeys dot products of a step are summed over the
+// A warp takes 32 tokens, kKeys at a time, the next ones on their way while
+// these are used, and the tokens of its next tile looked up meanwhile (17
+// sequences of up to 8192 tokens, 64/8 heads of 128 in fp32: 374 us without,
+// 199 us with).  Lane holds dims lane + 32 i of q, K, V and O.  The kRows * kKeys dot products of a step are summed over the
 // lanes by a butterfly that halves the number of values at each step, which
 // leaves each lane one product (31 shuffles for 32 products).
-template <int kRows>
+constexpr int kSimtChunk = 32, kSimtTile = kWarps * kSimtChunk;
+template <int kPer, int kRows>
 struct SimtCfg {
-  static constexpr int kKeys = kRows >= 4 ? 32 / kRows : 8;
-  static constexpr int kChunk = 16;
-  static constexpr int kTile = kWarps * kChunk;
+  static constexpr int kKeys = kPer == 8 ? 2 : kPer == 4 || kRows == 8 ? 4 : 8;
+  static constexpr int kCtas = kPer <= 2 ? 4 : kPer == 4 ? 3 : 2;  // per SM
 };
 
 template <typename T, int kPer, int kRows, bool kWeights>
-__global__ void __launch_bounds__(kThreads) attn_decode_simt_kernel(const __grid_constant__ DecodeArgs a) {
-  using C = SimtCfg<kRows>;
-  constexpr int kKeys = C::kKeys, kTile = C::kTile, kChunk = C::kChunk;
+__global__ void __launch_bounds__(kThreads, SimtCfg<kPer, kRows>::kCtas) attn_decode_simt_kernel(const __grid_constant__ DecodeArgs a) {
+  using C = SimtCfg<kPer, kRows>;
+  constexpr int kKeys = C::kKeys, kTile = kSimtTile, kChunk = kSimtChunk;
   constexpr int kVals = kRows * kKeys;
   constexpr int kSame = 32 / kVals;    // lanes that hold the same product
   constexpr int kRowLanes = 32 / kRows;  // lanes of one row
@@ -899,6 +901,12 @@ __global__ void __launch_bounds__(kThreads) attn_decode_simt_kernel(const __grid
   bool begun = cur.t == 0, fresh = true;
   int parity = 0;
   const int my_row = lane / kRowLanes, my_key = (lane / kSame) % kKeys;
+  int page = -1, row = -1;  // of token `lane` of the warp's part of a tile
+  auto look_up = [&](const Cursor& c) {
+    locate_logical(a, c.b, c.h, c.t * kTile + warp * kChunk + lane, c.len, &page, &row);
+    locate_physical(a, c.b, c.len, &page, &row);
+  };
+  if (n > 0) look_up(cur);
 
   for (int i = 0; i < n; ++i) {
     const int h = cur.h, rt = cur.rt;
@@ -918,32 +926,41 @@ __global__ void __launch_bounds__(kThreads) attn_decode_simt_kernel(const __grid
       l = 0.f;
       fresh = false;
     }
-    int page = -1, row = 0;
     const int pos0 = cur.t * kTile + warp * kChunk;
-    if (lane < kChunk) {
-      locate_logical(a, cur.b, h, pos0 + lane, cur.len, &page, &row);
-      locate_physical(a, cur.b, cur.len, &page, &row);
-    }
-    const uint32_t mask = __ballot_sync(0xffffffffu, lane < kChunk && located(a, page, row, &fault));
+    const uint32_t mask = __ballot_sync(0xffffffffu, located(a, page, row, &fault));
+    const int this_page = page, this_row = row;
+    Cursor next = cur;
+    advance<kTile>(a, next, &fault);
+    if (i + 1 < n) look_up(next);
     if (mask != 0 || kWeights) {
-      const long long kh = h * a.c.ks[1], vh = h * a.c.vs[1];
-#pragma unroll 1
-      for (int k0 = 0; k0 < kChunk; k0 += kKeys) {
-        float kv[kKeys][kPer], vv[kKeys][kPer];
+      const T* kh = kbase + h * a.c.ks[1];
+      const T* vh = vbase + h * a.c.vs[1];
+      T kn[kKeys][kPer], vn[kKeys][kPer];
+      auto fetch = [&](int k0) {
 #pragma unroll
         for (int k = 0; k < kKeys; ++k) {
-          const int pg = __shfl_sync(0xffffffffu, page, k0 + k), in = __shfl_sync(0xffffffffu, row, k0 + k);
+          const int pg = __shfl_sync(0xffffffffu, this_page, k0 + k), in = __shfl_sync(0xffffffffu, this_row, k0 + k);
           const bool live = mask >> (k0 + k) & 1u;
-          const T* kp = kbase + (live ? pg * a.c.ks[0] + kh + in * a.c.ks[2] : 0);
-          const T* vp = vbase + (live ? pg * a.c.vs[0] + vh + in * a.c.vs[2] : 0);
+          const T* kp = kh + (live ? pg * a.c.ks[0] + in * a.c.ks[2] : 0);
+          const T* vp = vh + (live ? pg * a.c.vs[0] + in * a.c.vs[2] : 0);
 #pragma unroll
           for (int e = 0; e < kPer; ++e) {
             const int d = lane + 32 * e;
             const bool ok = live && d < a.c.D;
-            kv[k][e] = ok ? to_f32(kp[d]) : 0.f;
-            vv[k][e] = ok ? to_f32(vp[d]) : 0.f;
+            kn[k][e] = ok ? kp[d] : from_f32<T>(0.f);
+            vn[k][e] = ok ? vp[d] : from_f32<T>(0.f);
           }
         }
+      };
+      fetch(0);
+#pragma unroll 1
+      for (int k0 = 0; k0 < kChunk; k0 += kKeys) {
+        float kv[kKeys][kPer], vv[kKeys][kPer];
+#pragma unroll
+        for (int k = 0; k < kKeys; ++k)
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) kv[k][e] = to_f32(kn[k][e]), vv[k][e] = to_f32(vn[k][e]);
+        if (k0 + kKeys < kChunk) fetch(k0 + kKeys);
         float s[kVals];
 #pragma unroll
         for (int r = 0; r < kRows; ++r)
@@ -1032,7 +1049,7 @@ __global__ void __launch_bounds__(kThreads) attn_decode_simt_kernel(const __grid
       begun = true;
       fresh = true;
     }
-    advance<kTile>(a, cur, &fault);
+    cur = next;
   }
   if (fault) atomicOr(&g_page_fault, fault);
 }
@@ -1199,8 +1216,8 @@ Plan make_plan(const AttnPagedCache* c, bool fast, int Hq, int n_pages, bool lis
     p.kd = D <= 32 ? 1 : D <= 64 ? 2 : D <= 128 ? 4 : 8;
     p.rows = group == 1 ? 1 : group <= 2 ? 2 : group <= 4 ? 4 : kSimtRows;
     if (p.rows > group) p.rows = group;
-    p.tile = SimtCfg<8>::kTile;
-    per_sm = 4;
+    p.tile = kSimtTile;
+    per_sm = p.kd <= 2 ? SimtCfg<2, 1>::kCtas : p.kd == 4 ? SimtCfg<4, 1>::kCtas : SimtCfg<8, 1>::kCtas;
   }
   p.row_tiles = (group + p.rows - 1) / p.rows;
   const long long capacity = static_cast<long long>(listed ? n_pages : c->table_width) * c->page_size;

@@ -263,14 +263,54 @@ struct ScoreArgs {
 constexpr int kScoreLanes = 16;                 // lanes per page
 constexpr int kScoreSlots = 256 / kScoreLanes;  // pages a CTA takes at a time
 
+// 16-bit values as doubles without a conversion, of which the hardware does 16
+// a clock and SM against 64 multiply-adds: a value's bits at the top of a
+// double are the value times 2^-kShift (the difference of the two exponent
+// biases), zeros and subnormals included, as a double's own subnormals carry
+// on.  Infinities and NaN come out as finite values, so the caller looks for
+// them.
+template <typename T> struct Bits16 { static constexpr int kShift = 0; };
+template <> struct Bits16<__nv_bfloat16> {
+  static constexpr int kShift = 1023 - 127, kMove = 3;
+  static constexpr unsigned kMask = 0x8fffe000u;
+};
+template <> struct Bits16<__half> {
+  static constexpr int kShift = 1023 - 15, kMove = 6;
+  static constexpr unsigned kMask = 0x81fffc00u;
+};
+template <typename T>
+__device__ __forceinline__ double scaled_double(unsigned top) {  // the value in the upper half of `top`
+  // an arithmetic shift keeps the sign; its copies in the exponent go
+  return __hiloint2double(static_cast<int>(static_cast<unsigned>(static_cast<int>(top) >> Bits16<T>::kMove) & Bits16<T>::kMask), 0);
+}
+__device__ __forceinline__ double power_of_two(int e) { return __hiloint2double((1023 + e) << 20, 0); }
+
+// A lane's part of the sum of a page whose bounds hold infinities or NaN, or
+// whose sum came out NaN, by the definition: a part of q that is zero adds
+// nothing to it, unless the bound is NaN.  Rare, so out of the way.
+template <typename T>
+__device__ __noinline__ double odd_page_sum(const T* lo, const T* hi, const double* up, const double* down, int D, int sub) {
+  double sum = 0.0;
+#pragma unroll 1
+  for (int d = sub; d < D; d += kScoreLanes) {
+    const double h = to_f32(hi[d]), l = to_f32(lo[d]);
+    if (up[d] != 0.0 || h != h) sum = fma(up[d], h, sum);
+    if (down[d] != 0.0 || l != l) sum = fma(down[d], l, sum);
+  }
+  return sum;
+}
+
 // max(q min, q max) is q max where q >= 0 and q min where q < 0, so the sum
 // over the query heads needs only their summed positive and negative parts:
 // one fused multiply-add per bound whatever the group.  Products of 16-bit
 // values are exact in 64 bits and their sums as good as exact, so the choice
-// of pages does not depend on the order of the sum.
+// of pages does not depend on the order of the sum.  Half the bounds are
+// converted, half moved (Bits16): the two take different pipes.
 template <typename T, int kVec, int kPer>
-__global__ void __launch_bounds__(256, kPer == 1 ? 2 : 1) kv_page_score_kernel(const __grid_constant__ ScoreArgs a) {
+__global__ void __launch_bounds__(256, kPer == 1 ? 3 : 1) kv_page_score_kernel(const __grid_constant__ ScoreArgs a) {
   using V = Vec<T, kVec>;
+  constexpr bool kMoved = sizeof(T) == 2 && kVec == 8;
+  constexpr int kBatch = kPer == 1 ? 2 : 1;  // pages on their way together
   __shared__ double s_up[256], s_down[256];
   launch_dependents();
   grid_dependency_wait();
@@ -305,6 +345,8 @@ __global__ void __launch_bounds__(256, kPer == 1 ? 2 : 1) kv_page_score_kernel(c
       s_down[d] = down;
     }
     __syncthreads();
+    // Half the shift of the moved bounds goes to q, which keeps products of
+    // the largest and of the smallest values in range, half to their sum.
     double up[kPer][kVec], down[kPer][kVec];
 #pragma unroll
     for (int j = 0; j < kPer; ++j)
@@ -312,17 +354,14 @@ __global__ void __launch_bounds__(256, kPer == 1 ? 2 : 1) kv_page_score_kernel(c
       for (int e = 0; e < kVec; ++e) {
         const int d = (j * kScoreLanes + sub) * kVec + e;
         up[j][e] = s_up[d & 255];
-        down[j][e] = s_down[d & 255];
+        down[j][e] = kMoved ? s_down[d & 255] * power_of_two(Bits16<T>::kShift / 2) : s_down[d & 255];
       }
     const T* base = static_cast<const T*>(a.bounds) + h * a.b_h;
     unsigned long long* keys = a.keys + (static_cast<long long>(b) * a.c.heads + h) * a.c.table_width;
-    // kBatch turns at a time: the bounds of the next are on their way while
-    // these are summed.
-    constexpr int kBatch = kPer == 1 ? 4 : kPer == 2 ? 2 : 1;
-    V lo[kBatch][kPer], hi[kBatch][kPer];
-    int page[kBatch];
     int turn = 0;
-    auto load = [&](int p0) {
+    for (int p0 = first; p0 < last; p0 += kBatch * kScoreSlots) {
+      V lo[kBatch][kPer], hi[kBatch][kPer];
+      int page[kBatch];
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
         page[i] = __shfl_sync(0xffffffffu, ids, (lane & 16) + turn + i);
@@ -342,55 +381,60 @@ __global__ void __launch_bounds__(256, kPer == 1 ? 2 : 1) kv_page_score_kernel(c
         turn = 0;
         ids = look_up(p0 + kBatch * kScoreSlots);
       }
-    };
-    load(first);
-    for (int p0 = first; p0 < last; p0 += kBatch * kScoreSlots) {
-      double sum[kBatch], sum2[kBatch];
-      bool named[kBatch];
-      {
-        V l[kBatch][kPer], x[kBatch][kPer];
+      double sum[kBatch];
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          named[i] = page[i] >= 0;
-          sum[i] = sum2[i] = 0.0;
+      for (int i = 0; i < kBatch; ++i) {
+        double s_hi = 0.0, s_lo = 0.0;
+        bool odd = false;
+        if constexpr (kMoved) {
+          using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+          T2 seen(T(0.f), T(0.f));  // 0 * inf and 0 * NaN are NaN
 #pragma unroll
-          for (int j = 0; j < kPer; ++j) l[i][j] = lo[i][j], x[i][j] = hi[i][j];
-        }
-        if (p0 + kBatch * kScoreSlots < last) load(p0 + kBatch * kScoreSlots);
+          for (int j = 0; j < kPer; ++j)
 #pragma unroll
-        for (int j = 0; j < kPer; ++j)
-#pragma unroll
-          for (int e = 0; e < kVec; ++e)
-#pragma unroll
-            for (int i = 0; i < kBatch; ++i) {
-              sum[i] = fma(up[j][e], static_cast<double>(to_f32(x[i][j].v[e])), sum[i]);
-              sum2[i] = fma(down[j][e], static_cast<double>(to_f32(l[i][j].v[e])), sum2[i]);
+            for (int e = 0; e < kVec / 2; ++e) {
+              unsigned w;
+              T2 x;
+              memcpy(&w, &lo[i][j].v[2 * e], 4);
+              memcpy(&x, &lo[i][j].v[2 * e], 4);
+              seen = __hfma2(x, T2(T(0.f), T(0.f)), seen);
+              s_lo = fma(down[j][2 * e], scaled_double<T>(w << 16), s_lo);
+              s_lo = fma(down[j][2 * e + 1], scaled_double<T>(w), s_lo);
+              s_hi = fma(up[j][2 * e], static_cast<double>(to_f32(hi[i][j].v[2 * e])), s_hi);
+              s_hi = fma(up[j][2 * e + 1], static_cast<double>(to_f32(hi[i][j].v[2 * e + 1])), s_hi);
             }
-      }
-      // The turns' sums over the lanes: halves of the batch are exchanged until
-      // a lane has one turn, then that one is summed.
+          odd = __hisnan(seen.x) || __hisnan(seen.y);
+          sum[i] = fma(s_lo, power_of_two(Bits16<T>::kShift / 2), s_hi);
+        } else {
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) sum[i] += sum2[i];
-      int mine = 0, off = kScoreLanes / 2;
+          for (int j = 0; j < kPer; ++j)
 #pragma unroll
-      for (int left = kBatch; left > 1; left /= 2) {
-        const bool up_half = lane & off;
-#pragma unroll
-        for (int i = 0; i < left / 2; ++i) {
-          const double keep = up_half ? sum[i + left / 2] : sum[i], give = up_half ? sum[i] : sum[i + left / 2];
-          sum[i] = keep + __shfl_xor_sync(0xffffffffu, give, off);
+            for (int e = 0; e < kVec; ++e) {
+              s_hi = fma(up[j][e], static_cast<double>(to_f32(hi[i][j].v[e])), s_hi);
+              s_lo = fma(down[j][e], static_cast<double>(to_f32(lo[i][j].v[e])), s_lo);
+            }
+          sum[i] = s_hi + s_lo;
         }
-        mine += up_half ? left / 2 : 0;
-        off /= 2;
+        odd = odd || sum[i] != sum[i];
+        const unsigned odd_lanes = __ballot_sync(0xffffffffu, odd && page[i] >= 0);
+        if (odd_lanes >> (lane & 16) & 0xffffu)
+          sum[i] = odd_page_sum(base + page[i] * a.b_p, base + page[i] * a.b_p + a.b_m, s_up, s_down, a.c.D, sub);
       }
-      for (; off > 0; off /= 2) sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], off);
-      bool is_named = false;
+      // The sums over the page's lanes; of two pages the halves of the lanes
+      // take one each.
+      int mine = 0;
+      if constexpr (kBatch == 2) {
+        constexpr int off = kScoreLanes / 2;
+        mine = sub >= off;
+        const double keep = mine ? sum[1] : sum[0], give = mine ? sum[0] : sum[1];
+        sum[0] = keep + __shfl_xor_sync(0xffffffffu, give, off);
+      }
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i)
-        if (i == mine) is_named = named[i];
+      for (int o = kScoreLanes / 2 / kBatch; o > 0; o >>= 1) sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], o);
       const int p = p0 + mine * kScoreSlots + slot;
       // a page the table does not name ranks last
-      if (p < last && sub % (kScoreLanes / kBatch) == 0) keys[p] = is_named ? order_key(sum[0]) : 0ull;
+      const bool named = (mine ? page[kBatch - 1] : page[0]) >= 0;
+      if (p < last && sub % (kScoreLanes / kBatch) == 0) keys[p] = named ? order_key(sum[0]) : 0ull;
     }
   }
   if (fault) atomicOr(&g_page_fault, fault);
@@ -592,7 +636,8 @@ int pick_room(long long most, int key_bytes) {
 
 template <typename... Params, typename... Args>
 bool launch_pick(void (*kern)(Params...), int warps, unsigned units, size_t smem, cudaStream_t stream, const Args&... args) {
-  if (smem > 32 * 1024 &&
+  // 48 KiB without asking, PickSmem among them
+  if (smem + sizeof(PickSmem) > 48 * 1024 &&
       cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kPickRoomBytes) != cudaSuccess)
     return false;
   return launch_after(kern, dim3(units), dim3(warps * 32), smem, stream, 1, args...);
@@ -936,9 +981,10 @@ extern "C" int launch_kv_select_pages(const AttnPagedCache* cache, const void* q
   const long long units = static_cast<long long>(cache->B) * cache->heads;
   // Pages per CTA: as many as leave eight CTAs per SM, two of which run at once
   // (measured: 2 and 16 per SM 4 % slower on 32 contexts of 1024 pages).
-  int per = 4 * kScoreSlots;
-  while (per < cache->table_width && units * ((cache->table_width + per - 1) / per) > 148 * 8) per += 4 * kScoreSlots;
-  const int chunks = (cache->table_width + per - 1) / per;
+  const long long wanted = units < 148 * 8 ? 148 * 8 / units : 1;
+  constexpr int kTurns = 4 * kScoreSlots;
+  const int per = static_cast<int>(((cache->table_width + wanted - 1) / wanted + kTurns - 1) / kTurns * kTurns);
+  const int chunks = per > 0 ? (cache->table_width + per - 1) / per : 0;
   if (units > 0x7fffffffLL || static_cast<long long>(cache->B) * chunks > 0x7fffffffLL)
     return ATTN_ERR_INVALID_ARGUMENT;
   const long long contiguous[2] = {static_cast<long long>(Hq) * cache->D, cache->D};

@@ -81,7 +81,9 @@ bool launch_after(void (*kern)(Params...), dim3 grid, dim3 block, size_t smem, c
   cfg.stream = stream;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess;
+  if (cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess) return true;
+  cudaGetLastError();  // reported by the caller's status
+  return false;
 }
 
 // (Loads of what other kernels write, lengths and tables among it, are plain

@@ -13,7 +13,7 @@ Cache layout, common to all of them:
   size;
 * ``block_table``: int32 ``[B, W]``; token t of sequence b lies in page
   ``block_table[b, t // page_size]``, row ``t % page_size``.  Entries behind a
-  sequence's last page are not read;
+  sequence's last page do not matter;
 * ``seq_lens``: int32 ``[B]``, the tokens of each sequence in the cache, the
   newest included.  Zero or less is an empty sequence, such as an unused row of
   a padded batch.
@@ -49,7 +49,8 @@ def attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, b
 
     weights: optional fp32 ``[B, Hkv, >= W * page_size]``, updated in place:
     each token's softmax weight, summed over the query heads of the kv head, is
-    added to it (``kv_evict`` takes it).  Not together with ``pages``.
+    added to it (``kv_evict`` takes it).  Needs ``4 * B * Hq * W * page_size``
+    bytes of scratch memory.  Not together with ``pages``.
     """
     return rocm_attn_ext.attn_decode(q, k_cache, v_cache, block_table, seq_lens,
                                      -1.0 if scale is None else float(scale), pages, weights)

@@ -76,6 +76,23 @@ def test_decode_long_split(attn, D, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("B,Hkv,L", [(1, 1, 64), (1, 2, 128), (2, 1, 300), (1, 8, 517), (5, 8, 1000), (32, 8, 100),
+                                     (40, 16, 64)])
+@pytest.mark.parametrize("width", [None, 700])
+def test_decode_short_caches_and_wide_tables(attn, B, Hkv, L, width, dtype):
+    # few tiles by the table's width (one launch, clusters of each size) and many, by the same lengths
+    lens = [max(0, L - 37 * b) for b in range(B)]
+    _decode(attn, lens, 4 * Hkv, Hkv, 128, 16, dtype, seed=B, width=width)
+
+
+def test_decode_masked_tail_of_nan(attn):
+    # a chunk whose later 16 tokens are absent, in every position of the tile, with NaN behind them
+    for n in range(1, 140, 3):
+        _decode(attn, [n], 2, 1, 64, 32, BF16, seed=n)
+        _decode(attn, [n], 2, 1, 64, 48, F16, seed=n, width=300)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
 def test_decode_unaligned_and_mixed_strides(attn, dtype):
     # rows that are not 16-byte aligned, K and V of different strides, strided q
     k, v, table, ln = make_cache([77, 200], 2, 64, 16, dtype)
@@ -400,6 +417,22 @@ def test_select_ties_nan_and_bad_pages(attn):
     assert got[0, 0].tolist() == [0, 1, 2, 3, 7]
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+def test_select_infinite_bounds(attn, dtype):
+    # +inf and -inf in bounds, largest and smallest finite values and subnormals of the type; no q is zero
+    k, v, table, ln = make_cache([900], 2, 64, 4, dtype, poison=False)
+    bounds = bounds_ref(k, table, ln, torch.zeros(k.shape[0], 2, 2, 64, dtype=dtype))
+    fi = torch.finfo(dtype)
+    for i, (page, what, x) in enumerate([(3, 1, math.inf), (50, 0, -math.inf), (100, 1, fi.max), (130, 0, -fi.max),
+                                         (150, 1, fi.smallest_normal / 4), (160, 0, -math.inf), (160, 1, math.inf)]):
+        bounds[int(table[0, page]), 0, what, i] = x
+    q = _q(1, 4, 64, dtype, seed=8)
+    q[q == 0] = 1
+    for top in (2, 4, 6, 20):
+        got = attn.kv_select_pages(q.cuda(), bounds.cuda(), table.cuda(), ln.cuda(), 4, top)
+        assert torch.equal(got.cpu(), select_ref(q, bounds, table, ln, 4, top))
+
+
 def test_select_decides_by_less_than_32_bits(attn):
     # two pages whose scores differ by less than half a step of 32 bits
     bounds = torch.zeros(3, 1, 2, 2)
@@ -468,6 +501,22 @@ def test_evict_ties_and_nan(attn):
     w[2, 0, 33] = math.inf
     w[2, 0, 34] = -math.inf
     _check_evict(attn, k, v, table, ln, new, w, budget, 10)
+
+
+@pytest.mark.parametrize("n", [4000, 7930, 8190, 12000, 41500])
+def test_evict_sizes_of_the_key_store(attn, n):
+    # capacities about the limits of shared memory without and with opting in, and beyond what it holds
+    c = _evict_case([n, n - 1], 1, 8, 16, F16, 600, seed=n)
+    _check_evict(attn, *c, 600, 7)
+
+
+@pytest.mark.parametrize("n", [3900, 4090, 21000])
+def test_select_sizes_of_the_key_store(attn, n):
+    k, v, table, ln = make_cache([n], 1, 8, 1, F16, poison=False)
+    bounds = bounds_ref(k, table, ln, torch.zeros(k.shape[0], 1, 2, 8, dtype=F16))
+    q = _q(1, 2, 8, F16)
+    got = attn.kv_select_pages(q.cuda(), bounds.cuda(), table.cuda(), ln.cuda(), 1, 333)
+    assert torch.equal(got.cpu(), select_ref(q, bounds, table, ln, 1, 333))
 
 
 def test_evict_bad_pages(attn):
