@@ -979,9 +979,9 @@ extern "C" int launch_kv_select_pages(const AttnPagedCache* cache, const void* q
   if (top < 1 || Hq < 0 || Hq % cache->heads != 0 || cache->heads > 65535) return ATTN_ERR_INVALID_ARGUMENT;
   if (cache->B == 0) return ATTN_OK;
   const long long units = static_cast<long long>(cache->B) * cache->heads;
-  // Pages per CTA: as many as leave eight CTAs per SM, two of which run at once
-  // (measured: 2 and 16 per SM 4 % slower on 32 contexts of 1024 pages).
-  const long long wanted = units < 148 * 8 ? 148 * 8 / units : 1;
+  // Pages per CTA: as many as leave four CTAs per SM, three of which run at
+  // once (32 contexts of 1024 pages: 34.8 us with eight, 32.9 us with four).
+  const long long wanted = units < 148 * 4 ? 148 * 4 / units : 1;
   constexpr int kTurns = 4 * kScoreSlots;
   const int per = static_cast<int>(((cache->table_width + wanted - 1) / wanted + kTurns - 1) / kTurns * kTurns);
   const int chunks = per > 0 ? (cache->table_width + per - 1) / per : 0;
