@@ -106,13 +106,14 @@ def build_kernel_lib(force: bool = False, verbose: bool = False) -> str:
         jobs = [("attn_general.cu", "attn_general.o", ()), ("attn_kernel.cu", "attn_kernel.o", ()),
                 ("attn_group.cu", "attn_group.o", ()),
                 ("attn_decode.cu", "attn_decode.o", ()), ("kv_cache.cu", "kv_cache.o", ()),
-                ("attn_kernel.cu", "attn_kernel_wdtest.o", ("RA_WATCHDOG_TEST",))]
+                ("attn_kernel.cu", "attn_kernel_wdtest.o", ("RA_WATCHDOG_TEST",)),
+                ("attn_decode.cu", "attn_decode_wdtest.o", ("RA_WATCHDOG_TEST",))]
         with ThreadPoolExecutor(len(jobs)) as ex:
-            general, kernel, group, decode, cache, wd = ex.map(
+            general, kernel, group, decode, cache, wd, wd_decode = ex.map(
                 lambda j: _compile(os.path.join(CSRC, j[0]), os.path.join(OBJ_DIR, j[1]), defines=j[2],
                                    verbose=verbose), jobs)
         _link([kernel, group, general, decode, cache], KERNEL_LIB)
-        _link([wd, group, general, decode, cache], WATCHDOG_TEST_LIB)
+        _link([wd, group, general, wd_decode, cache], WATCHDOG_TEST_LIB)
     return KERNEL_LIB
 
 

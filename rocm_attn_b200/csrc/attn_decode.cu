@@ -21,14 +21,24 @@
 //     and a second small kernel joins them in the order of the tokens, so
 //     results do not depend on timing.  It is launched early and waits on the
 //     grid before it (programmatic launch), which hides its launch.
-//   * Each warp has its own ring of K/V chunks in shared memory filled by
-//     16-byte asynchronous copies, through page ids looked up one chunk ahead;
-//     warps meet only where a unit ends.  The chunk freed last is the scratch
-//     space of that meeting, so the ring stays full meanwhile.
+//   * Where the block table can only name a few tiles per CTA, the CTAs of a
+//     unit form a cluster and join over its shared memory instead: one launch
+//     and no workspace.
+//   * Each warp has its own ring of K/V chunks in shared memory, filled by TMA
+//     (or 16-byte asynchronous copies) through page ids looked up chunks
+//     ahead; warps meet only where a unit ends.  The chunk freed last is the
+//     scratch space of that meeting, so the ring stays full meanwhile.
 //
 // Two kernels share that frame: attn_decode_mma_kernel (fp16/bf16, D a
 // multiple of 8, 16-byte rows) on warp-level tensor cores, and
 // attn_decode_simt_kernel (fp32, any D <= 256, any strides).
+//
+// Measured on B200 (calls in a row): 64 sequences of up to 16384 tokens, 64/8
+// heads of 128, fp16, 2.75 GB of K and V: 408 us, 6.75 TB/s, where a copy does
+// 6.54; 24 of up to 4096, 32/8 heads, bf16, with weights: 55 us (floor 41); one
+// of 517 tokens: 7.4 us on the device.  Each call has about 8 us that are
+// not reading: lengths and first look-ups 3, first fill of the rings 2.5, the
+// ends of the runs and the join the rest.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -251,6 +261,12 @@ __device__ __forceinline__ Cursor schedule(const DecodeArgs& a, ScheduleSmem& s,
   return a.c.B <= 128 ? schedule_by<kTile, false>(a, s, run, fault) : schedule_by<kTile, true>(a, s, run, fault);
 }
 
+// The first query row of the unit at c.
+template <typename T>
+__device__ __forceinline__ const T* query_rows(const DecodeArgs& a, const Cursor& c) {
+  return static_cast<const T*>(a.q) + c.b * a.q_b + (static_cast<long long>(c.h) * a.group + c.rt * a.rows) * a.q_h;
+}
+
 // Output rows of empty sequences are zeros.
 template <typename T>
 __device__ __forceinline__ void zero_empty_rows(const DecodeArgs& a, int* fault) {
@@ -267,7 +283,8 @@ __device__ __forceinline__ void zero_empty_rows(const DecodeArgs& a, int* fault)
 // value only the next needs, so that the loads of several tokens overlap: its
 // logical page (row < 0: no such token), then its physical page.
 __device__ __forceinline__ void locate_logical(const DecodeArgs& a, int b, int h, int pos, int len, int* lp, int* row) {
-  const int j = static_cast<int>((__umulhi(static_cast<unsigned>(pos), a.ps_mul) + static_cast<unsigned>(pos)) >> a.ps_shift);
+  const unsigned p = static_cast<unsigned>(pos);
+  const int j = static_cast<int>((__umulhi(p, a.ps_mul) + p) >> a.ps_shift);
   *row = pos - j * a.c.page_size;
   *lp = j;
   if (a.pages) {
@@ -331,7 +348,10 @@ __device__ __forceinline__ Place place_of(const DecodeArgs& a, const Cursor& c, 
 // A warp's chunk is kKeys tokens: K rows, then V rows, of kD 16-bit elements,
 // 16-byte columns XOR-swizzled by the row so that ldmatrix reads every bank
 // once.  Its size, 4 kKeys kD bytes, is that of 16 rows of O in fp32 or more,
-// which is what the freed chunk holds where a unit ends.
+// which is what the freed chunk holds where a unit ends.  Rings of two chunks:
+// with three, 64 long sequences read 6.39 TB/s instead of 6.73.  Two CTAs of
+// four warps per SM (one at D = 256, whose accumulators and query heads take
+// the registers): while one ends a unit the other reads.
 template <int kD>
 struct MmaCfg {
   static constexpr int kKeys = kD <= 64 ? 32 : 16;
@@ -376,6 +396,7 @@ __device__ __forceinline__ float4 cluster_load4(const float* p, int rank) {
 struct TmaMaps {
   CUtensorMap k, v;
   unsigned long long wait_ns;
+  int lose;  // watchdog test build only: CTA 0's first wait is for bytes that never come
 };
 
 template <bool kBf16, int kD, int kNT, bool kWeights, bool kTma>
@@ -447,7 +468,7 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
   auto prefetch_q = [&](const Cursor& c) {
     constexpr int kLines = kD / 64;  // of 128 bytes in a row
     const int rows = min(a.rows, a.group - c.rt * a.rows);
-    const T* q = static_cast<const T*>(a.q) + c.b * a.q_b + (static_cast<long long>(c.h) * a.group + c.rt * a.rows) * a.q_h;
+    const T* q = query_rows<T>(a, c);
     for (int e = lane; e < rows * kLines; e += 32)
       if (e % kLines * 64 < a.c.D) prefetch_l1(q + (e / kLines) * a.q_h + e % kLines * 64);
   };
@@ -476,8 +497,11 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
   };
   auto physical = [&](int s) { locate_physical(a, last_b, last_len, &page[s], &row[s]); };
   const uint64_t policy = l2_policy_evict_first();
+  uint32_t phase = 0, in_flight = 0;  // of each stage's barrier; chunks asked for and not yet seen
+  bool gave_up = false;
   auto issue = [&](int stage) {
-    const uint32_t mask = __ballot_sync(0xffffffffu, located(a, page[0], row[0], &fault));
+    uint32_t mask = __ballot_sync(0xffffffffu, located(a, page[0], row[0], &fault));
+    if (gave_up) mask = 0;
     if (lane == 0) s_mask[warp][stage] = mask;
     if constexpr (kTma) {
       // One lane asks for the boxes, of 16 rows, that hold tokens.  All rows of
@@ -486,7 +510,12 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
         int boxes = 0;
 #pragma unroll
         for (int g = 0; g < kKeys / 16; ++g) boxes += mask >> (g * 16) & 1u;
-        if (lane == 0) mbar_arrive_expect_tx(&s_full[warp][stage], boxes * 16 * (kD * 4));
+        int bytes = boxes * 16 * (kD * 4);
+#ifdef RA_WATCHDOG_TEST
+        if (maps.lose && blockIdx.x == 0 && threadIdx.x == 0 && in_flight == 0 && phase == 0) bytes += 16;
+#endif
+        if (lane == 0) mbar_arrive_expect_tx(&s_full[warp][stage], bytes);
+        in_flight |= 1u << stage;
 #pragma unroll
         for (int g = 0; g < kKeys / 16; ++g) {
           const int pg = __shfl_sync(0xffffffffu, page[0], g * 16), in = __shfl_sync(0xffffffffu, row[0], g * 16);
@@ -561,7 +590,6 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
   float m[kNT][2], l[kNT][2];  // of query heads 8 t + 2 (lane % 4) + {0, 1}
   bool begun = a.cluster ? true : cur.t == 0, fresh = true;
   int stage = 0;
-  uint32_t phase = 0;  // of each stage's barrier
 
   // Scores of tokens lane / 4 + {0, 8} of the chunk's g-th 16 and of two heads
   // of column tile t, for the weights.
@@ -588,7 +616,7 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
       if (fresh) {
         // A new unit: its query heads as B fragments (heads behind the last are zero).
         const int rows = min(a.rows, a.group - cur.rt * a.rows);
-        const T* q = static_cast<const T*>(a.q) + cur.b * a.q_b + (static_cast<long long>(cur.h) * a.group + cur.rt * a.rows) * a.q_h;
+        const T* q = query_rows<T>(a, cur);
 #pragma unroll
         for (int t = 0; t < kNT; ++t) {
           const int r = t * 8 + (lane >> 2);
@@ -612,21 +640,32 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
       if (mask != 0 || kWeights) {
         const uint32_t chunk = ring_addr + stage * C::kStageBytes;
         const uint32_t kaddr = chunk + (lane & 15) * 128 + (((lane >> 4) ^ (lane & 7)) << 4);
-        const uint32_t vaddr = chunk + kKeys * kD * 2 + ((lane >> 4) * 8 + (lane & 7)) * 128 + (((lane >> 3 & 1) ^ (lane & 7)) << 4);
+        const uint32_t vaddr =
+            chunk + kKeys * kD * 2 + ((lane >> 4) * 8 + (lane & 7)) * 128 + (((lane >> 3 & 1) ^ (lane & 7)) << 4);
         if constexpr (kTma) {
           if (mask != 0) {
-            // A wait that runs out marks the launch; the CTA goes on, at once
-            // from then on, so that its warps still meet.
-            if (!mbar_wait(&s_full[warp][stage], phase >> stage & 1u, &s_abort, &s_code, 1, maps.wait_ns)) fault |= kFaultWait;
-            phase ^= 1u << stage;
+            // A wait that runs out marks the launch; the warp asks for nothing
+            // more, whose barrier could not tell it from what is missing, and
+            // goes on without, so that the CTA's warps still meet.
+            if (!gave_up) {
+              const bool there = mbar_wait(&s_full[warp][stage], phase >> stage & 1u, &s_abort, &s_code, 1, maps.wait_ns);
+              if (__all_sync(0xffffffffu, there)) {
+                phase ^= 1u << stage;
+                in_flight &= ~(1u << stage);
+              } else {
+                gave_up = true;
+                fault |= kFaultWait;
+              }
+            }
             if (mask != 0xffffffffu >> (32 - kKeys)) {
               // Rows of a box that hold no token have come along; V's are
               // cleared, as no weight, not even zero, may meet them.
 #pragma unroll 1
               for (int e = lane; e < kKeys * kCols; e += 32) {
                 const int r = e % kKeys, c = e / kKeys;
+                unsigned char* v_at = ring + stage * C::kStageBytes + kKeys * kD * 2 + (c / 8) * (kKeys * 128);
                 if (!(mask >> r & 1u))
-                  *reinterpret_cast<uint4*>(ring + stage * C::kStageBytes + kKeys * kD * 2 + (c / 8) * (kKeys * 128) + r * 128 + (c % 8) * 16) = make_uint4(0, 0, 0, 0);
+                  *reinterpret_cast<uint4*>(v_at + r * 128 + (c % 8) * 16) = make_uint4(0, 0, 0, 0);
               }
               fence_proxy_async_smem();
               __syncwarp();
@@ -812,9 +851,8 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
           const int n_w = (unit_T - w + a.cluster - 1) / a.cluster;
           ms[w] = cluster_load(&s_cm[r], w);
           ls[w] = cluster_load(&s_cl[r], w);
-          ys[w] = cluster_load4(reinterpret_cast<const float*>(smem + ((r >> 4) * kStages + n_w % kStages) * C::kStageBytes) +
-                                    (r & 15) * kD + c4 * 4,
-                                w);
+          const unsigned char* part = smem + ((r >> 4) * kStages + n_w % kStages) * C::kStageBytes;
+          ys[w] = cluster_load4(reinterpret_cast<const float*>(part) + (r & 15) * kD + c4 * 4, w);
         }
       }
       float M = -INFINITY, L = 0.f;
@@ -842,13 +880,14 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
     cluster_sync();
   } else if (a.cluster == 1 && n == 0) {
     const int rows = min(a.rows, a.group - cur_rt * a.rows);
-    for (int e = threadIdx.x; e < rows * a.c.D; e += kThreads) static_cast<T*>(a.out)[unit_row0 * a.c.D + e] = from_f32<T>(0.f);
+    T* out = static_cast<T*>(a.out) + unit_row0 * a.c.D;
+    for (int e = threadIdx.x; e < rows * a.c.D; e += kThreads) out[e] = from_f32<T>(0.f);
   }
   if constexpr (kTma) {
-    if (s_abort) {
-      // Copies still in flight must not outlive the CTA's shared memory.
+    // Copies still in flight must not outlive the CTA's shared memory.
+    if (gave_up) {
       for (int s = 0; s < kStages; ++s)
-        if (s_mask[warp][s] != 0) mbar_wait(&s_full[warp][s], phase >> s & 1u, &s_late, &s_code, 1);
+        if (in_flight >> s & 1u) mbar_wait(&s_full[warp][s], phase >> s & 1u, &s_late, &s_code, 1);
     }
   } else {
     cp_async_wait<0>();
@@ -863,9 +902,10 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
 // A warp takes 32 tokens, kKeys at a time, the next ones on their way while
 // these are used, and the tokens of its next tile looked up meanwhile (17
 // sequences of up to 8192 tokens, 64/8 heads of 128 in fp32: 374 us without,
-// 199 us with).  Lane holds dims lane + 32 i of q, K, V and O.  The kRows * kKeys dot products of a step are summed over the
-// lanes by a butterfly that halves the number of values at each step, which
-// leaves each lane one product (31 shuffles for 32 products).
+// 199 us with).  Lane holds dims lane + 32 i of q, K, V and O.  The kRows *
+// kKeys dot products of a step are summed over the lanes by a butterfly that
+// halves the number of values at each step, which leaves each lane one product
+// (31 shuffles for 32 products).
 constexpr int kSimtChunk = 32, kSimtTile = kWarps * kSimtChunk;
 template <int kPer, int kRows>
 struct SimtCfg {
@@ -874,7 +914,8 @@ struct SimtCfg {
 };
 
 template <typename T, int kPer, int kRows, bool kWeights>
-__global__ void __launch_bounds__(kThreads, SimtCfg<kPer, kRows>::kCtas) attn_decode_simt_kernel(const __grid_constant__ DecodeArgs a) {
+__global__ void __launch_bounds__(kThreads, SimtCfg<kPer, kRows>::kCtas)
+    attn_decode_simt_kernel(const __grid_constant__ DecodeArgs a) {
   using C = SimtCfg<kPer, kRows>;
   constexpr int kKeys = C::kKeys, kTile = kSimtTile, kChunk = kSimtChunk;
   constexpr int kVals = kRows * kKeys;
@@ -913,7 +954,7 @@ __global__ void __launch_bounds__(kThreads, SimtCfg<kPer, kRows>::kCtas) attn_de
     const int rows = min(a.rows, a.group - rt * a.rows);
     const long long row0 = static_cast<long long>(cur.b) * a.Hq + h * a.group + rt * a.rows;
     if (fresh) {
-      const T* qp = static_cast<const T*>(a.q) + cur.b * a.q_b + (static_cast<long long>(h) * a.group + rt * a.rows) * a.q_h;
+      const T* qp = query_rows<T>(a, cur);
 #pragma unroll
       for (int r = 0; r < kRows; ++r)
 #pragma unroll
@@ -1082,7 +1123,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_decode_join_kernel(const
   if (lane < kJoinWarps && c + lane < gridDim.x) early_ml = a.part_ml[slot(lane)];
 #pragma unroll
   for (int k = 0; k < 2; ++k)
-    if (ask && k * 128 + lane * 4 < a.D4) early[k] = *reinterpret_cast<const float4*>(a.part_o + slot(warp) * a.D4 + k * 128 + lane * 4);
+    if (ask && k * 128 + lane * 4 < a.D4)
+      early[k] = *reinterpret_cast<const float4*>(a.part_o + slot(warp) * a.D4 + k * 128 + lane * 4);
   const int4 meta = a.meta[c];
   if (meta.z == 0 || r >= meta.y) return;
   float M = -INFINITY, L = 0.f;
@@ -1227,10 +1269,18 @@ Plan make_plan(const AttnPagedCache* c, bool fast, int Hq, int n_pages, bool lis
   if (grid < 1) grid = 1;
   p.cluster = 0;
   if (p.mma) {
-    const long long unit_tiles = (capacity + p.tile - 1) / p.tile, units = static_cast<long long>(c->B) * c->heads * p.row_tiles;
+    const long long unit_tiles = (capacity + p.tile - 1) / p.tile;
+    const long long units = static_cast<long long>(c->B) * c->heads * p.row_tiles;
     int cl = 1;
     while (cl < kMaxCluster && cl < unit_tiles && units * cl * 2 <= static_cast<long long>(sms) * per_sm) cl *= 2;
-    const long long slots = static_cast<long long>(sms) * per_sm, most = units * cl * 2 >= slots && units * cl <= slots ? 4 : 2;
+    // One launch of clusters where a CTA gets at most two tiles, or four if
+    // the clusters leave less than half of the GPU idle; not where units far
+    // outnumber the CTAs that fit, whose set-up would then repeat.  Measured, in
+    // clusters against runs, us: 8 units of 1 tile 4.6 / 6.4, 32 of 8 tiles
+    // 7.4 / 8.2, 32 of 32 tiles 11.3 / 12.2, 512 of 2 tiles 12.5 / 14.0; but 8 of
+    // 32 tiles 10.4 / 9.5, 512 of 8 tiles 27.0 / 25.5, 2048 of 2 tiles 40.7 / 35.2.
+    const long long slots = static_cast<long long>(sms) * per_sm;
+    const int most = units * cl * 2 >= slots && units * cl <= slots ? 4 : 2;
     if (unit_tiles <= cl * most && units * cl <= 2 * slots) {
       p.cluster = cl;
       grid = units * cl;
@@ -1316,6 +1366,7 @@ bool launch_mma_any(const DecodeArgs& a, const Plan& p, cudaStream_t stream) {
   TmaMaps maps;
   const unsigned long long limit = wait_limit_ns();
   maps.wait_ns = limit != 0 ? limit : kWaitTimeoutNs;
+  maps.lose = drop_arrival_requested();
   auto encode = [&](CUtensorMap* map, const void* base, const long long* st) {
     return make_tensor_map_4d(map, base, kBf16, a.c.D, a.c.page_size, a.c.heads, a.c.num_pages, st[2], st[1], st[0], 64,
                               16) == 0;

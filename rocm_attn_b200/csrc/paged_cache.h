@@ -39,6 +39,7 @@ int check_paged_cache(const AttnPagedCache* c, int tensors, PagedView* view);
 int check_device();
 int sm_count();
 unsigned long long wait_limit_ns();  // the setting of attn_set_wait_limit_ns
+int drop_arrival_requested();        // watchdog test build only
 
 // Faults a kernel records: a page or length out of range, a wait that ran out.
 constexpr int kFaultPage = 1, kFaultWait = 2;

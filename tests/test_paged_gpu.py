@@ -1,11 +1,14 @@
 """The paged key-value cache operators against their definitions in 64 bits
 (paged_ref.py): attention of one new token, the cache's writer, page bounds,
 page selection and eviction."""
+import ctypes
 import math
+import os
 
 import pytest
 import torch
 
+import rocm_attn_b200
 from paged_ref import (bounds_ref, decode_ref, decode_tolerance, evict_ref, make_cache, rows, select_ref)
 
 pytestmark = pytest.mark.gpu
@@ -655,6 +658,54 @@ def test_generation_run(attn):
     for i in range(20):
         step(i % 2 == 1)
     assert attn.check_status(0) == 0
+
+
+# ---------------------------------------------------------------------------
+# the watchdog (tests/test_watchdog_gpu.py says how the test build works)
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("lens,D,width", [([300, 40], 128, None), ([2000, 700], 64, None), ([5000], 128, 400),
+                                          ([900], 256, 200)])
+def test_watchdog_fires_and_recovers(lens, D, width):
+    # CTA 0's first wait is for 16 bytes more than come: it ends by the limit, the kernel reports it and
+    # returns, and the next launch is clean
+    from test_paged_cpu import LL3, PagedCache
+
+    lib = ctypes.CDLL(os.path.join(os.path.dirname(rocm_attn_b200.KERNEL_LIB_PATH), "librocm_attn_wdtest.so"))
+    lib.attn_set_wait_limit_ns.argtypes = [ctypes.c_ulonglong]
+    lib.launch_attn_decode.argtypes = [ctypes.c_void_p] * 4 + [ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_int,
+                                                                ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+                                                                ctypes.c_size_t, ctypes.c_void_p]
+    k, v, table, ln = make_cache(lens, 2, D, 16, BF16, width=width)
+    q = _q(len(lens), 4, D, BF16)
+    dk, dv, dt, dl, dq = (t.cuda() for t in (k, v, table, ln, q))
+    out = torch.zeros_like(dq)
+    st = LL3(*dk.stride()[:3])
+    c = PagedCache(dk.data_ptr(), dv.data_ptr(), k.shape[0], 2, 16, D, 1, st, st, dt.data_ptr(), dt.shape[1], dt.shape[1],
+                   dl.data_ptr(), len(lens))
+    size = ctypes.c_size_t()
+    assert lib.attn_decode_workspace_bytes(ctypes.byref(c), 4, False, 0, False, ctypes.byref(size)) == 0
+    space = torch.empty(max(16, size.value), dtype=torch.uint8, device="cuda")
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+    def run():
+        assert lib.launch_attn_decode(ctypes.byref(c), dq.data_ptr(), None, out.data_ptr(), 4, -1.0, None, 0, None, None,
+                                      space.data_ptr(), size.value, stream) == 0
+        status = ctypes.c_int(-1)
+        assert lib.attn_get_status(stream, ctypes.byref(status)) == 0
+        return status.value
+
+    assert run() == 0
+    lib.attn_set_wait_limit_ns(1_000_000)
+    lib.attn_test_drop_arrival(1)
+    try:
+        assert run() == 7
+    finally:
+        lib.attn_test_drop_arrival(0)
+        lib.attn_set_wait_limit_ns(0)
+    assert run() == 0
+    _close(out, decode_ref(q, k, v, table, ln), max(lens), BF16)
 
 
 # ---------------------------------------------------------------------------
