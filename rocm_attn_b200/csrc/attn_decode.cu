@@ -1215,6 +1215,7 @@ __global__ void __launch_bounds__(256) attn_decode_weights_kernel(const __grid_c
   if (t >= len) return;
   const long long r0 = static_cast<long long>(b) * a.Hq + static_cast<long long>(h) * a.group;
   float sum = 0.f;
+#pragma unroll 4
   for (int g = 0; g < a.group; ++g) sum += ex2_approx(a.x[(r0 + g) * a.x_stride + t] - a.lse2[r0 + g]);
   float* w = weights + b * w_b + h * w_h + t;
   *w += sum;
