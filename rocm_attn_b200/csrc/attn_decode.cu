@@ -1338,7 +1338,8 @@ bool launch_mma(const DecodeArgs& a, const TmaMaps& maps, int grid, cudaStream_t
       done[dev] = true;
     }
   }
-  return launch_after(kern, dim3(grid), dim3(kThreads), MmaCfg<kD>::kRingBytes, stream, a.cluster, a, maps);
+  const bool ahead = a.cluster <= 1 || 2 * grid <= MmaCfg<kD>::kCtas * sm_count();
+  return launch_after(kern, dim3(grid), dim3(kThreads), MmaCfg<kD>::kRingBytes, stream, a.cluster, ahead, a, maps);
 }
 
 // Column tiles of eight query heads: 1, 2 or 4.
@@ -1383,7 +1384,7 @@ bool launch_simt_rows(const DecodeArgs& a, int grid, cudaStream_t stream) {
                     : a.rows <= 2 ? attn_decode_simt_kernel<T, kPer, 2, kWeights>
                     : a.rows <= 4 ? attn_decode_simt_kernel<T, kPer, 4, kWeights>
                                   : attn_decode_simt_kernel<T, kPer, 8, kWeights>;
-  return launch_after(kern, dim3(grid), dim3(kThreads), 0, stream, 1, a);
+  return launch_after(kern, dim3(grid), dim3(kThreads), 0, stream, 1, true, a);
 }
 
 template <typename T, bool kWeights>
@@ -1500,13 +1501,13 @@ extern "C" int launch_attn_decode(const AttnPagedCache* cache, const void* q, co
   const dim3 grid(p.grid, p.rows), block(kJoinWarps * 32);
   bool ok = true;
   if (!p.cluster) switch (cache->dtype) {
-    case ATTN_F16: ok = launch_after(attn_decode_join_kernel<__half>, grid, block, 0, stream, 1, a); break;
-    case ATTN_BF16: ok = launch_after(attn_decode_join_kernel<__nv_bfloat16>, grid, block, 0, stream, 1, a); break;
-    default: ok = launch_after(attn_decode_join_kernel<float>, grid, block, 0, stream, 1, a); break;
+    case ATTN_F16: ok = launch_after(attn_decode_join_kernel<__half>, grid, block, 0, stream, 1, true, a); break;
+    case ATTN_BF16: ok = launch_after(attn_decode_join_kernel<__nv_bfloat16>, grid, block, 0, stream, 1, true, a); break;
+    default: ok = launch_after(attn_decode_join_kernel<float>, grid, block, 0, stream, 1, true, a); break;
   }
   if (ok && weights) {
     const dim3 wgrid((view.capacity() + 255) / 256, cache->heads, cache->B);
-    ok = wgrid.x == 0 || launch_after(attn_decode_weights_kernel, wgrid, dim3(256), 0, stream, 1, a, weights,
+    ok = wgrid.x == 0 || launch_after(attn_decode_weights_kernel, wgrid, dim3(256), 0, stream, 1, true, a, weights,
                                       weights_strides[0], weights_strides[1]);
   }
   return ok ? ATTN_OK : ATTN_ERR_LAUNCH;

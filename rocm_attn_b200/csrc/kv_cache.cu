@@ -649,7 +649,7 @@ bool launch_pick(void (*kern)(Params...), int warps, unsigned units, size_t smem
   if (smem + sizeof(PickSmem) > 48 * 1024 &&
       cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kPickRoomBytes) != cudaSuccess)
     return false;
-  return launch_after(kern, dim3(units), dim3(warps * 32), smem, stream, 1, args...);
+  return launch_after(kern, dim3(units), dim3(warps * 32), smem, stream, 1, true, args...);
 }
 
 // CTA (head, b): the last place, and the pick - 1 largest of the others.
@@ -813,7 +813,7 @@ bool launch_rows_typed(const RowsArgs& a, bool append, dim3 grid, cudaStream_t s
   const auto kern = !append    ? kv_rows_kernel<T, kVec, false, true>
                     : a.bounds ? kv_rows_kernel<T, kVec, true, true>
                                : kv_rows_kernel<T, kVec, true, false>;
-  return launch_after(kern, grid, dim3(kRowsWarps * 32), 0, stream, 1, a);
+  return launch_after(kern, grid, dim3(kRowsWarps * 32), 0, stream, 1, true, a);
 }
 
 int launch_rows(RowsArgs& a, AttnDType dtype, int vec, bool append, cudaStream_t stream) {
@@ -850,7 +850,7 @@ bool negative(const long long* s, int n) {
 
 template <typename T, int kVec, int kPer>
 bool launch_score(const ScoreArgs& a, dim3 grid, cudaStream_t stream) {
-  return launch_after(kv_page_score_kernel<T, kVec, kPer>, grid, dim3(256), 0, stream, 1, a);
+  return launch_after(kv_page_score_kernel<T, kVec, kPer>, grid, dim3(256), 0, stream, 1, true, a);
 }
 
 template <typename T>
@@ -1094,16 +1094,16 @@ extern "C" int launch_kv_evict(const AttnPagedCache* cache, const float* weights
   bool ok;
   switch (cache->dtype) {
     case ATTN_F16:
-      ok = w.vec == 8 ? launch_after(kv_evict_copy_kernel<__half, 8>, grid, block, 0, stream, 1, a)
-                      : launch_after(kv_evict_copy_kernel<__half, 1>, grid, block, 0, stream, 1, a);
+      ok = w.vec == 8 ? launch_after(kv_evict_copy_kernel<__half, 8>, grid, block, 0, stream, 1, true, a)
+                      : launch_after(kv_evict_copy_kernel<__half, 1>, grid, block, 0, stream, 1, true, a);
       break;
     case ATTN_BF16:
-      ok = w.vec == 8 ? launch_after(kv_evict_copy_kernel<__nv_bfloat16, 8>, grid, block, 0, stream, 1, a)
-                      : launch_after(kv_evict_copy_kernel<__nv_bfloat16, 1>, grid, block, 0, stream, 1, a);
+      ok = w.vec == 8 ? launch_after(kv_evict_copy_kernel<__nv_bfloat16, 8>, grid, block, 0, stream, 1, true, a)
+                      : launch_after(kv_evict_copy_kernel<__nv_bfloat16, 1>, grid, block, 0, stream, 1, true, a);
       break;
     default:
-      ok = w.vec == 4 ? launch_after(kv_evict_copy_kernel<float, 4>, grid, block, 0, stream, 1, a)
-                      : launch_after(kv_evict_copy_kernel<float, 1>, grid, block, 0, stream, 1, a);
+      ok = w.vec == 4 ? launch_after(kv_evict_copy_kernel<float, 4>, grid, block, 0, stream, 1, true, a)
+                      : launch_after(kv_evict_copy_kernel<float, 1>, grid, block, 0, stream, 1, true, a);
       break;
   }
   return ok ? ATTN_OK : ATTN_ERR_LAUNCH;

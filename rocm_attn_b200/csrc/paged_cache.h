@@ -60,28 +60,32 @@ __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepco
 // its launch overlaps that work.  The wait ends when the grid before has
 // completed, and so, as that grid waited too, everything before it.  Back to
 // back this hides about a microsecond per kernel.  `cluster` CTAs per cluster
-// (1 or 0: none); clusters are launched after the work before them, since
-// eight CTAs' room at once is hard to find beside it (32 units of 512 tokens:
-// 7.6 us against 9.6 us).
+// (1 or 0: none); `ahead` false launches after the work before it: clusters
+// that need more than half of the GPU, since eight CTAs' room at once is hard to
+// find beside that work (256 CTAs: 7.4 us a call against 9.6 us ahead).
 template <typename... Params, typename... Args>
 bool launch_after(void (*kern)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, int cluster,
-                  const Args&... args) {
-  cudaLaunchAttribute attr;
+                  bool ahead, const Args&... args) {
+  cudaLaunchAttribute attr[2];
+  int n = 0;
   if (cluster > 1) {
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = cluster;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  } else {
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = cluster;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (ahead) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
   if (cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess) return true;
   cudaGetLastError();  // reported by the caller's status
   return false;
