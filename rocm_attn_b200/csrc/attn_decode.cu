@@ -34,11 +34,11 @@
 // attn_decode_simt_kernel (fp32, any D <= 256, any strides).
 //
 // Measured on B200 (calls in a row): 64 sequences of up to 16384 tokens, 64/8
-// heads of 128, fp16, 2.75 GB of K and V: 408 us, 6.75 TB/s, where a copy does
-// 6.54; 24 of up to 4096, 32/8 heads, bf16, with weights: 55 us (floor 41); one
-// of 517 tokens: 7.4 us on the device.  Each call has about 8 us that are
-// not reading: lengths and first look-ups 3, first fill of the rings 2.5, the
-// ends of the runs and the join the rest.
+// heads of 128, fp16, 2.75 GB of K and V: 402 to 430 us by box, 6.4 to 6.8
+// TB/s, where a copy does 6.54; 24 of up to 4096, 32/8 heads, bf16, with
+// weights: 55 us (floor 41); one of 517 tokens: 7.9 us.  A call in two launches
+// has about 8 us that are not reading: lengths and first look-ups 3, first fill
+// of the rings 2.5, the ends of the runs and the join the rest.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -1272,16 +1272,21 @@ Plan make_plan(const AttnPagedCache* c, bool fast, int Hq, int n_pages, bool lis
   if (p.mma) {
     const long long unit_tiles = (capacity + p.tile - 1) / p.tile;
     const long long units = static_cast<long long>(c->B) * c->heads * p.row_tiles;
-    int cl = 1;
-    while (cl < kMaxCluster && cl < unit_tiles && units * cl * 2 <= static_cast<long long>(sms) * per_sm) cl *= 2;
-    // One launch of clusters where a CTA gets at most two tiles, or four if
-    // the clusters leave less than half of the GPU idle; not where units far
-    // outnumber the CTAs that fit, whose set-up would then repeat.  Measured, in
-    // clusters against runs, us: 8 units of 1 tile 4.6 / 6.4, 32 of 8 tiles
-    // 7.4 / 8.2, 32 of 32 tiles 11.3 / 12.2, 512 of 2 tiles 12.5 / 14.0; but 8 of
-    // 32 tiles 10.4 / 9.5, 512 of 8 tiles 27.0 / 25.5, 2048 of 2 tiles 40.7 / 35.2.
     const long long slots = static_cast<long long>(sms) * per_sm;
-    const int most = units * cl * 2 >= slots && units * cl <= slots ? 4 : 2;
+    // One launch of clusters where a CTA gets at most two tiles, or four if
+    // the clusters leave no more than three quarters of the GPU idle; not where
+    // units far outnumber the CTAs that fit, whose set-up would then repeat.
+    // Measured, in clusters against runs, us: 8 units of 1 tile 4.6 / 6.4, 32 of 8
+    // tiles 7.4 / 8.2, 32 of 32 tiles 11.3 / 12.2, 512 of 2 tiles 12.5 / 14.0; but
+    // 8 of 32 tiles 10.4 / 9.5, 512 of 8 tiles 27.0 / 25.5, 2048 of 2 tiles 40.7 /
+    // 35.2.  Clusters grow beyond half of the GPU only for more than four
+    // tiles per CTA, as up to there a call starts beside the one before it: 32
+    // units of 8 tiles, calls in a row, 8.4 us in 128 CTAs, 9.7 us in 256.
+    int cl = 1;
+    while (cl < kMaxCluster && cl < unit_tiles && units * cl * 2 <= slots &&
+           (units * cl * 4 <= slots || unit_tiles > 4 * cl))
+      cl *= 2;
+    const int most = units * cl * 4 >= slots && units * cl <= slots ? 4 : 2;
     if (unit_tiles <= cl * most && units * cl <= 2 * slots) {
       p.cluster = cl;
       grid = units * cl;
