@@ -183,7 +183,8 @@ ATTN_API int attn_library_version(void);
  * until the call's work on `stream` is done; calls that may run at the same
  * time need one each.
  * Limits: 1 <= D <= 256, page_size >= 1, heads >= 1,
- * table_width * page_size <= 2^31 - 65537.
+ * table_width * page_size <= 2^31 - 65537, and for launch_attn_decode as many
+ * tiles of 64 tokens in B * heads sequences of that capacity as fit 31 bits.
  */
 typedef struct AttnPagedCache {
   void* k;

@@ -661,6 +661,146 @@ def test_generation_run(attn):
 
 
 # ---------------------------------------------------------------------------
+# views, empty calls, large batches, captured runs
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+def test_unaligned_views(attn, dtype):
+    # every tensor a view whose rows are not 16-byte aligned, or with gaps between them
+    def odd(t):
+        x = torch.full((*t.shape[:-1], t.shape[-1] + 3), math.nan, dtype=t.dtype, device="cuda")[..., 1:1 + t.shape[-1]]
+        return x.copy_(t)
+
+    lens, D, ps = [70, 33], 64, 16
+    k, v, table, ln = make_cache(lens, 2, D, ps, dtype, spare=9)
+    x, y = torch.randn(2, 2, 5, D).to(dtype), torch.randn(2, 2, 5, D).to(dtype)
+    gk, gv = odd(k), odd(v)
+    bounds = odd(torch.zeros(k.shape[0], 2, 2, D, dtype=dtype))
+    long = torch.tensor([75, 38], dtype=torch.int32)
+    attn.kv_append(odd(x), odd(y), gk, gv, table.cuda(), long.cuda(), bounds=bounds)
+    for b, n in enumerate(lens):
+        for s in range(5):
+            t = n + s
+            k[int(table[b, t // ps]), :, t % ps], v[int(table[b, t // ps]), :, t % ps] = x[b, :, s], y[b, :, s]
+    assert _same(gk, k) and _same(gv, v)
+    attn.kv_page_bounds(gk, table.cuda(), long.cuda(), bounds=bounds)
+    want = bounds_ref(k, table, long, torch.zeros(k.shape[0], 2, 2, D, dtype=dtype))
+    used = torch.cat([table[0, :5], table[1, :3]]).long()
+    assert _same(bounds.cpu()[used], want[used])
+    q = _q(2, 4, D, dtype)
+    pages = attn.kv_select_pages(odd(q), bounds, table.cuda(), long.cuda(), ps, 3)
+    assert torch.equal(pages.cpu(), select_ref(q, want, table, long, ps, 3))
+    _close(attn.attn_decode(odd(q), gk, gv, table.cuda(), long.cuda(), pages=pages),
+           decode_ref(q, k, v, table, long, pages=pages.cpu()), 48, dtype)
+    free = [p for p in range(k.shape[0]) if p not in used.tolist()]
+    new = torch.tensor(free[:4], dtype=torch.int32).reshape(2, 2)
+    w = torch.rand(2, 2, table.shape[1] * ps)
+    kept, _ = evict_ref(w, long, 20, 3)
+    _, _, got = attn.kv_evict(gk, gv, table.cuda(), long.cuda(), odd(w), new.cuda(), 20, recent=3)
+    assert torch.equal(got.cpu(), kept)
+    for b in range(2):
+        for h in range(2):
+            t = kept[b, h].long()
+            assert torch.equal(rows(gk.cpu(), new[b], h, range(20)), rows(k, table[b], h, t))
+            assert torch.equal(rows(gv.cpu(), new[b], h, range(20)), rows(v, table[b], h, t))
+    assert attn.check_status(0) == 0
+
+
+def test_empty_calls(attn):
+    k = torch.zeros(4, 2, 16, 64, dtype=F16, device="cuda")
+    t, n = torch.zeros(0, 3, dtype=torch.int32, device="cuda"), torch.zeros(0, dtype=torch.int32, device="cuda")
+    none = torch.zeros(0, 2, 1, 64, dtype=F16, device="cuda")
+    attn.kv_append(none, none, k, k, t, n)
+    assert (attn.kv_page_bounds(k, t, n) == 0).all()
+    assert attn.kv_select_pages(none, torch.zeros(4, 2, 2, 64, dtype=F16, device="cuda"), t, n, 16, 3).shape == (0, 2, 3)
+    a, b, c = attn.kv_evict(k, k, t, n, torch.zeros(0, 2, 48, device="cuda"), t, 5)
+    assert a.shape == (0,) and b.shape == (0, 2, 48) and c.shape == (0, 2, 5)
+    # no new tokens, and tables without pages
+    t1, n1 = torch.zeros(1, 0, dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    attn.kv_append(none.new_zeros(1, 2, 0, 64), none.new_zeros(1, 2, 0, 64), k, k, t1, n1)
+    assert (attn.kv_page_bounds(k, t1, n1) == 0).all()
+    got = attn.kv_select_pages(none.new_zeros(1, 2, 1, 64), torch.zeros(4, 2, 2, 64, dtype=F16, device="cuda"), t1, n1, 16, 3)
+    assert (got == -1).all()
+    assert attn.check_status(0) == 0
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_more_sequences_than_a_grid_dimension(attn, dtype):
+    B, D, ps = 70001, 8, 4
+    k, v = (torch.randn(B, 1, ps, D, device="cuda").to(dtype) for _ in range(2))
+    table = torch.randperm(B, device="cuda").to(torch.int32)[:, None]
+    lens = torch.ones(B, dtype=torch.int32, device="cuda")
+    lens[5::7] = 0
+    x, y = (torch.randn(B, 1, 1, D, device="cuda").to(dtype) for _ in range(2))
+    bounds = torch.zeros(B, 1, 2, D, dtype=dtype, device="cuda")
+    attn.kv_append(x, y, k, v, table, lens, bounds=bounds)
+    page, live = table[:, 0].long(), lens > 0
+    assert torch.equal(k[page[live], 0, 0], x[live, 0, 0]) and torch.equal(bounds[page[live], 0, 1], x[live, 0, 0])
+    assert torch.equal(attn.kv_page_bounds(k, table, lens), bounds)
+    out = attn.attn_decode(torch.randn(B, 2, 1, D, device="cuda").to(dtype), k, v, table, lens)
+    assert torch.equal(out[live], y[live].expand(-1, 2, 1, D)) and (out[~live] == 0).all()  # one token has all the weight
+    pages = attn.kv_select_pages(out, bounds, table, lens, ps, 1)
+    assert torch.equal(pages[:, 0, 0] == 0, live)
+    new = torch.arange(B, dtype=torch.int32, device="cuda")[:, None]
+    k2, v2 = torch.cat([k, k * 0]), torch.cat([v, v * 0])
+    n, w, kept = attn.kv_evict(k2, v2, table, lens, torch.ones(B, 1, ps, device="cuda"), new + B, 2)
+    assert torch.equal(n, lens) and torch.equal(kept[:, 0, 0] == 0, live) and (kept[:, 0, 1] == -1).all()
+    assert torch.equal(k2[B:][live, 0, 0], x[live, 0, 0]) and torch.equal(v2[B:][live, 0, 0], y[live, 0, 0])
+    assert attn.check_status(0) == 0
+
+
+def test_captured_steps(attn):
+    # append, weights and eviction captured together and replayed on new values, lengths and pages
+    lens, D, ps, budget = [90, 41], 64, 16, 40
+    k, v, table, ln = make_cache(lens, 2, D, ps, F16, spare=20, poison=False)
+    free = [p for p in range(k.shape[0]) if p not in table.flatten().tolist()]
+    new = torch.tensor(free[:6], dtype=torch.int32).reshape(2, 3)
+    gk, gv, gt, gl, gn = k.cuda(), v.cuda(), table.cuda(), ln.cuda(), new.cuda()
+    x, y = torch.randn(2, 2, 1, D).to(F16), torch.randn(2, 2, 1, D).to(F16)
+    q = _q(2, 4, D, F16)
+    gx, gy, gq = x.cuda(), y.cuda(), q.cuda()
+    w = torch.zeros(2, 2, table.shape[1] * ps, device="cuda")
+
+    def step():
+        attn.kv_append(gx, gy, gk, gv, gt, gl)
+        out = attn.attn_decode(gq, gk, gv, gt, gl, weights=w)
+        return out, attn.kv_evict(gk, gv, gt, gl, w, gn, budget, recent=4)
+
+    step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out, (n2, w2, kept) = step()
+    for i, n in enumerate(([90, 41], [17, 90], [64, 1])):
+        x, y, q = torch.randn(2, 2, 1, D).to(F16), torch.randn(2, 2, 1, D).to(F16), _q(2, 4, D, F16, seed=i)
+        now = torch.tensor(n, dtype=torch.int32)
+        full = torch.tensor([p for p in range(k.shape[0]) if p not in new.flatten().tolist()])
+        table = full[torch.randperm(len(full))[:2 * table.shape[1]]].reshape(2, -1).to(torch.int32)
+        gk.copy_(k), gv.copy_(v), gx.copy_(x), gy.copy_(y), gq.copy_(q), gl.copy_(now), gt.copy_(table)
+        start = torch.rand(w.shape)
+        w.copy_(start)
+        g.replay()
+        torch.cuda.synchronize()
+        kk, vv = k.clone(), v.clone()
+        for b in range(2):
+            t = n[b] - 1
+            kk[int(table[b, t // ps]), :, t % ps], vv[int(table[b, t // ps]), :, t % ps] = x[b, :, 0], y[b, :, 0]
+        ref = decode_ref(q, kk, vv, table, now)
+        _close(out, ref, 90, F16)
+        # the bound of test_decode_weights: 2 (68 2^-23 5 + 2^-21 + 90 2^-23) of a weight of at most 1
+        assert torch.allclose(w.cpu().double(), start.double() + ref[3], rtol=0, atol=1e-4 * 2)
+        want, lens2 = evict_ref(w.cpu(), now, budget, 4)
+        assert torch.equal(kept.cpu(), want) and torch.equal(n2.cpu(), lens2.int())
+        for b in range(2):
+            for h in range(2):
+                m = int(lens2[b])
+                assert torch.equal(rows(gk.cpu(), new[b], h, range(m)), rows(kk, table[b], h, want[b, h, :m].long()))
+                assert torch.equal(w2[b, h, :m].cpu(), w.cpu()[b, h][want[b, h, :m].long()])
+    assert attn.check_status(0) == 0
+
+
+# ---------------------------------------------------------------------------
 # the watchdog (tests/test_watchdog_gpu.py says how the test build works)
 # ---------------------------------------------------------------------------
 
