@@ -217,8 +217,9 @@ typedef struct AttnPagedCache {
  *        together with `pages` (ATTN_ERR_UNSUPPORTED).
  * softmax_scale as in launch_attn_forward.  With weights the workspace holds
  * the scores, 4 * B * Hq * table_width * page_size bytes; without, it does not
- * grow with the lengths (and may be empty: the pointer is then only checked). `listed` tells the workspace call
- * whether `pages` will be given, `weights` whether weights will be.
+ * grow with the lengths and may be empty (the pointer is then only checked).
+ * `listed` tells the workspace call whether `pages` will be given, `weights`
+ * whether weights will be.
  */
 ATTN_API int attn_decode_workspace_bytes(const AttnPagedCache* cache, int Hq, bool listed, int n_pages, bool weights,
                                          size_t* bytes);

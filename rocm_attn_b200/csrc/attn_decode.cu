@@ -1315,7 +1315,7 @@ int check_decode(const AttnPagedCache* c, int Hq, const void* pages, int n_pages
   const int st = check_paged_cache(c, kCacheK | kCacheV, view);
   if (st != ATTN_OK) return st;
   if (Hq < 0 || n_pages < 0) return ATTN_ERR_INVALID_ARGUMENT;
-  if (c->heads == 0 ? Hq != 0 : Hq % c->heads != 0) return ATTN_ERR_INVALID_ARGUMENT;
+  if (Hq % c->heads != 0) return ATTN_ERR_INVALID_ARGUMENT;
   if (static_cast<long long>(c->B) * Hq > 0x7fffffffLL) return ATTN_ERR_INVALID_ARGUMENT;
   if (static_cast<long long>(n_pages) * c->page_size > kMaxCapacity) return ATTN_ERR_INVALID_ARGUMENT;
   if (pages && weights) return ATTN_ERR_UNSUPPORTED;
