@@ -150,12 +150,14 @@ __global__ void __launch_bounds__(kRowsWarps * 32) kv_rows_kernel(const __grid_c
     fault |= kFaultPage;
     len = cap;
   }
-  int page = -1, lp = 0;
+  int page = -1;
   long long base = 0;
   if (first < len) {
-    lp = static_cast<int>(first) / ps + run;
-    base = static_cast<long long>(lp) * ps;
-    if (base < len) page = paged_page(a.c, b, lp, &fault);
+    // 64 bits: fewer tokens may be new than there is room for in `runs` pages,
+    // and the pages behind the last new one may lie past 2^31.
+    const long long lp = static_cast<long long>(static_cast<int>(first) / ps) + run;
+    base = lp * ps;
+    if (base < len) page = paged_page(a.c, b, static_cast<int>(lp), &fault);
   }
   if (fault && lane == 0) atomicOr(&g_page_fault, fault);
   if (page < 0) return;

@@ -1,0 +1,37 @@
+"""The paged key-value cache operators at the ends of what their documentation
+allows: the largest tables, scores and weights at the ends of their types'
+ranges, work on several streams, captured runs."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+
+MAX_CAPACITY = 2 ** 31 - 65537  # tokens a block table may name
+
+
+def _wide_table():
+    """A block table of one sequence, pages of one token, as wide as allowed (8.6 GB): page 0 throughout."""
+    return torch.zeros(1, MAX_CAPACITY, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("D", [8, 5])
+def test_append_at_the_end_of_the_widest_table(attn, D):
+    # one new token where 131072 are offered: the pages of the others would lie behind position 2^31
+    S = 131072
+    table = _wide_table()
+    table[0, -S:] = torch.arange(1, S + 1, dtype=torch.int32, device="cuda")
+    lens = torch.tensor([MAX_CAPACITY], dtype=torch.int32, device="cuda")
+    new = torch.ones(1, dtype=torch.int32, device="cuda")
+    k, v = (torch.randn(1, 1, S, D, device="cuda").to(F16) for _ in range(2))
+    kc, vc = (torch.zeros(S + 2, 1, 1, D, dtype=F16, device="cuda") for _ in range(2))
+    attn.kv_append(k, v, kc, vc, table, lens, new_lens=new)
+    for c, x in ((kc, k), (vc, v)):
+        assert torch.equal(c[S, 0, 0], x[0, 0, 0])
+        assert (c[:S] == 0).all() and (c[S + 1] == 0).all()
+    attn.kv_append(k, v, kc, vc, table, lens)  # all of them new
+    for c, x in ((kc, k), (vc, v)):
+        assert torch.equal(c[1:S + 1, 0, 0], x[0, 0])
+        assert (c[0] == 0).all() and (c[S + 1] == 0).all()
+    assert attn.check_status(0) == 0
