@@ -669,7 +669,9 @@ __global__ void __launch_bounds__(kWarps * 32)
   const unsigned long long* k = keys + (static_cast<long long>(b) * c.heads + h) * c.table_width;
   int* out = pages + (static_cast<long long>(b) * c.heads + h) * top;
   if (n <= top) {
-    for (int i = threadIdx.x; i < top; i += kWarps * 32) out[i] = i < n ? i : -1;
+    // unsigned: `top` may be the largest int, and a step past it must not wrap
+    for (unsigned i = threadIdx.x; i < static_cast<unsigned>(top); i += kWarps * 32)
+      out[i] = i < static_cast<unsigned>(n) ? static_cast<int>(i) : -1;
     return;
   }
   if (threadIdx.x == 0) out[top - 1] = n - 1;

@@ -35,3 +35,18 @@ def test_append_at_the_end_of_the_widest_table(attn, D):
         assert torch.equal(c[1:S + 1, 0, 0], x[0, 0])
         assert (c[0] == 0).all() and (c[S + 1] == 0).all()
     assert attn.check_status(0) == 0
+
+
+@pytest.mark.parametrize("width", [4, 5000])
+def test_select_of_the_longest_list(attn, width):
+    # the list's length is the largest int: the pages there are, and -1 to its end
+    top = 2 ** 31 - 1
+    table = torch.zeros(1, width, dtype=torch.int32, device="cuda")
+    lens = torch.tensor([3 * 16], dtype=torch.int32, device="cuda")
+    bounds = torch.zeros(1, 1, 2, 8, dtype=F16, device="cuda")
+    q = torch.ones(1, 1, 1, 8, dtype=F16, device="cuda")
+    pages = attn.kv_select_pages(q, bounds, table, lens, 16, top)
+    assert pages.shape == (1, 1, top)
+    assert pages[0, 0, :4].tolist() == [0, 1, 2, -1]
+    assert int(pages[0, 0, 3:].max()) == -1 and int(pages[0, 0, 3:].min()) == -1
+    assert attn.check_status(0) == 0
