@@ -330,7 +330,7 @@ __global__ void __launch_bounds__(256, kPer == 1 ? 3 : 1) kv_page_score_kernel(c
   int fault = 0;
   const int len = paged_len(a.c, b, &fault);
   const int pages = static_cast<int>((static_cast<long long>(len) + a.c.page_size - 1) / a.c.page_size);
-  const int first = chunk * a.pages, last = min(pages, first + a.pages);
+  const int first = chunk * a.pages, last = first + min(pages - first, a.pages);  // first < table_width
   if (first < last) {
     // Page ids of the next 16 turns, one per lane of the page's lanes.
     auto look_up = [&](int p0) {
@@ -998,12 +998,12 @@ extern "C" int launch_kv_select_pages(const AttnPagedCache* cache, const void* q
   const long long units = static_cast<long long>(cache->B) * cache->heads;
   // Pages per CTA: as many as leave four CTAs per SM, three of which run at
   // once (32 contexts of 1024 pages: 34.8 us with eight, 32.9 us with four).
+  // In 64 bits: the width rounded up can pass 2^31.
   const long long wanted = units < 148 * 4 ? 148 * 4 / units : 1;
   constexpr int kTurns = 4 * kScoreSlots;
-  const int per = static_cast<int>(((cache->table_width + wanted - 1) / wanted + kTurns - 1) / kTurns * kTurns);
-  const int chunks = per > 0 ? (cache->table_width + per - 1) / per : 0;
-  if (units > 0x7fffffffLL || static_cast<long long>(cache->B) * chunks > 0x7fffffffLL)
-    return ATTN_ERR_INVALID_ARGUMENT;
+  const long long per = ((cache->table_width + wanted - 1) / wanted + kTurns - 1) / kTurns * kTurns;
+  const long long chunks = per > 0 ? (cache->table_width + per - 1) / per : 0;
+  if (units > 0x7fffffffLL || cache->B * chunks > 0x7fffffffLL) return ATTN_ERR_INVALID_ARGUMENT;
   const long long contiguous[2] = {static_cast<long long>(Hq) * cache->D, cache->D};
   const long long* qs = q_strides ? q_strides : contiguous;
   if ((Hq > 0 && !q) || !pages || (cache->num_pages > 0 && !bounds) || !bounds_strides || negative(bounds_strides, 3) ||
@@ -1027,10 +1027,10 @@ extern "C" int launch_kv_select_pages(const AttnPagedCache* cache, const void* q
   a.bounds = bounds;
   a.b_p = bounds_strides[0], a.b_h = bounds_strides[1], a.b_m = bounds_strides[2];
   a.keys = static_cast<unsigned long long*>(workspace);
-  a.chunks = chunks;
-  a.pages = per;
+  a.chunks = static_cast<int>(chunks);
+  a.pages = static_cast<int>(per);  // kTurns divides 2^31 - 65536, the widest table and one, so this fits too
   if (chunks > 0) {
-    const dim3 grid(static_cast<unsigned>(cache->B) * chunks, cache->heads);
+    const dim3 grid(static_cast<unsigned>(cache->B * chunks), cache->heads);
     bool ok;
     switch (cache->dtype) {
       case ATTN_F16: ok = launch_score_typed<__half>(a, w.vec, grid, stream); break;

@@ -50,3 +50,22 @@ def test_select_of_the_longest_list(attn, width):
     assert pages[0, 0, :4].tolist() == [0, 1, 2, -1]
     assert int(pages[0, 0, 3:].max()) == -1 and int(pages[0, 0, 3:].min()) == -1
     assert attn.check_status(0) == 0
+
+
+@pytest.mark.parametrize("lens", [[5000], [MAX_CAPACITY], [MAX_CAPACITY, 40, MAX_CAPACITY - 3]], ids=str)
+def test_select_from_the_widest_table(attn, lens):
+    # pages of one token; scores 0 but for a few pages up to the end (8 bytes of scratch memory a table entry)
+    B, D = len(lens), 8
+    table = _wide_table().expand(B, -1)
+    places = [3, 17, 4990, 10 ** 9, MAX_CAPACITY - 40, MAX_CAPACITY - 5]
+    table[0, places] = torch.arange(1, len(places) + 1, dtype=torch.int32, device="cuda")
+    bounds = torch.zeros(len(places) + 1, 1, 2, D, dtype=F16, device="cuda")
+    bounds[1:, 0, 1] = 1
+    q = torch.ones(B, 1, 1, D, dtype=F16, device="cuda")
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    pages = attn.kv_select_pages(q, bounds, table, n, 1, 8)
+    for b, length in enumerate(lens):
+        best = [p for p in places if p < length - 1]
+        rest = [p for p in range(20) if p not in best][:7 - len(best)]  # ties to the lower page
+        assert pages[b, 0].tolist() == sorted(best + rest) + [length - 1]
+    assert attn.check_status(0) == 0
