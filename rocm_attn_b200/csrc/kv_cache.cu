@@ -999,7 +999,7 @@ extern "C" int launch_kv_select_pages(const AttnPagedCache* cache, const void* q
   // Pages per CTA: as many as leave four CTAs per SM, three of which run at
   // once (32 contexts of 1024 pages: 34.8 us with eight, 32.9 us with four).
   // In 64 bits: the width rounded up can pass 2^31.
-  const long long wanted = units < 148 * 4 ? 148 * 4 / units : 1;
+  const long long target = 4LL * sm_count(), wanted = units < target ? target / units : 1;
   constexpr int kTurns = 4 * kScoreSlots;
   const long long per = ((cache->table_width + wanted - 1) / wanted + kTurns - 1) / kTurns * kTurns;
   const long long chunks = per > 0 ? (cache->table_width + per - 1) / per : 0;
