@@ -206,7 +206,7 @@ typedef struct AttnPagedCache {
  *        contiguous; Hq a multiple of cache->heads, query heads
  *        [h * Hq / heads, (h + 1) * Hq / heads) read kv head h
  *   out  [B, Hq, D] contiguous, fully overwritten; zeros for a sequence with
- *        no token
+ *        no token (one whose every score is -inf gives NaN, as the formula)
  *   pages  null, or int32 [B, heads, n_pages]: only the tokens of these logical
  *        pages (t / page_size) are attended to.  Entries that name no page of
  *        the sequence (such as -1) add nothing, one named twice counts twice.

@@ -4,7 +4,8 @@
 // For sequence b, query head i of the g heads that read kv head h, and the
 // tokens t of the sequence (all of them, or those of the listed pages):
 //   x_t = scale * log2(e) * (q_i . k_t),  M = max x_t,  L = sum 2^(x_t - M),
-//   o_i = sum 2^(x_t - M) v_t / L,  and 0 where L is 0 (no token),
+//   o_i = sum 2^(x_t - M) v_t / L,  and 0 where there is no token
+//   (where there are tokens and every x_t is -inf, 0 / 0: NaN, as the formula),
 //   weights[b, h, t] += sum_i 2^(x_t - M_i - log2 L_i)   when asked for.
 //
 // Every K and V element is used by the g query heads of one token only, so up
@@ -139,6 +140,21 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(flo
 
 // 2^(x - m) for a running maximum that may still be -inf (no token yet).
 __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.f : m; }
+
+// The running maximum of tokens starts here, below which only -inf lies, so
+// that M = -inf says that there is no token (the result is 0), and a sum of 0
+// beside another M that all scores are -inf (the result is 0 / 0).
+constexpr float kLowest = -3.402823466e38f;
+__device__ __forceinline__ float quotient(float sum, float M, float L) {
+  return L == 0.f && M == -INFINITY ? 0.f : sum / L;
+}
+__device__ __forceinline__ float inverse(float M, float L) {
+  return L != 0.f ? 1.f / L : M == -INFINITY ? 0.f : __int_as_float(0x7fffffff);
+}
+// log2 of the sum, for the weights: 2^(x - this) is 0, or NaN.
+__device__ __forceinline__ float log2_sum(float M, float L) {
+  return L != 0.f ? M + log2f(L) : M == -INFINITY ? INFINITY : __int_as_float(0x7fffffff);
+}
 
 // ---------------------------------------------------------------------------
 // The run of tiles of one CTA
@@ -715,10 +731,9 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-              const float mn = fmaxf(m[t][e], mx);
-              top[e] = finite_max(mn);
+              top[e] = fmaxf(fmaxf(m[t][e], mx), kLowest);  // there is a token among the 16
               f[e] = ex2_approx(m[t][e] - top[e]);
-              m[t][e] = mn;
+              m[t][e] = top[e];
             }
             if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
               l[t][0] *= f[0];
@@ -807,11 +822,11 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
               sum.w += y.w * f;
             }
             if (p.whole) {
-              const float inv = L == 0.f ? 0.f : 1.f / L;
+              const float inv = inverse(M, L);
               T* out = static_cast<T*>(a.out) + (p.row0 + r) * a.c.D + c4 * 4;
               *reinterpret_cast<uint2*>(out) =
                   make_uint2(pack2<kBf16>(sum.x * inv, sum.y * inv), pack2<kBf16>(sum.z * inv, sum.w * inv));
-              if (kWeights && c4 == 0) a.lse2[p.row0 + r] = L == 0.f ? INFINITY : M + log2f(L);
+              if (kWeights && c4 == 0) a.lse2[p.row0 + r] = log2_sum(M, L);
             } else if (a.cluster) {
               // kept for the cluster in the other chunk of warp 0 (or 1), which is free: there are no more tiles
               *reinterpret_cast<float4*>(cluster_part(r) + c4 * 4) = sum;
@@ -871,11 +886,11 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
           sum.w += ys[w].w * f;
         }
       }
-      const float inv = L == 0.f ? 0.f : 1.f / L;
+      const float inv = inverse(M, L);
       T* out = static_cast<T*>(a.out) + (unit_row0 + r) * a.c.D + c4 * 4;
       *reinterpret_cast<uint2*>(out) =
           make_uint2(pack2<kBf16>(sum.x * inv, sum.y * inv), pack2<kBf16>(sum.z * inv, sum.w * inv));
-      if (kWeights && c4 == 0) a.lse2[unit_row0 + r] = L == 0.f ? INFINITY : M + log2f(L);
+      if (kWeights && c4 == 0) a.lse2[unit_row0 + r] = log2_sum(M, L);
     }
     cluster_sync();
   } else if (a.cluster == 1 && n == 0) {
@@ -1025,10 +1040,11 @@ __global__ void __launch_bounds__(kThreads, SimtCfg<kPer, kRows>::kCtas)
         }
 #pragma unroll
         for (int rest = kSame / 2; rest > 0; rest >>= 1) s[0] += __shfl_xor_sync(0xffffffffu, s[0], rest);
-        const float x = (mask >> (k0 + my_key) & 1u) ? s[0] * a.scale_log2 : -INFINITY;
+        const bool is = mask >> (k0 + my_key) & 1u;
+        const float x = is ? s[0] * a.scale_log2 : -INFINITY;
         if (kWeights && my_row < rows && lane % kSame == 0)
           a.x[(row0 + my_row) * a.x_stride + pos0 + k0 + my_key] = x;
-        float mx = x;
+        float mx = is ? fmaxf(x, kLowest) : -INFINITY;
 #pragma unroll
         for (int w = kSame; w < kRowLanes; w <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
         const float mn = fmaxf(m, mx);
@@ -1077,8 +1093,8 @@ __global__ void __launch_bounds__(kThreads, SimtCfg<kPer, kRows>::kCtas)
           sum += s_o[w][r][d] * f;
         }
         if (p.whole) {
-          static_cast<T*>(a.out)[(p.row0 + r) * a.c.D + d] = from_f32<T>(L == 0.f ? 0.f : sum / L);
-          if (kWeights && d == 0) a.lse2[p.row0 + r] = L == 0.f ? INFINITY : M + log2f(L);
+          static_cast<T*>(a.out)[(p.row0 + r) * a.c.D + d] = from_f32<T>(quotient(sum, M, L));
+          if (kWeights && d == 0) a.lse2[p.row0 + r] = log2_sum(M, L);
         } else {
           const long long at = static_cast<long long>(p.slot) * a.rows + r;
           a.part_o[at * a.D4 + d] = sum;
@@ -1198,8 +1214,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_decode_join_kernel(const
 #pragma unroll
   for (int w = 0; w < kJoinWarps; ++w) sum += reinterpret_cast<const float*>(s_o[w])[d];
   const long long row = meta.x + r;
-  static_cast<T*>(a.out)[row * a.c.D + d] = from_f32<T>(L == 0.f ? 0.f : sum / L);
-  if (a.lse2 && d == 0) a.lse2[row] = L == 0.f ? INFINITY : M + log2f(L);
+  static_cast<T*>(a.out)[row * a.c.D + d] = from_f32<T>(quotient(sum, M, L));
+  if (a.lse2 && d == 0) a.lse2[row] = log2_sum(M, L);
 }
 
 // weights[b, h, t] += sum over the group of 2^(x_t - lse2), one thread per

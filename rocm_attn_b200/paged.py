@@ -40,7 +40,8 @@ def attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, b
 
     q: ``[B, Hq, 1, D]`` in the cache's type, Hq a multiple of Hkv (query heads
     ``h * Hq // Hkv`` and following read kv head ``h``).  ``scale`` defaults to
-    1/sqrt(D).  Returns O ``[B, Hq, 1, D]``; an empty sequence gives zeros.
+    1/sqrt(D).  Returns O ``[B, Hq, 1, D]``; an empty sequence gives zeros, one
+    that has tokens and only scores of -inf NaN, as the formula does.
 
     pages: optional int32 ``[B, Hkv, n]`` of logical pages (``t // page_size``),
     as ``kv_select_pages`` returns: only their tokens are attended to.  Entries

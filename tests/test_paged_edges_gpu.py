@@ -1,8 +1,12 @@
 """The paged key-value cache operators at the ends of what their documentation
 allows: the largest tables, scores and weights at the ends of their types'
 ranges, work on several streams, captured runs."""
+import math
+
 import pytest
 import torch
+
+from paged_ref import decode_ref, decode_tolerance, make_cache
 
 pytestmark = pytest.mark.gpu
 
@@ -68,4 +72,48 @@ def test_select_from_the_widest_table(attn, lens):
         best = [p for p in places if p < length - 1]
         rest = [p for p in range(20) if p not in best][:7 - len(best)]  # ties to the lower page
         assert pages[b, 0].tolist() == sorted(best + rest) + [length - 1]
+    assert attn.check_status(0) == 0
+
+
+def _q(B, Hq, D, dtype, seed=1):
+    return torch.randn(B, Hq, 1, D, generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("D", [64, 128, 256, 33])
+@pytest.mark.parametrize("width", [None, 900])  # one launch, and runs over the whole grid
+@pytest.mark.parametrize("lens", [[1, 16, 70, 0, 150], [3000, 5, 700, 0, 40]], ids=str)
+def test_every_score_minus_infinity(attn, lens, width, D, dtype):
+    # The formula's 0 / 0 where all of a sequence's scores are -inf, zeros only where there is no token; a part
+    # of them weighs nothing.  Of five sequences: all -inf, the first 5 finite, all but the last -inf, empty,
+    # all -inf for kv head 0 alone.
+    k, v, table, ln = make_cache(lens, 2, D, 16, dtype, width=width)
+    q = _q(5, 6, D, dtype).abs() + 0.1
+    ps = 16
+    for b, heads, gone in ((0, (0, 1), range(lens[0])), (1, (0, 1), range(5, lens[1])), (2, (0, 1), range(lens[2] - 1)),
+                           (4, (0,), range(lens[4]))):
+        for t in gone:
+            k[int(table[b, t // ps]), list(heads), t % ps, D // 2] = -math.inf
+    args = tuple(t.cuda() for t in (q, k, v, table, ln))
+    o, absum, smax, w = decode_ref(q, k, v, table, ln)
+    assert o[0].isnan().all() and o[4, :3].isnan().all() and not o[1:4].isnan().any() and not o[4, 3:].isnan().any()
+    # the bound from the finite scores: what weighs nothing adds nothing
+    k0 = k.masked_fill(k == -math.inf, 0.0)
+    smax = decode_ref(q, k0, v, table, ln)[2]
+    tol = decode_tolerance(o, absum, smax, max(lens), D, dtype)
+    cap = table.shape[1] * ps
+    weights = torch.zeros(5, 2, cap, device="cuda")
+    pages = torch.arange(table.shape[1], dtype=torch.int32).expand(5, 2, -1).contiguous().cuda()
+    for out in (attn.attn_decode(*args), attn.attn_decode(*args, pages=pages), attn.attn_decode(*args, weights=weights)):
+        out = out.cpu().double()
+        assert torch.equal(out.isnan(), o.isnan())
+        ok = ~o.isnan()
+        assert ((out - o).abs() <= tol)[ok].all()
+        assert (out[3] == 0).all()
+    got = weights.cpu()
+    assert torch.equal(got.isnan(), w.isnan())
+    # a weight's bound, as in the tests of the weights: a score's exponential and the denominator, summed over 3 heads
+    rel = 2 * ((D + 4) * 2.0 ** -23 * float(smax.max()) + 2.0 ** -21 + max(lens) * 2.0 ** -23) + 4 * 2.0 ** -24
+    ok = ~w.isnan()
+    assert ((got.double() - w).abs() <= rel * w)[ok].all()
     assert attn.check_status(0) == 0
