@@ -608,7 +608,8 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
   int stage = 0;
 
   // Scores of tokens lane / 4 + {0, 8} of the chunk's g-th 16 and of two heads
-  // of column tile t, for the weights.
+  // of column tile t, for the weights: -inf where there is no token, and a
+  // token's own -inf as the lowest finite value, which weighs nothing either.
   auto keep_scores = [&](int t, int g, float x0, float x1, float y0, float y1) {
     const int rows = min(a.rows, a.group - cur.rt * a.rows), r = t * 8 + (lane & 3) * 2;
     const long long row0 = static_cast<long long>(cur.b) * a.Hq + cur.h * a.group + cur.rt * a.rows;
@@ -723,7 +724,13 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
               for (int e = 0; e < 4; ++e)
                 if (!(live >> ((e >> 1) * 8 + (lane >> 2)) & 1u)) s[t][e] = -INFINITY;
             }
-            if constexpr (kWeights) keep_scores(t, g, s[t][0], s[t][1], s[t][2], s[t][3]);
+            if constexpr (kWeights) {
+              float x[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                x[e] = live >> ((e >> 1) * 8 + (lane >> 2)) & 1u ? fmaxf(s[t][e], kLowest) : -INFINITY;
+              keep_scores(t, g, x[0], x[1], x[2], x[3]);
+            }
             float f[2], top[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
@@ -1042,9 +1049,9 @@ __global__ void __launch_bounds__(kThreads, SimtCfg<kPer, kRows>::kCtas)
         for (int rest = kSame / 2; rest > 0; rest >>= 1) s[0] += __shfl_xor_sync(0xffffffffu, s[0], rest);
         const bool is = mask >> (k0 + my_key) & 1u;
         const float x = is ? s[0] * a.scale_log2 : -INFINITY;
+        float mx = is ? fmaxf(x, kLowest) : -INFINITY;  // what the weights keep: -inf is an absent token alone
         if (kWeights && my_row < rows && lane % kSame == 0)
-          a.x[(row0 + my_row) * a.x_stride + pos0 + k0 + my_key] = x;
-        float mx = is ? fmaxf(x, kLowest) : -INFINITY;
+          a.x[(row0 + my_row) * a.x_stride + pos0 + k0 + my_key] = mx;
 #pragma unroll
         for (int w = kSame; w < kRowLanes; w <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
         const float mn = fmaxf(m, mx);
@@ -1232,7 +1239,10 @@ __global__ void __launch_bounds__(256) attn_decode_weights_kernel(const __grid_c
   const long long r0 = static_cast<long long>(b) * a.Hq + static_cast<long long>(h) * a.group;
   float sum = 0.f;
 #pragma unroll 4
-  for (int g = 0; g < a.group; ++g) sum += ex2_approx(a.x[(r0 + g) * a.x_stride + t] - a.lse2[r0 + g]);
+  for (int g = 0; g < a.group; ++g) {
+    const float x = a.x[(r0 + g) * a.x_stride + t], p = ex2_approx(x - a.lse2[r0 + g]);
+    sum += x == -INFINITY ? 0.f : p;  // an absent token gets nothing, not even of a sum that is NaN
+  }
   float* w = weights + b * w_b + h * w_h + t;
   *w += sum;
 }

@@ -117,3 +117,24 @@ def test_every_score_minus_infinity(attn, lens, width, D, dtype):
     ok = ~w.isnan()
     assert ((got.double() - w).abs() <= rel * w)[ok].all()
     assert attn.check_status(0) == 0
+
+
+@pytest.mark.parametrize("dtype,D", [(F16, 64), (BF16, 128), (BF16, 256), (F32, 64), (F16, 33)])
+@pytest.mark.parametrize("width", [None, 900])
+def test_weights_of_absent_tokens_beside_nan(attn, dtype, D, width):
+    # a sequence whose softmax is NaN: its tokens' weights are NaN, those of tokens in a page outside the cache stay
+    k, v, table, ln = make_cache([100, 100], 2, D, 16, dtype, width=width)
+    q = _q(2, 6, D, dtype)
+    k[int(table[0, 1]), 0, 7, 3] = math.nan
+    table[0, 3], table[1, 3] = -1, 2 ** 30
+    start = torch.rand(2, 2, table.shape[1] * 16, generator=torch.Generator().manual_seed(4))
+    w = start.cuda()
+    attn.attn_decode(q.cuda(), k.cuda(), v.cuda(), table.cuda(), ln.cuda(), weights=w)
+    w = w.cpu()
+    live = torch.ones(100, dtype=torch.bool)
+    live[48:64] = False
+    assert w[0, 0, :100][live].isnan().all()
+    assert torch.equal(w[0, 0, 48:64], start[0, 0, 48:64])
+    assert (w[0, 1, :100][live] > start[0, 1, :100][live]).any() and not w[0, 1].isnan().any()
+    assert torch.equal(w[1, :, 48:64], start[1, :, 48:64]) and torch.equal(w[:, :, 100:], start[:, :, 100:])
+    assert attn.check_status(0) == 8
