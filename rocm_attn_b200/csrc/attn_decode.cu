@@ -424,6 +424,12 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
   constexpr int kCols = kD / 8;                // 16-byte columns of a row
   constexpr int kSteps = kD / 16;              // 16-wide steps of the head dim
   constexpr int kRowsPerCopy = 32 / kCols;     // rows of one 16-byte copy of the warp
+  // A warp's weights, and so its L and O, are kept times this power of two:
+  // fp16 ends 2^-14 below 1 with its full precision and 2^-25 below with all,
+  // and tokens beside one that takes nearly everything lie there.  With it
+  // weights down to 2^-29 of the largest keep their bits, and those from 2^-40
+  // on still count.
+  constexpr float kUp = kBf16 ? 1.f : 32768.f;
 
   extern __shared__ __align__(1024) unsigned char smem[];
   __shared__ ScheduleSmem s_sched;
@@ -753,10 +759,10 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
                 o[t][j][3] *= f[1];
               }
             }
-            // P is rounded to the input type for P V (half a step, 2^-9 or 2^-12
-            // of each weight); its sum is taken before the rounding.
+            // P is rounded to the input type for P V, by half a step (2^-8 or
+            // 2^-11 of each weight) at most; its sum is taken before that.
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[t][e] = ex2_approx(s[t][e] - top[e & 1]);
+            for (int e = 0; e < 4; ++e) s[t][e] = ex2_approx(s[t][e] - top[e & 1]) * kUp;
             l[t][0] += s[t][0] + s[t][2];
             l[t][1] += s[t][1] + s[t][3];
             pf[t][0] = transpose_8x8(pack2<kBf16>(s[t][0], s[t][1]));
@@ -818,7 +824,7 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
             float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
-              const float f = ex2_approx(s_m[w][r] - finite_max(M));
+              const float f = ex2_approx(s_m[w][r] - finite_max(M)) * (1.f / kUp);
               const float4 y = *reinterpret_cast<const float4*>(
                   reinterpret_cast<const float*>(smem + (w * kStages + stage) * C::kStageBytes) + at * kD +
                   ((c4 ^ ((at >> 1 & 3) << 1)) << 2));

@@ -92,6 +92,23 @@ def decode_tolerance(o, absum, smax, n, D, dtype):
     return tol
 
 
+def decode_bound(o, absum, smax, n, D, dtype, vmax=0.0):
+    """Elementwise bound of |kernel - o| that holds for small weights too: decode_tolerance with the fp16
+    kernel's own ends of P.
+
+    It keeps P times 2^15, so that weights from 2^-29 of the largest of their warp on are normal numbers and
+    off by half a step; smaller ones are off by at most 2^-25 2^-15 = 2^-40 of the largest, each times its |v| <=
+    vmax (0: there are none).  O is rounded to the output type, subnormals of fp16 by 2^-25."""
+    half = torch.finfo(dtype).eps / 2
+    rel = 2 * ((D + 4) * 2.0 ** -23 * smax + 2.0 ** -21 + n * 2.0 ** -23)
+    tol = rel * absum + half * o.abs() + 1e-30
+    if dtype != torch.float32:
+        tol = tol + half * absum * (1 + rel)
+    if dtype == torch.float16:
+        tol = tol + n * 2.0 ** -40 * vmax + 2.0 ** -25
+    return tol
+
+
 def bounds_ref(k, table, lens, out):
     ps = k.shape[2]
     for b in range(table.shape[0]):

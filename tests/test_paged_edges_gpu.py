@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from paged_ref import decode_ref, decode_tolerance, make_cache
+from paged_ref import decode_bound, decode_ref, decode_tolerance, make_cache
 
 pytestmark = pytest.mark.gpu
 
@@ -138,3 +138,36 @@ def test_weights_of_absent_tokens_beside_nan(attn, dtype, D, width):
     assert (w[0, 1, :100][live] > start[0, 1, :100][live]).any() and not w[0, 1].isnan().any()
     assert torch.equal(w[1, :, 48:64], start[1, :, 48:64]) and torch.equal(w[:, :, 100:], start[:, :, 100:])
     assert attn.check_status(0) == 8
+
+
+@pytest.mark.parametrize("octaves", [12.0, 20.5, 24.625, 25.125, 28.0])
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("D", [64, 128, 256, 33])
+@pytest.mark.parametrize("L,width", [(150, None), (150, 900), (3000, None)])
+def test_small_weights_beside_a_large_one(attn, L, width, D, dtype, octaves):
+    # Every eighth token takes all the weight and has a zero V row; the others, `octaves` powers of two below,
+    # make up the whole output.  Scores are exact: q is one column of K.
+    k, v, table, ln = make_cache([L, L - 9], 2, D, 16, dtype, width=width)
+    ps = 16
+    for b in range(2):
+        t = torch.arange(int(ln[b]))
+        page, row = table[b, t // ps].long(), t % ps
+        sink = t % 8 == (3 if b else 0)
+        k[page, :, row, 0] = torch.where(sink, 0.0, -octaves).to(dtype)[:, None]
+        x = (v[page, :, row].abs().clamp(max=3) + 1) * 2.0 ** 12
+        v[page, :, row] = torch.where(sink[:, None, None], 0.0, x).to(dtype)
+    q = torch.zeros(2, 6, 1, D).to(dtype)
+    q[..., 0] = 1
+    scale = math.log(2.0)
+    o, absum, _, w = decode_ref(q, k, v, table, ln, scale)
+    smax = torch.full((2, 6, 1, 1), octaves * scale, dtype=torch.float64)
+    tol = decode_bound(o, absum, smax, L, D, dtype)
+    assert (tol < 0.02 * o.abs()).all()  # the outputs are of such weights alone
+    args = tuple(t.cuda() for t in (q, k, v, table, ln))
+    weights = torch.zeros(2, 2, table.shape[1] * ps, device="cuda")
+    for out in (attn.attn_decode(*args, scale=scale), attn.attn_decode(*args, scale=scale, weights=weights)):
+        err = (out.cpu().double() - o).abs()
+        assert (err <= tol).all(), f"error {(err / tol).max():.2f} of the bound"
+    rel = 2 * ((D + 4) * 2.0 ** -23 * octaves * scale + 2.0 ** -21 + L * 2.0 ** -23) + 4 * 2.0 ** -24
+    assert ((weights.cpu().double() - w).abs() <= rel * w).all()
+    assert attn.check_status(0) == 0
