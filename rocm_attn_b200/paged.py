@@ -39,9 +39,10 @@ def attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, b
     ``softmax(scale * q K^T) V``.
 
     q: ``[B, Hq, 1, D]`` in the cache's type, Hq a multiple of Hkv (query heads
-    ``h * Hq // Hkv`` and following read kv head ``h``).  ``scale`` defaults to
-    1/sqrt(D).  Returns O ``[B, Hq, 1, D]``; an empty sequence gives zeros, one
-    that has tokens and only scores of -inf NaN, as the formula does.
+    ``h * Hq // Hkv`` and following read kv head ``h``).  ``scale`` is positive
+    and finite, 1/sqrt(D) if not given.  Returns O ``[B, Hq, 1, D]``; an empty
+    sequence gives zeros, one that has tokens and only scores of -inf NaN, as
+    the formula does.
 
     pages: optional int32 ``[B, Hkv, n]`` of logical pages (``t // page_size``),
     as ``kv_select_pages`` returns: only their tokens are attended to.  Entries
@@ -54,7 +55,7 @@ def attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, b
     bytes of scratch memory.  Not together with ``pages``.
     """
     return rocm_attn_ext.attn_decode(q, k_cache, v_cache, block_table, seq_lens,
-                                     -1.0 if scale is None else float(scale), pages, weights)
+                                     None if scale is None else float(scale), pages, weights)
 
 
 def kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
