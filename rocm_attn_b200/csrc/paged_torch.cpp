@@ -8,7 +8,6 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
-#include <cmath>
 #include <optional>
 #include <tuple>
 
@@ -156,12 +155,7 @@ Tensor workspace(size_t bytes, const c10::Device& dev) {
 cudaStream_t stream_of(const c10::Device& dev) { return at::cuda::getCurrentCUDAStream(dev.index()).stream(); }
 
 Tensor attn_decode(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& block_table,
-                   const Tensor& seq_lens, std::optional<double> scale, const OptTensor& pages,
-                   const OptTensor& weights) {
-  // The launcher takes anything else as the default; a caller who gives such a scale does not mean that.
-  const float softmax_scale = scale ? static_cast<float>(*scale) : -1.0f;
-  TORCH_CHECK(!scale || (softmax_scale > 0.f && std::isfinite(softmax_scale)),
-              "scale must be positive and finite in 32 bits, got ", *scale);
+                   const Tensor& seq_lens, double scale, const OptTensor& pages, const OptTensor& weights) {
   check_cuda(q, "q");
   check_cache_tensor(k_cache, "k_cache");
   check_cache_tensor(v_cache, "v_cache");
@@ -195,7 +189,7 @@ Tensor attn_decode(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache
   // an empty list has no data, but is a list all the same
   static const int none = 0;
   const int* list_ptr = !pages ? nullptr : n_pages > 0 ? list.data_ptr<int>() : &none;
-  check_launch(launch_attn_decode(&c.c, x.data_ptr(), qs, out.data_ptr(), Hq, softmax_scale, list_ptr,
+  check_launch(launch_attn_decode(&c.c, x.data_ptr(), qs, out.data_ptr(), Hq, static_cast<float>(scale), list_ptr,
                                   n_pages, weights ? weights->data_ptr<float>() : nullptr, weights ? ws : nullptr,
                                   space.data_ptr(), bytes, stream_of(dev)),
                "launch_attn_decode");
@@ -337,7 +331,7 @@ std::tuple<Tensor, Tensor, Tensor> kv_evict(const Tensor& k_cache, const Tensor&
 
 void bind_paged(py::module& m) {
   m.def("attn_decode", &attn_decode, "Attention of one new token per sequence over a paged cache", py::arg("q"),
-        py::arg("k_cache"), py::arg("v_cache"), py::arg("block_table"), py::arg("seq_lens"), py::arg("scale") = py::none(),
+        py::arg("k_cache"), py::arg("v_cache"), py::arg("block_table"), py::arg("seq_lens"), py::arg("scale") = -1.0,
         py::arg("pages") = py::none(), py::arg("weights") = py::none());
   m.def("kv_append", &kv_append, "Write new tokens to a paged cache", py::arg("k"), py::arg("v"), py::arg("k_cache"),
         py::arg("v_cache"), py::arg("block_table"), py::arg("seq_lens"), py::arg("new_lens") = py::none(),

@@ -25,6 +25,8 @@ page_size`` are left out; ``check_status`` then returns 8.
 """
 from __future__ import annotations
 
+import ctypes
+import math
 from typing import Optional, Tuple
 
 import torch
@@ -54,8 +56,14 @@ def attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, b
     added to it (``kv_evict`` takes it).  Needs ``4 * B * Hq * W * page_size``
     bytes of scratch memory.  Not together with ``pages``.
     """
-    return rocm_attn_ext.attn_decode(q, k_cache, v_cache, block_table, seq_lens,
-                                     None if scale is None else float(scale), pages, weights)
+    if scale is None:
+        scale = -1.0  # the binding's default
+    else:
+        # as 32 bits, what the kernels get; the binding takes other scales as not given
+        scale = ctypes.c_float(scale).value
+        if not 0.0 < scale < math.inf:
+            raise ValueError("attn_decode: scale must be positive and finite in 32 bits")
+    return rocm_attn_ext.attn_decode(q, k_cache, v_cache, block_table, seq_lens, scale, pages, weights)
 
 
 def kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
