@@ -140,12 +140,13 @@ static std::vector<torch::Tensor> attn_forward_batch(std::vector<torch::Tensor> 
   return outs;
 }
 
-// Synchronises the current stream of `device` and returns (and clears) the
-// kernel status: 0 when every earlier launch completed its waits and met only
-// valid pages and lengths.
+// Synchronises `device`, since kernels of every stream share its status words,
+// and returns (and clears) the kernel status: 0 when every earlier launch
+// completed its waits and met only valid pages and lengths.
 static int check_status(int64_t device) {
   const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));
   cudaStream_t stream = at::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(device)).stream();
+  c10::cuda::device_synchronize();
   int status = 0;
   const int st = attn_get_status(stream, &status);
   TORCH_CHECK(st == ATTN_OK, "attn_get_status: ", status_text(st));

@@ -171,3 +171,20 @@ def test_small_weights_beside_a_large_one(attn, L, width, D, dtype, octaves):
     rel = 2 * ((D + 4) * 2.0 ** -23 * octaves * scale + 2.0 ** -21 + L * 2.0 ** -23) + 4 * 2.0 ** -24
     assert ((weights.cpu().double() - w).abs() <= rel * w).all()
     assert attn.check_status(0) == 0
+
+
+def test_status_covers_every_stream(attn):
+    # a bad page met late on another stream is reported by the check that follows the call
+    k, v, table, ln = make_cache([100], 2, 64, 16, BF16)
+    table[0, 3] = -7
+    args = tuple(t.cuda() for t in (_q(1, 4, 64, BF16), k, v, table, ln))
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):  # kernels loaded and memory at hand, which may synchronise
+        attn.attn_decode(*args)
+        torch.cuda._sleep(1000)
+    side.synchronize()
+    assert attn.check_status(0) == 8
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)  # about 0.1 s of work before it
+        attn.attn_decode(*args)
+    assert attn.check_status(0) == 8 and attn.check_status(0) == 0
