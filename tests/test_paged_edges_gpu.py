@@ -188,3 +188,46 @@ def test_status_covers_every_stream(attn):
         torch.cuda._sleep(200_000_000)  # about 0.1 s of work before it
         attn.attn_decode(*args)
     assert attn.check_status(0) == 8 and attn.check_status(0) == 0
+
+
+def _marked_case(D, n, dtype, trend):
+    """One sequence whose every 64 tokens add the same amount to one column of the output, at scores whose
+    maximum rises (or falls) along the sequence: q picks column 0 of K, the score in powers of two."""
+    k, v, table, ln = make_cache([n], 1, D, 16, dtype)
+    t = torch.arange(n)
+    tile = t // 64
+    level = ((tile * 5) % 4 + 12 * (tile if trend > 0 else int(tile[-1]) - tile) // int(tile[-1])).double() - 8
+    page, row = table[0, t // 16].long(), t % 16
+    k[page, 0, row] = 0
+    k[page, 0, row, 0] = level.to(dtype)
+    v[page, 0, row] = 0
+    v[page, 0, row, tile % D] = (2.0 ** -level).to(dtype)
+    q = torch.zeros(1, 4, 1, D).to(dtype)
+    q[..., 0] = 1
+    return (q, k, v, table, ln), tile, level
+
+
+@pytest.mark.parametrize("trend", [1, -1])
+@pytest.mark.parametrize("D,dtype", [(64, F16), (64, BF16), (128, F16), (128, BF16), (256, BF16), (64, F32), (100, F16)])
+def test_every_part_of_a_long_sequence_counts(attn, D, dtype, trend):
+    # one sequence over every CTA of the grid, more parts than the join takes in one turn: a tile of 64 tokens that
+    # is missing, counted twice or scaled by a power of two would be beyond the bound
+    n, scale = 40001, math.log(2.0)
+    case, tile, level = _marked_case(D, n, dtype, trend)
+    o, absum, _, w = decode_ref(*case, scale)
+    tol = decode_bound(o, absum, torch.full((1, 4, 1, 1), 8 * scale, dtype=torch.float64), n, D, dtype)
+    part = torch.zeros(int(tile[-1]) + 1, dtype=torch.float64).index_add_(0, tile, torch.exp2(level) * torch.exp2(-level))
+    part = part / torch.exp2(level).sum()  # what a tile adds to its column
+    column = torch.arange(len(part)) % D
+    full = tile.bincount() == 64
+    assert (part[full] > 2 * tol[0, 0, 0, column[full]]).all()
+    args = tuple(t.cuda() for t in case)
+    weights = torch.zeros(1, 1, case[3].shape[1] * 16, device="cuda")
+    out = attn.attn_decode(*args, scale=scale)
+    for got in (out, attn.attn_decode(*args, scale=scale, weights=weights)):
+        err = (got.cpu().double() - o).abs()
+        assert (err <= tol).all(), f"error {(err / tol).max():.2f} of the bound"
+    rel = 2 * ((D + 4) * 2.0 ** -23 * 8 * scale + 2.0 ** -21 + n * 2.0 ** -23) + 5 * 2.0 ** -24
+    assert ((weights.cpu().double() - w).abs() <= rel * w).all()
+    assert torch.equal(out, attn.attn_decode(*args, scale=scale))
+    assert attn.check_status(0) == 0
