@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from paged_ref import decode_bound, decode_ref, decode_tolerance, make_cache
+from paged_ref import bounds_ref, decode_bound, decode_ref, decode_tolerance, make_cache, select_ref
 
 pytestmark = pytest.mark.gpu
 
@@ -230,4 +230,48 @@ def test_every_part_of_a_long_sequence_counts(attn, D, dtype, trend):
     rel = 2 * ((D + 4) * 2.0 ** -23 * 8 * scale + 2.0 ** -21 + n * 2.0 ** -23) + 5 * 2.0 ** -24
     assert ((weights.cpu().double() - w).abs() <= rel * w).all()
     assert torch.equal(out, attn.attn_decode(*args, scale=scale))
+    assert attn.check_status(0) == 0
+
+
+@pytest.mark.parametrize("dtype,D,ps", [(BF16, 128, 16), (F16, 64, 24), (F32, 33, 8)])
+def test_captured_bounds_and_selection_follow_lengths_and_pages(attn, dtype, D, ps):
+    # bounds, selection and the attention over it, captured and replayed on other keys, lengths and pages
+    W, top = 60, 5
+    k, v, table, ln = make_cache([50, 0, 300, 3], 2, D, ps, dtype, width=W, poison=False, spare=240)
+    dk, dv, dt, dl = (t.cuda() for t in (k, v, table, ln))
+    q = _q(4, 8, D, dtype)
+    dq = q.cuda()
+    kept_bounds = torch.zeros(k.shape[0], 2, 2, D, dtype=dtype, device="cuda")
+
+    def step():
+        fresh = attn.kv_page_bounds(dk, dt, dl)
+        attn.kv_page_bounds(dk, dt, dl, bounds=kept_bounds)
+        pages = attn.kv_select_pages(dq, fresh, dt, dl, ps, top)
+        return fresh, pages, attn.attn_decode(dq, dk, dv, dt, dl, pages=pages)
+
+    dt.copy_(torch.arange(4 * W, dtype=torch.int32).reshape(4, W))
+    step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        fresh, pages, out = step()
+    kept = torch.zeros(kept_bounds.shape, dtype=dtype)
+    for i, new in enumerate(([50, 0, 300, 3], [1, W * ps, 5, 0], [300, 301, 302, 303])):
+        gen = torch.Generator().manual_seed(i)
+        k = torch.randn(k.shape, generator=gen).to(dtype)
+        q = torch.randn(q.shape, generator=gen).to(dtype)
+        ln = torch.tensor(new, dtype=torch.int32)
+        table = torch.randperm(k.shape[0], generator=gen)[:4 * W].reshape(4, W).to(torch.int32)
+        kept = torch.randn(kept.shape, generator=gen).to(dtype)
+        for d, t in ((dk, k), (dq, q), (dl, ln), (dt, table), (kept_bounds, kept)):
+            d.copy_(t)
+        g.replay()
+        torch.cuda.synchronize()
+        want = bounds_ref(k, table, ln, torch.zeros(kept.shape, dtype=dtype))
+        assert torch.equal(fresh.cpu(), want)
+        assert torch.equal(kept_bounds.cpu(), bounds_ref(k, table, ln, kept.clone()))
+        chosen = select_ref(q, want, table, ln, ps, top)
+        assert torch.equal(pages.cpu(), chosen)
+        o, absum, smax, _ = decode_ref(q, k, v, table, ln, pages=chosen)
+        assert ((out.cpu().double() - o).abs() <= decode_bound(o, absum, smax, top * ps, D, dtype, vmax=8.0)).all()
     assert attn.check_status(0) == 0
