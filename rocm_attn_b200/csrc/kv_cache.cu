@@ -1060,7 +1060,8 @@ extern "C" int launch_kv_evict(const AttnPagedCache* cache, const float* weights
       budget > static_cast<long long>(new_width) * cache->page_size)
     return ATTN_ERR_INVALID_ARGUMENT;
   if (cache->B == 0) return ATTN_OK;
-  if (!weights || !weights_strides || negative(weights_strides, 2) || !new_table || !new_weights || !kept || !new_lens)
+  if ((!weights && view.capacity() > 0) || !weights_strides || negative(weights_strides, 2) || !new_table ||
+      !new_weights || !kept || !new_lens)
     return ATTN_ERR_INVALID_ARGUMENT;
   if (!aligned_to(weights, 4) || !aligned_to(new_table, 4) || !aligned_to(new_weights, 4) || !aligned_to(kept, 4) ||
       !aligned_to(new_lens, 4))

@@ -275,3 +275,17 @@ def test_captured_bounds_and_selection_follow_lengths_and_pages(attn, dtype, D, 
         o, absum, smax, _ = decode_ref(q, k, v, table, ln, pages=chosen)
         assert ((out.cpu().double() - o).abs() <= decode_bound(o, absum, smax, top * ps, D, dtype, vmax=8.0)).all()
     assert attn.check_status(0) == 0
+
+
+def test_table_without_pages(attn):
+    # a block table of no entries names no token: weights of no elements go with it
+    k = torch.zeros(4, 2, 16, 64, dtype=F16, device="cuda")
+    t, n = torch.zeros(3, 0, dtype=torch.int32, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
+    w = torch.zeros(3, 2, 0, device="cuda")
+    q = torch.ones(3, 4, 1, 64, dtype=F16, device="cuda")
+    assert (attn.attn_decode(q, k, k, t, n, weights=w) == 0).all()
+    new = torch.arange(3, dtype=torch.int32, device="cuda")[:, None]
+    lens, new_w, kept = attn.kv_evict(k, k.clone(), t, n, w, new, 5, recent=2)
+    assert lens.tolist() == [0, 0, 0] and (new_w == 0).all() and (kept == -1).all()
+    assert new_w.shape == (3, 2, 16) and kept.shape == (3, 2, 5)
+    assert attn.check_status(0) == 0
