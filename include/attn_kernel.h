@@ -215,6 +215,10 @@ typedef struct AttnPagedCache {
  *        no two of which share memory: weights[b, h, t] += the sum of the
  *        softmax weights of token t over the query heads of kv head h.  Not
  *        together with `pages` (ATTN_ERR_UNSUPPORTED).
+ * Products are summed and the softmax is held in 32 bits; for fp16 and bf16
+ * caches with 16-byte rows each softmax weight is rounded to the cache's type
+ * before the product with V (half a step; fp16 weights below 2^-29 of the
+ * largest by at most 2^-40 of that).
  * softmax_scale as in launch_attn_forward.  With weights the workspace holds
  * the scores, 4 * B * Hq * table_width * page_size bytes; without, it does not
  * grow with the lengths and may be empty (the pointer is then only checked).
@@ -264,10 +268,11 @@ ATTN_API int launch_kv_page_bounds(const AttnPagedCache* cache, void* bounds, co
  *   score = sum over the dims d of max[d] * p[d] + min[d] * m[d],
  * p and m being the sums of q's positive and negative parts over the query
  * heads of the kv head: the sum of max(q * min, q * max), an upper bound of the
- * summed scores of any token of the page (a part of q that is zero adds
- * nothing, whatever the bound).  Ties go to the lower page, NaN counts as
- * largest.  Sums are taken in 64 bits, since a score
- * next to the border decides a page.  top >= 1; cache->k and v are not used.
+ * summed scores of any token of the page.  A part of q that is zero adds
+ * nothing, even beside an infinite bound; a bound that is NaN makes the score
+ * NaN.  Ties go to the lower page, NaN counts as largest.  Sums are taken in 64
+ * bits, since a score next to the border decides a page.  top >= 1; cache->k
+ * and v are not used.
  */
 ATTN_API int kv_select_pages_workspace_bytes(const AttnPagedCache* cache, size_t* bytes);
 ATTN_API int launch_kv_select_pages(const AttnPagedCache* cache, const void* q, const long long* q_strides, int Hq,

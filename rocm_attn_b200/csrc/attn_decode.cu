@@ -1308,12 +1308,15 @@ Plan make_plan(const AttnPagedCache* c, bool fast, int Hq, int n_pages, bool lis
     // One launch of clusters where a CTA gets at most two tiles, or four if
     // the clusters leave no more than three quarters of the GPU idle; not where
     // units far outnumber the CTAs that fit, whose set-up would then repeat.
-    // Measured, in clusters against runs, us: 8 units of 1 tile 4.6 / 6.4, 32 of 8
-    // tiles 7.4 / 8.2, 32 of 32 tiles 11.3 / 12.2, 512 of 2 tiles 12.5 / 14.0; but
-    // 8 of 32 tiles 10.4 / 9.5, 512 of 8 tiles 27.0 / 25.5, 2048 of 2 tiles 40.7 /
-    // 35.2.  Clusters grow beyond half of the GPU only for more than four
-    // tiles per CTA, as up to there a call starts beside the one before it: 32
-    // units of 8 tiles, calls in a row, 8.4 us in 128 CTAs, 9.7 us in 256.
+    // Clusters grow beyond half of the GPU only for more than four tiles per
+    // CTA, as up to there a call starts beside the one before it.  Measured at
+    // D = 128 and full lengths, calls in a row, us, as this rule has it in
+    // clusters / in runs: 8 units of 1 tile 4.5 / 6.5, of 8 tiles 6.7 / 7.2, of 16
+    // 8.0 / 8.5; 32 units of 1 tile 4.9 / 7.1, of 4 tiles 7.1 / 7.6, of 8 8.4 / 8.2,
+    // of 16 11.0 / 10.7, of 32 14.4 / 13.9; 128 of 4 tiles 9.0 / 10.0; 512 of 2 tiles
+    // 13.2 / 14.1.  Left to runs: 8 of 32 tiles 10.4 / 9.5, 512 of 4 tiles 18.7 /
+    // 19.7, of 8 28.7 / 29.5, 2048 of 2 tiles 42.7 / 32.2.  32 units of 8 tiles in
+    // clusters of eight, 256 CTAs, take 9.9.
     int cl = 1;
     while (cl < kMaxCluster && cl < unit_tiles && units * cl * 2 <= slots &&
            (units * cl * 4 <= slots || unit_tiles > 4 * cl))

@@ -46,6 +46,11 @@ def attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, b
     sequence gives zeros, one that has tokens and only scores of -inf NaN, as
     the formula does.
 
+    Scores and softmax are held in 32 bits.  With fp16 and bf16 each softmax
+    weight is rounded to that type for the product with V, by half a step (2^-11
+    and 2^-8 of it) at most, as attention on tensor cores does; the error
+    against exact arithmetic is about 1.2 times that of rounding O alone.
+
     pages: optional int32 ``[B, Hkv, n]`` of logical pages (``t // page_size``),
     as ``kv_select_pages`` returns: only their tokens are attended to.  Entries
     that name no page of the sequence (-1) add nothing; one named twice counts
@@ -54,7 +59,9 @@ def attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, b
     weights: optional fp32 ``[B, Hkv, >= W * page_size]``, updated in place:
     each token's softmax weight, summed over the query heads of the kv head, is
     added to it (``kv_evict`` takes it).  Needs ``4 * B * Hq * W * page_size``
-    bytes of scratch memory.  Not together with ``pages``.
+    bytes of scratch memory, so the table had better be as wide as the lengths
+    need.  Not together with ``pages``: steps that read listed pages leave the
+    weights as they are, so a loop that evicts by them takes whole steps too.
     """
     if scale is None:
         scale = -1.0  # the binding's default
@@ -108,8 +115,9 @@ def kv_select_pages(q: torch.Tensor, bounds: torch.Tensor, block_table: torch.Te
     sum over d of ``max * p + min * m``, p and m being q's positive and negative
     parts summed over the kv head's query heads.  That is the sum of ``max(q *
     min, q * max)``, an upper bound of the summed scores of any token of the
-    page.  Ties go to
-    the lower page and NaN counts as largest.  Scores are summed in 64 bits.
+    page.  A part that is zero adds nothing, even beside an infinite bound; a NaN
+    bound makes the score NaN.  Ties go to the lower page and NaN counts as
+    largest.  Scores are summed in 64 bits.
     """
     return rocm_attn_ext.kv_select_pages(q, bounds, block_table, seq_lens, int(page_size), int(top))
 
