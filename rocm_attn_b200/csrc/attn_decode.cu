@@ -35,8 +35,8 @@
 // attn_decode_simt_kernel (fp32, any D <= 256, any strides).
 //
 // Measured on B200 (calls in a row): 64 sequences of up to 16384 tokens, 64/8
-// heads of 128, fp16, 2.75 GB of K and V: 402 to 430 us by box, 6.4 to 6.8
-// TB/s, where a copy does 6.54; 24 of up to 4096, 32/8 heads, bf16, with
+// heads of 128, fp16, 2.75 GB of K and V: 402 to 433 us on different GPUs, 6.4
+// to 6.8 TB/s, where a copy does 6.54; 24 of up to 4096, 32/8 heads, bf16, with
 // weights: 55 us (floor 41); one of 517 tokens: 7.9 us.  A call in two launches
 // has about 8 us that are not reading: lengths and first look-ups 3, first fill
 // of the rings 2.5, the ends of the runs and the join the rest.
@@ -425,10 +425,9 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
   constexpr int kSteps = kD / 16;              // 16-wide steps of the head dim
   constexpr int kRowsPerCopy = 32 / kCols;     // rows of one 16-byte copy of the warp
   // A warp's weights, and so its L and O, are kept times this power of two:
-  // fp16 ends 2^-14 below 1 with its full precision and 2^-25 below with all,
-  // and tokens beside one that takes nearly everything lie there.  With it
-  // weights down to 2^-29 of the largest keep their bits, and those from 2^-40
-  // on still count.
+  // fp16 has its full precision down to 2^-14 and nothing below 2^-25, where
+  // the tokens beside one that takes nearly everything lie.  With it weights
+  // down to 2^-29 of the largest keep their bits, and those down to 2^-40 count.
   constexpr float kUp = kBf16 ? 1.f : 32768.f;
 
   extern __shared__ __align__(1024) unsigned char smem[];

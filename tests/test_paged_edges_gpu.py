@@ -289,3 +289,42 @@ def test_table_without_pages(attn):
     assert lens.tolist() == [0, 0, 0] and (new_w == 0).all() and (kept == -1).all()
     assert new_w.shape == (3, 2, 16) and kept.shape == (3, 2, 5)
     assert attn.check_status(0) == 0
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_decode_and_evict_over_the_widest_table(attn, dtype):
+    # 2^31 - 65537 tokens in pages of one, the same page but for the last, whose score makes it weigh as much
+    # as 2^31 others.  All sums are of equal powers of two and exact up to the join of at most 600 parts.
+    n, D = MAX_CAPACITY, 8
+    table = _wide_table()
+    table[0, -1] = 1
+    k, v = torch.zeros(8, 1, 1, D, dtype=dtype), torch.zeros(8, 1, 1, D, dtype=dtype)
+    k[1, 0, 0, 0] = 31
+    v[0], v[1] = 1, 3
+    q = torch.zeros(1, 1, 1, D, dtype=dtype, device="cuda")
+    q[..., 0] = 1
+    k, v = k.cuda(), v.cuda()
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    total = n - 1 + 2.0 ** 31
+    rel = 600 * 2.0 ** -24 + 2.0 ** -20
+    want = (n - 1 + 3 * 2.0 ** 31) / total
+    out = attn.attn_decode(q, k, v, table, lens, scale=math.log(2.0))
+    assert ((out.double() - want).abs() <= want * (rel + torch.finfo(dtype).eps / 2)).all()
+    w = torch.zeros(1, 1, n, device="cuda")
+    assert torch.equal(attn.attn_decode(q, k, v, table, lens, scale=math.log(2.0), weights=w), out)
+    # log2 of the sum, 32, is off by half a step of 2^-18
+    rel = rel + 2.0 ** -18
+    assert abs(float(w[0, 0, -1]) * total / 2.0 ** 31 - 1) <= rel
+    lo, hi = float(w[0, 0, :-1].min()), float(w[0, 0, :-1].max())
+    assert lo == hi and abs(lo * total - 1) <= rel
+    w[0, 0, n - 100] = 2
+    w[0, 0, 5] = 1
+    new = torch.arange(2, 7, dtype=torch.int32, device="cuda")[None]
+    new_lens, new_w, kept = attn.kv_evict(k, v, table, lens, w, new, 5, recent=2)
+    # the two largest, of the others, all equal, the lowest, and the last two
+    assert kept[0, 0].tolist() == [0, 5, n - 100, n - 2, n - 1] and new_lens.tolist() == [5]
+    assert torch.equal(new_w[0, 0], w[0, 0, kept[0, 0].long()])
+    assert (k[2:6] == k[0]).all() and torch.equal(k[6], k[1]) and torch.equal(v[6], v[1]) and (k[7] == 0).all()
+    bounds = attn.kv_page_bounds(k, table, lens)
+    assert torch.equal(bounds[:2, :, 0], k[:2, :, 0]) and torch.equal(bounds[:2, :, 1], k[:2, :, 0])
+    assert attn.check_status(0) == 0
