@@ -300,6 +300,97 @@ ATTN_API int launch_kv_evict(const AttnPagedCache* cache, const float* weights, 
                              const int* new_table, long long new_stride, int new_width, int budget, int recent,
                              float* new_weights, int* kept, int* new_lens, cudaStream_t stream);
 
+/*
+ * Attention of drafted tokens over the cache, for programs that check several
+ * guesses of the next tokens in one call: out = softmax(scale * q K^T) V, each
+ * drafted token over the sequence's context and the drafted tokens it follows.
+ *   q    [B, Hq, S, D], element strides over (batch, head, token) in q_strides,
+ *        null = contiguous; Hq as for launch_attn_decode, 0 <= S <= 1024
+ *   out  [B, Hq, S, D] contiguous, fully overwritten
+ *   new_lens  null (S everywhere), or int32 [B] device memory: how many of the
+ *        S tokens of sequence b are drafted, n (at most S, negative is none)
+ * seq_lens counts the drafted tokens: token s of sequence b lies at position
+ * seq_lens[b] - n + s, where launch_kv_append puts it when given the same
+ * lengths; the positions before are the context.
+ *   parents  null, or int32 [B, S] device memory, parents_stride entries from
+ *        one sequence to the next (0: one tree for all): the drafted token that
+ *        s follows, below s, or -1, where it follows the context.  Token s
+ *        attends to the context, itself, its parent, the parent's parent and so
+ *        on.  Null is a chain: token s follows s - 1.
+ * An entry of parents[b, 0..n) that is no earlier token counts as -1 and is
+ * reported as ATTN_ERR_BAD_PAGE.  Rows s >= n, and those of sequences without
+ * tokens, are zeros; a row that has tokens and only scores of -inf is NaN, as
+ * the formula.  Precision as for launch_attn_decode.
+ */
+ATTN_API int attn_tree_workspace_bytes(const AttnPagedCache* cache, int Hq, int S, size_t* bytes);
+ATTN_API int launch_attn_tree(const AttnPagedCache* cache, const void* q, const long long* q_strides, void* out, int Hq,
+                              int S, float softmax_scale, const int* parents, long long parents_stride,
+                              const int* new_lens, void* workspace, size_t workspace_bytes, cudaStream_t stream);
+
+/*
+ * Moves the drafted tokens that were accepted to the front of the drafted ones:
+ * with base = seq_lens[b] - new_lens[b], K and V of position base + kept[b, i]
+ * go to position base + i.
+ *   new_lens  int32 [B]: the drafted tokens of each sequence, as above
+ *   kept      int32 [B, n], kept_stride entries from one sequence to the next:
+ *             drafted tokens in ascending order; the first -1 ends a list
+ *   lens      int32 [B], written: base + the length of the list, the tokens of
+ *             the sequence from then on (seq_lens is left as it is)
+ * A list also ends at an entry that is not larger than the one before or names
+ * no drafted token, which is reported as ATTN_ERR_BAD_PAGE.  Rows behind the
+ * last kept token are left as they are, and so are page bounds: they still
+ * bound the tokens.  Two sequences of a call must not write to one page.
+ */
+ATTN_API int launch_kv_compact(const AttnPagedCache* cache, const int* new_lens, const int* kept, long long kept_stride,
+                               int n, int* lens, cudaStream_t stream);
+
+/*
+ * Who holds which pages.  refs (int32 [num_pages]) counts the holders of each
+ * page, 0 where it is free; sequence b holds the first held[b] (int32) pages
+ * of its row of the block table.
+ *
+ * launch_kv_resize makes every sequence hold the pages its seq_lens needs, no
+ * fewer and no more: pages behind are given back, pages that it lacks are
+ * taken, those free at the call's start from the lowest on, sequence after
+ * sequence.  A sequence that lacks pages of which there are not enough, those
+ * for the sequences before it counted, takes none.  Changes
+ * cache->block_table (through `table`, the same memory), held and refs;
+ * missing (int32 [B]) receives the pages that a sequence lacked and did not
+ * get, else 0.  Entries of the table behind those held are left as they are.
+ * cache->k and v are not used.
+ *
+ * Counts of held outside [0, table_width], lengths that need more pages than
+ * table_width, and table entries outside the cache are reported as
+ * ATTN_ERR_BAD_PAGE (and taken as the nearest valid count, or left out), and
+ * so is a page given back by more than hold it, whose count then is negative;
+ * such a page is never given out.
+ */
+ATTN_API int kv_resize_workspace_bytes(const AttnPagedCache* cache, size_t* bytes);
+ATTN_API int launch_kv_resize(const AttnPagedCache* cache, int* table, int* held, int* refs, int* missing,
+                              void* workspace, size_t workspace_bytes, cudaStream_t stream);
+
+/*
+ * The sequences of the next step as continuations of the present ones (beams,
+ * or several samples of one prompt): new sequence i, 0 <= i < n, continues
+ * sequence parents[i] (int32 [n]; -1 is an empty sequence), with its tokens.
+ *   new_table  int32 [n, table_width] contiguous, written: the parent's pages, -1
+ *              behind them; new_held, new_lens int32 [n], written
+ * Full pages are shared.  A last page that is partly filled goes to the first
+ * sequence that continues the parent if nobody else held it, and is copied
+ * (its tokens' rows) to a free page for each other one; free pages are those free at the
+ * call's start, from the lowest on.  All present sequences give up what they
+ * hold: refs counts the new ones' pages afterwards.  If there are fewer free
+ * pages than copies, nothing is changed, all new sequences are empty and
+ * *missing (int32) receives how many are lacking, else 0.  Tokens of a parent
+ * behind the pages it holds are left out and, like parents outside [-1, B) (taken
+ * as -1), reported as ATTN_ERR_BAD_PAGE.  The written arrays must not overlap
+ * the cache's table, lengths or held.
+ */
+ATTN_API int kv_fork_workspace_bytes(const AttnPagedCache* cache, int n, size_t* bytes);
+ATTN_API int launch_kv_fork(const AttnPagedCache* cache, const int* held, int* refs, const int* parents, int n,
+                            int* new_table, int* new_held, int* new_lens, int* missing, void* workspace,
+                            size_t workspace_bytes, cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -74,14 +74,15 @@ def check_status(device: int = 0) -> int:
     """Synchronise ``device`` and return (and clear) the kernel status: 0 when
     every earlier launch completed; 7 when a kernel gave up on a wait (its
     output is then invalid); 8 when a kernel of the paged cache met a
-    block-table entry or a length that is out of range (the tokens concerned
-    were left out)."""
+    block-table entry, a length, a parent or a count of holders that is out of
+    range (what it concerns was left out)."""
     return int(rocm_attn_ext.check_status(int(device)))
 
 
 from .pipeline import attn_forward_pinned  # noqa: E402  (host-resident inputs, transfers overlapped)
 from .paged import attn_decode, kv_append, kv_evict, kv_page_bounds, kv_select_pages  # noqa: E402  (paged key-value cache)
+from .branches import attn_tree, kv_compact, kv_fork, kv_resize  # noqa: E402  (drafted tokens and shared pages on it)
 
 __all__ = ["attn_forward", "attn_forward_batch", "attn_forward_pinned", "attn_decode", "kv_append", "kv_evict",
-           "kv_page_bounds", "kv_select_pages", "check_status", "rocm_attn_ext", "KERNEL_LIB_PATH",
-           "SUPPORTED_HEAD_DIMS", "SUPPORTED_DTYPES", "MAX_HEAD_DIM"]
+           "kv_page_bounds", "kv_select_pages", "attn_tree", "kv_compact", "kv_fork", "kv_resize", "check_status",
+           "rocm_attn_ext", "KERNEL_LIB_PATH", "SUPPORTED_HEAD_DIMS", "SUPPORTED_DTYPES", "MAX_HEAD_DIM"]

@@ -348,16 +348,18 @@ int status_word_read_clear_single(cudaStream_t stream, int* host) {
 
 extern "C" int attn_get_status(cudaStream_t stream, int* status) {
   if (!status) return ATTN_ERR_INVALID_ARGUMENT;
-  int single = 0, grouped = 0, decode = 0, cache = 0;
+  int single = 0, grouped = 0, decode = 0, cache = 0, pages = 0, tree = 0;
   if (ra::status_word_read_clear_single(stream, &single) != 0 ||
       ra::status_word_read_clear_grouped(stream, &grouped) != 0 ||
       ra::page_word_read_clear_decode(stream, &decode) != 0 ||
-      ra::page_word_read_clear_cache(stream, &cache) != 0 || cudaStreamSynchronize(stream) != cudaSuccess)
+      ra::page_word_read_clear_cache(stream, &cache) != 0 || ra::page_word_read_clear_pages(stream, &pages) != 0 ||
+      ra::page_word_read_clear_tree(stream, &tree) != 0 || cudaStreamSynchronize(stream) != cudaSuccess)
     return ATTN_ERR_LAUNCH;
-  if (single != 0 || grouped != 0 || ((decode | cache) & ra::kFaultWait) != 0)
+  const int paged = decode | cache | pages | tree;
+  if (single != 0 || grouped != 0 || (paged & ra::kFaultWait) != 0)
     *status = ATTN_ERR_WATCHDOG;
   else
-    *status = (decode == 0 && cache == 0) ? ATTN_OK : ATTN_ERR_BAD_PAGE;
+    *status = paged == 0 ? ATTN_OK : ATTN_ERR_BAD_PAGE;
   return ATTN_OK;
 }
 

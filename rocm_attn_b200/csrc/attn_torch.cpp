@@ -19,6 +19,7 @@ namespace py = pybind11;
 
 // The paged key-value cache's part of the module (paged_torch.cpp).
 void bind_paged(py::module& m);
+void bind_branches(py::module& m);
 
 const char* status_text(int s) {
   switch (s) {
@@ -162,6 +163,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("check_status", &check_status, "Read and clear the kernel watchdog status", py::arg("device") = 0);
   m.def("library_version", &attn_library_version);
   bind_paged(m);
+  bind_branches(m);
   m.def("set_wait_limit_ns", [](uint64_t ns) { return static_cast<uint64_t>(attn_set_wait_limit_ns(ns)); },
         "Limit of each pipeline wait of the tensor-core kernel for later launches (0: default 2 s); returns the "
         "previous value. For tests of the watchdog path.",

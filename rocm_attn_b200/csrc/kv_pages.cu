@@ -1,0 +1,657 @@
+// Pages of a paged key-value cache changing hands: the move of accepted drafted
+// tokens to their places (launch_kv_compact), the pages that lengths need
+// (launch_kv_resize) and sequences that continue others (launch_kv_fork).
+//
+// All of them are short: a few thousand table entries, the counts of the
+// pages, and for a fork the rows of a partly filled page per copy.  The time
+// of small calls is that of their dependent loads (a length, a table entry, a
+// count, each half a microsecond), so these are kept few and in parallel.
+//
+// A free page is one whose count is 0 at the start of the call; pages are
+// given out from the lowest on, in the order of the sequences, so results do
+// not depend on timing.  Finding them is one pass over the counts by a cluster
+// of CTAs: each warp counts its stretch, the cluster's prefix sum gives each
+// stretch the rank of its first free page, and a second pass (over the L2)
+// writes the pages of the ranks that were asked for to a list.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <limits.h>
+#include <stdint.h>
+
+#include "paged_cache.h"
+#include "sm100_ptx.cuh"
+
+namespace ra {
+
+namespace {
+
+__device__ int g_page_fault = 0;
+
+constexpr int kFindCluster = 8;  // CTAs that look for free pages
+constexpr int kFindWarps = 32;
+constexpr int kFindThreads = kFindWarps * 32;
+constexpr int kStep = 256;  // pages a warp looks at in one turn
+constexpr int kCopyAhead = 4;  // rows a thread copies in one turn
+
+template <typename E, int kVec>
+struct alignas(sizeof(E) * kVec) Vec {
+  E v[kVec];
+};
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ int cluster_load(const int* p, int rank) {
+  uint32_t at;
+  int x;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_addr(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(x) : "r"(at) : "memory");
+  return x;
+}
+
+// ---------------------------------------------------------------------------
+// Free pages
+// ---------------------------------------------------------------------------
+
+struct FindSmem {
+  int warp_count[kFindWarps];
+  int total;  // free pages of this CTA's stretch, read by the cluster
+  long long warp_sum[kFindWarps];
+};
+
+// The stretch of pages of this warp, a multiple of kStep long but for the last.
+struct Stretch {
+  long long lo, hi;
+};
+__device__ __forceinline__ Stretch stretch(int num_pages) {
+  const int w = blockIdx.x * kFindWarps + (threadIdx.x >> 5);
+  const long long warps = static_cast<long long>(kFindCluster) * kFindWarps;
+  const long long per = ((num_pages + warps - 1) / warps + kStep - 1) / kStep * kStep;
+  Stretch s{w * per, (w + 1) * per};
+  if (s.lo > num_pages) s.lo = num_pages;
+  if (s.hi > num_pages) s.hi = num_pages;
+  return s;
+}
+
+// Free pages of the warp's stretch.
+__device__ __forceinline__ int count_free(const int* refs, const Stretch& s) {
+  const int lane = threadIdx.x & 31;
+  int n = 0;
+  for (long long p = s.lo; p < s.hi; p += kStep) {
+    int r[kStep / 32];
+#pragma unroll
+    for (int i = 0; i < kStep / 32; ++i) {
+      const long long at = p + i * 32 + lane;
+      r[i] = at < s.hi ? *(refs + at) : 1;
+    }
+#pragma unroll
+    for (int i = 0; i < kStep / 32; ++i) n += __popc(__ballot_sync(0xffffffffu, r[i] == 0));
+  }
+  return n;
+}
+
+// After count_free by every warp: the rank of the first free page of this
+// warp's stretch, and the free pages of all.  Holds one cluster barrier.
+__device__ __forceinline__ long long first_rank(FindSmem& s, int count, long long* all) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (lane == 0) s.warp_count[warp] = count;
+  __syncthreads();
+  if (warp == 0) {
+    const int sum = __reduce_add_sync(0xffffffffu, s.warp_count[lane]);
+    if (lane == 0) s.total = sum;
+  }
+  cluster_sync();
+  long long rank = 0;
+  *all = 0;
+  for (int c = 0; c < kFindCluster; ++c) {
+    const int x = cluster_load(&s.total, c);
+    if (c < static_cast<int>(blockIdx.x)) rank += x;
+    *all += x;
+  }
+  for (int w = 0; w < warp; ++w) rank += s.warp_count[w];
+  return rank;
+}
+
+// Writes the stretch's free pages of rank below `wanted` to their places in `order`.
+__device__ __forceinline__ void list_free(const int* refs, const Stretch& s, long long rank, long long wanted,
+                                          int* order) {
+  const int lane = threadIdx.x & 31;
+  for (long long p = s.lo; p < s.hi && rank < wanted; p += kStep) {
+    int r[kStep / 32];
+#pragma unroll
+    for (int i = 0; i < kStep / 32; ++i) {
+      const long long at = p + i * 32 + lane;
+      r[i] = at < s.hi ? *(refs + at) : 1;
+    }
+#pragma unroll
+    for (int i = 0; i < kStep / 32; ++i) {
+      const unsigned free = __ballot_sync(0xffffffffu, r[i] == 0);
+      const long long at = rank + __popc(free & ((1u << lane) - 1u));
+      if (r[i] == 0 && at < wanted) order[at] = static_cast<int>(p + i * 32 + lane);
+      rank += __popc(free);
+    }
+  }
+}
+
+// Sum of `x` over the threads of the CTA before this one, and of all.
+__device__ __forceinline__ long long cta_prefix(FindSmem& s, int x, long long* all) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long upto = x;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += y;
+  }
+  __syncthreads();  // the sums of the turn before have been read
+  if (lane == 31) s.warp_sum[warp] = upto;
+  __syncthreads();
+  long long before = upto - x;
+  *all = 0;
+#pragma unroll 8
+  for (int w = 0; w < kFindWarps; ++w) {
+    const long long y = s.warp_sum[w];
+    if (w < warp) before += y;
+    *all += y;
+  }
+  return before;
+}
+
+// What the table's row b holds: held[b], or the nearest count that its width allows.
+__device__ __forceinline__ int held_pages(const PagedView& c, const int* held, int b, int* fault) {
+  const int n = *(held + b);
+  if (n >= 0 && n <= c.table_width) return n;
+  *fault |= kFaultPage;
+  return n < 0 ? 0 : c.table_width;
+}
+
+__device__ __forceinline__ void change_refs(const PagedView& c, int* refs, int page, int by, int* fault) {
+  if (static_cast<unsigned>(page) >= static_cast<unsigned>(c.num_pages))
+    *fault |= kFaultPage;
+  else if (atomicAdd(refs + page, by) + by < 0)
+    *fault |= kFaultPage;
+}
+
+// ---------------------------------------------------------------------------
+// The pages that lengths need
+// ---------------------------------------------------------------------------
+
+struct ResizeArgs {
+  PagedView c;
+  int *table, *held, *refs, *missing;
+  int *have, *start;  // [B] workspace: held pages, rank of the first page taken
+  int* order;         // workspace: free pages by rank
+};
+
+__global__ void __launch_bounds__(kFindThreads) kv_resize_kernel(const __grid_constant__ ResizeArgs a) {
+  __shared__ FindSmem s;
+  launch_dependents();
+  grid_dependency_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int fault = 0;
+  auto want_of = [&](int b) {
+    const int len = paged_len(a.c, b, &fault);
+    return static_cast<int>((static_cast<long long>(len) + a.c.page_size - 1) / a.c.page_size);
+  };
+  // What each sequence lacks, and the sum of it over those before: all of it
+  // in every CTA, which saves a barrier.
+  long long wanted = 0;
+  for (long long b0 = 0; b0 < a.c.B; b0 += kFindThreads) {
+    const long long b = b0 + threadIdx.x;
+    int have = 0, need = 0;
+    if (b < a.c.B) {
+      have = held_pages(a.c, a.held, b, &fault);
+      need = max(0, want_of(b) - have);
+    }
+    long long all;
+    const long long at = wanted + cta_prefix(s, need, &all);
+    if (b < a.c.B && blockIdx.x == 0) {
+      a.have[b] = have;
+      a.start[b] = static_cast<int>(at < INT_MAX ? at : INT_MAX);
+    }
+    wanted += all;
+  }
+  long long free = 0;
+  if (wanted > 0) {
+    const Stretch mine = stretch(a.c.num_pages);
+    const long long rank = first_rank(s, count_free(a.refs, mine), &free);
+    list_free(a.refs, mine, rank, wanted, a.order);
+  }
+  cluster_sync();
+  // Several warps to a sequence where there are few.
+  constexpr int kWarpsAll = kFindCluster * kFindWarps;
+  const int split = a.c.B < kWarpsAll ? kWarpsAll / a.c.B : 1;
+  const long long w = static_cast<long long>(blockIdx.x) * kFindWarps + warp;
+  for (long long u = w; u < static_cast<long long>(a.c.B) * split; u += kWarpsAll) {
+    const int b = static_cast<int>(u / split), part = static_cast<int>(u % split);
+    const int have = a.have[b], want = want_of(b), start = a.start[b];
+    int* row = a.table + b * a.c.table_stride;
+    const bool granted = want <= have || static_cast<long long>(start) + (want - have) <= free;
+    for (long long j = static_cast<long long>(have) + part * 32 + lane; granted && j < want; j += split * 32) {
+      const int page = a.order[start + (j - have)];
+      row[j] = page;
+      a.refs[page] = 1;
+    }
+    for (long long j = static_cast<long long>(want) + part * 32 + lane; j < have; j += split * 32)
+      change_refs(a.c, a.refs, row[j], -1, &fault);
+    if (part == 0 && lane == 0) {
+      a.held[b] = granted ? want : have;
+      a.missing[b] = granted ? 0 : want - have;
+    }
+  }
+  if (fault) atomicOr(&g_page_fault, fault);
+}
+
+// ---------------------------------------------------------------------------
+// Sequences that continue others
+// ---------------------------------------------------------------------------
+
+struct ForkArgs {
+  PagedView c;
+  const int *held, *parents;
+  int* refs;
+  int n;
+  int *new_table, *new_held, *new_lens, *missing;
+  int *first, *kids;  // [B] workspace: the first sequence that continues this one, and how many do
+  int* copy;          // [n] workspace: which free page a new sequence's last page is copied to, or -1
+  int* order;         // workspace: free pages by rank
+  int cols;           // 16-byte (or element) columns of a row
+  int chunks;         // CTAs per head's K (or V) rows of a copied page
+};
+
+// A new sequence's parent and what it takes from it: len tokens in `full` full
+// pages and `rest` rows of another.
+struct Branch {
+  int parent, len, full, rest;
+};
+__device__ __forceinline__ Branch branch_of_parent(const ForkArgs& a, int parent, int* fault) {
+  const int have = held_pages(a.c, a.held, parent, fault), room = have * a.c.page_size;
+  int len = paged_len(a.c, parent, fault);
+  if (len > room) {
+    *fault |= kFaultPage;
+    len = room;
+  }
+  const int full = len / a.c.page_size;
+  return Branch{parent, len, full, len - full * a.c.page_size};
+}
+__device__ __forceinline__ Branch branch_of(const ForkArgs& a, int i, int* fault) {
+  const int parent = *(a.parents + i);
+  if (parent >= 0 && parent < a.c.B) return branch_of_parent(a, parent, fault);
+  if (parent != -1) *fault |= kFaultPage;
+  return Branch{-1, 0, 0, 0};
+}
+
+// Which new sequences copy their last page, and where to: one cluster.
+__global__ void __launch_bounds__(kFindThreads) kv_fork_plan_kernel(const __grid_constant__ ForkArgs a) {
+  __shared__ FindSmem s;
+  launch_dependents();
+  grid_dependency_wait();
+  int fault = 0;
+  const long long id = static_cast<long long>(blockIdx.x) * kFindThreads + threadIdx.x;
+  for (long long b = id; b < a.c.B; b += kFindCluster * kFindThreads) {
+    a.first[b] = INT_MAX;
+    a.kids[b] = 0;
+  }
+  cluster_sync();
+  for (long long i = id; i < a.n; i += kFindCluster * kFindThreads) {
+    const int parent = *(a.parents + i);
+    if (parent >= 0 && parent < a.c.B) {
+      atomicMin(a.first + parent, static_cast<int>(i));
+      atomicAdd(a.kids + parent, 1);
+    }
+  }
+  const Stretch mine = stretch(a.c.num_pages);
+  long long free;
+  const long long rank = first_rank(s, count_free(a.refs, mine), &free);  // a cluster barrier: first is complete
+  long long wanted = 0;
+  for (long long i0 = 0; i0 < a.n; i0 += kFindThreads) {
+    const long long i = i0 + threadIdx.x;
+    bool copies = false;
+    if (i < a.n) {
+      const Branch br = branch_of(a, static_cast<int>(i), &fault);
+      if (br.rest > 0) {
+        const int page = paged_page(a.c, br.parent, br.full, &fault);
+        copies = page >= 0 && (a.first[br.parent] != i || *(a.refs + page) != 1);
+      }
+    }
+    long long all;
+    const long long at = wanted + cta_prefix(s, copies ? 1 : 0, &all);
+    if (i < a.n && blockIdx.x == 0) a.copy[i] = copies ? static_cast<int>(at) : -1;
+    wanted += all;
+  }
+  if (wanted <= free) list_free(a.refs, mine, rank, wanted, a.order);
+  if (id == 0) *a.missing = static_cast<int>(wanted > free ? wanted - free : 0);
+  if (fault) atomicOr(&g_page_fault, fault);
+  cluster_sync();  // no CTA leaves while its count may be read
+}
+
+// The tables and counts, and the copies: the CTAs (i, 0) do row i of the
+// tables, CTA (i, y) its share of new sequence i's copy, K or V rows of one head.
+template <typename E, int kVec>
+__global__ void __launch_bounds__(256) kv_fork_copy_kernel(const __grid_constant__ ForkArgs a) {
+  using V = Vec<E, kVec>;
+  launch_dependents();
+  grid_dependency_wait();
+  int fault = 0;
+  const int i = blockIdx.x;
+  const bool fits = *a.missing == 0;
+  if (blockIdx.y == 0) {
+    if (i < a.n) {
+      const Branch br = branch_of(a, i, &fault);
+      const int count = fits ? br.full + (br.rest > 0) : 0, copy = a.copy[i];
+      int* row = a.new_table + static_cast<long long>(i) * a.c.table_width;
+      for (int j = threadIdx.x; j < a.c.table_width; j += 256) {
+        int page = -1;
+        if (j < count) {
+          const bool copied = copy >= 0 && j == br.full;
+          page = copied ? a.order[copy] : *(a.c.table + static_cast<long long>(br.parent) * a.c.table_stride + j);
+          if (copied) a.refs[page] = 1;
+        }
+        row[j] = page;
+      }
+      if (threadIdx.x == 0) {
+        a.new_held[i] = count;
+        a.new_lens[i] = fits ? br.len : 0;
+      }
+    }
+    if (fits && i < a.c.B) {
+      // One holder less, and as many more as continue it.
+      const Branch br = branch_of_parent(a, i, &fault);
+      const int have = held_pages(a.c, a.held, i, &fault), kids = a.kids[i];
+      const bool keeps = kids > 0 && br.rest > 0 && a.copy[a.first[i]] < 0;
+      for (int j = threadIdx.x; j < have; j += 256) {
+        const int by = (j < br.full ? kids : j == br.full && keeps ? 1 : 0) - 1;
+        if (by != 0) change_refs(a.c, a.refs, *(a.c.table + i * a.c.table_stride + j), by, &fault);
+      }
+    }
+  }
+  if (fits && i < a.n && a.copy[i] >= 0) {
+    const Branch br = branch_of(a, i, &fault);
+    const long long from = *(a.c.table + static_cast<long long>(br.parent) * a.c.table_stride + br.full);
+    const long long to = a.order[a.copy[i]];
+    const int hv = blockIdx.y / a.chunks, chunk = blockIdx.y - hv * a.chunks;
+    const bool is_v = hv >= a.c.heads;
+    const int h = is_v ? hv - a.c.heads : hv;
+    const long long* st = is_v ? a.c.vs : a.c.ks;
+    const int in = threadIdx.x / a.cols, at_once = 256 / a.cols;
+    E* x = static_cast<E*>(is_v ? a.c.v : a.c.k) + h * st[1] + static_cast<long long>(threadIdx.x - in * a.cols) * kVec;
+    if (in < at_once) {
+      const long long step = static_cast<long long>(a.chunks) * at_once;
+      for (long long r0 = chunk * at_once + in; r0 < br.rest; r0 += kCopyAhead * step) {
+        V row[kCopyAhead];
+#pragma unroll
+        for (int p = 0; p < kCopyAhead; ++p)
+          if (r0 + p * step < br.rest)
+            row[p] = *reinterpret_cast<const V*>(x + from * st[0] + (r0 + p * step) * st[2]);
+#pragma unroll
+        for (int p = 0; p < kCopyAhead; ++p)
+          if (r0 + p * step < br.rest) *reinterpret_cast<V*>(x + to * st[0] + (r0 + p * step) * st[2]) = row[p];
+      }
+    }
+  }
+  if (fault) atomicOr(&g_page_fault, fault);
+}
+
+// ---------------------------------------------------------------------------
+// Accepted tokens to their places
+// ---------------------------------------------------------------------------
+
+struct CompactArgs {
+  PagedView c;
+  const int *new_lens, *kept;
+  long long kept_stride;
+  int n;
+  int* lens;
+  int cols;  // 16-byte (or element) columns of a row
+};
+
+// Warp (b, head), lane a column of K or V: a kept token's place is never behind
+// it, and the places of the tokens of one turn never among the sources of a later one, so
+// each lane moves its column by itself, the rows of a turn read before any of
+// them is written.
+constexpr int kMoveWarps = 4, kMoveAhead = 16;
+
+template <typename E, int kVec>
+__global__ void __launch_bounds__(kMoveWarps * 32) kv_compact_kernel(const __grid_constant__ CompactArgs a) {
+  using V = Vec<E, kVec>;
+  launch_dependents();
+  grid_dependency_wait();
+  const int lane = threadIdx.x & 31;
+  const long long task = static_cast<long long>(blockIdx.x) * kMoveWarps + (threadIdx.x >> 5);
+  const int b = static_cast<int>(task / a.c.heads), h = static_cast<int>(task - static_cast<long long>(b) * a.c.heads);
+  if (b >= a.c.B) return;
+  int fault = 0;
+  const int* list = a.kept + b * a.kept_stride;
+  int kept = lane < a.n ? list[lane] : -1;
+  const long long len = *(a.c.lens + b);
+  const int drafted = *(a.new_lens + b);
+  const long long base = len - (drafted > 0 ? drafted : 0);
+  const int cap = a.c.capacity();
+  if (len > cap) fault |= kFaultPage;
+  long long count = 0;
+  int last = -1;  // the kept token before this turn's
+  for (int i0 = 0; i0 < a.n; i0 += 32) {
+    if (i0 > 0) kept = i0 + lane < a.n ? list[i0 + lane] : -1;
+    int before = __shfl_up_sync(0xffffffffu, kept, 1);
+    if (lane == 0) before = last;
+    last = __shfl_sync(0xffffffffu, kept, 31);
+    const bool ok = kept > before && kept < drafted;
+    const unsigned bad = __ballot_sync(0xffffffffu, !ok);
+    const int here = bad ? __ffs(bad) - 1 : 32;
+    if (here < 32 && i0 + here < a.n && __shfl_sync(0xffffffffu, kept, here) != -1) fault |= kFaultPage;
+    // Where this lane's token comes from and goes to; one that stays, or lies
+    // in no page, is not moved.
+    int from_page = -1, to_page = -1, from_row = 0, to_row = 0;
+    const long long from = base + kept, to = base + i0 + lane;
+    if (lane < here && from != to && to >= 0 && from < cap) {
+      const int fp = static_cast<int>(from) / a.c.page_size, tp = static_cast<int>(to) / a.c.page_size;
+      from_row = static_cast<int>(from) - fp * a.c.page_size;
+      to_row = static_cast<int>(to) - tp * a.c.page_size;
+      from_page = paged_page(a.c, b, fp, &fault);
+      to_page = paged_page(a.c, b, tp, &fault);
+    }
+    const unsigned moves = __ballot_sync(0xffffffffu, from_page >= 0 && to_page >= 0);
+    for (int half = 0; half < 32; half += kMoveAhead) {
+      if ((moves >> half & (0xffffffffu >> (32 - kMoveAhead))) == 0) continue;
+      for (int c0 = 0; c0 < 2 * a.cols; c0 += 32) {
+        const int c = c0 + lane;
+        const bool is_v = c >= a.cols, live = c < 2 * a.cols;
+        const long long* st = is_v ? a.c.vs : a.c.ks;
+        E* x = static_cast<E*>(is_v ? a.c.v : a.c.k) + h * st[1] + static_cast<long long>(is_v ? c - a.cols : c) * kVec;
+        V row[kMoveAhead];
+#pragma unroll
+        for (int p = 0; p < kMoveAhead; ++p) {
+          const long long pg = __shfl_sync(0xffffffffu, from_page, half + p);
+          const int in = __shfl_sync(0xffffffffu, from_row, half + p);
+          if (live && (moves >> (half + p) & 1u)) row[p] = *reinterpret_cast<const V*>(x + pg * st[0] + in * st[2]);
+        }
+#pragma unroll
+        for (int p = 0; p < kMoveAhead; ++p) {
+          const long long pg = __shfl_sync(0xffffffffu, to_page, half + p);
+          const int in = __shfl_sync(0xffffffffu, to_row, half + p);
+          if (live && (moves >> (half + p) & 1u)) *reinterpret_cast<V*>(x + pg * st[0] + in * st[2]) = row[p];
+        }
+      }
+    }
+    count += here;
+    if (here < 32) break;
+  }
+  if (h == 0 && lane == 0) {
+    const long long now = base + count;
+    a.lens[b] = static_cast<int>(now > 0 ? now : 0);
+  }
+  if (fault) atomicOr(&g_page_fault, fault);
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+
+size_t round_up(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
+
+// Places of a call's arrays of ints in its workspace.
+struct ResizePlan {
+  size_t have_at, start_at, order_at, bytes;
+};
+ResizePlan resize_plan(const AttnPagedCache* c) {
+  const size_t rows = round_up(sizeof(int) * static_cast<size_t>(c->B));
+  const long long most = static_cast<long long>(c->B) * c->table_width;
+  const size_t listed = static_cast<size_t>(most < c->num_pages ? most : c->num_pages);
+  return ResizePlan{0, rows, 2 * rows, 2 * rows + round_up(sizeof(int) * listed)};
+}
+struct ForkPlan {
+  size_t first_at, kids_at, copy_at, order_at, bytes;
+};
+ForkPlan fork_plan(const AttnPagedCache* c, int n) {
+  const size_t old = round_up(sizeof(int) * static_cast<size_t>(c->B)), now = round_up(sizeof(int) * static_cast<size_t>(n));
+  const size_t listed = static_cast<size_t>(n < c->num_pages ? n : c->num_pages);
+  return ForkPlan{0, old, 2 * old, 2 * old + now, 2 * old + now + round_up(sizeof(int) * listed)};
+}
+
+// Elements per access: 16 bytes where rows, strides and addresses of K and V
+// allow them, else one.
+int access_width(const AttnPagedCache* c) {
+  const int vec = c->dtype == ATTN_F32 ? 4 : 8;
+  bool fits = c->D % vec == 0 && aligned_to(c->k, 16) && aligned_to(c->v, 16);
+  for (int i = 0; i < 3; ++i) fits = fits && c->k_strides[i] % vec == 0 && c->v_strides[i] % vec == 0;
+  return fits ? vec : 1;
+}
+
+}  // namespace
+
+int page_word_read_clear_pages(cudaStream_t stream, int* host) {
+  static const int zero = 0;
+  return cudaMemcpyFromSymbolAsync(host, g_page_fault, sizeof(int), 0, cudaMemcpyDeviceToHost, stream) ==
+                     cudaSuccess &&
+                 cudaMemcpyToSymbolAsync(g_page_fault, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, stream) ==
+                     cudaSuccess
+             ? 0
+             : -1;
+}
+
+}  // namespace ra
+
+extern "C" int launch_kv_compact(const AttnPagedCache* cache, const int* new_lens, const int* kept,
+                                 long long kept_stride, int n, int* lens, cudaStream_t stream) {
+  using namespace ra;
+  CompactArgs a;
+  int st = check_paged_cache(cache, kCacheK | kCacheV, &a.c);
+  if (st != ATTN_OK) return st;
+  if (n < 0 || kept_stride < 0) return ATTN_ERR_INVALID_ARGUMENT;
+  if (cache->B == 0) return ATTN_OK;
+  if (!new_lens || (n > 0 && !kept) || !lens) return ATTN_ERR_INVALID_ARGUMENT;
+  if (!aligned_to(new_lens, 4) || !aligned_to(kept, 4) || !aligned_to(lens, 4)) return ATTN_ERR_MISALIGNED;
+  const long long blocks = (static_cast<long long>(cache->B) * cache->heads + kMoveWarps - 1) / kMoveWarps;
+  if (blocks > 0x7fffffffLL) return ATTN_ERR_INVALID_ARGUMENT;
+  st = check_device();
+  if (st != ATTN_OK) return st;
+  a.new_lens = new_lens;
+  a.kept = kept;
+  a.kept_stride = kept_stride;
+  a.n = n;
+  a.lens = lens;
+  const int vec = access_width(cache);
+  a.cols = cache->D / vec;
+  const dim3 grid(static_cast<unsigned>(blocks)), block(kMoveWarps * 32);
+  const auto kern = cache->dtype == ATTN_F32 ? (vec == 4 ? kv_compact_kernel<uint32_t, 4> : kv_compact_kernel<uint32_t, 1>)
+                                             : (vec == 8 ? kv_compact_kernel<uint16_t, 8> : kv_compact_kernel<uint16_t, 1>);
+  return launch_after(kern, grid, block, 0, stream, 1, true, a) ? ATTN_OK : ATTN_ERR_LAUNCH;
+}
+
+extern "C" int kv_resize_workspace_bytes(const AttnPagedCache* cache, size_t* bytes) {
+  using namespace ra;
+  if (!bytes) return ATTN_ERR_INVALID_ARGUMENT;
+  PagedView view;
+  const int st = check_paged_cache(cache, 0, &view);
+  if (st != ATTN_OK) return st;
+  *bytes = resize_plan(cache).bytes;
+  return ATTN_OK;
+}
+
+extern "C" int launch_kv_resize(const AttnPagedCache* cache, int* table, int* held, int* refs, int* missing,
+                                void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+  using namespace ra;
+  ResizeArgs a;
+  int st = check_paged_cache(cache, 0, &a.c);
+  if (st != ATTN_OK) return st;
+  if (cache->B == 0) return ATTN_OK;
+  if (table != cache->block_table || !held || (cache->num_pages > 0 && !refs) || !missing || !workspace)
+    return ATTN_ERR_INVALID_ARGUMENT;
+  if (!aligned_to(held, 4) || !aligned_to(refs, 4) || !aligned_to(missing, 4) || !aligned_to(workspace, 16))
+    return ATTN_ERR_MISALIGNED;
+  const ResizePlan p = resize_plan(cache);
+  if (workspace_bytes < p.bytes) return ATTN_ERR_INVALID_ARGUMENT;
+  st = check_device();
+  if (st != ATTN_OK) return st;
+  char* ws = static_cast<char*>(workspace);
+  a.table = table;
+  a.held = held;
+  a.refs = refs;
+  a.missing = missing;
+  a.have = reinterpret_cast<int*>(ws + p.have_at);
+  a.start = reinterpret_cast<int*>(ws + p.start_at);
+  a.order = reinterpret_cast<int*>(ws + p.order_at);
+  return launch_after(kv_resize_kernel, dim3(kFindCluster), dim3(kFindThreads), 0, stream, kFindCluster, true, a)
+             ? ATTN_OK
+             : ATTN_ERR_LAUNCH;
+}
+
+extern "C" int kv_fork_workspace_bytes(const AttnPagedCache* cache, int n, size_t* bytes) {
+  using namespace ra;
+  if (!bytes || n < 0) return ATTN_ERR_INVALID_ARGUMENT;
+  PagedView view;
+  const int st = check_paged_cache(cache, kCacheK | kCacheV, &view);
+  if (st != ATTN_OK) return st;
+  *bytes = fork_plan(cache, n).bytes;
+  return ATTN_OK;
+}
+
+extern "C" int launch_kv_fork(const AttnPagedCache* cache, const int* held, int* refs, const int* parents, int n,
+                              int* new_table, int* new_held, int* new_lens, int* missing, void* workspace,
+                              size_t workspace_bytes, cudaStream_t stream) {
+  using namespace ra;
+  ForkArgs a;
+  int st = check_paged_cache(cache, kCacheK | kCacheV, &a.c);
+  if (st != ATTN_OK) return st;
+  if (n < 0) return ATTN_ERR_INVALID_ARGUMENT;
+  if ((cache->B > 0 && !held) || (cache->num_pages > 0 && !refs) || !missing || !workspace ||
+      (n > 0 && (!parents || (cache->table_width > 0 && !new_table) || !new_held || !new_lens)))
+    return ATTN_ERR_INVALID_ARGUMENT;
+  for (const void* p : {static_cast<const void*>(held), static_cast<const void*>(refs), static_cast<const void*>(parents),
+                        static_cast<const void*>(new_table), static_cast<const void*>(new_held),
+                        static_cast<const void*>(new_lens), static_cast<const void*>(missing)})
+    if (!aligned_to(p, 4)) return ATTN_ERR_MISALIGNED;
+  if (!aligned_to(workspace, 16)) return ATTN_ERR_MISALIGNED;
+  const ForkPlan p = fork_plan(cache, n);
+  const int vec = access_width(cache);
+  a.cols = cache->D / vec;
+  // Rows per thread: up to two turns of kCopyAhead.
+  const long long per = 2LL * kCopyAhead * (256 / a.cols);
+  a.chunks = static_cast<int>((cache->page_size + per - 1) / per);
+  while (a.chunks > 1 && 2LL * cache->heads * a.chunks > 65535) a.chunks = (a.chunks + 1) / 2;
+  if (workspace_bytes < p.bytes || 2LL * cache->heads > 65535) return ATTN_ERR_INVALID_ARGUMENT;
+  st = check_device();
+  if (st != ATTN_OK) return st;
+  char* ws = static_cast<char*>(workspace);
+  a.held = held;
+  a.parents = parents;
+  a.refs = refs;
+  a.n = n;
+  a.new_table = new_table;
+  a.new_held = new_held;
+  a.new_lens = new_lens;
+  a.missing = missing;
+  a.first = reinterpret_cast<int*>(ws + p.first_at);
+  a.kids = reinterpret_cast<int*>(ws + p.kids_at);
+  a.copy = reinterpret_cast<int*>(ws + p.copy_at);
+  a.order = reinterpret_cast<int*>(ws + p.order_at);
+  if (!launch_after(kv_fork_plan_kernel, dim3(kFindCluster), dim3(kFindThreads), 0, stream, kFindCluster, true, a))
+    return ATTN_ERR_LAUNCH;
+  const int rows = n > cache->B ? n : cache->B;
+  if (rows == 0) return ATTN_OK;
+  const dim3 grid(static_cast<unsigned>(rows), static_cast<unsigned>(2 * cache->heads * a.chunks)), block(256);
+  const auto kern = cache->dtype == ATTN_F32
+                        ? (vec == 4 ? kv_fork_copy_kernel<uint32_t, 4> : kv_fork_copy_kernel<uint32_t, 1>)
+                        : (vec == 8 ? kv_fork_copy_kernel<uint16_t, 8> : kv_fork_copy_kernel<uint16_t, 1>);
+  return launch_after(kern, grid, block, 0, stream, 1, true, a) ? ATTN_OK : ATTN_ERR_LAUNCH;
+}

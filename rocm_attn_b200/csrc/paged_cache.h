@@ -44,10 +44,12 @@ int drop_arrival_requested();        // watchdog test build only
 // Faults a kernel records: a page or length out of range, a wait that ran out.
 constexpr int kFaultPage = 1, kFaultWait = 2;
 
-// Copies of the fault words of the two translation units into *host and
-// resets, queued on `stream` (see attn_get_status).
+// Copies of the fault words of the translation units into *host and resets,
+// queued on `stream` (see attn_get_status).
 int page_word_read_clear_decode(cudaStream_t stream, int* host);
 int page_word_read_clear_cache(cudaStream_t stream, int* host);
+int page_word_read_clear_pages(cudaStream_t stream, int* host);
+int page_word_read_clear_tree(cudaStream_t stream, int* host);
 
 inline bool aligned_to(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
