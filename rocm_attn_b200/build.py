@@ -109,13 +109,14 @@ def build_kernel_lib(force: bool = False, verbose: bool = False) -> str:
                 ("attn_decode.cu", "attn_decode.o", ()), ("kv_cache.cu", "kv_cache.o", ()),
                 ("attn_tree.cu", "attn_tree.o", ()), ("kv_pages.cu", "kv_pages.o", ()),
                 ("attn_kernel.cu", "attn_kernel_wdtest.o", ("RA_WATCHDOG_TEST",)),
-                ("attn_decode.cu", "attn_decode_wdtest.o", ("RA_WATCHDOG_TEST",))]
+                ("attn_decode.cu", "attn_decode_wdtest.o", ("RA_WATCHDOG_TEST",)),
+                ("attn_tree.cu", "attn_tree_wdtest.o", ("RA_WATCHDOG_TEST",))]
         with ThreadPoolExecutor(len(jobs)) as ex:
-            general, kernel, group, decode, cache, tree, pages, wd, wd_decode = ex.map(
+            general, kernel, group, decode, cache, tree, pages, wd, wd_decode, wd_tree = ex.map(
                 lambda j: _compile(os.path.join(CSRC, j[0]), os.path.join(OBJ_DIR, j[1]), defines=j[2],
                                    verbose=verbose), jobs)
         _link([kernel, group, general, decode, cache, tree, pages], KERNEL_LIB)
-        _link([wd, group, general, wd_decode, cache, tree, pages], WATCHDOG_TEST_LIB)
+        _link([wd, group, general, wd_decode, cache, wd_tree, pages], WATCHDOG_TEST_LIB)
     return KERNEL_LIB
 
 

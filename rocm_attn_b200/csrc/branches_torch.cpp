@@ -44,9 +44,15 @@ Tensor attn_tree(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, 
               "q's heads must be a multiple of the cache's heads");
   TORCH_CHECK(q.size(2) <= 1024, "at most 1024 drafted tokens per sequence");
   const int Hq = static_cast<int>(q.size(1)), S = static_cast<int>(q.size(2));
-  const Tensor x = q.size(3) > 1 && q.stride(3) != 1 ? q.contiguous() : q;
+  Tensor x = q.size(3) > 1 && q.stride(3) != 1 ? q.contiguous() : q;
   long long qs[3], tree_stride = 0;
   strides_of(x, 0, 3, qs);
+  // a copy of a q whose rows are not 16-byte aligned costs less than the kernel that could read it
+  const int64_t vec = 16 / x.element_size();
+  if (c.c.D % vec == 0 && (reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 || qs[0] % vec || qs[1] % vec || qs[2] % vec)) {
+    x = x.clone(at::MemoryFormat::Contiguous);
+    strides_of(x, 0, 3, qs);
+  }
   Tensor tree, n;
   if (parents) {
     tree = int_rows(*parents, "parents", c.c.B, dev, &tree_stride);
