@@ -45,6 +45,7 @@ struct TreeArgs {
   int Hq, group, S;
   int rows;                  // group * S rows per kv head, in row_tiles tiles of unit_rows
   int unit_rows, row_tiles;
+  int tile;                  // tokens per tile
   float scale_log2;
   const int* parents;        // or null: a chain
   long long parents_stride;
@@ -53,11 +54,19 @@ struct TreeArgs {
   float2* part_ml;           // [2 gridDim.x][unit_rows]
   float4* part_o;            // [2 gridDim.x][D4][unit_rows]: a row of threads writes and reads it in a row
   int D4;                    // D / 4, rounded up
-  // pos / page_size for pos < 2^31 as (umulhi(pos, ps_mul) + pos) >> ps_shift:
+  // x / page_size, x / S and x / tile for x < 2^31 as (umulhi(x, mul) + x) >> shift:
   // Granlund and Montgomery, Division by Invariant Integers using
   // Multiplication (1994), figure 4.1.
-  unsigned ps_mul;
-  int ps_shift;
+  unsigned ps_mul, s_mul, t_mul;
+  int ps_shift, s_shift, t_shift;
+  __device__ __forceinline__ int page_at(int pos) const {
+    const unsigned p = static_cast<unsigned>(pos);
+    return static_cast<int>((__umulhi(p, ps_mul) + p) >> ps_shift);
+  }
+  __device__ __forceinline__ int head_at(int row) const {
+    const unsigned r = static_cast<unsigned>(row);
+    return static_cast<int>((__umulhi(r, s_mul) + r) >> s_shift);
+  }
 };
 
 template <typename T> __device__ __forceinline__ float to_f32(T x);
@@ -92,22 +101,27 @@ struct Seq {
   int len, n, base;
 };
 
-__device__ __forceinline__ Seq seq_of(const TreeArgs& a, int b, int* fault) {
-  Seq s;
-  int n = a.S;
-  if (a.new_lens) {
-    n = *(a.new_lens + b);
-    if (n > a.S) {
-      *fault |= kFaultPage;
-      n = a.S;
-    }
-    if (n < 0) n = 0;
+// What memory holds of a sequence, asked for well before it is used.
+struct RawSeq {
+  int len, n;
+};
+__device__ __forceinline__ RawSeq raw_seq(const TreeArgs& a, int b) {
+  RawSeq r{0, 0};
+  if (b < a.c.B) {
+    r.len = *(a.c.lens + b);
+    r.n = a.new_lens ? *(a.new_lens + b) : a.S;
   }
-  s.n = n;
-  s.base = max(*(a.c.lens + b), 0) - n;
-  s.len = paged_len(a.c, b, fault);
+  return r;
+}
+__device__ __forceinline__ Seq seq_from(const TreeArgs& a, const RawSeq& r, int* fault) {
+  Seq s;
+  s.n = max(min(r.n, a.S), 0);
+  s.len = max(min(r.len, a.c.capacity()), 0);
+  s.base = max(r.len, 0) - s.n;
+  if (r.n > a.S || r.len > a.c.capacity()) *fault |= kFaultPage;
   return s;
 }
+__device__ __forceinline__ Seq seq_of(const TreeArgs& a, int b, int* fault) { return seq_from(a, raw_seq(a, b), fault); }
 
 // A place in the row of tiles: tile t of the T tiles of the unit (sequence b,
 // kv head h, tile rt of its rows).
@@ -116,23 +130,24 @@ struct Cursor {
   Seq s;
 };
 
-template <int kTile>
-__device__ __forceinline__ int tiles_of(const Seq& s) {
-  return s.n > 0 ? (s.len + kTile - 1) / kTile : 0;
+__device__ __forceinline__ int tiles_of(const TreeArgs& a, const Seq& s) {
+  const unsigned x = static_cast<unsigned>(s.len + a.tile - 1);
+  return s.n > 0 ? static_cast<int>((__umulhi(x, a.t_mul) + x) >> a.t_shift) : 0;
 }
 
-template <int kTile>
-__device__ __forceinline__ void advance(const TreeArgs& a, Cursor& c, int* fault) {
-  if (++c.t < c.T) return;
+// To the next unit; `ahead` is the sequence behind c.b, on its way.
+__device__ __forceinline__ void next_unit(const TreeArgs& a, Cursor& c, RawSeq& ahead, int* fault) {
   c.t = 0;
   if (++c.rt < a.row_tiles) return;
   c.rt = 0;
   if (++c.h < a.c.heads) return;
   c.h = 0;
   c.T = 0;
+#pragma unroll 1
   while (c.T == 0 && ++c.b < a.c.B) {
-    c.s = seq_of(a, c.b, fault);
-    c.T = tiles_of<kTile>(c.s);
+    c.s = seq_from(a, ahead, fault);
+    ahead = raw_seq(a, c.b + 1);
+    c.T = tiles_of(a, c.s);
   }
 }
 
@@ -157,7 +172,7 @@ struct ScheduleSmem {
 // Works out this CTA's run and its first tile; all its threads share the
 // batch.  The host keeps the number of tiles the block table can name below
 // 2^31.
-template <int kTile, int kThreads>
+template <int kThreads>
 __device__ __forceinline__ Cursor schedule(const TreeArgs& a, ScheduleSmem<kThreads>& s, Run* run, int* fault) {
   constexpr int kWarps = kThreads / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -166,9 +181,10 @@ __device__ __forceinline__ Cursor schedule(const TreeArgs& a, ScheduleSmem<kThre
   const int b0 = from < a.c.B ? static_cast<int>(from) : a.c.B, b1 = min(a.c.B - b0, seg) + b0;
   int mine = 0, T = 0;
   Seq q = {};
+#pragma unroll 1
   for (int b = b0; b < b1; ++b) {
     q = seq_of(a, b, fault);
-    T = tiles_of<kTile>(q);
+    T = tiles_of(a, q);
     mine += T;
   }
   int upto = mine;
@@ -194,9 +210,10 @@ __device__ __forceinline__ Cursor schedule(const TreeArgs& a, ScheduleSmem<kThre
   if (run->n > 0 && run->first >= before * units && run->first - before * units < mine * units) {
     int in = run->first - before * units, b = b0;
     if (seg > 1) {
+#pragma unroll 1
       for (;; ++b) {
         q = seq_of(a, b, fault);
-        T = tiles_of<kTile>(q);
+        T = tiles_of(a, q);
         if (in < T * units || b + 1 >= b1) break;
         in -= T * units;
       }
@@ -205,7 +222,7 @@ __device__ __forceinline__ Cursor schedule(const TreeArgs& a, ScheduleSmem<kThre
     s.first = Cursor{b, h, hu - h * a.row_tiles, in - hu * T, T, q};
   }
   __syncthreads();
-  return s.first;
+  return run->n > 0 ? s.first : Cursor{};  // nobody has written a first tile of an empty run
 }
 
 // Output rows of sequences without tokens, or without drafted ones, are zeros.
@@ -213,52 +230,67 @@ template <typename T, int kThreads>
 __device__ __forceinline__ void zero_empty_rows(const TreeArgs& a, int* fault) {
   const long long bytes = static_cast<long long>(a.Hq) * a.S * a.c.D * sizeof(T);
   const bool wide = bytes % 16 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0;
+#pragma unroll 1
   for (int b = blockIdx.x; b < a.c.B; b += gridDim.x) {
     const Seq s = seq_of(a, b, fault);
     if (s.len > 0 && s.n > 0) continue;
     unsigned char* o = static_cast<unsigned char*>(a.out) + b * bytes;
     if (wide) {
+#pragma unroll 1
       for (long long i = threadIdx.x; i < bytes / 16; i += kThreads) reinterpret_cast<uint4*>(o)[i] = make_uint4(0, 0, 0, 0);
     } else {
+#pragma unroll 1
       for (long long i = threadIdx.x; i < bytes / static_cast<long long>(sizeof(T)); i += kThreads)
         reinterpret_cast<T*>(o)[i] = from_f32<T>(0.f);
     }
   }
 }
 
-// The drafted tokens that each one follows, checked: par[s] < s.
-template <int kThreads>
-__device__ __forceinline__ void load_parents(const TreeArgs& a, int b, int n, int* par, int thread, int* fault) {
-  for (int s = thread; s < n; s += kThreads) {
-    int p = s - 1;
-    if (a.parents) {
-      p = *(a.parents + b * a.parents_stride + s);
-      if (p < -1 || p >= s) {
-        *fault |= kFaultPage;
-        p = -1;
-      }
-    }
-    par[s] = p;
+// The drafted tokens that each one follows: the first kParShared of them in
+// shared memory, the others where they are.
+constexpr int kParShared = 256;
+struct Tree {
+  const int* shared;
+  const int* global;  // null: a chain
+  __device__ __forceinline__ int parent(int s, int* fault) const {
+    if (!global) return s - 1;
+    const int p = s < kParShared ? shared[s] : global[s];
+    if (p >= -1 && p < s) return p;
+    *fault |= kFaultPage;
+    return -1;
   }
-}
-
-// One of them, where they are not at hand.
-__device__ __noinline__ int parent_of(const TreeArgs& a, int b, int s) {
-  const int p = a.parents ? *(a.parents + b * a.parents_stride + s) : s - 1;
-  return p < -1 || p >= s ? -1 : p;
+};
+__device__ __forceinline__ const int* tree_of(const TreeArgs& a, int b) {
+  return a.parents ? a.parents + b * a.parents_stride : nullptr;
 }
 
 // Bits of the kWords * 32 positions from `pos0` on that drafted token s of the
 // sequence may see (s < n), beside those the sequence has there.
 template <int kWords>
-__device__ __forceinline__ void visible(const Seq& q, int s, int pos0, const int* par, uint32_t (&bits)[kWords]) {
+__device__ __forceinline__ void visible(const Seq& q, int s, int pos0, const Tree& tree, uint32_t (&bits)[kWords],
+                                        int* fault) {
 #pragma unroll
   for (int w = 0; w < kWords; ++w) {
     // positions below base: all of them
     const int in = q.base - (pos0 + 32 * w);
     bits[w] = in >= 32 ? 0xffffffffu : in > 0 ? (1u << in) - 1u : 0u;
   }
-  for (int p = s; p >= 0; p = par[p]) {
+  if (!tree.global) {
+    // a chain: also those up to s
+#pragma unroll
+    for (int w = 0; w < kWords; ++w) {
+      const int in = q.base + s + 1 - (pos0 + 32 * w);
+      const uint32_t upto = in >= 32 ? 0xffffffffu : in > 0 ? (1u << in) - 1u : 0u;
+      bits[w] |= upto;
+    }
+    if (q.base < 0) {
+#pragma unroll
+      for (int w = 0; w < kWords; ++w) bits[w] = q.base + s >= 0 ? bits[w] : 0u;
+    }
+    return;
+  }
+#pragma unroll 1
+  for (int p = s; p >= 0; p = tree.parent(p, fault)) {
     const int at = q.base + p - pos0;
     if (at < 0) break;  // ancestors only lie further ahead
 #pragma unroll
@@ -270,8 +302,7 @@ __device__ __forceinline__ void visible(const Seq& q, int s, int pos0, const int
 // Where token `pos` lies: its physical page and row, or page -1.
 __device__ __forceinline__ int page_of(const TreeArgs& a, const Cursor& c, int pos, int* row, int* fault) {
   if (pos >= c.s.len) return -1;
-  const unsigned p = static_cast<unsigned>(pos);
-  const int lp = static_cast<int>((__umulhi(p, a.ps_mul) + p) >> a.ps_shift);
+  const int lp = a.page_at(pos);
   *row = pos - lp * a.c.page_size;
   return paged_page(a.c, c.b, lp, fault);
 }
@@ -314,7 +345,7 @@ struct SimtCfg {
   static constexpr int kPitch = kDP + 4;  // floats; rows 4 banks apart
   static constexpr int kPPitch = kSimtTile + 4;
   static constexpr size_t kBytes = sizeof(float) * ((kSimtRows + kSimtTile) * kPitch + kSimtRows * kPPitch) +
-                                   sizeof(long long) * 2 * kSimtTile + sizeof(int) * kMaxDrafted;
+                                   sizeof(long long) * 2 * kSimtTile + sizeof(int) * kParShared;
 };
 
 template <typename T, int kDP>
@@ -327,6 +358,7 @@ __global__ void __launch_bounds__(kSimtThreads) attn_tree_simt_kernel(const __gr
   float* s_p = s_kv + kSimtTile * C::kPitch;
   long long* s_at = reinterpret_cast<long long*>(s_p + kSimtRows * C::kPPitch);  // K, then V offsets; -1: no token
   int* s_par = reinterpret_cast<int*>(s_at + 2 * kSimtTile);
+  Tree tree{s_par, nullptr};
   __shared__ ScheduleSmem<kSimtThreads> s_sched;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, D = a.c.D;
   int fault = 0;
@@ -334,8 +366,9 @@ __global__ void __launch_bounds__(kSimtThreads) attn_tree_simt_kernel(const __gr
   grid_dependency_wait();
   if (tid == 0) a.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
   Run run;
-  Cursor cur = schedule<kSimtTile>(a, s_sched, &run, &fault);
+  Cursor cur = schedule(a, s_sched, &run, &fault);
   zero_empty_rows<T, kSimtThreads>(a, &fault);
+  RawSeq ahead = raw_seq(a, cur.b + 1);
   float o[4][kCols], m[4], l[4];
   bool begun = cur.t == 0, fresh = true;
   const T* kbase = static_cast<const T*>(a.c.k);
@@ -357,7 +390,8 @@ __global__ void __launch_bounds__(kSimtThreads) attn_tree_simt_kernel(const __gr
         const int head = gr / a.S, s = gr - head * a.S;
         s_q[r * C::kPitch + d] = gr < a.rows && d < D ? to_f32(q[head * a.q_h + s * a.q_s + d]) : 0.f;
       }
-      load_parents<kSimtThreads>(a, cur.b, cur.s.n, s_par, tid, &fault);
+      tree.global = tree_of(a, cur.b);
+      for (int e = tid; tree.global && e < min(cur.s.n, kParShared); e += kSimtThreads) s_par[e] = tree.global[e];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         m[r] = -INFINITY;
@@ -399,7 +433,7 @@ __global__ void __launch_bounds__(kSimtThreads) attn_tree_simt_kernel(const __gr
     uint32_t see[2] = {0, 0};
     if (tx < 4) {
       const int gr = cur.rt * kSimtRows + ty * 4 + tx, s = gr % a.S;
-      if (gr < a.rows && s < cur.s.n) visible<2>(cur.s, s, pos0, s_par, see);
+      if (gr < a.rows && s < cur.s.n) visible<2>(cur.s, s, pos0, tree, see, &fault);
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -484,7 +518,7 @@ __global__ void __launch_bounds__(kSimtThreads) attn_tree_simt_kernel(const __gr
       fresh = true;
     }
     __syncthreads();  // the tile's buffers are free
-    advance<kSimtTile>(a, cur, &fault);
+    if (++cur.t == cur.T) next_unit(a, cur, ahead, &fault);
   }
   if (fault) atomicOr(&g_page_fault, fault);
 }
@@ -493,100 +527,146 @@ __global__ void __launch_bounds__(kSimtThreads) attn_tree_simt_kernel(const __gr
 // Tensor-core kernel: fp16 and bf16, D a multiple of 8, 16-byte rows
 // ---------------------------------------------------------------------------
 
-// 128 rows (or two tiles of 128) of a kv head are the rows of the tcgen05
-// products, 64 tokens a tile: S = Q K^T into tensor memory, a thread per row
-// takes the softmax of it and writes P over it, O += P V.  Up to 128 rows the
-// floor is the time to read the cache: 64 tokens of D = 128 are 32 KB, 1400
-// clocks of an SM's share of the bandwidth, beside 384 + 256 of the two products and about 800
-// of the softmax.  Warp roles:
-//   warps 0-3 (4-7)  softmax of row tile 0 (1), and its Q and O
-//   next warp        the products, one elected lane; V of tiles that end early
-//   last warp        copies: boxes of K and V rows by TMA, page ids looked up a
-//                    group of tiles ahead
-// S has two buffers, so S(j + 1) is computed while the softmax takes S(j); the
-// products are issued S(j + 1), P(j) V(j), and at the end of a unit P(j) V(j)
-// first, as the next unit's Q takes the place of this one's.  Two CTAs per SM
-// where they fit hide each other's ends of units and waits.
-template <int kD_, int kTiles_>
+// The rows of a kv head are the rows of the tcgen05 products: S = Q K^T into
+// tensor memory, a thread per row takes the softmax of it and writes P over it,
+// O += P V.  Up to 128 rows the floor is the time to read the cache, 2800 clocks
+// for 64 KB as an SM's share, the K and V of 128 tokens at D = 128.
+//   up to 128 rows   tiles of 64 tokens, two score buffers, so that S(j + 1) is
+//                    there when the softmax of tile j ends; two CTAs per SM (one
+//                    at D = 256) hide each other's waits and ends of units.
+//                    Q of the next unit is copied during this one where there
+//                    is room: a load takes some 5000 clocks beside so many copies.
+//   more rows        256 at a time over the same tiles of 128 tokens: two
+//                    streams, each with its S and O in tensor memory and a
+//                    warpgroup for the softmax, one CTA per SM.
+// Warp roles: softmax warpgroups, then one warp of which a thread issues the
+// products, and one that copies K and V (one for each with two streams), page ids
+// looked up ahead: boxes of rows by TMA where 8 divides the page size, else by
+// 16-byte asynchronous copies.  It also mends V of tiles that end early.
+template <int kD_, bool kTwo_>
 struct TcCfg {
-  static constexpr int kD = kD_, kTiles = kTiles_;
-  static constexpr int kBN = 64;
-  static constexpr int kRows = 128 * kTiles;
-  static constexpr int kCtas = kTiles == 1 && kD <= 128 ? 2 : 1;  // per SM
-  static constexpr int kStages = kD == 64 ? 5 : kTiles == 2 ? 4 : 2;  // of K and of V
-  static constexpr uint32_t kQBytes = 128u * kD * 2;      // a Q tile
-  static constexpr uint32_t kQBlock = 128u * 128;         // 64 columns of it
-  static constexpr uint32_t kKVBytes = kBN * kD * 2u;     // a K or V tile
-  static constexpr uint32_t kKVBlock = kBN * 128u;        // 64 columns of it
-  static constexpr size_t kSmemBytes = 1024 + kTiles * kQBytes + 2 * kStages * kKVBytes;
-  static constexpr uint32_t kColO = 2 * kTiles * kBN;     // after the S buffers
-  static constexpr uint32_t kTmemCols = kColO + kTiles * kD <= 256 ? 256 : 512;
-  static constexpr int kMmaWarp = 4 * kTiles, kTmaWarp = kMmaWarp + 1;
-  static constexpr int kThreads = 128 * kTiles + 64;
+  static constexpr int kD = kD_;
+  static constexpr bool kTwo = kTwo_;
+  static constexpr int kStreams = kTwo ? 2 : 1;
+  static constexpr int kCtas = kTwo || kD == 256 ? 1 : 2;  // per SM
+  static constexpr int kBN = kTwo ? 128 : 64;              // tokens per tile
+  static constexpr int kRows = 128 * kStreams;
+  static constexpr uint32_t kQBytes = 128u * kD * 2;       // a Q tile
+  // Q tiles there is room for: two row tiles; at D = 64 this unit's and the
+  // next one's; otherwise one, or two of up to 64 rows.
+  static constexpr int kQTiles = kTwo || kD == 64 ? 2 : 1;
+  static constexpr uint32_t kSlotBytes = kBN * kD * 2u;  // a K or V tile
+  static constexpr uint32_t kSlotBlock = kBN * 128u;     // 64 columns of it
+  static constexpr int kKSlots = kTwo ? (kD == 64 ? 5 : 2) : kD == 64 ? 4 : 2;
+  static constexpr int kVSlots = kTwo ? (kD == 64 ? 5 : 3) : kD == 64 ? 4 : kD == 128 ? 2 : 3;
+  static constexpr uint32_t kColO = 2 * kBN;               // after the scores: two buffers, or one of each stream
+  static constexpr uint32_t kTmemCols = kColO + kStreams * kD <= 256 ? 256 : 512;
+  static constexpr int kSoftThreads = 128 * kStreams;
+  static constexpr int kMmaWarp = 4 * kStreams, kCopyWarp = kMmaWarp + 1;
+  static constexpr int kThreads = kSoftThreads + 32 + 32 * kStreams;
+  static constexpr uint32_t kTileBytes = kQTiles * kQBytes + (kKSlots + kVSlots) * kSlotBytes;
+  static constexpr size_t kCtlBytes = 3072;
+  static constexpr size_t kSmemBytes = kTileBytes + kCtlBytes;
+  static_assert(kSmemBytes <= (kCtas == 1 ? 232448 : 115712), "shared memory of a CTA");
 };
-constexpr int kHoles = 8;  // tiles whose holes are remembered: a ring deeper than the stages by two
+// A wait that did not end at once: mbar_wait's polling, once in the program.
+__device__ __noinline__ bool wait_long(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* code,
+                                       unsigned long long limit_ns) {
+  return mbar_wait(bar, parity, abort_flag, code, 1, limit_ns);
+}
+
+constexpr int kHoles = 8;  // tiles, and units, that are remembered: more than the copies may be ahead
 
 template <typename C>
-struct __align__(8) TcCtl {
-  uint64_t q_full[C::kTiles];
-  uint64_t k_full[C::kStages], k_empty[C::kStages], v_full[C::kStages], v_empty[C::kStages];
-  uint64_t s_full[C::kTiles][2], p_full[C::kTiles][2], pv_done[C::kTiles], o_done[C::kTiles];
-  uint64_t mma_done, group_met[C::kTiles];
-  unsigned long long hole[kHoles];  // tokens of a tile that lie in no page of the cache
-  uint32_t odd[2][kMaxDrafted / 32];  // drafted tokens of this unit (the last) with infinite or NaN values
+struct __align__(16) TcCtl {
+  uint64_t q_full;                          // a unit's Q (kSoftThreads arrivals)
+  uint64_t k_full[C::kKSlots], k_empty[C::kKSlots], v_full[C::kVSlots], v_empty[C::kVSlots];
+  uint64_t v_raw[C::kVSlots];               // V has come, and is to be mended before it is full
+  uint64_t s_full[2], p_full[2];            // of a score buffer
+  uint64_t o_done;                          // the last product of a unit
+  uint64_t met;                             // the softmax threads meet
+  uint64_t mma_done;
+  unsigned long long hole[kHoles][2];       // tokens of a tile that lie in no page of the cache
+  int4 mend[kHoles];                        // of tiles to mend: first drafted row, rows, draft of row 0, unit
+  uint32_t odd[kHoles][kMaxDrafted / 256];  // of a unit: eights of drafted tokens with infinite or NaN values
+  ScheduleSmem<C::kThreads> sched;
   uint32_t tmem_base;
   int abort_flag, code;
+  int par[2][kParShared];
 };
 
 // The two caches as [num_pages, heads, page_size, D] tensors read in boxes of
 // `rows` rows by 64 columns.
 struct TcMaps {
   CUtensorMap k, v;
-  int rows;
+  int rows, boxes;  // rows of a box, boxes of a tile; 0: no boxes, 16-byte copies
   unsigned long long wait_ns;
   int lose;  // watchdog test build only: CTA 0's first K copy is for bytes that never come
 };
 
-template <bool kBf16, int kD, int kTiles>
-__global__ void __launch_bounds__(TcCfg<kD, kTiles>::kThreads, TcCfg<kD, kTiles>::kCtas)
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+// Whether the phase has completed, without waiting for it.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok)
+      : "r"(smem_addr(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+template <bool kBf16, int kD, bool kTwo>
+__global__ void __launch_bounds__(TcCfg<kD, kTwo>::kThreads, TcCfg<kD, kTwo>::kCtas)
     attn_tree_tc_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ TcMaps maps) {
-  using C = TcCfg<kD, kTiles>;
+  using C = TcCfg<kD, kTwo>;
   using T = typename std::conditional<kBf16, __nv_bfloat16, __half>::type;
-  constexpr int kBN = C::kBN, kStages = C::kStages, kThreads = C::kThreads;
-  static_assert(kHoles >= kStages + 2, "the softmax may be two tiles behind the copies' ring");
+  constexpr int kBN = C::kBN, kWords = kBN / 32;
+  static_assert(sizeof(TcCtl<C>) <= C::kCtlBytes, "control block");
   // fp16 has its full precision down to 2^-14: P is kept times 2^7 (at most
   // 2^15, as the maximum it refers to may be 2^8 below the largest score).
   constexpr float kUp = kBf16 ? 0.f : 7.f;
 
-  extern __shared__ uint8_t smem_raw[];
-  __shared__ TcCtl<C> ctl;
-  __shared__ ScheduleSmem<kThreads> s_sched;
-  __shared__ int s_par[kTiles][kMaxDrafted];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* sQ = smem;
-  uint8_t* sK = smem + kTiles * C::kQBytes;
-  uint8_t* sV = sK + kStages * C::kKVBytes;
+  uint8_t* sK = smem + C::kQTiles * C::kQBytes;
+  uint8_t* sV = sK + C::kKSlots * C::kSlotBytes;
+  TcCtl<C>& ctl = *reinterpret_cast<TcCtl<C>*>(smem + C::kTileBytes);
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x) / 32, 0), lane = threadIdx.x & 31;
   int fault = 0;
 
   if (threadIdx.x == 0) {
     ctl.abort_flag = ctl.code = 0;
-    for (int t = 0; t < kTiles; ++t) {
-      mbar_init(&ctl.q_full[t], 128);
-      for (int i = 0; i < 2; ++i) {
-        mbar_init(&ctl.s_full[t][i], 1);
-        mbar_init(&ctl.p_full[t][i], 128);
-      }
-      mbar_init(&ctl.pv_done[t], 1);
-      mbar_init(&ctl.o_done[t], 1);
-      mbar_init(&ctl.group_met[t], 128);
-    }
-    for (int s = 0; s < kStages; ++s) {
+    mbar_init(&ctl.q_full, C::kSoftThreads);
+    for (int s = 0; s < C::kKSlots; ++s) {
       mbar_init(&ctl.k_full[s], 1);
       mbar_init(&ctl.k_empty[s], 1);
+    }
+    for (int s = 0; s < C::kVSlots; ++s) {
       mbar_init(&ctl.v_full[s], 1);
       mbar_init(&ctl.v_empty[s], 1);
+      mbar_init(&ctl.v_raw[s], 1);
     }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&ctl.s_full[s], 1);
+      mbar_init(&ctl.p_full[s], 128);
+    }
+    mbar_init(&ctl.o_done, 1);
+    mbar_init(&ctl.met, C::kSoftThreads);
     mbar_init(&ctl.mma_done, 1);
     fence_mbar_init();
   }
@@ -594,7 +674,7 @@ __global__ void __launch_bounds__(TcCfg<kD, kTiles>::kThreads, TcCfg<kD, kTiles>
     tmem_alloc(smem_addr(&ctl.tmem_base), C::kTmemCols);
     tmem_relinquish();
   }
-  if (warp == C::kTmaWarp && lane == 0) {
+  if (warp == C::kCopyWarp && lane == 0) {
     tma_prefetch_desc(&maps.k);
     tma_prefetch_desc(&maps.v);
   }
@@ -608,155 +688,74 @@ __global__ void __launch_bounds__(TcCfg<kD, kTiles>::kThreads, TcCfg<kD, kTiles>
   grid_dependency_wait();
   if (threadIdx.x == 0) a.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
   Run run;
-  Cursor cur = schedule<kBN>(a, s_sched, &run, &fault);
+  Cursor cur = schedule(a, ctl.sched, &run, &fault);
   const int n = run.n;
-  zero_empty_rows<T, kThreads>(a, &fault);
+  RawSeq ahead = raw_seq(a, cur.b + 1);
 
   const unsigned long long wait_ns = maps.wait_ns;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
-    const bool there =
-        __all_sync(0xffffffffu, mbar_wait(bar, parity, &ctl.abort_flag, &ctl.code, 1, wait_ns));
+    const bool there = __all_sync(0xffffffffu, mbar_try_wait(smem_addr(bar), parity) ||
+                                                   wait_long(bar, parity, &ctl.abort_flag, &ctl.code, wait_ns));
     if (!there) fault |= kFaultWait;
     return there;
   };
-  int last_k = -1, last_v = -1;  // last tiles whose copies went out (copying warp)
+  int last_copy[2] = {-1, -1};  // the last tile whose copies of K and V went out (copying warps)
+  // The tile of V to mend, when the copies of the next one are out, and the
+  // parities of v_raw.
+  int late = -1, late_slot = 0;
+  uint32_t raw = 0;
+  // Q of the next unit is copied during this one where there is room for two.
+  const bool early_q = !kTwo && (C::kQTiles == 2 || a.rows <= 64);
+  const int q_rows = early_q && C::kQTiles == 1 ? 64 : 128;  // of a Q tile
+  const uint32_t q_block = q_rows * 128, q_tile = q_block * (kD / 64);
 
-  if (warp == C::kTmaWarp) {
+  if (warp >= C::kCopyWarp) {
     // ---------------------------------------------------------------- copies
-    const int R = maps.rows, boxes = kBN / R, group = 32 / boxes;  // tiles per look-up
-    const uint64_t policy = a.row_tiles > 1 ? l2_policy_evict_last() : l2_policy_evict_first();
-    const int my_tile = lane / boxes, my_box = lane % boxes;
-    struct Group {
-      int page, row, live;  // of this lane's box: table entry, first row, rows that are tokens
-      int count, h;
-    };
-    Cursor look = cur;
-    int left = n;
-    auto look_up = [&](Group& g) {
-      g.count = min(min(group, look.T - look.t), left);
-      g.h = look.h;
-      g.page = -1;
-      g.row = g.live = 0;
-      if (left <= 0) return;
-      const int pos = (look.t + my_tile) * kBN + my_box * R;
-      if (my_tile < g.count && pos < look.s.len) {
-        const unsigned p = static_cast<unsigned>(pos);
-        const int lp = static_cast<int>((__umulhi(p, a.ps_mul) + p) >> a.ps_shift);
-        g.row = pos - lp * a.c.page_size;
-        g.live = min(R, look.s.len - pos);
-        g.page = *(a.c.table + static_cast<long long>(look.b) * a.c.table_stride + lp);
-      }
-      left -= g.count;
-      look.t += g.count - 1;
-      if (left > 0) advance<kBN>(a, look, &fault);
-    };
-    Group now, next;
-    look_up(now);
-    look_up(next);
-    int in = 0;
+    const bool does[2] = {!kTwo || warp == C::kCopyWarp, !kTwo || warp != C::kCopyWarp};  // K, V
+    int left = n, slot[2] = {0, 0};
+    uint32_t parity[2] = {1, 1};  // of the slots' `empty`: the first round finds it so
     bool ok = true;
-    for (int j = 0; j < n && ok; ++j) {
-      const int slot = j % kStages;
-      const uint32_t parity = ((j / kStages) & 1) ^ 1;
-      const bool mine = my_tile == in && now.live > 0;
-      const bool there = mine && static_cast<unsigned>(now.page) < static_cast<unsigned>(a.c.num_pages);
-      uint32_t bytes = __popc(__ballot_sync(0xffffffffu, there)) * R * (kD * 2);
-      unsigned long long hole = 0;
-      if (__any_sync(0xffffffffu, mine && !there)) {
-        unsigned long long bits = 0;
-        if (mine && !there) {
-          fault |= kFaultPage;
-          bits = (R == 64 ? ~0ull : (1ull << R) - 1) << (my_box * R);
-        }
-        const uint32_t lo = __reduce_or_sync(0xffffffffu, static_cast<uint32_t>(bits));
-        const uint32_t hi = __reduce_or_sync(0xffffffffu, static_cast<uint32_t>(bits >> 32));
-        hole = static_cast<unsigned long long>(hi) << 32 | lo;
-      }
-      ok = wait(&ctl.k_empty[slot], parity);
-      if (!ok) break;
-      if (lane == 0) {
-        ctl.hole[j % kHoles] = hole;
-        uint32_t expected = bytes;
-#ifdef RA_WATCHDOG_TEST
-        if (maps.lose && blockIdx.x == 0 && j == 0) expected += 16;
-#endif
-        mbar_arrive_expect_tx(&ctl.k_full[slot], expected);
-      }
-      __syncwarp();
-      if (there) {
-#pragma unroll
-        for (int c = 0; c < kD / 64; ++c)
-          tma_load_4d(smem_addr(sK + slot * C::kKVBytes + c * C::kKVBlock + my_box * R * 128), &maps.k,
-                      &ctl.k_full[slot], c * 64, now.row, now.h, now.page, policy);
-      }
-      last_k = j;
-      ok = wait(&ctl.v_empty[slot], parity);
-      if (!ok) break;
-      if (lane == 0) mbar_arrive_expect_tx(&ctl.v_full[slot], bytes);
-      __syncwarp();
-      if (there) {
-#pragma unroll
-        for (int c = 0; c < kD / 64; ++c)
-          tma_load_4d(smem_addr(sV + slot * C::kKVBytes + c * C::kKVBlock + my_box * R * 128), &maps.v,
-                      &ctl.v_full[slot], c * 64, now.row, now.h, now.page, policy);
-      }
-      last_v = j;
-      if (++in == now.count) {
-        in = 0;
-        now = next;
-        look_up(next);
-      }
-    }
-  } else if (warp == C::kMmaWarp) {
-    // -------------------------------------------------------------- products
-    constexpr uint32_t idesc_s = umma_idesc_f16(kBf16, 128, kBN, false);
-    constexpr uint32_t idesc_o = umma_idesc_f16(kBf16, 128, kD, true);
-    const bool leader = elect_one();
-    int unit = 0;  // of the run, at tile j (+ 1 while the next unit's S is issued)
-    auto issue_s = [&](int j, bool first, int u) {
-      const int slot = j % kStages;
-      if (!wait(&ctl.k_full[slot], (j / kStages) & 1)) return false;
-      if (first) {
-        for (int t = 0; t < kTiles; ++t)
-          if (!wait(&ctl.q_full[t], u & 1)) return false;
-      }
-      tc_fence_after();
-      if (leader) {
-        const uint64_t kd = sw128_desc(smem_addr(sK + slot * C::kKVBytes), 16, 1024);
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
-          const uint64_t qd = sw128_desc(smem_addr(sQ + t * C::kQBytes), 16, 1024);
-#pragma unroll
-          for (int k = 0; k < kD / 16; ++k)
-            umma_ss(tmem + (2 * t + (j & 1)) * kBN, sw128_desc_step(qd, (k / 4) * C::kQBlock + (k % 4) * 32),
-                    sw128_desc_step(kd, (k / 4) * C::kKVBlock + (k % 4) * 32), idesc_s, k > 0 ? 1u : 0u);
-          umma_commit(&ctl.s_full[t][j & 1]);
-        }
-        umma_commit(&ctl.k_empty[slot]);
-      }
-      __syncwarp();
-      return true;
+    auto full = [&](int kv, int s) { return kv ? &ctl.v_full[s] : &ctl.k_full[s]; };
+    auto empty = [&](int kv, int s) { return kv ? &ctl.v_empty[s] : &ctl.k_empty[s]; };
+    auto to_next = [&](int kv) {
+      if (++slot[kv] == (kv ? C::kVSlots : C::kKSlots)) slot[kv] = 0, parity[kv] ^= 1;
     };
+
     // V of a tile as the product may see it: rows that are no tokens are zeros
     // (no weight, not even zero, may meet what lies there), and so are infinite and
     // NaN values of drafted tokens, which some rows do not follow; the rows
     // that do add them at the end.
-    auto mend_v = [&](uint8_t* v, const Cursor& c, unsigned long long hole, int u) {
-      const int pos0 = c.t * kBN, live = c.s.len - pos0;
-      unsigned long long absent = hole;
-      if (live < kBN) absent |= ~0ull << live;
-      if (absent) {
-        for (int e = lane; e < kBN * (kD / 8); e += 32) {
-          const int r = e / (kD / 8), col = e % (kD / 8);
-          if (absent >> r & 1u)
-            *reinterpret_cast<uint4*>(v + (col / 8) * C::kKVBlock + r * 128 + (((col % 8) ^ (r & 7)) << 4)) =
-                make_uint4(0, 0, 0, 0);
-        }
+    constexpr int kCols = kD / 8, kPer = kCols >= 32 ? 1 : 32 / kCols;  // 16-byte columns of a row, rows at once
+    const int col = lane % kCols, my_row = lane / kCols;
+    int unit = -1;
+    bool unit_begins = true;
+    // Notes what there is to mend of tile j, cur's or the look-up's; whether there is anything.
+    auto note_mend = [&](int j, const Seq& q, int t, bool begins, bool holes) {
+      if (begins) {
+        ++unit;
+        if (lane < kMaxDrafted / 256) ctl.odd[unit % kHoles][lane] = 0;
       }
-      const int from = max(0, c.s.base - pos0), rows = min(live, kBN) - from;
-      for (int e = lane; e < rows * (kD / 8); e += 32) {
-        const int r = from + e / (kD / 8), col = e % (kD / 8);
-        uint4* at = reinterpret_cast<uint4*>(v + (col / 8) * C::kKVBlock + r * 128 + (((col % 8) ^ (r & 7)) << 4));
+      const int pos0 = t * a.tile;
+      if (pos0 + a.tile <= q.base && !holes) return false;
+      if (lane == 0)
+        ctl.mend[j % kHoles] = make_int4(max(0, q.base - pos0), min(q.len - pos0, a.tile), pos0 - q.base, unit % kHoles);
+      __syncwarp();
+      return true;
+    };
+    auto mend = [&](int j, int in_slot, unsigned long long hole0, unsigned long long hole1) {
+      const int4 what = ctl.mend[j % kHoles];
+      uint8_t* v = sV + in_slot * C::kSlotBytes + (col / 8) * C::kSlotBlock;
+      auto place = [&](int r) { return reinterpret_cast<uint4*>(v + r * 128 + (((col % 8) ^ (r & 7)) << 4)); };
+#pragma unroll 1
+      for (int r = what.y + my_row; r < kBN; r += kPer) *place(r) = make_uint4(0, 0, 0, 0);
+      if (hole0 | hole1) {
+#pragma unroll 1
+        for (int r = my_row; r < kBN; r += kPer)
+          if ((r < 64 ? hole0 >> r : hole1 >> (r & 63)) & 1u) *place(r) = make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll 1
+      for (int r = what.x + my_row; r < what.y; r += kPer) {
+        uint4* at = place(r);
         uint32_t x[4] = {at->x, at->y, at->z, at->w};
         bool odd = false;
         constexpr uint32_t kExp = kBf16 ? 0x7f80u : 0x7c00u;
@@ -767,293 +766,614 @@ __global__ void __launch_bounds__(TcCfg<kD, kTiles>::kThreads, TcCfg<kD, kTiles>
         }
         if (odd) {
           *at = make_uint4(x[0], x[1], x[2], x[3]);
-          const int s = pos0 + r - c.s.base;
-          atomicOr(&ctl.odd[u & 1][s >> 5], 1u << (s & 31));
+          const int eight = (what.z + r) >> 3;
+          atomicOr(&ctl.odd[what.w][eight >> 5], 1u << (eight & 31));
         }
       }
       fence_proxy_async_smem();
       __syncwarp();
     };
-    bool ok = n > 0 && issue_s(0, true, 0);
-    bool first = true;
-    for (int j = 0; j < n && ok; ++j) {
-      const bool more = j + 1 < n, ends = cur.t + 1 == cur.T;
-      if (more && !ends) ok = issue_s(j + 1, false, unit);
-      if (!ok) break;
-      const int slot = j % kStages;
-      if (first) {
-        // (the softmax is past the unit before the last: this buffer is free)
-        for (int i = lane; i < kMaxDrafted / 32; i += 32) ctl.odd[unit & 1][i] = 0;
-        __syncwarp();
-      }
-      ok = wait(&ctl.v_full[slot], (j / kStages) & 1);
-      if (!ok) break;
-      const unsigned long long hole = ctl.hole[j % kHoles];
-      if ((cur.t + 1) * kBN > cur.s.base || hole) mend_v(sV + slot * C::kKVBytes, cur, hole, unit);
-      const uint64_t vd = sw128_desc(smem_addr(sV + slot * C::kKVBytes), C::kKVBlock, 1024);
-#pragma unroll
-      for (int t = 0; t < kTiles; ++t) {
-        ok = ok && wait(&ctl.p_full[t][j & 1], (j >> 1) & 1);
-        if (!ok) break;
-        tc_fence_after();
-        if (leader) {
-#pragma unroll
-          for (int k = 0; k < kBN / 16; ++k)
-            umma_ts(tmem + C::kColO + t * kD, tmem + (2 * t + (j & 1)) * kBN + k * 8, sw128_desc_step(vd, k * 2048),
-                    idesc_o, (!first || k > 0) ? 1u : 0u);
-          umma_commit(&ctl.pv_done[t]);
-          // A barrier of its own: by then the softmax may be two phases of pv_done behind or none.
-          if (ends || !more) umma_commit(&ctl.o_done[t]);
+    if (maps.boxes > 0) {
+      const int R = maps.rows, boxes = maps.boxes, group = 32 / boxes;  // tiles per look-up
+      const uint64_t policy = a.row_tiles > 1 ? l2_policy_evict_last() : l2_policy_evict_first();
+      const int my_tile = lane / boxes, my_box = lane - my_tile * boxes;
+      struct Group {
+        int page, row, live;  // of this lane's box: table entry, first row, whether it has tokens
+        int count, h, t;
+        bool begins;  // the unit, or this run's part of it
+        Seq s;
+      };
+      auto look_up = [&](Group& g) {
+        g = Group{-1, 0, 0, 0, cur.h, cur.t, unit_begins, cur.s};
+        if (left <= 0) return;
+        g.count = min(min(group, cur.T - cur.t), left);
+        const int pos = (cur.t + my_tile) * a.tile + my_box * R;
+        if (my_tile < g.count && pos < cur.s.len) {
+          const int lp = a.page_at(pos);
+          g.row = pos - lp * a.c.page_size;
+          g.live = 1;
+          g.page = *(a.c.table + static_cast<long long>(cur.b) * a.c.table_stride + lp);
         }
+        left -= g.count;
+        cur.t += g.count;
+        unit_begins = cur.t == cur.T;
+        if (left > 0 && unit_begins) next_unit(a, cur, ahead, &fault);
+      };
+      if (does[1] && a.tile < kBN) {
+        // Rows behind a tile's tokens: no copy reaches them.
+#pragma unroll 1
+        for (int v = 0; v < C::kVSlots; ++v)
+#pragma unroll 1
+          for (int r = a.tile + my_row; r < kBN; r += kPer)
+            *reinterpret_cast<uint4*>(sV + v * C::kSlotBytes + (col / 8) * C::kSlotBlock + r * 128 +
+                                      (((col % 8) ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();
         __syncwarp();
       }
-      if (!ok) break;
-      if (leader) umma_commit(&ctl.v_empty[slot]);
-      __syncwarp();
-      first = false;
-      advance<kBN>(a, cur, &fault);
-      if (ends) {
-        first = true;
-        ++unit;
-        if (more) ok = issue_s(j + 1, true, unit);
+      Group now, next;
+      look_up(now);
+      look_up(next);
+      int in = 0;
+      unsigned long long late_hole[2] = {0, 0};
+      auto mend_late = [&] {
+        const bool there = wait(&ctl.v_raw[late_slot], raw >> late_slot & 1u);
+        raw ^= 1u << late_slot;
+        if (there) {
+          mend(late, late_slot, late_hole[0], late_hole[1]);
+          if (lane == 0) mbar_arrive(&ctl.v_full[late_slot]);
+        }
+        late = -1;
+        return there;
+      };
+      for (int j = 0; j < n && ok; ++j) {
+        const bool mine = my_tile == in && now.live;
+        const bool good = mine && static_cast<unsigned>(now.page) < static_cast<unsigned>(a.c.num_pages);
+        const uint32_t have = __ballot_sync(0xffffffffu, good);
+        const uint32_t gone = __ballot_sync(0xffffffffu, mine && !good) >> (in * boxes);
+        unsigned long long hole[2] = {0, 0};
+#pragma unroll 1
+        for (int b = 0; gone && b < boxes; ++b)
+          if (gone >> b & 1u)
+#pragma unroll 1
+            for (int r = b * R; r < (b + 1) * R; r += 8) hole[r >> 6] |= 0xffull << (r & 63);
+        if (gone) fault |= kFaultPage;
+        bool to_mend = false;
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          if (!does[kv] || !ok) continue;
+          if (late >= 0 && !__all_sync(0xffffffffu, mbar_test(empty(kv, slot[kv]), parity[kv]))) ok = mend_late();
+          ok = ok && wait(empty(kv, slot[kv]), parity[kv]);
+          if (!ok) continue;
+          uint64_t* arrives = full(kv, slot[kv]);
+          if (kv == 1) {
+            to_mend = note_mend(j, now.s, now.t + in, now.begins && in == 0, gone != 0);
+            if (to_mend) arrives = &ctl.v_raw[slot[1]];
+          }
+          if (lane == 0) {
+            if (kv == 0) ctl.hole[j % kHoles][0] = hole[0], ctl.hole[j % kHoles][1] = hole[1];
+            uint32_t bytes = __popc(have) * R * (kD * 2);
+#ifdef RA_WATCHDOG_TEST
+            if (maps.lose && blockIdx.x == 0 && j == 0 && kv == 0) bytes += 16;
+#endif
+            mbar_arrive_expect_tx(arrives, bytes);
+          }
+          __syncwarp();
+          if (good) {
+            const uint32_t dst = smem_addr((kv ? sV : sK) + slot[kv] * C::kSlotBytes) + my_box * R * 128;
+#pragma unroll
+            for (int c = 0; c < kD / 64; ++c)
+              tma_load_4d(dst + c * C::kSlotBlock, kv ? &maps.v : &maps.k, arrives, c * 64, now.row, now.h, now.page,
+                          policy);
+          }
+          last_copy[kv] = j;
+          if (kv == 1) {
+            if (late >= 0) ok = mend_late();
+            if (to_mend) late = j, late_slot = slot[1], late_hole[0] = hole[0], late_hole[1] = hole[1];
+          }
+          to_next(kv);
+        }
+        if (++in == now.count) {
+          in = 0;
+          now = next;
+          look_up(next);
+        }
       }
+      if (ok && late >= 0) ok = mend_late();
+    } else {
+      // Lane looks up tokens lane + 32 w of a tile, and copies one 16-byte
+      // column (zeros behind D and where there is no token) of every kPer-th row.
+      constexpr int kLag = 2;  // tiles in flight before the first is waited for
+      const bool col_ok = col * 8 < a.c.D;
+      struct Look {
+        int page[kWords], row[kWords];  // row -1: no such token
+        int h, t;
+        bool begins;
+        Seq s;
+      };
+      auto look_up = [&](Look& k) {
+        k.h = cur.h;
+        k.t = cur.t;
+        k.s = cur.s;
+        k.begins = unit_begins;
+#pragma unroll
+        for (int w = 0; w < kWords; ++w) {
+          const int in = w * 32 + lane, pos = cur.t * a.tile + in;
+          k.page[w] = -1;
+          k.row[w] = -1;
+          if (left > 0 && in < a.tile && pos < cur.s.len) {
+            const int lp = a.page_at(pos);
+            k.row[w] = pos - lp * a.c.page_size;
+            k.page[w] = *(a.c.table + static_cast<long long>(cur.b) * a.c.table_stride + lp);
+          }
+        }
+        unit_begins = ++cur.t == cur.T;
+        if (--left > 0 && unit_begins) next_unit(a, cur, ahead, &fault);
+      };
+      int told = 0, told_slot[2] = {0, 0};  // tiles whose arrival has been told
+      uint32_t to_mend = 0;         // of the tiles from `told` on
+      auto tell = [&](int upto) {
+        fence_proxy_async_smem();
+        __syncwarp();
+#pragma unroll 1
+        for (; told < upto; ++told) {
+          if (to_mend & 1u) mend(told, told_slot[1], 0, 0);
+          to_mend >>= 1;
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv) {
+            if (!does[kv]) continue;
+            if (lane == 0) mbar_arrive(full(kv, told_slot[kv]));
+            if (++told_slot[kv] == (kv ? C::kVSlots : C::kKSlots)) told_slot[kv] = 0;
+          }
+        }
+      };
+      Look now, next;
+      look_up(now);
+      look_up(next);
+      for (int j = 0; j < n && ok; ++j) {
+        unsigned long long hole[2] = {0, 0};
+        bool good[kWords];
+#pragma unroll
+        for (int w = 0; w < kWords; ++w) {
+          good[w] = static_cast<unsigned>(now.page[w]) < static_cast<unsigned>(a.c.num_pages);
+          const uint32_t gone = __ballot_sync(0xffffffffu, now.row[w] >= 0 && !good[w]);
+          if (gone) fault |= kFaultPage;
+          hole[w / 2] |= static_cast<unsigned long long>(gone) << (w % 2 * 32);
+          good[w] = good[w] && now.row[w] >= 0;
+        }
+#pragma unroll 1
+        for (int kv = 0; kv < 2; ++kv) {
+          if (!does[kv] || !ok) continue;
+          if (!__all_sync(0xffffffffu, mbar_test(empty(kv, slot[kv]), parity[kv]))) {
+            // Nothing may wait for what has arrived meanwhile.
+            cp_async_wait_all();
+            tell(j);
+            ok = wait(empty(kv, slot[kv]), parity[kv]);
+            if (!ok) continue;
+          }
+          if (kv == 0 && lane == 0) ctl.hole[j % kHoles][0] = hole[0], ctl.hole[j % kHoles][1] = hole[1];
+          if (kv == 1 && note_mend(j, now.s, now.t, now.begins, false)) to_mend |= 1u << (j - told);
+          const long long* st = kv ? a.c.vs : a.c.ks;
+          const T* from = static_cast<const T*>(kv ? a.c.v : a.c.k) + (col_ok ? col * 8 : 0) + now.h * st[1];
+          const uint32_t dst = smem_addr((kv ? sV : sK) + slot[kv] * C::kSlotBytes) + (col / 8) * C::kSlotBlock;
+#pragma unroll
+          for (int w = 0; w < kWords; ++w) {
+            // element offset of this lane's token, or -1
+            const long long at = good[w] ? now.page[w] * st[0] + now.row[w] * st[2] : -1;
+#pragma unroll 4
+            for (int i = 0; i < 32; i += kPer) {
+              const int r = i + (kPer > 1 ? my_row : 0);
+              const long long off = __shfl_sync(0xffffffffu, at, r);
+              const bool there = off >= 0 && col_ok;
+              cp_async16(dst + (w * 32 + r) * 128 + (((col % 8) ^ (r & 7)) << 4), from + (there ? off : 0), there);
+            }
+          }
+          last_copy[kv] = j;
+          to_next(kv);
+        }
+        if (!ok) break;
+        cp_async_commit();
+        now = next;
+        look_up(next);
+        if (j >= kLag) {
+          cp_async_wait<kLag>();
+          tell(j - kLag + 1);
+        }
+      }
+      cp_async_wait_all();
+      if (ok) tell(n);
     }
-    // Every product this warp issued has retired before tensor memory is given back.
-    if (leader) umma_commit(&ctl.mma_done);
+  } else if (warp == C::kMmaWarp) {
+    // -------------------------------------------------------------- products
+    // One thread, and as few instructions as can be: it shares its scheduler
+    // with softmax warps, and every wait and product it issues is in the
+    // streams' way.
+    constexpr uint32_t idesc_s = umma_idesc_f16(kBf16, 128, kBN, false);
+    constexpr uint32_t idesc_o = umma_idesc_f16(kBf16, 128, kD, true);
+    if (elect_one()) {
+      auto wait_one = [&](uint64_t* bar, uint32_t parity) {
+        if (mbar_try_wait(smem_addr(bar), parity) ||
+            wait_long(bar, parity, &ctl.abort_flag, &ctl.code, wait_ns))
+          return true;
+        fault |= kFaultWait;
+        return false;
+      };
+      const uint64_t qd0 = sw128_desc(smem_addr(sQ), 16, 1024), kd0 = sw128_desc(smem_addr(sK), 16, 1024);
+      const uint64_t vd0 = sw128_desc(smem_addr(sV), C::kSlotBlock, 1024);
+      int k_slot = 0, v_slot = 0;
+      uint32_t k_parity = 0, v_parity = 0, p_parity = 0;
+      const uint32_t q_step = q_block >> 4;
+      // S into buffer st for the K at hand, of the run's u-th unit, whose Q is
+      // waited for at its first tile.  `begins`: the first product with this K,
+      // `frees`: the last.
+      auto issue_s = [&](int st, bool begins, bool frees, bool first, int u) {
+        if (begins && !wait_one(&ctl.k_full[k_slot], k_parity)) return false;
+        if (first && !wait_one(&ctl.q_full, u & 1)) return false;
+        tc_fence_after();
+        const uint64_t kd = sw128_desc_step(kd0, k_slot * C::kSlotBytes);
+        const uint64_t qd = sw128_desc_step(qd0, (kTwo ? st : early_q ? u & 1 : 0) * q_tile);
+#pragma unroll
+        for (int k = 0; k < kD / 16; ++k)
+          umma_ss(tmem + st * kBN, qd + (k / 4) * q_step + (k % 4) * 2,
+                  sw128_desc_step(kd, (k / 4) * C::kSlotBlock + (k % 4) * 32), idesc_s, k > 0 ? 1u : 0u);
+        umma_commit(&ctl.s_full[st]);
+        if (frees) {
+          umma_commit(&ctl.k_empty[k_slot]);
+          if (++k_slot == C::kKSlots) k_slot = 0, k_parity ^= 1;
+        }
+        return true;
+      };
+      // O += P V from buffer st with the V at hand; `anew`: O begins, `ends`: the
+      // unit's last product.
+      auto issue_pv = [&](int st, bool begins, bool frees, bool anew, bool ends) {
+        if (begins && !wait_one(&ctl.v_full[v_slot], v_parity)) return false;
+        if (!wait_one(&ctl.p_full[st], p_parity >> st & 1u)) return false;
+        p_parity ^= 1u << st;
+        tc_fence_after();
+        const uint64_t vd = sw128_desc_step(vd0, v_slot * C::kSlotBytes);
+#pragma unroll
+        for (int k = 0; k < kBN / 16; ++k)
+          umma_ts(tmem + C::kColO + (kTwo ? st * kD : 0), tmem + st * kBN + k * 8, sw128_desc_step(vd, k * 2048), idesc_o,
+                  (!anew || k > 0) ? 1u : 0u);
+        if (frees) {
+          umma_commit(&ctl.v_empty[v_slot]);
+          if (++v_slot == C::kVSlots) v_slot = 0, v_parity ^= 1;
+        }
+        if (ends) umma_commit(&ctl.o_done);
+        return true;
+      };
+      bool ok = n > 0;
+      int unit = 0, j = 0;
+      if constexpr (!kTwo) ok = ok && issue_s(0, true, true, true, 0);
+      while (ok && j < n) {
+        const int count = min(cur.T - cur.t, n - j);  // tiles of the unit in this run
+        for (int i = 0; i < count && ok; ++i, ++j) {
+          const bool closes = i + 1 == count;
+          if constexpr (!kTwo) {
+            // S(j + 1), then P(j) V(j); the other way round before a new unit,
+            // whose Q may still be on its way.
+            if (!closes) ok = issue_s((j + 1) & 1, true, true, false, unit);
+            ok = ok && issue_pv(j & 1, true, true, i == 0, closes);
+            if (closes && j + 1 < n) ok = ok && issue_s((j + 1) & 1, true, true, true, unit + 1);
+          } else {
+            // S0(j), P1(j - 1) V(j - 1), S1(j), P0(j) V(j): each stream's softmax
+            // runs beside the other's products.  (V(j - 1) is at hand until P1.)
+            ok = issue_s(0, true, false, i == 0, unit);
+            if (i > 0) ok = ok && issue_pv(1, false, true, i == 1, false);
+            ok = ok && issue_s(1, false, true, false, unit);
+            ok = ok && issue_pv(0, true, false, i == 0, false);
+            if (closes) ok = ok && issue_pv(1, false, true, i == 0, true);
+          }
+        }
+        ++unit;
+        if (ok && j < n) next_unit(a, cur, ahead, &fault);
+      }
+      // Every product has retired before tensor memory is given back.
+      umma_commit(&ctl.mma_done);
+      volatile int no_abort = 0;
+      mbar_wait(&ctl.mma_done, 0, &no_abort, &ctl.code, 1);
+    }
     __syncwarp();
-    volatile int no_abort = 0;
-    mbar_wait(&ctl.mma_done, 0, &no_abort, &ctl.code, 1);
   } else {
     // --------------------------------------------------------------- softmax
-    const int t = warp >> 2, in_tile = (warp & 3) * 32 + lane, tid = threadIdx.x & 127;
+    const int st = warp >> 2, in_tile = (warp & 3) * 32 + lane;
+    const int row_off = st * 128 + in_tile;  // row within the unit
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t tO = tmem + lane_off + C::kColO + t * kD;
+    const uint32_t tO = tmem + lane_off + C::kColO + st * kD;
     const float c = a.scale_log2;
     const uint64_t c2 = f2(c, c);
-    int* par = s_par[t];
-    int par_b = -1;
     uint32_t met = 0;
-    // The 128 threads of the row tile meet (by a wait that ends, as all here).
+    // The softmax threads meet (by a wait that ends, as all here).
     auto meet = [&] {
-      mbar_arrive(&ctl.group_met[t]);
-      const bool there = wait(&ctl.group_met[t], met);
+      mbar_arrive(&ctl.met);
+      const bool there = wait(&ctl.met, met);
       met ^= 1;
       return there;
     };
-
-    // Q of a unit's rows to shared memory (rows behind the last are zeros) and
-    // its sequence's tree.  The S products of the unit before have retired.
-    auto load_unit = [&](const Cursor& u) {
-      if (!meet()) return false;  // nobody looks at the tree before any more
-      if (u.b != par_b) {
-        load_parents<128>(a, u.b, u.s.n, par, tid, &fault);
-        par_b = u.b;
+    // Starts the copy of a unit's Q rows, those of warps that have any (zeros
+    // behind the last and behind D), and of its sequence's tree.
+    auto copy_unit = [&](const Cursor& u, int tile, int par_buf, bool tree) {
+      constexpr int kCols = kD / 8, kAtOnce = C::kSoftThreads / kCols;  // columns of a row, rows at once
+      static_assert(kAtOnce % 4 == 0, "rows at once");
+      const int col = threadIdx.x % kCols, r0 = threadIdx.x / kCols;
+      const int used = (min(a.rows - u.rt * C::kRows, C::kRows) + 31) & ~31;
+      const T* q = static_cast<const T*>(a.q) + u.b * a.q_b + static_cast<long long>(u.h) * a.group * a.q_h + col * 8;
+      const uint32_t to = smem_addr(sQ) + tile * q_tile + (col / 8) * q_block;
+#pragma unroll 2
+      for (int r = r0; r < used; r += kAtOnce) {
+        const int gr = u.rt * C::kRows + r, head = a.head_at(gr), s = gr - head * a.S;
+        const bool there = gr < a.rows && col * 8 < a.c.D;
+        cp_async16(to + (r >> 7) * q_tile + (r & 127) * 128 + (((col % 8) ^ (r & 7)) << 4),
+                   there ? q + head * a.q_h + s * a.q_s : a.q, there);
       }
-      const T* q = static_cast<const T*>(a.q) + u.b * a.q_b + static_cast<long long>(u.h) * a.group * a.q_h;
-      uint8_t* to = sQ + t * C::kQBytes;
-      constexpr int kChunks = kD / 8;
-#pragma unroll 8
-      for (int e = tid; e < 128 * kChunks; e += 128) {
-        const int r = e / kChunks, col = e % kChunks, gr = u.rt * C::kRows + t * 128 + r;
-        const int head = gr / a.S, s = gr - head * a.S;
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (gr < a.rows && col * 8 < a.c.D)
-          x = *reinterpret_cast<const uint4*>(q + head * a.q_h + s * a.q_s + col * 8);
-        *reinterpret_cast<uint4*>(to + (col / 8) * C::kQBlock + r * 128 + (((col % 8) ^ (r & 7)) << 4)) = x;
-      }
-      fence_proxy_async_smem();
-      mbar_arrive(&ctl.q_full[t]);
-      return meet();  // the tree is there
-    };
-
-    float m = -INFINITY, l = 0.f;  // running maximum of the scaled scores that P refers to, sum of P
-    bool begun = cur.t == 0, first = true;
-    int unit = 0, gr = 0, s_row = 0;  // this thread's row of the kv head, and the drafted token it is
-    bool dead = true;                 // no row of the result, or a drafted token that is not there
-    auto row_of = [&](const Cursor& u) {
-      gr = u.rt * C::kRows + t * 128 + in_tile;
-      s_row = gr % a.S;
-      dead = gr >= a.rows || s_row >= u.s.n;
-    };
-    bool ok = n > 0 && load_unit(cur);
-    if (ok) row_of(cur);
-    for (int j = 0; j < n && ok; ++j) {
-      const uint32_t tS = tmem + lane_off + (2 * t + (j & 1)) * kBN;
-      ok = wait(&ctl.s_full[t][j & 1], (j >> 1) & 1);
-      if (!ok) break;
-      tc_fence_after();
-      if (!__all_sync(0xffffffffu, dead)) {
-        uint32_t u[2][32];
-        tmem_ld32(tS, u[0]);
-        tmem_ld32(tS + 32, u[1]);
-        const int pos0 = cur.t * kBN;
-        const unsigned long long hole = ctl.hole[j % kHoles];
-        bool any = true;
-        uint32_t see[2] = {0xffffffffu, 0xffffffffu};
-        const bool masked = pos0 + kBN > cur.s.base || hole;
-        if (masked) {
-          if (dead) see[0] = see[1] = 0;
-          else visible<2>(cur.s, s_row, pos0, par, see);
-          // behind the table's end, or in no page
-          unsigned long long there = ~hole;
-          if (cur.s.len - pos0 < kBN) there &= ~(~0ull << (cur.s.len - pos0));
-          see[0] &= static_cast<uint32_t>(there);
-          see[1] &= static_cast<uint32_t>(there >> 32);
-          any = (see[0] | see[1]) != 0;
-        }
-        tmem_wait_ld();
-        float s[kBN];
-#pragma unroll
-        for (int i = 0; i < kBN; ++i) s[i] = __uint_as_float(u[i / 32][i % 32]);
-        if (masked) {
-#pragma unroll
-          for (int i = 0; i < kBN; ++i)
-            if (!(see[i / 32] >> (i % 32) & 1u)) s[i] = -INFINITY;
-        }
-        float mx[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-        for (int i = 4; i < kBN - 4; i += 8) {
-          mx[0] = fmax3(mx[0], s[i + 0], s[i + 4]);
-          mx[1] = fmax3(mx[1], s[i + 1], s[i + 5]);
-          mx[2] = fmax3(mx[2], s[i + 2], s[i + 6]);
-          mx[3] = fmax3(mx[3], s[i + 3], s[i + 7]);
-        }
-        const float top = fmax3(fmax3(mx[0], mx[1], s[kBN - 4]), fmax3(mx[2], mx[3], s[kBN - 3]),
-                                fmaxf(s[kBN - 2], s[kBN - 1]));
-        const float mb = any ? fmaxf(top * c, kLowest) : -INFINITY;
-        // The maximum that P refers to moves, and O is rescaled, only when it
-        // has grown by more than 2^8; O / L is the same in exact arithmetic.
-        const bool grow = mb > m + 8.f;
-        if (__any_sync(0xffffffffu, grow)) {
-          float alpha = 1.f;
-          if (grow) {
-            alpha = ex2_approx(m - mb);  // 0 where m is -inf
-            l *= alpha;
-            m = mb;
-          }
-          if (!first) {
-            ok = wait(&ctl.pv_done[t], (j - 1) & 1);
-            if (!ok) break;
-            tc_fence_after();
+      if (tree && a.parents) {
+        const int* par = tree_of(a, u.b);
 #pragma unroll 1
-            for (int cc = 0; cc < kD; cc += 32) {
-              uint32_t o[32];
-              tmem_ld32(tO + cc, o);
-              tmem_wait_ld();
-#pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-              tmem_st32(tO + cc, o);
-            }
-          }
-        }
-        const float sub = kUp - finite_max(m);
-        const uint64_t sub2 = f2(sub, sub);
-        uint64_t sum0 = f2(0.f, 0.f), sum1 = f2(0.f, 0.f);
-        uint32_t pk[32];
-        // P is rounded to the input type for P V, by half a step of each weight
-        // at most; its sum is taken before that.
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          float x0, x1;
-          f2_split(f2_fma(f2(s[2 * i], s[2 * i + 1]), c2, sub2), x0, x1);
-          x0 = ex2_approx(x0);
-          x1 = ex2_approx(x1);
-          if (i % 2) sum1 = f2_add(sum1, f2(x0, x1));
-          else sum0 = f2_add(sum0, f2(x0, x1));
-          pk[i] = pack2<kBf16>(x0, x1);
-        }
-        tmem_st32(tS, pk);
-        float a0, a1, b0, b1;
-        f2_split(sum0, a0, a1);
-        f2_split(sum1, b0, b1);
-        l += (a0 + a1) + (b0 + b1);
-        tmem_wait_st();
+        for (int e = threadIdx.x; e < min(u.s.n, kParShared); e += C::kSoftThreads)
+          cp_async4(smem_addr(&ctl.par[par_buf][e]), par + e);
       }
-      tc_fence_before();
-      mbar_arrive(&ctl.p_full[t][j & 1]);
+    };
+    auto q_arrived = [&] {
+      cp_async_wait_all();
+      fence_proxy_async_smem();
+      mbar_arrive(&ctl.q_full);
+    };
 
-      const bool ends = cur.t + 1 == cur.T, last = j + 1 == n;
+    bool ok = n > 0;
+    if (ok) copy_unit(cur, 0, 0, true);  // before the flood of K and V
+    zero_empty_rows<T, C::kSoftThreads>(a, &fault);
+    int par_buf = 0, unit = 0, j = 0;
+    if (ok) {
+      q_arrived();
+      ok = meet();
+    }
+    bool begun = cur.t == 0;
+    while (ok && j < n) {
+      // The unit at cur, or the part of it in this run: tiles j .. j + count - 1.
+      const int count = min(cur.T - cur.t, n - j), j1 = j + count;
+      const bool last = j1 == n;
       Cursor nxt = cur;
-      if (!last) advance<kBN>(a, nxt, &fault);
-      if (ends || last) {
-        // The unit, or this CTA's part of it, ends.
-        if (!last && !load_unit(nxt)) break;
-        ok = wait(&ctl.o_done[t], unit & 1);
+      if (!last) next_unit(a, nxt, ahead, &fault);
+      const bool new_tree = nxt.b != cur.b;
+      if (early_q && !last) copy_unit(nxt, (unit + 1) & 1, par_buf ^ 1, new_tree);
+      const Tree tree{ctl.par[par_buf], tree_of(a, cur.b)};
+      const int gr = cur.rt * C::kRows + row_off, s_row = gr - a.head_at(gr) * a.S;
+      const bool dead = gr >= a.rows || s_row >= cur.s.n;  // no row of the result, or a drafted token that is not there
+      const bool warp_dead = __all_sync(0xffffffffu, dead);
+      float m = -INFINITY, l = 0.f;  // running maximum of the scaled scores that P refers to, sum of P
+      bool first = true;
+      for (int jj = j; jj < j1; ++jj) {
+        const int buf = kTwo ? st : jj & 1;
+        const uint32_t tS = tmem + lane_off + buf * kBN;
+        ok = wait(&ctl.s_full[buf], (kTwo ? jj : jj >> 1) & 1);
         if (!ok) break;
         tc_fence_after();
-        const Place p = place_of(a, cur, begun, run, run.first + j, threadIdx.x == 0);
-        const float M = dead ? -INFINITY : m, inv = inverse(M, l);
-        uint32_t odd = 0;
-        if (lane * 32 < cur.s.n) odd = ctl.odd[unit & 1][lane];
-        const bool mend = __any_sync(0xffffffffu, odd != 0);
-        if (!__all_sync(0xffffffffu, gr >= a.rows)) {
+        if (!warp_dead) {
+          const int pos0 = (cur.t + jj - j) * a.tile;
+          const unsigned long long hole0 = ctl.hole[jj % kHoles][0], hole1 = ctl.hole[jj % kHoles][1];
+          const bool masked = pos0 + a.tile > cur.s.base || (hole0 | hole1) != 0;
+          bool any = true;
+          uint32_t see[kWords];
+          if (masked) {
+            if (dead) {
+#pragma unroll
+              for (int w = 0; w < kWords; ++w) see[w] = 0;
+            } else {
+              visible<kWords>(cur.s, s_row, pos0, tree, see, &fault);
+            }
+            any = false;
+#pragma unroll
+            for (int w = 0; w < kWords; ++w) {
+              // behind the table's end or the tile's, or in no page
+              const int in = min(cur.s.len - pos0, a.tile) - 32 * w;
+              see[w] &= in >= 32 ? 0xffffffffu : in > 0 ? (1u << in) - 1u : 0u;
+              see[w] &= ~static_cast<uint32_t>((w < 2 ? hole0 : hole1) >> (w % 2 * 32));
+              any = any || see[w] != 0;
+            }
+          }
+          // Tiles of 128 tokens are read from tensor memory twice, 64 scores at a
+          // time, for their maximum and for P: all at once would not fit the
+          // registers.  Those that do not count are -inf there after the first
+          // time.  (The loops are kept short: a CTA's first pass over them comes
+          // from a cold instruction cache.)
+          float s[64];
+          auto load_scores = [&](int hf) {
+            uint32_t u[2][32];
+            tmem_ld32(tS + hf * 64, u[0]);
+            tmem_ld32(tS + hf * 64 + 32, u[1]);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 64; ++i) s[i] = __uint_as_float(u[i / 32][i % 32]);
+          };
+          float top = -INFINITY;
 #pragma unroll 1
-          for (int cc = 0; cc < kD; cc += 32) {
+          for (int hf = 0; hf < kBN / 64; ++hf) {
+            load_scores(hf);
+            uint32_t lo = see[0], hi = see[1];
+            if (kWords == 4 && hf) lo = see[kWords - 2], hi = see[kWords - 1];
+            const int tail = a.tile - hf * 64;
+            if (masked || tail < 64) {
+              if (!masked) lo = 0xffffffffu, hi = tail >= 64 ? 0xffffffffu : (1u << (tail - 32)) - 1u;
+#pragma unroll
+              for (int i = 0; i < 64; ++i)
+                if (!((i < 32 ? lo : hi) >> (i % 32) & 1u)) s[i] = -INFINITY;
+              if constexpr (kBN > 64) {
+                uint32_t u[2][32];
+#pragma unroll
+                for (int i = 0; i < 64; ++i) u[i / 32][i % 32] = __float_as_uint(s[i]);
+                tmem_st32(tS + hf * 64, u[0]);
+                tmem_st32(tS + hf * 64 + 32, u[1]);
+                tmem_wait_st();
+              }
+            }
+            float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+            for (int i = 4; i < 60; i += 8) {
+              mx[0] = fmax3(mx[0], s[i + 0], s[i + 4]);
+              mx[1] = fmax3(mx[1], s[i + 1], s[i + 5]);
+              mx[2] = fmax3(mx[2], s[i + 2], s[i + 6]);
+              mx[3] = fmax3(mx[3], s[i + 3], s[i + 7]);
+            }
+            top = fmax3(top, fmax3(mx[0], mx[1], s[60]), fmax3(fmax3(mx[2], mx[3], s[61]), s[62], s[63]));
+          }
+          const float mb = any ? fmaxf(top * c, kLowest) : -INFINITY;
+          // The maximum that P refers to moves, and O is rescaled, only when it
+          // has grown by more than 2^8; O / L is the same in exact arithmetic.
+          const bool grow = mb > m + 8.f;
+          if (__any_sync(0xffffffffu, grow)) {
+            float alpha = 1.f;
+            if (grow) {
+              alpha = ex2_approx(m - mb);  // 0 where m is -inf
+              l *= alpha;
+              m = mb;
+            }
+            if (!first) {
+              if constexpr (!kTwo) {
+                // The product before may not have retired, which frees its V.
+                // (With two streams it has, as S has been written over its P.)
+                ok = wait(&ctl.v_empty[(jj - 1) % C::kVSlots], ((jj - 1) / C::kVSlots) & 1);
+                if (!ok) break;
+                tc_fence_after();
+              }
+#pragma unroll 1
+              for (int cc = 0; cc < kD; cc += 32) {
+                uint32_t o[32];
+                tmem_ld32(tO + cc, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                tmem_st32(tO + cc, o);
+              }
+            }
+          }
+          const float sub = kUp - finite_max(m);
+          const uint64_t sub2 = f2(sub, sub);
+          uint64_t sum0 = f2(0.f, 0.f), sum1 = f2(0.f, 0.f);
+          // P is rounded to the input type for P V, by half a step of each weight
+          // at most; its sum is taken before that.
+#pragma unroll 1
+          for (int hf = 0; hf < kBN / 64; ++hf) {
+            uint32_t pk[32];
+            if constexpr (kBN > 64) load_scores(hf);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              float x0, x1;
+              f2_split(f2_fma(f2(s[2 * i], s[2 * i + 1]), c2, sub2), x0, x1);
+              x0 = ex2_approx(x0);
+              x1 = ex2_approx(x1);
+              if (i % 2) sum1 = f2_add(sum1, f2(x0, x1));
+              else sum0 = f2_add(sum0, f2(x0, x1));
+              pk[i] = pack2<kBf16>(x0, x1);
+            }
+            tmem_st32(tS + hf * 32, pk);
+          }
+          float a0, a1, b0, b1;
+          f2_split(sum0, a0, a1);
+          f2_split(sum1, b0, b1);
+          l += (a0 + a1) + (b0 + b1);
+          tmem_wait_st();
+        }
+        tc_fence_before();
+        mbar_arrive(&ctl.p_full[buf]);
+        first = false;
+      }
+      if (!ok) break;
+
+      // The unit, or this run's part of it, ends.
+      if (early_q && !last) q_arrived();
+      ok = wait(&ctl.o_done, unit & 1);
+      if (!ok) break;
+      tc_fence_after();
+      // (no product reads this unit's Q any more)
+      if (!early_q && !last) copy_unit(nxt, 0, par_buf ^ 1, new_tree);
+      Cursor at_end = cur;
+      at_end.t += count - 1;
+      const Place p = place_of(a, at_end, begun, run, run.first + j1 - 1, threadIdx.x == 0);
+      // Whether drafted tokens have values that the products left out.
+      bool mend = false;
+#pragma unroll
+      for (int w = 0; w < kMaxDrafted / 256; ++w) mend = mend || ctl.odd[unit % kHoles][w] != 0;
+      float M = m;
+      if (dead) M = -INFINITY;
+      const float inv = inverse(M, l);
+      if (!__all_sync(0xffffffffu, gr >= a.rows)) {
+#pragma unroll 1
+        for (int cc = 0; cc < kD; cc += 32) {
+          float o[32];
+          {
             uint32_t u[32];
             tmem_ld32(tO + cc, u);
             tmem_wait_ld();
-            float o[32];
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = __uint_as_float(u[i]);
-            if (mend && !dead) {
-              // the infinite and NaN values of drafted tokens this row follows, which the product left out
-              for (int f = s_row; f >= 0; f = nxt.b == cur.b || last ? par[f] : parent_of(a, cur.b, f)) {
-                if (!(ctl.odd[unit & 1][f >> 5] >> (f & 31) & 1u)) continue;
-                int row = 0, ignore = 0;
-                const int page = page_of(a, cur, cur.s.base + f, &row, &ignore);
-                if (page < 0) continue;
-                const T* v = static_cast<const T*>(a.c.v) + page * a.c.vs[0] + cur.h * a.c.vs[1] + row * a.c.vs[2];
+          }
+          if (mend && !dead) {
+            // the infinite and NaN values of drafted tokens this row follows, which the products left out
+#pragma unroll 1
+            for (int f = s_row; f >= 0; f = tree.parent(f, &fault)) {
+              if (!(ctl.odd[unit % kHoles][f >> 8] >> (f >> 3 & 31) & 1u)) continue;
+              int row = 0;
+              const int page = page_of(a, cur, cur.s.base + f, &row, &fault);
+              if (page < 0) continue;
+              const T* v = static_cast<const T*>(a.c.v) + page * a.c.vs[0] + cur.h * a.c.vs[1] + row * a.c.vs[2];
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                  const float x = cc + i < a.c.D ? to_f32(v[cc + i]) : 0.f;
-                  if (!isfinite(x)) o[i] += x;
-                }
+              for (int i = 0; i < 32; ++i) {
+                const float x = cc + i < a.c.D ? to_f32(v[cc + i]) : 0.f;
+                if (!isfinite(x)) o[i] += x;
               }
             }
-            if (gr >= a.rows) {
-            } else if (p.whole) {
-              T* out = static_cast<T*>(a.out) + (p.row0 + gr) * a.c.D + cc;
-#pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = M == -INFINITY ? 0.f : o[i] * inv;
-#pragma unroll
-              for (int i = 0; i < 32; i += 8)
-                if (cc + i < a.c.D)
-                  *reinterpret_cast<uint4*>(out + i) =
-                      make_uint4(pack2<kBf16>(o[i], o[i + 1]), pack2<kBf16>(o[i + 2], o[i + 3]),
-                                 pack2<kBf16>(o[i + 4], o[i + 5]), pack2<kBf16>(o[i + 6], o[i + 7]));
-            } else {
-              float4* part = a.part_o + (static_cast<long long>(p.slot) * a.D4 + cc / 4) * C::kRows + t * 128 + in_tile;
-#pragma unroll
-              for (int i = 0; i < 32; i += 4)
-                if (cc + i < a.c.D) part[i / 4 * C::kRows] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-            }
           }
-          if (gr < a.rows && !p.whole)
-            a.part_ml[static_cast<long long>(p.slot) * C::kRows + t * 128 + in_tile] = make_float2(M, l);
+          if (gr >= a.rows) {
+          } else if (p.whole) {
+            T* out = static_cast<T*>(a.out) + (p.row0 + gr) * a.c.D + cc;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = M == -INFINITY ? 0.f : o[i] * inv;
+#pragma unroll
+            for (int i = 0; i < 32; i += 8)
+              if (cc + i < a.c.D)
+                *reinterpret_cast<uint4*>(out + i) =
+                    make_uint4(pack2<kBf16>(o[i], o[i + 1]), pack2<kBf16>(o[i + 2], o[i + 3]),
+                               pack2<kBf16>(o[i + 4], o[i + 5]), pack2<kBf16>(o[i + 6], o[i + 7]));
+          } else {
+            float4* part = a.part_o + (static_cast<long long>(p.slot) * a.D4 + cc / 4) * C::kRows + row_off;
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              if (cc + i < a.c.D) part[i / 4 * C::kRows] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          }
         }
-        tc_fence_before();  // O has been read before the next unit's first product overwrites it (p_full orders the two)
-        m = -INFINITY;
-        l = 0.f;
-        begun = true;
-        ++unit;
-        if (!last) row_of(nxt);
+        if (gr < a.rows && !p.whole)
+          a.part_ml[static_cast<long long>(p.slot) * C::kRows + row_off] = make_float2(M, l);
       }
-      first = ends;
+      tc_fence_before();  // O has been read before the next unit's first product overwrites it (p_full orders the two)
+      if (!last) {
+        if (!early_q) q_arrived();
+        ok = meet();  // the tree is there
+        if (!ok) break;
+      }
+      begun = true;
+      ++unit;
+      if (new_tree) par_buf ^= 1;
       cur = nxt;
+      j = j1;
     }
+    cp_async_wait_all();
   }
 
   tc_fence_before();
   __syncthreads();
-  if (warp == C::kTmaWarp && ctl.abort_flag) {
+  if (warp >= C::kCopyWarp && maps.boxes > 0 && ctl.abort_flag) {
     // Some role gave up on a wait: copies already asked for land before the
     // CTA's shared memory goes.
-    for (int s = 0; s < kStages; ++s) {
-      volatile int no_abort = 0;
-      const int k = last_k - (last_k - s + kStages * 2) % kStages;  // last tile in slot s
-      if (k >= 0) mbar_wait(&ctl.k_full[s], (k / kStages) & 1, &no_abort, &ctl.code, 1);
-      const int v = last_v - (last_v - s + kStages * 2) % kStages;
-      if (v >= 0) mbar_wait(&ctl.v_full[s], (v / kStages) & 1, &no_abort, &ctl.code, 1);
+    for (int kv = 0; kv < 2; ++kv) {
+      const int slots = kv ? C::kVSlots : C::kKSlots, last = kv ? last_copy[1] : last_copy[0];
+      for (int s = 0; s < slots; ++s) {
+        volatile int no_abort = 0;
+        const int j = last - (last - s + slots) % slots;  // the last tile in slot s
+        if (last < 0 || j < 0) continue;
+        if (kv && late >= 0 && s == late_slot)
+          wait_long(&ctl.v_raw[s], raw >> s & 1u, &no_abort, &ctl.code, kWaitTimeoutNs);
+        else
+          wait_long(kv ? &ctl.v_full[s] : &ctl.k_full[s], (j / slots) & 1, &no_abort, &ctl.code, kWaitTimeoutNs);
+      }
     }
   }
   if (warp == C::kMmaWarp) {
@@ -1144,23 +1464,23 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_tree_join_kernel(const _
 struct Plan {
   bool tc;  // the tensor-core kernel
   int kd;   // head dim the kernel is compiled for
-  int row_tiles_each;  // tiles of 128 rows a CTA takes at once (tensor cores)
+  bool two_tiles;  // a CTA takes two tiles of 128 rows at once (tensor cores)
   int unit_rows, row_tiles, tile;
+  int box_rows, boxes;  // of a tile of K or V, by TMA; 0: 16-byte copies
   int grid;
   long long tiles;  // the block table can name
   size_t meta_at, ml_at, o_at, bytes;
 };
 
-// What the tensor-core kernel asks of the cache: 16-byte rows, read in boxes
-// of 8 rows at least, which lie in one page.
+// What the tensor-core kernel asks of the cache: 16-byte rows.
 bool tc_takes(const AttnPagedCache* c) {
-  if (c->dtype == ATTN_F32 || c->D % 8 != 0 || c->page_size % 8 != 0 || c->num_pages == 0) return false;
+  if (c->dtype == ATTN_F32 || c->D % 8 != 0) return false;
   for (int i = 0; i < 3; ++i)
     if (c->k_strides[i] % 8 != 0 || c->v_strides[i] % 8 != 0) return false;
   return aligned_to(c->k, 16) && aligned_to(c->v, 16);
 }
 
-// `fast`: q, out and the tensor maps allow the tensor-core kernel too.
+// `fast`: q and out allow the tensor-core kernel too.
 Plan make_plan(const AttnPagedCache* c, bool fast, int Hq, int S, int sms) {
   Plan p;
   const int D = c->D;
@@ -1168,12 +1488,32 @@ Plan make_plan(const AttnPagedCache* c, bool fast, int Hq, int S, int sms) {
   int per_sm;
   p.tc = fast && tc_takes(c);
   p.kd = D <= 64 ? 64 : D <= 128 ? 128 : 256;
-  p.row_tiles_each = 1;
+  p.two_tiles = false;
   if (p.tc) {
-    if (p.kd == 128 && rows > 128) p.row_tiles_each = 2;
-    p.unit_rows = 128 * p.row_tiles_each;
-    p.tile = TcCfg<128, 1>::kBN;
-    per_sm = p.kd <= 128 && p.row_tiles_each == 1 ? 2 : 1;
+    p.two_tiles = p.kd <= 128 && rows > 128;
+    p.unit_rows = p.two_tiles ? 256 : 128;
+    const int most = p.two_tiles ? TcCfg<128, true>::kBN : TcCfg<128, false>::kBN;
+    // A box is rows of one page, a multiple of 8 that divides its size, and a
+    // tile is whole boxes.  A warp takes some 600 clocks for a tile and 80 for
+    // each box of 64 columns; a tile takes 1600 (3900 with two streams) all
+    // the same, so a shorter tile of fewer boxes can be the quicker one, but need
+    // not: pages of 24 rows at D = 64, tiles of 64 tokens in eight boxes 32.0
+    // us, of 48 in two 38.4.
+    p.tile = most;
+    p.box_rows = p.boxes = 0;
+    double best = 0;
+    for (int r = 8; r <= most && c->page_size % 8 == 0; r += 8) {
+      const int boxes = most / r, tokens = boxes * r;
+      if (c->page_size % r != 0 || tokens <= most - 32) continue;  // (the kernel masks the last 31 at most)
+      const int copy = 600 + 80 * (p.kd / 64) * boxes * (p.two_tiles ? 1 : 2), least = p.two_tiles ? 3900 : 1600;
+      const double cost = static_cast<double>(copy > least ? copy : least) / tokens;
+      if (p.boxes > 0 && cost > best) continue;
+      best = cost;
+      p.box_rows = r;
+      p.boxes = boxes;
+      p.tile = tokens;
+    }
+    per_sm = p.two_tiles || p.kd == 256 ? 1 : 2;
   } else {
     p.unit_rows = kSimtRows;
     p.tile = kSimtTile;
@@ -1193,6 +1533,14 @@ Plan make_plan(const AttnPagedCache* c, bool fast, int Hq, int S, int sms) {
   p.o_at = p.ml_at + up(sizeof(float2) * 2 * parts * p.unit_rows);
   p.bytes = p.o_at + up(sizeof(float4) * 2 * parts * p.unit_rows * D4);
   return p;
+}
+
+// Multiplier and shift of a division by d (see TreeArgs).
+void divisor(int d, unsigned* mul, int* shift) {
+  const unsigned long long x = static_cast<unsigned long long>(d);
+  *shift = 0;
+  while ((1ull << *shift) < x) ++*shift;
+  *mul = static_cast<unsigned>((((1ull << *shift) - x) << 32) / x + 1);
 }
 
 // The checks of a call that need no device.  Returns ATTN_OK or a status.
@@ -1227,33 +1575,40 @@ bool launch_big(void (*kern)(Params...), std::mutex& mu, bool (&done)[64], int g
   return launch_after(kern, dim3(grid), dim3(threads), smem, stream, 1, true, args...);
 }
 
-template <bool kBf16, int kD, int kTiles>
+template <bool kBf16, int kD, bool kTwo>
 bool launch_tc(const TreeArgs& a, const TcMaps& maps, int grid, cudaStream_t stream) {
-  using C = TcCfg<kD, kTiles>;
+  using C = TcCfg<kD, kTwo>;
   static bool done[64] = {};
   static std::mutex mu;
-  return launch_big(attn_tree_tc_kernel<kBf16, kD, kTiles>, mu, done, grid, C::kThreads, C::kSmemBytes, stream, a, maps);
+  return launch_big(attn_tree_tc_kernel<kBf16, kD, kTwo>, mu, done, grid, C::kThreads, C::kSmemBytes, stream, a, maps);
 }
 
 template <bool kBf16>
 bool launch_tc_d(const TreeArgs& a, const TcMaps& maps, const Plan& p, cudaStream_t stream) {
-  if (p.kd == 64) return launch_tc<kBf16, 64, 1>(a, maps, p.grid, stream);
-  if (p.kd == 256) return launch_tc<kBf16, 256, 1>(a, maps, p.grid, stream);
-  return p.row_tiles_each == 2 ? launch_tc<kBf16, 128, 2>(a, maps, p.grid, stream)
-                               : launch_tc<kBf16, 128, 1>(a, maps, p.grid, stream);
+  switch (p.kd) {
+    case 64: return p.two_tiles ? launch_tc<kBf16, 64, true>(a, maps, p.grid, stream)
+                                : launch_tc<kBf16, 64, false>(a, maps, p.grid, stream);
+    case 128: return p.two_tiles ? launch_tc<kBf16, 128, true>(a, maps, p.grid, stream)
+                                 : launch_tc<kBf16, 128, false>(a, maps, p.grid, stream);
+    default: return launch_tc<kBf16, 256, false>(a, maps, p.grid, stream);
+  }
 }
 
-// The caches' tensor maps; false where TMA cannot describe them.
-bool make_maps(const AttnPagedCache* c, TcMaps* m) {
-  m->rows = c->page_size % 64 == 0 ? 64 : c->page_size % 32 == 0 ? 32 : c->page_size % 16 == 0 ? 16 : 8;
+// The caches' tensor maps; boxes = 0 where TMA does not suit them.
+TcMaps make_maps(const AttnPagedCache* c, const Plan& p) {
+  TcMaps m;
   const unsigned long long limit = wait_limit_ns();
-  m->wait_ns = limit != 0 ? limit : kWaitTimeoutNs;
-  m->lose = drop_arrival_requested();
+  m.wait_ns = limit != 0 ? limit : kWaitTimeoutNs;
+  m.lose = drop_arrival_requested();
+  m.rows = p.box_rows;
+  m.boxes = p.boxes;
   auto encode = [&](CUtensorMap* map, const void* base, const long long* st) {
     return make_tensor_map_4d(map, base, c->dtype == ATTN_BF16, c->D, c->page_size, c->heads, c->num_pages, st[2], st[1],
-                              st[0], 64, m->rows) == 0;
+                              st[0], 64, m.rows) == 0;
   };
-  return encode(&m->k, c->k, c->k_strides) && encode(&m->v, c->v, c->v_strides);
+  if (m.boxes > 0 && (c->num_pages == 0 || !encode(&m.k, c->k, c->k_strides) || !encode(&m.v, c->v, c->v_strides)))
+    m.boxes = 0;
+  return m;
 }
 
 template <typename T, int kDP>
@@ -1322,9 +1677,7 @@ extern "C" int launch_attn_tree(const AttnPagedCache* cache, const void* q, cons
     return ATTN_ERR_MISALIGNED;
   st = check_device();
   if (st != ATTN_OK) return st;
-  TcMaps maps;
-  const bool fast = tc_takes(cache) && aligned_to(q, 16) && aligned_to(out, 16) && qs[0] % 8 == 0 && qs[1] % 8 == 0 &&
-                    qs[2] % 8 == 0 && make_maps(cache, &maps);
+  const bool fast = aligned_to(q, 16) && aligned_to(out, 16) && qs[0] % 8 == 0 && qs[1] % 8 == 0 && qs[2] % 8 == 0;
   const Plan p = make_plan(cache, fast, Hq, S, sm_count());
   if (workspace_bytes < p.bytes || p.tiles > 0x7fffffffLL - 65536) return ATTN_ERR_INVALID_ARGUMENT;
 
@@ -1352,14 +1705,16 @@ extern "C" int launch_attn_tree(const AttnPagedCache* cache, const void* q, cons
   a.part_ml = reinterpret_cast<float2*>(ws + p.ml_at);
   a.part_o = reinterpret_cast<float4*>(ws + p.o_at);
   a.D4 = (D + 3) / 4;
-  const unsigned long long ps = static_cast<unsigned long long>(cache->page_size);
-  a.ps_shift = 0;
-  while ((1ull << a.ps_shift) < ps) ++a.ps_shift;
-  a.ps_mul = static_cast<unsigned>((((1ull << a.ps_shift) - ps) << 32) / ps + 1);
+  divisor(cache->page_size, &a.ps_mul, &a.ps_shift);
+  divisor(S, &a.s_mul, &a.s_shift);
+  divisor(p.tile, &a.t_mul, &a.t_shift);
+  a.tile = p.tile;
 
   bool ok;
-  if (p.tc) ok = cache->dtype == ATTN_BF16 ? launch_tc_d<true>(a, maps, p, stream) : launch_tc_d<false>(a, maps, p, stream);
-  else switch (cache->dtype) {
+  if (p.tc) {
+    const TcMaps maps = make_maps(cache, p);
+    ok = cache->dtype == ATTN_BF16 ? launch_tc_d<true>(a, maps, p, stream) : launch_tc_d<false>(a, maps, p, stream);
+  } else switch (cache->dtype) {
     case ATTN_F16: ok = launch_simt_d<__half>(a, p, stream); break;
     case ATTN_BF16: ok = launch_simt_d<__nv_bfloat16>(a, p, stream); break;
     default: ok = launch_simt_d<float>(a, p, stream); break;
