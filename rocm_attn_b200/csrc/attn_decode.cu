@@ -34,6 +34,10 @@
 // multiple of 8, 16-byte rows) on warp-level tensor cores, and
 // attn_decode_simt_kernel (fp32, any D <= 256, any strides).
 //
+// The tensor-core kernel also serves attention of drafted tokens (attn_tree.cu)
+// where a kv head has up to eight rows (query head, token): kTree, with the rows
+// as its query heads and the tokens that a row does not follow left out.
+//
 // Measured on B200 (calls in a row): 64 sequences of up to 16384 tokens, 64/8
 // heads of 128, fp16, 2.75 GB of K and V: 402 to 433 us on different GPUs, 6.4
 // to 6.8 TB/s, where a copy does 6.54; 24 of up to 4096, 32/8 heads, bf16, with
@@ -87,6 +91,12 @@ struct DecodeArgs {
   // Multiplication (1994), figure 4.1.
   unsigned ps_mul;
   int ps_shift;
+  // Drafted tokens (kTree): a query head here is row i * S + s, query head i and
+  // drafted token s, of a kv head, eight at most.  As for launch_attn_tree.
+  int S;
+  const int* parents;
+  long long parents_stride;
+  const int* new_lens;
 };
 
 __device__ __forceinline__ void prefetch_l1(const void* p) { asm volatile("prefetch.global.L1 [%0];" ::"l"(p)); }
@@ -166,13 +176,29 @@ struct Cursor {
   int b, h, rt, t, T, len;
 };
 
+// Drafted tokens of sequence b.
+__device__ __forceinline__ int drafted_of(const DecodeArgs& a, int b, int* fault) {
+  if (!a.new_lens) return a.S;
+  const int n = *(a.new_lens + b);
+  if (n > a.S) *fault |= kFaultPage;
+  return max(min(n, a.S), 0);
+}
+
+// The tokens that are attended to: none where no row asks.
+template <bool kTree>
+__device__ __forceinline__ int seq_len(const DecodeArgs& a, int b, int* fault) {
+  const int len = paged_len(a.c, b, fault);
+  if constexpr (kTree) return drafted_of(a, b, fault) > 0 ? len : 0;
+  return len;
+}
+
 template <int kTile>
 __device__ __forceinline__ int tiles_of(const DecodeArgs& a, int len) {
   const int n = a.pages ? (len > 0 ? a.n_pages * a.c.page_size : 0) : len;
   return (n + kTile - 1) / kTile;
 }
 
-template <int kTile>
+template <int kTile, bool kTree = false>
 __device__ __forceinline__ void advance(const DecodeArgs& a, Cursor& c, int* fault) {
   c.t += max(a.cluster, 1);
   if (c.t < c.T) return;
@@ -183,7 +209,7 @@ __device__ __forceinline__ void advance(const DecodeArgs& a, Cursor& c, int* fau
   c.h = 0;
   c.T = 0;
   while (c.T == 0 && ++c.b < a.c.B) {
-    c.len = paged_len(a.c, c.b, fault);
+    c.len = seq_len<kTree>(a, c.b, fault);
     c.T = tiles_of<kTile>(a, c.len);
   }
 }
@@ -209,7 +235,7 @@ struct ScheduleSmem {
 // tiles the block table can name below 2^31.  kWhole: the threads of the CTA
 // share the batch; otherwise each warp looks at all of it by itself, without
 // barriers, which is quicker for batches that a few loads per lane cover.
-template <int kTile, bool kWhole>
+template <int kTile, bool kWhole, bool kTree>
 __device__ __forceinline__ Cursor schedule_by(const DecodeArgs& a, ScheduleSmem& s, Run* run, int* fault) {
   constexpr int kShare = kWhole ? kThreads : 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, id = kWhole ? threadIdx.x : lane;
@@ -217,7 +243,7 @@ __device__ __forceinline__ Cursor schedule_by(const DecodeArgs& a, ScheduleSmem&
   const int b0 = min(a.c.B, id * seg), b1 = min(a.c.B, b0 + seg);
   int mine = 0, len = 0, T = 0;
   for (int b = b0; b < b1; ++b) {
-    len = paged_len(a.c, b, fault);
+    len = seq_len<kTree>(a, b, fault);
     T = tiles_of<kTile>(a, len);
     mine += T;
   }
@@ -250,7 +276,7 @@ __device__ __forceinline__ Cursor schedule_by(const DecodeArgs& a, ScheduleSmem&
     int in = run->first - before * units, b = b0;
     if (seg > 1) {
       for (;; ++b) {
-        len = paged_len(a.c, b, fault);
+        len = seq_len<kTree>(a, b, fault);
         T = tiles_of<kTile>(a, len);
         if (in < T * units || b + 1 >= b1) break;
         in -= T * units;
@@ -272,9 +298,10 @@ __device__ __forceinline__ Cursor schedule_by(const DecodeArgs& a, ScheduleSmem&
   }
 }
 
-template <int kTile>
+template <int kTile, bool kTree = false>
 __device__ __forceinline__ Cursor schedule(const DecodeArgs& a, ScheduleSmem& s, Run* run, int* fault) {
-  return a.c.B <= 128 ? schedule_by<kTile, false>(a, s, run, fault) : schedule_by<kTile, true>(a, s, run, fault);
+  return a.c.B <= 128 ? schedule_by<kTile, false, kTree>(a, s, run, fault)
+                      : schedule_by<kTile, true, kTree>(a, s, run, fault);
 }
 
 // The first query row of the unit at c.
@@ -284,11 +311,11 @@ __device__ __forceinline__ const T* query_rows(const DecodeArgs& a, const Cursor
 }
 
 // Output rows of empty sequences are zeros.
-template <typename T>
+template <typename T, bool kTree = false>
 __device__ __forceinline__ void zero_empty_rows(const DecodeArgs& a, int* fault) {
   const long long per_seq = static_cast<long long>(a.Hq) * a.c.D;
   for (int b = blockIdx.x; b < a.c.B; b += gridDim.x) {
-    if (paged_len(a.c, b, fault) > 0 && !(a.pages && a.n_pages == 0)) continue;
+    if (seq_len<kTree>(a, b, fault) > 0 && !(a.pages && a.n_pages == 0)) continue;
     T* o = static_cast<T*>(a.out) + b * per_seq;
     for (long long i = threadIdx.x; i < per_seq; i += kThreads) o[i] = from_f32<T>(0.f);
   }
@@ -415,7 +442,7 @@ struct TmaMaps {
   int lose;  // watchdog test build only: CTA 0's first wait is for bytes that never come
 };
 
-template <bool kBf16, int kD, int kNT, bool kWeights, bool kTma>
+template <bool kBf16, int kD, int kNT, bool kWeights, bool kTma, bool kTree>
 __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
     attn_decode_mma_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ TmaMaps maps) {
   using C = MmaCfg<kD>;
@@ -437,6 +464,9 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
   __shared__ uint64_t s_full[kWarps][kStages];
   __shared__ int s_abort, s_code, s_late;
   __shared__ float s_cm[8 * kNT], s_cl[8 * kNT];  // of this CTA's part of a cluster's unit
+  // kTree: of each drafted token those it follows and itself (0: it is not
+  // there), and of this unit (and the last) those with infinite or NaN values.
+  __shared__ uint32_t s_follows[32], s_odd[2];
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int fault = 0;
@@ -450,6 +480,7 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
     }
     if (threadIdx.x == 0) s_abort = s_code = s_late = 0;
   }
+  if (kTree && threadIdx.x < 2) s_odd[threadIdx.x] = 0;
   launch_dependents();
   grid_dependency_wait();
   int n;
@@ -463,15 +494,15 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
     cur.h = hu / a.row_tiles;
     cur.rt = hu - cur.h * a.row_tiles;
     cur.t = blockIdx.x % a.cluster;
-    cur.len = a.pages ? paged_len(a.c, cur.b, &fault) : a.c.capacity();
+    cur.len = a.pages ? seq_len<kTree>(a, cur.b, &fault) : a.c.capacity();
     cur.T = tiles_of<kTile>(a, cur.len);
     n = (cur.T - cur.t + a.cluster - 1) / a.cluster;
     if (threadIdx.x < 8 * kNT) s_cm[threadIdx.x] = -INFINITY, s_cl[threadIdx.x] = 0.f;
   } else {
     if (threadIdx.x == 0) a.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
-    cur = schedule<kTile>(a, s_sched, &run, &fault);
+    cur = schedule<kTile, kTree>(a, s_sched, &run, &fault);
     n = run.n;
-    zero_empty_rows<T>(a, &fault);
+    zero_empty_rows<T, kTree>(a, &fault);
     __syncthreads();  // the set-up above
   }
 
@@ -512,7 +543,7 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
       if (warp == 0 && ahead.t == 0) prefetch_q(ahead);
       if (kKeys == 32 || lane < kKeys)
         locate_logical(a, last_b, ahead.h, ahead.t * kTile + warp * kKeys + lane, last_len, &page[s], &row[s]);
-      advance<kTile>(a, ahead, &fault);
+      advance<kTile, kTree>(a, ahead, &fault);
       ++looked;
     }
   };
@@ -594,7 +625,7 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
   if (a.cluster) {
     if (!a.pages) {
       // The length: what was looked up behind it does not count.
-      cur.len = ahead.len = last_len = paged_len(a.c, cur.b, &fault);
+      cur.len = ahead.len = last_len = seq_len<kTree>(a, cur.b, &fault);
       cur.T = ahead.T = tiles_of<kTile>(a, cur.len);
       n = max(0, (cur.T - cur.t + a.cluster - 1) / a.cluster);
 #pragma unroll
@@ -611,6 +642,9 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
   float m[kNT][2], l[kNT][2];  // of query heads 8 t + 2 (lane % 4) + {0, 1}
   bool begun = a.cluster ? true : cur.t == 0, fresh = true;
   int stage = 0;
+  // kTree: where the drafted tokens begin, and those that the thread's rows follow.
+  int base = 0, odd_now = 0;
+  uint32_t follows[kNT][2];
 
   // Scores of tokens lane / 4 + {0, 8} of the chunk's g-th 16 and of two heads
   // of column tile t, for the weights: -inf where there is no token, and a
@@ -654,6 +688,34 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
           m[t][0] = m[t][1] = -INFINITY;
           l[t][0] = l[t][1] = 0.f;
         }
+        if constexpr (kTree) {
+          // Lane s walks up from drafted token s, all lanes a step at a time.
+          const int n_draft = drafted_of(a, cur.b, &fault);
+          base = max(*(a.c.lens + cur.b), 0) - n_draft;
+          int parent = lane - 1;
+          if (a.parents && lane < n_draft) {
+            parent = *(a.parents + cur.b * a.parents_stride + lane);
+            if (parent < -1 || parent >= lane) {
+              fault |= kFaultPage;
+              parent = -1;
+            }
+          }
+          uint32_t mine = lane < n_draft ? 1u << lane : 0u;
+          int at = lane < n_draft ? parent : -1;
+          while (__any_sync(0xffffffffu, at >= 0)) {
+            const int up = __shfl_sync(0xffffffffu, parent, at & 31);
+            if (at >= 0) {
+              mine |= 1u << at;
+              at = up;
+            }
+          }
+          if (warp == 0) s_follows[lane] = mine;
+#pragma unroll
+          for (int t = 0; t < kNT; ++t)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              follows[t][e] = __shfl_sync(0xffffffffu, mine, (cur.rt * a.rows + t * 8 + (lane & 3) * 2 + e) % a.S);
+        }
         fresh = false;
       }
       if constexpr (!kTma) cp_async_wait<kStages - 1>();
@@ -692,6 +754,36 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
               fence_proxy_async_smem();
               __syncwarp();
             }
+          }
+        }
+        const int chunk_pos = cur.t * kTile + warp * kKeys;  // of the chunk's first token
+        if constexpr (kTree) {
+          if (mask != 0 && chunk_pos + kKeys > base) {
+            // Infinite and NaN values of drafted tokens, which some rows do not
+            // follow, become zeros; the rows that do add them at the unit's end.
+            const int r0 = max(0, base - chunk_pos);
+            bool found = false;
+#pragma unroll 1
+            for (int e = lane; e < (kKeys - r0) * kCols; e += 32) {
+              const int r = r0 + e / kCols, c = e % kCols;
+              if (!(mask >> r & 1u)) continue;
+              uint4* v_at = reinterpret_cast<uint4*>(ring + stage * C::kStageBytes + kKeys * kD * 2 +
+                                                     (c / 8) * (kKeys * 128) + r * 128 + (c % 8) * 16);
+              uint32_t x[4] = {v_at->x, v_at->y, v_at->z, v_at->w};
+              bool odd = false;
+              constexpr uint32_t kExp = kBf16 ? 0x7f80u : 0x7c00u;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                if ((x[i] & kExp) == kExp) x[i] &= 0xffff0000u, odd = true;
+                if ((x[i] >> 16 & kExp) == kExp) x[i] &= 0xffffu, odd = true;
+              }
+              if (!odd) continue;
+              found = true;
+              *v_at = make_uint4(x[0], x[1], x[2], x[3]);
+              atomicOr(&s_odd[odd_now], 1u << ((chunk_pos + r - base) & 31));
+            }
+            if (__any_sync(0xffffffffu, found)) fence_proxy_async_smem();
+            __syncwarp();
           }
         }
 #pragma unroll
@@ -736,16 +828,39 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
                 x[e] = live >> ((e >> 1) * 8 + (lane >> 2)) & 1u ? fmaxf(s[t][e], kLowest) : -INFINITY;
               keep_scores(t, g, x[0], x[1], x[2], x[3]);
             }
+            // Whether tokens of the 16 are drafted: then a row sees those it
+            // follows, and may see none.
+            const bool drafts = kTree && chunk_pos + g * 16 + 16 > base;
             float f[2], top[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              float mx = fmaxf(s[t][e], s[t][e + 2]);
+              float mx;
+              if (drafts) {
+                mx = -INFINITY;
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                  const int d = chunk_pos + g * 16 + k * 8 + (lane >> 2) - base;
+                  const bool sees =
+                      (live >> (k * 8 + (lane >> 2)) & 1u) && (d < 0 || (d < 32 && (follows[t][e] >> d & 1u)));
+                  if (!sees) s[t][e + 2 * k] = -INFINITY;
+                  if (sees) mx = fmaxf(mx, fmaxf(s[t][e + 2 * k], kLowest));
+                }
+              } else {
+                mx = fmaxf(s[t][e], s[t][e + 2]);
+              }
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-              top[e] = fmaxf(fmaxf(m[t][e], mx), kLowest);  // there is a token among the 16
-              f[e] = ex2_approx(m[t][e] - top[e]);
-              m[t][e] = top[e];
+              top[e] = fmaxf(fmaxf(m[t][e], mx), drafts ? -INFINITY : kLowest);  // there is a token among the 16
+              if constexpr (kTree) {
+                const float to = finite_max(top[e]);
+                f[e] = ex2_approx(m[t][e] - to);
+                m[t][e] = top[e];
+                top[e] = to;
+              } else {
+                f[e] = ex2_approx(m[t][e] - top[e]);
+                m[t][e] = top[e];
+              }
             }
             if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
               l[t][0] *= f[0];
@@ -833,6 +948,31 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
               sum.z += y.z * f;
               sum.w += y.w * f;
             }
+            if constexpr (kTree) {
+              const uint32_t seen = s_follows[(cur.rt * a.rows + r) % a.S];
+              if (seen == 0) {  // no such drafted token
+                M = -INFINITY;
+                L = 0.f;
+                sum = make_float4(0.f, 0.f, 0.f, 0.f);
+              }
+              // what the products left out
+#pragma unroll 1
+              for (uint32_t left = seen & s_odd[odd_now]; left != 0; left &= left - 1) {
+                const int pos = base + __ffs(left) - 1;
+                int page = 0, row = 0;
+                locate_logical(a, cur.b, cur.h, pos, cur.len, &page, &row);
+                locate_physical(a, cur.b, cur.len, &page, &row);
+                if (!located(a, page, row, &fault)) continue;
+                const T* v = static_cast<const T*>(a.c.v) + page * a.c.vs[0] + cur.h * a.c.vs[1] + row * a.c.vs[2] + c4 * 4;
+                float* to[4] = {&sum.x, &sum.y, &sum.z, &sum.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const float x = to_f32(v[i]);
+                  if (!isfinite(x)) *to[i] += x;
+                }
+              }
+              if (e == threadIdx.x && threadIdx.x == 0) s_odd[odd_now ^ 1] = 0;
+            }
             if (p.whole) {
               const float inv = inverse(M, L);
               T* out = static_cast<T*>(a.out) + (p.row0 + r) * a.c.D + c4 * 4;
@@ -852,6 +992,7 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
           if constexpr (kTma) fence_proxy_async_smem();
           __syncthreads();  // all this is read before it is written again
         }
+        odd_now ^= 1;
         begun = true;
         fresh = true;
       }
@@ -859,7 +1000,7 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<kD>::kCtas)
     __syncwarp();
     issue(stage);
     stage = stage + 1 == kStages ? 0 : stage + 1;
-    if (i >= 0) advance<kTile>(a, cur, &fault);
+    if (i >= 0) advance<kTile, kTree>(a, cur, &fault);
   }
   if (a.cluster > 1) {
     // The parts of the cluster's CTAs are joined in their order, each CTA
@@ -1344,6 +1485,14 @@ Plan make_plan(const AttnPagedCache* c, bool fast, int Hq, int n_pages, bool lis
   return p;
 }
 
+// Multiplier and shift of the division by the page size (see DecodeArgs).
+void page_divisor(int page_size, DecodeArgs* a) {
+  const unsigned long long ps = static_cast<unsigned long long>(page_size);
+  a->ps_shift = 0;
+  while ((1ull << a->ps_shift) < ps) ++a->ps_shift;
+  a->ps_mul = static_cast<unsigned>((((1ull << a->ps_shift) - ps) << 32) / ps + 1);
+}
+
 // The checks of a call that need no device.  Returns ATTN_OK or a status.
 int check_decode(const AttnPagedCache* c, int Hq, const void* pages, int n_pages, bool weights, PagedView* view) {
   const int st = check_paged_cache(c, kCacheK | kCacheV, view);
@@ -1359,9 +1508,9 @@ int check_decode(const AttnPagedCache* c, int Hq, const void* pages, int n_pages
 
 // The first launch on a device opts the kernel in to its shared memory and to
 // the largest shared-memory share of the SM, so that two CTAs fit.
-template <bool kBf16, int kD, int kNT, bool kWeights, bool kTma>
+template <bool kBf16, int kD, int kNT, bool kWeights, bool kTma, bool kTree>
 bool launch_mma(const DecodeArgs& a, const TmaMaps& maps, int grid, cudaStream_t stream) {
-  auto kern = attn_decode_mma_kernel<kBf16, kD, kNT, kWeights, kTma>;
+  auto kern = attn_decode_mma_kernel<kBf16, kD, kNT, kWeights, kTma, kTree>;
   static bool done[64] = {};
   static std::mutex mu;
   int dev = 0;
@@ -1382,27 +1531,29 @@ bool launch_mma(const DecodeArgs& a, const TmaMaps& maps, int grid, cudaStream_t
 }
 
 // Column tiles of eight query heads: 1, 2 or 4.
-template <bool kBf16, int kD, bool kWeights, bool kTma>
+template <bool kBf16, int kD, bool kWeights, bool kTma, bool kTree>
 bool launch_mma_tiles(const DecodeArgs& a, const TmaMaps& maps, int grid, cudaStream_t stream) {
-  if (a.rows <= 8) return launch_mma<kBf16, kD, 1, kWeights, kTma>(a, maps, grid, stream);
-  if (a.rows <= 16) return launch_mma<kBf16, kD, 2, kWeights, kTma>(a, maps, grid, stream);
-  if constexpr (MmaCfg<kD>::kMaxHeads > 16) return launch_mma<kBf16, kD, 4, kWeights, kTma>(a, maps, grid, stream);
+  if (a.rows <= 8 || kTree) return launch_mma<kBf16, kD, 1, kWeights, kTma, kTree>(a, maps, grid, stream);
+  if constexpr (!kTree) {
+    if (a.rows <= 16) return launch_mma<kBf16, kD, 2, kWeights, kTma, false>(a, maps, grid, stream);
+    if constexpr (MmaCfg<kD>::kMaxHeads > 16) return launch_mma<kBf16, kD, 4, kWeights, kTma, false>(a, maps, grid, stream);
+  }
   return false;
 }
 
-template <bool kBf16, bool kWeights, bool kTma>
+template <bool kBf16, bool kWeights, bool kTma, bool kTree>
 bool launch_mma_d(const DecodeArgs& a, const TmaMaps& maps, int kd, int grid, cudaStream_t stream) {
   switch (kd) {
-    case 64: return launch_mma_tiles<kBf16, 64, kWeights, kTma>(a, maps, grid, stream);
-    case 128: return launch_mma_tiles<kBf16, 128, kWeights, kTma>(a, maps, grid, stream);
-    default: return launch_mma_tiles<kBf16, 256, kWeights, kTma>(a, maps, grid, stream);
+    case 64: return launch_mma_tiles<kBf16, 64, kWeights, kTma, kTree>(a, maps, grid, stream);
+    case 128: return launch_mma_tiles<kBf16, 128, kWeights, kTma, kTree>(a, maps, grid, stream);
+    default: return launch_mma_tiles<kBf16, 256, kWeights, kTma, kTree>(a, maps, grid, stream);
   }
 }
 
 // TMA where 16 divides the page size (a box is rows of one page) and the
 // strides suit it, else 16-byte copies (pages of 24 rows of 128 bytes: boxes
 // of 8 rows 143 us, copies 135 us).
-template <bool kBf16, bool kWeights>
+template <bool kBf16, bool kWeights, bool kTree = false>
 bool launch_mma_any(const DecodeArgs& a, const Plan& p, cudaStream_t stream) {
   TmaMaps maps;
   const unsigned long long limit = wait_limit_ns();
@@ -1413,8 +1564,8 @@ bool launch_mma_any(const DecodeArgs& a, const Plan& p, cudaStream_t stream) {
                               16) == 0;
   };
   if (a.c.page_size % 16 == 0 && a.c.num_pages > 0 && encode(&maps.k, a.c.k, a.c.ks) && encode(&maps.v, a.c.v, a.c.vs))
-    return launch_mma_d<kBf16, kWeights, true>(a, maps, p.kd, p.grid, stream);
-  return launch_mma_d<kBf16, kWeights, false>(a, maps, p.kd, p.grid, stream);
+    return launch_mma_d<kBf16, kWeights, true, kTree>(a, maps, p.kd, p.grid, stream);
+  return launch_mma_d<kBf16, kWeights, false, kTree>(a, maps, p.kd, p.grid, stream);
 }
 
 template <typename T, int kPer, bool kWeights>
@@ -1458,6 +1609,50 @@ int page_word_read_clear_decode(cudaStream_t stream, int* host) {
                      cudaSuccess
              ? 0
              : -1;
+}
+
+bool decode_rows_plan(const AttnPagedCache* c, int Hq, int S, int sms, size_t* bytes) {
+  const long long rows = static_cast<long long>(Hq / c->heads) * S;
+  if (!mma_takes(c) || rows > 8 || static_cast<long long>(c->B) * Hq * S > 0x7fffffffLL) return false;
+  const Plan p = make_plan(c, true, Hq * S, 0, false, false, sms);
+  if (p.tiles > 0x7fffffffLL - 65536) return false;
+  *bytes = p.bytes;
+  return true;
+}
+
+bool launch_decode_rows(const AttnPagedCache* c, const PagedView& view, const void* q, long long q_b, long long q_row,
+                        void* out, int Hq, int S, float scale, const int* parents, long long parents_stride,
+                        const int* new_lens, void* workspace, cudaStream_t stream) {
+  const Plan p = make_plan(c, true, Hq * S, 0, false, false, sm_count());
+  char* ws = static_cast<char*>(workspace);
+  DecodeArgs a = {};
+  a.c = view;
+  a.q = q;
+  a.q_b = q_b;
+  a.q_h = q_row;
+  a.out = out;
+  a.Hq = Hq * S;
+  a.group = Hq * S / c->heads;
+  a.rows = p.rows;
+  a.row_tiles = p.row_tiles;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.cluster = p.cluster;
+  a.meta = reinterpret_cast<int4*>(ws + p.meta_at);
+  a.part_ml = reinterpret_cast<float2*>(ws + p.ml_at);
+  a.part_o = reinterpret_cast<float*>(ws + p.o_at);
+  a.D4 = (c->D + 3) / 4 * 4;
+  page_divisor(c->page_size, &a);
+  a.S = S;
+  a.parents = parents;
+  a.parents_stride = parents_stride;
+  a.new_lens = new_lens;
+  const bool bf16 = c->dtype == ATTN_BF16;
+  if (!(bf16 ? launch_mma_any<true, false, true>(a, p, stream) : launch_mma_any<false, false, true>(a, p, stream)))
+    return false;
+  if (p.cluster) return true;
+  const dim3 grid(p.grid, p.rows), block(kJoinWarps * 32);
+  return bf16 ? launch_after(attn_decode_join_kernel<__nv_bfloat16>, grid, block, 0, stream, 1, true, a)
+              : launch_after(attn_decode_join_kernel<__half>, grid, block, 0, stream, 1, true, a);
 }
 
 }  // namespace ra
@@ -1530,10 +1725,10 @@ extern "C" int launch_attn_decode(const AttnPagedCache* cache, const void* q, co
   a.part_ml = reinterpret_cast<float2*>(ws + p.ml_at);
   a.part_o = reinterpret_cast<float*>(ws + p.o_at);
   a.D4 = (D + 3) / 4 * 4;
-  const unsigned long long ps = static_cast<unsigned long long>(cache->page_size);
-  a.ps_shift = 0;
-  while ((1ull << a.ps_shift) < ps) ++a.ps_shift;
-  a.ps_mul = static_cast<unsigned>((((1ull << a.ps_shift) - ps) << 32) / ps + 1);
+  page_divisor(cache->page_size, &a);
+  a.S = 0;
+  a.parents = a.new_lens = nullptr;
+  a.parents_stride = 0;
 
   if (!(weights ? launch_first<true>(a, p, cache->dtype, stream) : launch_first<false>(a, p, cache->dtype, stream)))
     return ATTN_ERR_LAUNCH;

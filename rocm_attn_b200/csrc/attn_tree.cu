@@ -1388,32 +1388,37 @@ __global__ void __launch_bounds__(TcCfg<kD, kTwo>::kThreads, TcCfg<kD, kTwo>::kC
 // ---------------------------------------------------------------------------
 
 // The unit that CTA blockIdx.x of the grid before began and did not finish:
-// warp (row tile, columns), lane a row and eight columns of it, its parts in the
-// order of the tokens.
-constexpr int kJoinWarps = 4, kJoinCols = 8;
+// lane a row and eight columns of it, its parts in the order of the tokens, or
+// by `split` warps that take every split-th of them where there are many (one
+// sequence of 4096 tokens, 8 kv heads: 37 parts each).
+constexpr int kJoinWarps = 8, kJoinCols = 8;
 
 template <typename T>
-__global__ void __launch_bounds__(kJoinWarps * 32) attn_tree_join_kernel(const __grid_constant__ TreeArgs a) {
+__global__ void __launch_bounds__(kJoinWarps * 32) attn_tree_join_kernel(const __grid_constant__ TreeArgs a, int split) {
+  __shared__ float2 s_ml[kJoinWarps][32];
+  __shared__ float4 s_o[kJoinWarps][2][32];
   launch_dependents();
   grid_dependency_wait();
-  const int c = blockIdx.x, lane = threadIdx.x & 31;
-  const int col_tiles = (a.c.D + kJoinCols - 1) / kJoinCols;
-  const int w = blockIdx.y * kJoinWarps + (threadIdx.x >> 5), rows32 = w / col_tiles, d = (w - rows32 * col_tiles) * kJoinCols;
+  const int c = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int col_tiles = (a.c.D + kJoinCols - 1) / kJoinCols, first = warp & (split - 1);
+  const int w = (blockIdx.y * kJoinWarps + warp) / split, rows32 = w / col_tiles, d = (w - rows32 * col_tiles) * kJoinCols;
   const int4 meta = a.meta[c];
+  if (meta.z == 0) return;
   const int r = rows32 * 32 + lane, gr = meta.y * a.unit_rows + r;
-  if (meta.z == 0 || r >= a.unit_rows || gr >= a.rows) return;
-  const bool two = d / 4 + 1 < a.D4;
+  const bool live = r < a.unit_rows && gr < a.rows, two = d / 4 + 1 < a.D4;
   float M = -INFINITY, L = 0.f;
   float4 o[2] = {};
-  for (int i0 = 0; i0 <= meta.z; i0 += 4) {
+#pragma unroll 1
+  for (int i0 = first; live && i0 <= meta.z; i0 += 4 * split) {
     float2 ml[4];
     float4 y[4][2];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
+      const int part = i0 + i * split;
       ml[i] = make_float2(-INFINITY, 0.f);
       y[i][0] = y[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (i0 + i <= meta.z) {
-        const long long slot = i0 + i == 0 ? 2 * c + 1 : 2 * (c + i0 + i);
+      if (part <= meta.z) {
+        const long long slot = part == 0 ? 2 * c + 1 : 2 * (c + part);
         ml[i] = a.part_ml[slot * a.unit_rows + r];
         const float4* at = a.part_o + (slot * a.D4 + d / 4) * a.unit_rows + r;
         y[i][0] = *at;
@@ -1439,6 +1444,34 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_tree_join_kernel(const _
       }
     }
   }
+  if (split > 1) {
+    s_ml[warp][lane] = make_float2(M, L);
+    s_o[warp][0][lane] = o[0];
+    s_o[warp][1][lane] = o[1];
+    __syncthreads();
+    if (first != 0) return;
+    float top = M;
+    for (int k = 1; k < split; ++k) top = fmaxf(top, s_ml[warp + k][lane].x);
+    float f = ex2_approx(M - finite_max(top));
+    L *= f;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) o[k].x *= f, o[k].y *= f, o[k].z *= f, o[k].w *= f;
+    for (int i = 1; i < split; ++i) {
+      const float2 ml = s_ml[warp + i][lane];
+      f = ex2_approx(ml.x - finite_max(top));
+      L = fmaf(ml.y, f, L);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const float4 y = s_o[warp + i][k][lane];
+        o[k].x = fmaf(y.x, f, o[k].x);
+        o[k].y = fmaf(y.y, f, o[k].y);
+        o[k].z = fmaf(y.z, f, o[k].z);
+        o[k].w = fmaf(y.w, f, o[k].w);
+      }
+    }
+    M = top;
+  }
+  if (!live) return;
   T* out = static_cast<T*>(a.out) + (static_cast<long long>(meta.x) * a.S + gr) * a.c.D + d;
   const float inv = inverse(M, L);
   const float x[8] = {o[0].x, o[0].y, o[0].z, o[0].w, o[1].x, o[1].y, o[1].z, o[1].w};
@@ -1655,6 +1688,8 @@ extern "C" int attn_tree_workspace_bytes(const AttnPagedCache* cache, int Hq, in
   // q or out may turn out to need the other kernel: room for either
   const Plan fast = make_plan(cache, true, Hq, S, sms), other = make_plan(cache, false, Hq, S, sms);
   *bytes = fast.bytes > other.bytes ? fast.bytes : other.bytes;
+  size_t few = 0;
+  if (decode_rows_plan(cache, Hq, S, sms, &few) && few > *bytes) *bytes = few;
   return ATTN_OK;
 }
 
@@ -1678,11 +1713,25 @@ extern "C" int launch_attn_tree(const AttnPagedCache* cache, const void* q, cons
   st = check_device();
   if (st != ATTN_OK) return st;
   const bool fast = aligned_to(q, 16) && aligned_to(out, 16) && qs[0] % 8 == 0 && qs[1] % 8 == 0 && qs[2] % 8 == 0;
-  const Plan p = make_plan(cache, fast, Hq, S, sm_count());
-  if (workspace_bytes < p.bytes || p.tiles > 0x7fffffffLL - 65536) return ATTN_ERR_INVALID_ARGUMENT;
-
+  const int sms = sm_count();
   float scale = softmax_scale;
   if (!(scale > 0.f) || !isfinite(scale)) scale = 1.0f / sqrtf(static_cast<float>(D));
+  // Up to eight rows (which must lie evenly in memory) fill one column tile of
+  // attn_decode's products, where a tile's softmax is not one warp's work of some
+  // 1100 clocks: 8 rows, D = 128, that kernel / this one, us: one sequence of 4096
+  // tokens 14.3 / 19.5, 24 of up to 4096 57.0 / 62.5, 16 of up to 16384 138 / 154;
+  // 16 rows 19.9 / 19.7, 77.4 / 63.2, 172 / 155.
+  const bool even = S == 1 || Hq == 1 || qs[1] == S * qs[2];
+  size_t few = 0;
+  if (fast && even && decode_rows_plan(cache, Hq, S, sms, &few)) {
+    if (workspace_bytes < few) return ATTN_ERR_INVALID_ARGUMENT;
+    return launch_decode_rows(cache, view, q, qs[0], S == 1 ? qs[1] : qs[2], out, Hq, S, scale, parents, parents_stride,
+                              new_lens, workspace, stream)
+               ? ATTN_OK
+               : ATTN_ERR_LAUNCH;
+  }
+  const Plan p = make_plan(cache, fast, Hq, S, sms);
+  if (workspace_bytes < p.bytes || p.tiles > 0x7fffffffLL - 65536) return ATTN_ERR_INVALID_ARGUMENT;
   char* ws = static_cast<char*>(workspace);
   TreeArgs a;
   a.c = view;
@@ -1721,12 +1770,16 @@ extern "C" int launch_attn_tree(const AttnPagedCache* cache, const void* q, cons
   }
   if (!ok) return ATTN_ERR_LAUNCH;
   const int used = a.rows < p.unit_rows ? a.rows : p.unit_rows;
-  const int join_warps = (used + 31) / 32 * ((D + kJoinCols - 1) / kJoinCols);
-  const dim3 grid(p.grid, (join_warps + kJoinWarps - 1) / kJoinWarps), block(kJoinWarps * 32);
+  const long long items = static_cast<long long>((used + 31) / 32) * ((D + kJoinCols - 1) / kJoinCols);
+  // About how many CTAs share a unit, at full lengths.
+  const long long parts = p.grid / (static_cast<long long>(cache->B) * cache->heads * p.row_tiles);
+  int split = 1;
+  while (split < kJoinWarps && split * 4 <= parts) split *= 2;
+  const dim3 grid(p.grid, static_cast<unsigned>((items * split + kJoinWarps - 1) / kJoinWarps)), block(kJoinWarps * 32);
   switch (cache->dtype) {
-    case ATTN_F16: ok = launch_after(attn_tree_join_kernel<__half>, grid, block, 0, stream, 1, true, a); break;
-    case ATTN_BF16: ok = launch_after(attn_tree_join_kernel<__nv_bfloat16>, grid, block, 0, stream, 1, true, a); break;
-    default: ok = launch_after(attn_tree_join_kernel<float>, grid, block, 0, stream, 1, true, a); break;
+    case ATTN_F16: ok = launch_after(attn_tree_join_kernel<__half>, grid, block, 0, stream, 1, true, a, split); break;
+    case ATTN_BF16: ok = launch_after(attn_tree_join_kernel<__nv_bfloat16>, grid, block, 0, stream, 1, true, a, split); break;
+    default: ok = launch_after(attn_tree_join_kernel<float>, grid, block, 0, stream, 1, true, a, split); break;
   }
   return ok ? ATTN_OK : ATTN_ERR_LAUNCH;
 }

@@ -51,6 +51,15 @@ int page_word_read_clear_cache(cudaStream_t stream, int* host);
 int page_word_read_clear_pages(cudaStream_t stream, int* host);
 int page_word_read_clear_tree(cudaStream_t stream, int* host);
 
+// Attention of drafted tokens on the kernel of attn_decode.cu, whose query
+// heads are then the rows (query head, token) of a kv head: whether it takes
+// the call (few rows, 16-bit types, 16-byte rows), its workspace, and the
+// launch, for a q of rows q_row elements apart and out as for launch_attn_tree.
+bool decode_rows_plan(const AttnPagedCache* c, int Hq, int S, int sms, size_t* bytes);
+bool launch_decode_rows(const AttnPagedCache* c, const PagedView& view, const void* q, long long q_b, long long q_row,
+                        void* out, int Hq, int S, float scale, const int* parents, long long parents_stride,
+                        const int* new_lens, void* workspace, cudaStream_t stream);
+
 inline bool aligned_to(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
 #ifdef __CUDACC__
