@@ -10,9 +10,9 @@
 // A free page is one whose count is 0 at the start of the call; pages are
 // given out from the lowest on, in the order of the sequences, so results do
 // not depend on timing.  Finding them is one pass over the counts by a cluster
-// of CTAs: each warp counts its stretch, the cluster's prefix sum gives each
-// stretch the rank of its first free page, and a second pass (over the L2)
-// writes the pages of the ranks that were asked for to a list.
+// of CTAs: each warp counts its stretch and keeps its bits, the cluster's prefix
+// sum gives each stretch the rank of its first free page, and the pages of the
+// ranks that were asked for are written to a list.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -28,10 +28,11 @@ namespace {
 
 __device__ int g_page_fault = 0;
 
-constexpr int kFindCluster = 8;  // CTAs that look for free pages
+constexpr int kFindMost = 8;  // CTAs that look for free pages, one cluster: the grid
 constexpr int kFindWarps = 32;
 constexpr int kFindThreads = kFindWarps * 32;
 constexpr int kStep = 256;  // pages a warp looks at in one turn
+constexpr int kTurnsKept = 8;  // turns whose bits are kept (half a million pages); others are looked at again
 constexpr int kCopyAhead = 4;  // rows a thread copies in one turn
 
 template <typename E, int kVec>
@@ -58,6 +59,7 @@ struct FindSmem {
   int warp_count[kFindWarps];
   int total;  // free pages of this CTA's stretch, read by the cluster
   long long warp_sum[kFindWarps];
+  unsigned bits[kFindWarps][kTurnsKept][kStep / 32];
 };
 
 // The stretch of pages of this warp, a multiple of kStep long but for the last.
@@ -66,7 +68,7 @@ struct Stretch {
 };
 __device__ __forceinline__ Stretch stretch(int num_pages) {
   const int w = blockIdx.x * kFindWarps + (threadIdx.x >> 5);
-  const long long warps = static_cast<long long>(kFindCluster) * kFindWarps;
+  const long long warps = static_cast<long long>(gridDim.x) * kFindWarps;
   const long long per = ((num_pages + warps - 1) / warps + kStep - 1) / kStep * kStep;
   Stretch s{w * per, (w + 1) * per};
   if (s.lo > num_pages) s.lo = num_pages;
@@ -74,20 +76,36 @@ __device__ __forceinline__ Stretch stretch(int num_pages) {
   return s;
 }
 
-// Free pages of the warp's stretch.
-__device__ __forceinline__ int count_free(const int* refs, const Stretch& s) {
+// Which of the kStep pages from p on are free: lane i gets the bits of pages p +
+// 32 i and following (lanes behind kStep / 32 nothing).
+__device__ __forceinline__ unsigned free_bits(const int* refs, long long p, long long hi) {
   const int lane = threadIdx.x & 31;
-  int n = 0;
-  for (long long p = s.lo; p < s.hi; p += kStep) {
-    int r[kStep / 32];
+  int r[kStep / 32];
 #pragma unroll
-    for (int i = 0; i < kStep / 32; ++i) {
-      const long long at = p + i * 32 + lane;
-      r[i] = at < s.hi ? *(refs + at) : 1;
-    }
-#pragma unroll
-    for (int i = 0; i < kStep / 32; ++i) n += __popc(__ballot_sync(0xffffffffu, r[i] == 0));
+  for (int i = 0; i < kStep / 32; ++i) {
+    const long long at = p + i * 32 + lane;
+    r[i] = at < hi ? *(refs + at) : 1;
   }
+  unsigned mine = 0;
+#pragma unroll
+  for (int i = 0; i < kStep / 32; ++i) {
+    const unsigned b = __ballot_sync(0xffffffffu, r[i] == 0);
+    if (lane == i) mine = b;
+  }
+  return mine;
+}
+
+// Free pages of the warp's stretch.
+__device__ __forceinline__ int count_free(FindSmem& sm, const int* refs, const Stretch& s) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int n = 0, turn = 0;
+#pragma unroll 2
+  for (long long p = s.lo; p < s.hi; p += kStep, ++turn) {
+    const unsigned b = free_bits(refs, p, s.hi);
+    if (turn < kTurnsKept && lane < kStep / 32) sm.bits[warp][turn][lane] = b;
+    n += __reduce_add_sync(0xffffffffu, __popc(b));
+  }
+  __syncwarp();
   return n;
 }
 
@@ -104,7 +122,7 @@ __device__ __forceinline__ long long first_rank(FindSmem& s, int count, long lon
   cluster_sync();
   long long rank = 0;
   *all = 0;
-  for (int c = 0; c < kFindCluster; ++c) {
+  for (int c = 0; c < static_cast<int>(gridDim.x); ++c) {
     const int x = cluster_load(&s.total, c);
     if (c < static_cast<int>(blockIdx.x)) rank += x;
     *all += x;
@@ -114,21 +132,18 @@ __device__ __forceinline__ long long first_rank(FindSmem& s, int count, long lon
 }
 
 // Writes the stretch's free pages of rank below `wanted` to their places in `order`.
-__device__ __forceinline__ void list_free(const int* refs, const Stretch& s, long long rank, long long wanted,
-                                          int* order) {
-  const int lane = threadIdx.x & 31;
-  for (long long p = s.lo; p < s.hi && rank < wanted; p += kStep) {
-    int r[kStep / 32];
-#pragma unroll
+__device__ __forceinline__ void list_free(const FindSmem& sm, const int* refs, const Stretch& s, long long rank,
+                                          long long wanted, int* order) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int turn = 0;
+  for (long long p = s.lo; p < s.hi && rank < wanted; p += kStep, ++turn) {
+    const unsigned mine = turn < kTurnsKept ? (lane < kStep / 32 ? sm.bits[warp][turn][lane] : 0u)
+                                            : free_bits(refs, p, s.hi);
+#pragma unroll 4
     for (int i = 0; i < kStep / 32; ++i) {
-      const long long at = p + i * 32 + lane;
-      r[i] = at < s.hi ? *(refs + at) : 1;
-    }
-#pragma unroll
-    for (int i = 0; i < kStep / 32; ++i) {
-      const unsigned free = __ballot_sync(0xffffffffu, r[i] == 0);
+      const unsigned free = __shfl_sync(0xffffffffu, mine, i);
       const long long at = rank + __popc(free & ((1u << lane) - 1u));
-      if (r[i] == 0 && at < wanted) order[at] = static_cast<int>(p + i * 32 + lane);
+      if ((free >> lane & 1u) && at < wanted) order[at] = static_cast<int>(p + i * 32 + lane);
       rank += __popc(free);
     }
   }
@@ -165,11 +180,36 @@ __device__ __forceinline__ int held_pages(const PagedView& c, const int* held, i
   return n < 0 ? 0 : c.table_width;
 }
 
-__device__ __forceinline__ void change_refs(const PagedView& c, int* refs, int page, int by, int* fault) {
-  if (static_cast<unsigned>(page) >= static_cast<unsigned>(c.num_pages))
-    *fault |= kFaultPage;
-  else if (atomicAdd(refs + page, by) + by < 0)
-    *fault |= kFaultPage;
+// Changes the counts of the pages that row[first], row[first + step], ... below
+// `end` name by by_of(index) (0: none): kBatch entries, then as many counts, on
+// their way at once, as each takes the better part of a microsecond.
+constexpr int kBatch = 8;
+template <typename By>
+__device__ __forceinline__ void change_refs(const PagedView& c, int* refs, const int* row, long long first,
+                                            long long end, int step, By by_of, int* fault) {
+  for (long long j = first; j < end; j += static_cast<long long>(kBatch) * step) {
+    int page[kBatch], by[kBatch], was[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const long long at = j + static_cast<long long>(k) * step;
+      by[k] = at < end ? by_of(at) : 0;
+      page[k] = by[k] != 0 ? row[at] : 0;
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      was[k] = 0;
+      if (by[k] == 0) continue;
+      if (static_cast<unsigned>(page[k]) >= static_cast<unsigned>(c.num_pages)) {
+        *fault |= kFaultPage;
+        by[k] = 0;
+      } else {
+        was[k] = atomicAdd(refs + page[k], by[k]);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k)
+      if (was[k] + by[k] < 0) *fault |= kFaultPage;
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -179,12 +219,13 @@ __device__ __forceinline__ void change_refs(const PagedView& c, int* refs, int p
 struct ResizeArgs {
   PagedView c;
   int *table, *held, *refs, *missing;
-  int *have, *start;  // [B] workspace: held pages, rank of the first page taken
+  int *have, *start;  // [B] workspace (rows from kFindThreads on): held pages, rank of the first page taken
   int* order;         // workspace: free pages by rank
 };
 
 __global__ void __launch_bounds__(kFindThreads) kv_resize_kernel(const __grid_constant__ ResizeArgs a) {
   __shared__ FindSmem s;
+  __shared__ int s_have[kFindThreads], s_start[kFindThreads];
   launch_dependents();
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -205,35 +246,42 @@ __global__ void __launch_bounds__(kFindThreads) kv_resize_kernel(const __grid_co
     }
     long long all;
     const long long at = wanted + cta_prefix(s, need, &all);
-    if (b < a.c.B && blockIdx.x == 0) {
+    const int start = static_cast<int>(at < INT_MAX ? at : INT_MAX);
+    if (b0 == 0) {
+      s_have[threadIdx.x] = have;
+      s_start[threadIdx.x] = start;
+    } else if (b < a.c.B && blockIdx.x == 0) {
       a.have[b] = have;
-      a.start[b] = static_cast<int>(at < INT_MAX ? at : INT_MAX);
+      a.start[b] = start;
     }
     wanted += all;
   }
   long long free = 0;
   if (wanted > 0) {
     const Stretch mine = stretch(a.c.num_pages);
-    const long long rank = first_rank(s, count_free(a.refs, mine), &free);
-    list_free(a.refs, mine, rank, wanted, a.order);
+    const long long rank = first_rank(s, count_free(s, a.refs, mine), &free);
+    list_free(s, a.refs, mine, rank, wanted, a.order);
   }
   cluster_sync();
   // Several warps to a sequence where there are few.
-  constexpr int kWarpsAll = kFindCluster * kFindWarps;
-  const int split = a.c.B < kWarpsAll ? kWarpsAll / a.c.B : 1;
+  const int all_warps = gridDim.x * kFindWarps, split = a.c.B < all_warps ? all_warps / a.c.B : 1;
   const long long w = static_cast<long long>(blockIdx.x) * kFindWarps + warp;
-  for (long long u = w; u < static_cast<long long>(a.c.B) * split; u += kWarpsAll) {
+  for (long long u = w; u < static_cast<long long>(a.c.B) * split; u += all_warps) {
     const int b = static_cast<int>(u / split), part = static_cast<int>(u % split);
-    const int have = a.have[b], want = want_of(b), start = a.start[b];
+    const int have = b < kFindThreads ? s_have[b] : a.have[b], start = b < kFindThreads ? s_start[b] : a.start[b];
+    const int want = want_of(b);
     int* row = a.table + b * a.c.table_stride;
     const bool granted = want <= have || static_cast<long long>(start) + (want - have) <= free;
-    for (long long j = static_cast<long long>(have) + part * 32 + lane; granted && j < want; j += split * 32) {
-      const int page = a.order[start + (j - have)];
-      row[j] = page;
-      a.refs[page] = 1;
+    if (granted) {
+#pragma unroll 8
+      for (long long j = static_cast<long long>(have) + part * 32 + lane; j < want; j += split * 32) {
+        const int page = *(a.order + start + (j - have));
+        row[j] = page;
+        a.refs[page] = 1;
+      }
     }
-    for (long long j = static_cast<long long>(want) + part * 32 + lane; j < have; j += split * 32)
-      change_refs(a.c, a.refs, row[j], -1, &fault);
+    change_refs(a.c, a.refs, row, static_cast<long long>(want) + part * 32 + lane, have, split * 32,
+                [](long long) { return -1; }, &fault);
     if (part == 0 && lane == 0) {
       a.held[b] = granted ? want : have;
       a.missing[b] = granted ? 0 : want - have;
@@ -253,7 +301,9 @@ struct ForkArgs {
   int n;
   int *new_table, *new_held, *new_lens, *missing;
   int *first, *kids;  // [B] workspace: the first sequence that continues this one, and how many do
-  int* copy;          // [n] workspace: which free page a new sequence's last page is copied to, or -1
+  int4* copy;         // [n] workspace, of the new sequence: parent, tokens, page to copy (or none), rank of the free page
+  int2* list;         // [n] workspace, by rank of the free page: page to copy and its rows
+  int* copies;        // workspace: how many
   int* order;         // workspace: free pages by rank
   int cols;           // 16-byte (or element) columns of a row
   int chunks;         // CTAs per head's K (or V) rows of a copied page
@@ -288,12 +338,28 @@ __global__ void __launch_bounds__(kFindThreads) kv_fork_plan_kernel(const __grid
   grid_dependency_wait();
   int fault = 0;
   const long long id = static_cast<long long>(blockIdx.x) * kFindThreads + threadIdx.x;
-  for (long long b = id; b < a.c.B; b += kFindCluster * kFindThreads) {
+  for (long long b = id; b < a.c.B; b += gridDim.x * kFindThreads) {
     a.first[b] = INT_MAX;
     a.kids[b] = 0;
   }
+  // A new sequence, its partly filled page (-1: none) and whether others hold that too.
+  struct Want {
+    Branch br;
+    int page;
+    bool shared;
+  };
+  auto look = [&](long long i) {
+    Want w{{-1, 0, 0, 0}, -1, false};
+    if (i < a.n) {
+      w.br = branch_of(a, static_cast<int>(i), &fault);
+      if (w.br.rest > 0) w.page = paged_page(a.c, w.br.parent, w.br.full, &fault);
+      if (w.page >= 0) w.shared = *(a.refs + w.page) != 1;
+    }
+    return w;
+  };
+  Want want = look(threadIdx.x);  // ahead of the barriers: four loads that wait for one another
   cluster_sync();
-  for (long long i = id; i < a.n; i += kFindCluster * kFindThreads) {
+  for (long long i = id; i < a.n; i += gridDim.x * kFindThreads) {
     const int parent = *(a.parents + i);
     if (parent >= 0 && parent < a.c.B) {
       atomicMin(a.first + parent, static_cast<int>(i));
@@ -302,74 +368,77 @@ __global__ void __launch_bounds__(kFindThreads) kv_fork_plan_kernel(const __grid
   }
   const Stretch mine = stretch(a.c.num_pages);
   long long free;
-  const long long rank = first_rank(s, count_free(a.refs, mine), &free);  // a cluster barrier: first is complete
+  const long long rank = first_rank(s, count_free(s, a.refs, mine), &free);  // a cluster barrier: first is complete
   long long wanted = 0;
   for (long long i0 = 0; i0 < a.n; i0 += kFindThreads) {
     const long long i = i0 + threadIdx.x;
-    bool copies = false;
-    if (i < a.n) {
-      const Branch br = branch_of(a, static_cast<int>(i), &fault);
-      if (br.rest > 0) {
-        const int page = paged_page(a.c, br.parent, br.full, &fault);
-        copies = page >= 0 && (a.first[br.parent] != i || *(a.refs + page) != 1);
-      }
-    }
+    if (i0 > 0) want = look(i);
+    const bool copies = want.page >= 0 && (want.shared || a.first[want.br.parent] != i);
     long long all;
     const long long at = wanted + cta_prefix(s, copies ? 1 : 0, &all);
-    if (i < a.n && blockIdx.x == 0) a.copy[i] = copies ? static_cast<int>(at) : -1;
+    if (i < a.n && blockIdx.x == 0) {
+      a.copy[i] = make_int4(want.br.parent, want.br.len, copies ? want.page : -1, static_cast<int>(at));
+      if (copies) a.list[at] = make_int2(want.page, want.br.rest);
+    }
     wanted += all;
   }
-  if (wanted <= free) list_free(a.refs, mine, rank, wanted, a.order);
-  if (id == 0) *a.missing = static_cast<int>(wanted > free ? wanted - free : 0);
+  if (wanted <= free) list_free(s, a.refs, mine, rank, wanted, a.order);
+  if (id == 0) {
+    *a.missing = static_cast<int>(wanted > free ? wanted - free : 0);
+    *a.copies = wanted > free ? 0 : static_cast<int>(wanted);
+  }
   if (fault) atomicOr(&g_page_fault, fault);
   cluster_sync();  // no CTA leaves while its count may be read
 }
 
-// The tables and counts, and the copies: the CTAs (i, 0) do row i of the
-// tables, CTA (i, y) its share of new sequence i's copy, K or V rows of one head.
+// The tables and counts, and the copies, dealt out to a grid that fills the GPU
+// once: first row i of the tables, then the K or V rows of one head of a page.
 template <typename E, int kVec>
 __global__ void __launch_bounds__(256) kv_fork_copy_kernel(const __grid_constant__ ForkArgs a) {
   using V = Vec<E, kVec>;
   launch_dependents();
   grid_dependency_wait();
   int fault = 0;
-  const int i = blockIdx.x;
   const bool fits = *a.missing == 0;
-  if (blockIdx.y == 0) {
-    if (i < a.n) {
-      const Branch br = branch_of(a, i, &fault);
-      const int count = fits ? br.full + (br.rest > 0) : 0, copy = a.copy[i];
-      int* row = a.new_table + static_cast<long long>(i) * a.c.table_width;
-      for (int j = threadIdx.x; j < a.c.table_width; j += 256) {
-        int page = -1;
-        if (j < count) {
-          const bool copied = copy >= 0 && j == br.full;
-          page = copied ? a.order[copy] : *(a.c.table + static_cast<long long>(br.parent) * a.c.table_stride + j);
-          if (copied) a.refs[page] = 1;
+  const int copies = *a.copies;
+  const int rows = max(a.n, a.c.B), each = 2 * a.c.heads * a.chunks;
+  for (long long item = blockIdx.x; item < rows + static_cast<long long>(copies) * each; item += gridDim.x) {
+    if (item < rows) {
+      const int i = static_cast<int>(item);
+      if (i < a.n) {
+        const int4 plan = a.copy[i];
+        const int full = plan.y / a.c.page_size, rest = plan.y - full * a.c.page_size;
+        const int count = fits ? full + (rest > 0) : 0;
+        int* row = a.new_table + static_cast<long long>(i) * a.c.table_width;
+        for (int j = threadIdx.x; j < a.c.table_width; j += 256) {
+          int page = -1;
+          if (j < count) {
+            const bool copied = plan.z >= 0 && j == full;
+            page = copied ? a.order[plan.w] : *(a.c.table + static_cast<long long>(plan.x) * a.c.table_stride + j);
+            if (copied) a.refs[page] = 1;
+          }
+          row[j] = page;
         }
-        row[j] = page;
+        if (threadIdx.x == 0) {
+          a.new_held[i] = count;
+          a.new_lens[i] = fits ? plan.y : 0;
+        }
       }
-      if (threadIdx.x == 0) {
-        a.new_held[i] = count;
-        a.new_lens[i] = fits ? br.len : 0;
+      if (fits && i < a.c.B) {
+        // One holder less, and as many more as continue it.
+        const Branch br = branch_of_parent(a, i, &fault);
+        const int have = held_pages(a.c, a.held, i, &fault), kids = a.kids[i];
+        const bool keeps = kids > 0 && br.rest > 0 && a.copy[a.first[i]].z < 0;
+        change_refs(a.c, a.refs, a.c.table + i * a.c.table_stride, threadIdx.x, have, 256,
+                    [&](long long j) { return (j < br.full ? kids : j == br.full && keeps ? 1 : 0) - 1; }, &fault);
       }
+      continue;
     }
-    if (fits && i < a.c.B) {
-      // One holder less, and as many more as continue it.
-      const Branch br = branch_of_parent(a, i, &fault);
-      const int have = held_pages(a.c, a.held, i, &fault), kids = a.kids[i];
-      const bool keeps = kids > 0 && br.rest > 0 && a.copy[a.first[i]] < 0;
-      for (int j = threadIdx.x; j < have; j += 256) {
-        const int by = (j < br.full ? kids : j == br.full && keeps ? 1 : 0) - 1;
-        if (by != 0) change_refs(a.c, a.refs, *(a.c.table + i * a.c.table_stride + j), by, &fault);
-      }
-    }
-  }
-  if (fits && i < a.n && a.copy[i] >= 0) {
-    const Branch br = branch_of(a, i, &fault);
-    const long long from = *(a.c.table + static_cast<long long>(br.parent) * a.c.table_stride + br.full);
-    const long long to = a.order[a.copy[i]];
-    const int hv = blockIdx.y / a.chunks, chunk = blockIdx.y - hv * a.chunks;
+    const long long at = item - rows;
+    const int k = static_cast<int>(at / each), hc = static_cast<int>(at - static_cast<long long>(k) * each);
+    const int2 what = a.list[k];
+    const long long from = what.x, to = a.order[k];
+    const int hv = hc / a.chunks, chunk = hc - hv * a.chunks;
     const bool is_v = hv >= a.c.heads;
     const int h = is_v ? hv - a.c.heads : hv;
     const long long* st = is_v ? a.c.vs : a.c.ks;
@@ -377,15 +446,15 @@ __global__ void __launch_bounds__(256) kv_fork_copy_kernel(const __grid_constant
     E* x = static_cast<E*>(is_v ? a.c.v : a.c.k) + h * st[1] + static_cast<long long>(threadIdx.x - in * a.cols) * kVec;
     if (in < at_once) {
       const long long step = static_cast<long long>(a.chunks) * at_once;
-      for (long long r0 = chunk * at_once + in; r0 < br.rest; r0 += kCopyAhead * step) {
+      for (long long r0 = chunk * at_once + in; r0 < what.y; r0 += kCopyAhead * step) {
         V row[kCopyAhead];
 #pragma unroll
         for (int p = 0; p < kCopyAhead; ++p)
-          if (r0 + p * step < br.rest)
+          if (r0 + p * step < what.y)
             row[p] = *reinterpret_cast<const V*>(x + from * st[0] + (r0 + p * step) * st[2]);
 #pragma unroll
         for (int p = 0; p < kCopyAhead; ++p)
-          if (r0 + p * step < br.rest) *reinterpret_cast<V*>(x + to * st[0] + (r0 + p * step) * st[2]) = row[p];
+          if (r0 + p * step < what.y) *reinterpret_cast<V*>(x + to * st[0] + (r0 + p * step) * st[2]) = row[p];
       }
     }
   }
@@ -489,7 +558,16 @@ __global__ void __launch_bounds__(kMoveWarps * 32) kv_compact_kernel(const __gri
 
 size_t round_up(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 
-// Places of a call's arrays of ints in its workspace.
+// CTAs that look for free pages: as many as take one turn each, since a barrier
+// of several costs about what a turn does (384 sequences forked in a pool of
+// 5000 pages: 16.6 us with one CTA, 17.7 with eight).
+int find_ctas(int num_pages) {
+  int n = 1;
+  while (n < kFindMost && static_cast<long long>(n) * kFindWarps * kStep < num_pages) n *= 2;
+  return n;
+}
+
+// Places of a call's arrays in its workspace.
 struct ResizePlan {
   size_t have_at, start_at, order_at, bytes;
 };
@@ -500,12 +578,13 @@ ResizePlan resize_plan(const AttnPagedCache* c) {
   return ResizePlan{0, rows, 2 * rows, 2 * rows + round_up(sizeof(int) * listed)};
 }
 struct ForkPlan {
-  size_t first_at, kids_at, copy_at, order_at, bytes;
+  size_t first_at, kids_at, copy_at, list_at, copies_at, order_at, bytes;
 };
 ForkPlan fork_plan(const AttnPagedCache* c, int n) {
   const size_t old = round_up(sizeof(int) * static_cast<size_t>(c->B)), now = round_up(sizeof(int) * static_cast<size_t>(n));
   const size_t listed = static_cast<size_t>(n < c->num_pages ? n : c->num_pages);
-  return ForkPlan{0, old, 2 * old, 2 * old + now, 2 * old + now + round_up(sizeof(int) * listed)};
+  const size_t copy = 2 * old, list = copy + 4 * now, copies = list + 2 * now, order = copies + 256;
+  return ForkPlan{0, old, copy, list, copies, order, order + round_up(sizeof(int) * listed)};
 }
 
 // Elements per access: 16 bytes where rows, strides and addresses of K and V
@@ -591,7 +670,8 @@ extern "C" int launch_kv_resize(const AttnPagedCache* cache, int* table, int* he
   a.have = reinterpret_cast<int*>(ws + p.have_at);
   a.start = reinterpret_cast<int*>(ws + p.start_at);
   a.order = reinterpret_cast<int*>(ws + p.order_at);
-  return launch_after(kv_resize_kernel, dim3(kFindCluster), dim3(kFindThreads), 0, stream, kFindCluster, true, a)
+  const int ctas = find_ctas(cache->num_pages);
+  return launch_after(kv_resize_kernel, dim3(ctas), dim3(kFindThreads), 0, stream, ctas, true, a)
              ? ATTN_OK
              : ATTN_ERR_LAUNCH;
 }
@@ -625,11 +705,10 @@ extern "C" int launch_kv_fork(const AttnPagedCache* cache, const int* held, int*
   const ForkPlan p = fork_plan(cache, n);
   const int vec = access_width(cache);
   a.cols = cache->D / vec;
-  // Rows per thread: up to two turns of kCopyAhead.
-  const long long per = 2LL * kCopyAhead * (256 / a.cols);
-  a.chunks = static_cast<int>((cache->page_size + per - 1) / per);
-  while (a.chunks > 1 && 2LL * cache->heads * a.chunks > 65535) a.chunks = (a.chunks + 1) / 2;
-  if (workspace_bytes < p.bytes || 2LL * cache->heads > 65535) return ATTN_ERR_INVALID_ARGUMENT;
+  // Rows per thread: up to two turns of kCopyAhead, in large pages more.
+  const long long per = 2LL * kCopyAhead * (256 / a.cols), chunks = (cache->page_size + per - 1) / per;
+  a.chunks = static_cast<int>(chunks < 64 ? chunks : 64);
+  if (workspace_bytes < p.bytes || 2LL * cache->heads * a.chunks > 0x7fffffffLL) return ATTN_ERR_INVALID_ARGUMENT;
   st = check_device();
   if (st != ATTN_OK) return st;
   char* ws = static_cast<char*>(workspace);
@@ -643,13 +722,17 @@ extern "C" int launch_kv_fork(const AttnPagedCache* cache, const int* held, int*
   a.missing = missing;
   a.first = reinterpret_cast<int*>(ws + p.first_at);
   a.kids = reinterpret_cast<int*>(ws + p.kids_at);
-  a.copy = reinterpret_cast<int*>(ws + p.copy_at);
+  a.copy = reinterpret_cast<int4*>(ws + p.copy_at);
+  a.list = reinterpret_cast<int2*>(ws + p.list_at);
+  a.copies = reinterpret_cast<int*>(ws + p.copies_at);
   a.order = reinterpret_cast<int*>(ws + p.order_at);
-  if (!launch_after(kv_fork_plan_kernel, dim3(kFindCluster), dim3(kFindThreads), 0, stream, kFindCluster, true, a))
+  const int ctas = find_ctas(cache->num_pages);
+  if (!launch_after(kv_fork_plan_kernel, dim3(ctas), dim3(kFindThreads), 0, stream, ctas, true, a))
     return ATTN_ERR_LAUNCH;
   const int rows = n > cache->B ? n : cache->B;
   if (rows == 0) return ATTN_OK;
-  const dim3 grid(static_cast<unsigned>(rows), static_cast<unsigned>(2 * cache->heads * a.chunks)), block(256);
+  const long long items = rows + static_cast<long long>(n) * 2 * cache->heads * a.chunks, fill = 8LL * sm_count();
+  const dim3 grid(static_cast<unsigned>(items < fill ? items : fill)), block(256);
   const auto kern = cache->dtype == ATTN_F32
                         ? (vec == 4 ? kv_fork_copy_kernel<uint32_t, 4> : kv_fork_copy_kernel<uint32_t, 1>)
                         : (vec == 8 ? kv_fork_copy_kernel<uint16_t, 8> : kv_fork_copy_kernel<uint16_t, 1>);
