@@ -1613,7 +1613,7 @@ int page_word_read_clear_decode(cudaStream_t stream, int* host) {
 
 bool decode_rows_plan(const AttnPagedCache* c, int Hq, int S, int sms, size_t* bytes) {
   const long long rows = static_cast<long long>(Hq / c->heads) * S;
-  if (!mma_takes(c) || rows > 8 || static_cast<long long>(c->B) * Hq * S > 0x7fffffffLL) return false;
+  if (!mma_takes(c) || c->num_pages == 0 || rows > 8 || static_cast<long long>(c->B) * Hq * S > 0x7fffffffLL) return false;
   const Plan p = make_plan(c, true, Hq * S, 0, false, false, sms);
   if (p.tiles > 0x7fffffffLL - 65536) return false;
   *bytes = p.bytes;

@@ -1505,9 +1505,9 @@ struct Plan {
   size_t meta_at, ml_at, o_at, bytes;
 };
 
-// What the tensor-core kernel asks of the cache: 16-byte rows.
+// What the tensor-core kernel asks of the cache: 16-byte rows (and some).
 bool tc_takes(const AttnPagedCache* c) {
-  if (c->dtype == ATTN_F32 || c->D % 8 != 0) return false;
+  if (c->dtype == ATTN_F32 || c->D % 8 != 0 || c->num_pages == 0) return false;
   for (int i = 0; i < 3; ++i)
     if (c->k_strides[i] % 8 != 0 || c->v_strides[i] % 8 != 0) return false;
   return aligned_to(c->k, 16) && aligned_to(c->v, 16);

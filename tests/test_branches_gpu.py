@@ -1,14 +1,18 @@
 """The operators for drafted tokens and shared pages against their definitions
 (branches_ref.py): attention of a tree of drafted tokens, the move of accepted
 ones, sequences that continue others, and the pages that lengths need."""
+import ctypes
 import math
+import os
 import random
 
 import pytest
 import torch
 
+import rocm_attn_b200
 from branches_ref import (compact_ref, fork_ref, random_pool, random_tree, resize_ref, tree_bound, tree_ref)
 from paged_ref import make_cache
+from test_paged_cpu import LL3, PagedCache
 
 pytestmark = pytest.mark.gpu
 
@@ -331,6 +335,138 @@ def test_tree_captured_and_on_two_streams(attn, D, dtype):
         for (k, v, table, ln, q, par, new), out in zip(data, outs):
             assert torch.equal(out, attn.attn_tree(q, k, v, table, ln, par, new))
             _close(out, tree_ref(*(x.cpu() for x in (q, k, v, table, ln, par, new))), 800, dtype)
+
+
+@pytest.mark.parametrize("dtype,Hq,S", [(BF16, 4, 2), (BF16, 4, 5), (F16, 8, 30), (F32, 4, 5)])
+def test_offsets_past_32_bits(attn, dtype, Hq, S):
+    # the last pages of a cache of more than 2^32 bytes and 2^31 elements
+    ps, D = 256, 128
+    P = 2 ** 31 // (ps * D) + 64
+    cache = torch.zeros(P, 1, ps, D, dtype=dtype, device="cuda")
+    k, v, table, ln = make_cache([700], 1, D, ps, dtype, spare=0)
+    cache[P - 3:] = k.cuda()
+    far = (table + P - 3).cuda()
+    q, par = _q(1, Hq, S, D, dtype), _trees(1, S)
+    out = attn.attn_tree(q.cuda(), cache, cache, far, ln.cuda(), par.cuda())
+    _close(out, tree_ref(q, k, k, table, ln, par), 700, dtype)
+    if S != 5:
+        return
+    kept, new = ints([[1, 4]]), ints([5])
+    attn.kv_compact(cache, cache.clone(), far, ln.cuda(), kept.cuda(), new.cuda())
+    was = k.clone()
+    for i, a in enumerate((1, 4)):
+        k[int(table[0, (695 + i) // ps]), 0, (695 + i) % ps] = was[int(table[0, (695 + a) // ps]), 0, (695 + a) % ps]
+    assert torch.equal(cache[P - 3:].cpu().nan_to_num(7.0), k.nan_to_num(7.0))
+    # a fork whose source and copy lie there
+    refs = torch.ones(P, dtype=torch.int32, device="cuda")
+    refs[P - 5] = 0
+    t, h, n, m = attn.kv_fork(cache, cache.clone(), far, ints([3]).cuda(), ln.cuda(), refs, ints([0, 0]).cuda())
+    assert m.tolist() == [0] and t[1].tolist() == far[0, :2].tolist() + [P - 5] and n.tolist() == [700, 700]
+    assert torch.equal(cache[P - 5, :, :188], cache[int(far[0, 2]), :, :188]) and not cache[P - 5, :, 188:].any()
+    assert attn.check_status(0) == 0
+
+
+def test_more_sequences_than_a_grid_dimension(attn):
+    # 70000 sequences of one or two tokens
+    B, ps, D = 70000, 2, 64
+    lens = torch.tensor([1 + i % 2 for i in range(B)], dtype=torch.int32).cuda()
+    g = torch.Generator(device="cuda").manual_seed(1)
+    k, v = (torch.randn(B + 50000, 1, ps, D, generator=g, device="cuda", dtype=F16) for _ in range(2))
+    table, held = torch.full((B, 1), -1, dtype=torch.int32, device="cuda"), torch.zeros(B, dtype=torch.int32, device="cuda")
+    refs = torch.zeros(B + 50000, dtype=torch.int32, device="cuda")
+    refs[5] = 3
+    assert not attn.kv_resize(table, held, lens, refs, ps).any()
+    assert torch.equal(table[:, 0], torch.tensor([i for i in range(B + 1) if i != 5], dtype=torch.int32).cuda())
+    for S in (1, 9):
+        q = torch.randn(B, 1, S, D, generator=g, device="cuda", dtype=F16)
+        one = torch.ones(B, dtype=torch.int32, device="cuda")
+        out = attn.attn_tree(q, k, v, table, lens, new_lens=one).double()
+        kk, vv = k[table[:, 0].long(), 0].double(), v[table[:, 0].long(), 0].double()
+        x = (q[:, 0, 0].double()[:, None] * kk).sum(2) / 8
+        x[lens == 1, 1] = -math.inf
+        want = (torch.softmax(x, 1)[..., None] * vv).sum(1)
+        assert ((out[:, 0, 0] - want).abs() <= 2.0 ** -9 * (1 + want.abs())).all() and not out[:, :, 1:].any()
+    moved = attn.kv_compact(k, v, table, lens, torch.zeros(B, 1, dtype=torch.int32, device="cuda"), one)
+    assert torch.equal(moved, lens)
+    parents = torch.arange(B, dtype=torch.int32, device="cuda") // 2 * 2
+    t, h, n, m = attn.kv_fork(k, v, table, held, lens, refs, parents)
+    assert m.tolist() == [0] and torch.equal(n, lens[parents.long()])
+    assert torch.equal(t[::2], table[::2]) and int(refs.clamp(0, 1).sum()) == B + 1 and t.unique().numel() == B
+    assert torch.equal(k[t[1::2, 0].long(), :, 0], k[t[::2, 0].long(), :, 0])
+    assert attn.check_status(0) == 0
+
+
+@pytest.mark.parametrize("dtype,S", [(BF16, 1), (BF16, 40), (F16, 9), (F32, 3)])
+def test_cache_without_pages(attn, dtype, S):
+    k = torch.empty(0, 2, 16, 64, dtype=dtype, device="cuda")
+    q = torch.randn(2, 4, S, 64, device="cuda").to(dtype)
+    table, ln = ints([[0], [0]]).cuda(), ints([0, 0]).cuda()
+    assert not attn.attn_tree(q, k, k, table, ln).any() and attn.check_status(0) == 0
+    attn.attn_tree(q, k, k, table, ints([3, 0]).cuda())
+    assert attn.check_status(0) == 8 and attn.check_status(0) == 0
+    refs = torch.zeros(0, dtype=torch.int32, device="cuda")
+    held = ints([0, 0]).cuda()
+    assert attn.kv_resize(table, held, ints([5, 0]).cuda(), refs, 16).tolist() == [1, 0]
+    t, h, n, m = attn.kv_fork(k, k, table, held, ln, refs, ints([1, 0, -1]).cuda())
+    assert n.tolist() == [0, 0, 0] and m.tolist() == [0] and attn.check_status(0) == 0
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_rows_that_are_not_there_may_hold_anything(attn, D):
+    # queries behind the drafted tokens, in rows that share a warp with others
+    k, v, table, ln = make_cache([90, 200], 2, D, 16, BF16)
+    for S, Hq in ((2, 4), (7, 8), (40, 16)):
+        q, new = _q(2, Hq, S, D, BF16), ints([S - 1, 1])
+        q[0, :, S - 1:] = math.nan
+        q[1, :, 1:] = math.inf
+        out = attn.attn_tree(q.cuda(), k.cuda(), v.cuda(), table.cuda(), ln.cuda(), new_lens=new.cuda())
+        _close(out, tree_ref(q, k, v, table, ln, new_lens=new), 200, BF16)
+        assert not out[0, :, S - 1:].any() and not out[1, :, 1:].any()
+
+
+# ---------------------------------------------------------------------------
+# the watchdog (tests/test_watchdog_gpu.py says how the test build works)
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("lens,D,Hq,S,ps", [([300, 40], 128, 8, 9, 16), ([2000, 700], 64, 4, 30, 24), ([900], 256, 4, 12, 64),
+                                            ([3000, 50], 128, 8, 50, 32), ([700], 64, 16, 40, 16), ([300, 90], 128, 4, 3, 16)])
+def test_watchdog_fires_and_recovers(lens, D, Hq, S, ps):
+    # CTA 0's first wait is for 16 bytes more than come: it ends by the limit, the kernel reports it and
+    # returns, and the next launch is clean
+    lib = ctypes.CDLL(os.path.join(os.path.dirname(rocm_attn_b200.KERNEL_LIB_PATH), "librocm_attn_wdtest.so"))
+    p, i = ctypes.c_void_p, ctypes.c_int
+    lib.attn_set_wait_limit_ns.argtypes = [ctypes.c_ulonglong]
+    lib.launch_attn_tree.argtypes = [p, p, p, p, i, i, ctypes.c_float, p, ctypes.c_longlong, p, p, ctypes.c_size_t, p]
+    k, v, table, ln = make_cache(lens, 2, D, ps, BF16)
+    q, par = _q(len(lens), Hq, S, D, BF16), _trees(len(lens), S)
+    dk, dv, dt, dl, dq, dp = (t.cuda() for t in (k, v, table, ln, q, par))
+    out = torch.zeros_like(dq)
+    st = LL3(*dk.stride()[:3])
+    c = PagedCache(dk.data_ptr(), dv.data_ptr(), k.shape[0], 2, ps, D, 1, st, st, dt.data_ptr(), dt.shape[1], dt.shape[1],
+                   dl.data_ptr(), len(lens))
+    size = ctypes.c_size_t()
+    assert lib.attn_tree_workspace_bytes(ctypes.byref(c), Hq, S, ctypes.byref(size)) == 0
+    space = torch.empty(max(16, size.value), dtype=torch.uint8, device="cuda")
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+    def run():
+        assert lib.launch_attn_tree(ctypes.byref(c), dq.data_ptr(), None, out.data_ptr(), Hq, S, -1.0, dp.data_ptr(), S,
+                                    None, space.data_ptr(), size.value, stream) == 0
+        status = ctypes.c_int(-1)
+        assert lib.attn_get_status(stream, ctypes.byref(status)) == 0
+        return status.value
+
+    assert run() == 0
+    lib.attn_set_wait_limit_ns(1_000_000)
+    lib.attn_test_drop_arrival(1)
+    try:
+        assert run() == 7
+    finally:
+        lib.attn_test_drop_arrival(0)
+        lib.attn_set_wait_limit_ns(0)
+    assert run() == 0
+    _close(out, tree_ref(q, k, v, table, ln, par), max(lens), BF16)
 
 
 # ---------------------------------------------------------------------------
