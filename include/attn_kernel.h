@@ -320,7 +320,9 @@ ATTN_API int launch_kv_evict(const AttnPagedCache* cache, const float* weights, 
  * An entry of parents[b, 0..n) that is no earlier token counts as -1 and is
  * reported as ATTN_ERR_BAD_PAGE.  Rows s >= n, and those of sequences without
  * tokens, are zeros; a row that has tokens and only scores of -inf is NaN, as
- * the formula.  Precision as for launch_attn_decode.
+ * the formula.  Precision as for launch_attn_decode, but that fp16 weights are
+ * off by half a step only down to 2^-21 of the largest, and below by at most
+ * 2^-32 of that, where a kv head has more than eight rows (Hq / Hkv * S).
  */
 ATTN_API int attn_tree_workspace_bytes(const AttnPagedCache* cache, int Hq, int S, size_t* bytes);
 ATTN_API int launch_attn_tree(const AttnPagedCache* cache, const void* q, const long long* q_strides, void* out, int Hq,

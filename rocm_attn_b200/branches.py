@@ -59,7 +59,8 @@ def attn_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, blo
     ``scale`` is positive and finite, 1/sqrt(D) if not given.  Returns O ``[B,
     Hq, S, D]``: zeros for tokens behind the n and for empty sequences; NaN, as
     the formula gives, for a token that has only scores of -inf.  Precision is
-    that of ``attn_decode``.
+    that of ``attn_decode``; fp16 weights below 2^-21 of the largest may be off by
+    2^-32 of that where ``Hq / Hkv * S`` is above eight.
     """
     if scale is None:
         scale = -1.0  # the binding's default

@@ -16,6 +16,17 @@
 // so the host needs no lengths and a ragged batch loads every SM alike.  A
 // unit cut by the ends of runs leaves its parts (M, L and the unscaled O, fp32)
 // in the workspace and a second kernel joins them in the order of the tokens.
+//
+// What carries the products depends on the rows:
+//   up to 8, 16-bit   attn_decode's kernel, the rows as columns of mma.sync: 17
+//                     sequences of up to 2047 tokens, 16 kv heads of 64, five
+//                     rows 32.4 us, 35.5 here
+//   up to 128         tcgen05, tiles of 64 tokens, two CTAs per SM whose chains
+//                     of product, softmax and product fill each other's waits:
+//                     273 MB in 62 us, of which the join takes 3
+//   above             tcgen05, 256 rows in two streams over the same tiles of
+//                     128 tokens: K and V cross the copy engine once for both
+//   fp32, odd strides dot products on the plain cores
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -331,33 +342,55 @@ __device__ __forceinline__ Place place_of(const TreeArgs& a, const Cursor& c, bo
   return p;
 }
 
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
 // ---------------------------------------------------------------------------
 // SIMT kernel: fp32, any head dim, any strides
 // ---------------------------------------------------------------------------
 
 // 32 rows by 64 tokens per tile.  Thread (ty, tx) of 8 x 16 has rows 4 ty + {0
 // .. 3}: scores of tokens tx + 16 {0 .. 3}, and of O the columns 4 tx + {0 .. 3}
-// + 64 j.  K and then V lie in one buffer, in 32 bits.
+// + 64 j.  K and V lie in 32 bits, in a buffer each where copies of 16 bytes can
+// fill them (kWide: fp32, 16-byte rows), so that the next tile's come while this
+// one is worked on; else one after the other in one buffer.  fp32, us (in brackets
+// one buffer and an element per load): 3 sequences of 1500 tokens, 16/4 heads of
+// 64, 7 drafted 16.0 (30.5); 16 of up to 8192 96.9 (446); 16 of up to 4096, 32/8
+// heads of 128, 8 drafted 227 (808); 8 of up to 4096, 16/4 of 256 152 (596).  It
+// costs CTAs per SM (4, 2 and 1 at D = 64, 128 and 256 instead of 5, 3 and 2).
 constexpr int kSimtThreads = 128, kSimtRows = 32, kSimtTile = 64;
 
-template <int kDP>
+template <int kDP, bool kWide>
 struct SimtCfg {
   static constexpr int kPitch = kDP + 4;  // floats; rows 4 banks apart
   static constexpr int kPPitch = kSimtTile + 4;
-  static constexpr size_t kBytes = sizeof(float) * ((kSimtRows + kSimtTile) * kPitch + kSimtRows * kPPitch) +
-                                   sizeof(long long) * 2 * kSimtTile + sizeof(int) * kParShared;
+  static constexpr size_t kBytes = sizeof(float) * ((kSimtRows + (kWide ? 2 : 1) * kSimtTile) * kPitch + kSimtRows * kPPitch) +
+                                   sizeof(long long) * 4 * kSimtTile + sizeof(int) * kParShared;
 };
 
-template <typename T, int kDP>
+template <typename T, int kDP, bool kWide>
 __global__ void __launch_bounds__(kSimtThreads) attn_tree_simt_kernel(const __grid_constant__ TreeArgs a) {
-  using C = SimtCfg<kDP>;
+  using C = SimtCfg<kDP, kWide>;
   constexpr int kCols = kDP / 16;
   extern __shared__ __align__(16) float sm[];
   float* s_q = sm;
-  float* s_kv = s_q + kSimtRows * C::kPitch;
-  float* s_p = s_kv + kSimtTile * C::kPitch;
+  float* s_k = s_q + kSimtRows * C::kPitch;
+  float* s_v = kWide ? s_k + kSimtTile * C::kPitch : s_k;
+  float* s_p = s_v + kSimtTile * C::kPitch;
   long long* s_at = reinterpret_cast<long long*>(s_p + kSimtRows * C::kPPitch);  // K, then V offsets; -1: no token
-  int* s_par = reinterpret_cast<int*>(s_at + 2 * kSimtTile);
+  long long* s_next = s_at + 2 * kSimtTile;                                      // those of the next tile (kWide)
+  int* s_par = reinterpret_cast<int*>(s_next + 2 * kSimtTile);
   Tree tree{s_par, nullptr};
   __shared__ ScheduleSmem<kSimtThreads> s_sched;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, D = a.c.D;
@@ -374,20 +407,57 @@ __global__ void __launch_bounds__(kSimtThreads) attn_tree_simt_kernel(const __gr
   const T* kbase = static_cast<const T*>(a.c.k);
   const T* vbase = static_cast<const T*>(a.c.v);
 
-  // Rows of the cache at s_at to s_kv, zeros behind D and where there is no token.
-  auto load = [&](const T* base, const long long* at) {
-    for (int e = tid; e < kSimtTile * kDP; e += kSimtThreads) {
-      const int r = e / kDP, d = e % kDP;
-      s_kv[r * C::kPitch + d] = at[r] >= 0 && d < D ? to_f32(base[at[r] + d]) : 0.f;
+  // Rows of the cache to `to`, zeros behind D and where there is no token.
+  auto load = [&](float* to, const T* base, const long long* at) {
+    if constexpr (kWide) {
+#pragma unroll
+      for (int e = tid; e < kSimtTile * kDP / 4; e += kSimtThreads) {
+        const int r = e / (kDP / 4), d = e % (kDP / 4) * 4;
+        const bool is = at[r] >= 0 && d < D;
+        cp_async16(smem_addr(to + r * C::kPitch + d), base + (is ? at[r] + d : 0), is);
+      }
+      cp_async_commit();
+    } else {
+#pragma unroll 1
+      for (int e0 = tid; e0 < kSimtTile * kDP; e0 += 8 * kSimtThreads) {
+        float x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int e = e0 + k * kSimtThreads, r = e / kDP, d = e % kDP;
+          x[k] = at[r] >= 0 && d < D ? to_f32(base[at[r] + d]) : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int e = e0 + k * kSimtThreads;
+          to[e / kDP * C::kPitch + e % kDP] = x[k];
+        }
+      }
     }
+  };
+  // Token `pos`, this thread's of a tile, to its place in `at`.
+  auto locate = [&](int page, int row, long long* at) {
+    at[tid] = page < 0 ? -1 : page * a.c.ks[0] + cur.h * a.c.ks[1] + row * a.c.ks[2];
+    at[kSimtTile + tid] = page < 0 ? -1 : page * a.c.vs[0] + cur.h * a.c.vs[1] + row * a.c.vs[2];
   };
 
   for (int i = 0; i < run.n; ++i) {
+    const int pos0 = cur.t * kSimtTile;
+    int page = -1, row = 0;
+    if (fresh || !kWide) {
+      if (tid < kSimtTile) {
+        page = page_of(a, cur, pos0 + tid, &row, &fault);
+        locate(page, row, s_at);
+      }
+      __syncthreads();
+      load(s_k, kbase, s_at);
+      if constexpr (kWide) load(s_v, vbase, s_at + kSimtTile);
+    }
     if (fresh) {
       const T* q = static_cast<const T*>(a.q) + cur.b * a.q_b + static_cast<long long>(cur.h) * a.group * a.q_h;
+#pragma unroll 16
       for (int e = tid; e < kSimtRows * kDP; e += kSimtThreads) {
         const int r = e / kDP, d = e % kDP, gr = cur.rt * kSimtRows + r;
-        const int head = gr / a.S, s = gr - head * a.S;
+        const int head = a.head_at(gr), s = gr - head * a.S;
         s_q[r * C::kPitch + d] = gr < a.rows && d < D ? to_f32(q[head * a.q_h + s * a.q_s + d]) : 0.f;
       }
       tree.global = tree_of(a, cur.b);
@@ -401,15 +471,9 @@ __global__ void __launch_bounds__(kSimtThreads) attn_tree_simt_kernel(const __gr
       }
       fresh = false;
     }
-    const int pos0 = cur.t * kSimtTile;
-    if (tid < kSimtTile) {
-      int row = 0;
-      const int page = page_of(a, cur, pos0 + tid, &row, &fault);
-      s_at[tid] = page < 0 ? -1 : page * a.c.ks[0] + cur.h * a.c.ks[1] + row * a.c.ks[2];
-      s_at[kSimtTile + tid] = page < 0 ? -1 : page * a.c.vs[0] + cur.h * a.c.vs[1] + row * a.c.vs[2];
-    }
-    __syncthreads();
-    load(kbase, s_at);
+    const bool more = kWide && cur.t + 1 < cur.T && i + 1 < run.n;  // another tile of this unit
+    if (more && tid < kSimtTile) page = page_of(a, cur, pos0 + kSimtTile + tid, &row, &fault);
+    if constexpr (kWide) cp_async_wait<1>();  // V may be on its way
     __syncthreads();
     float x[4][4] = {};
 #pragma unroll 4
@@ -418,7 +482,7 @@ __global__ void __launch_bounds__(kSimtThreads) attn_tree_simt_kernel(const __gr
 #pragma unroll
       for (int r = 0; r < 4; ++r) q[r] = *reinterpret_cast<const float4*>(s_q + (ty * 4 + r) * C::kPitch + d);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) k[c] = *reinterpret_cast<const float4*>(s_kv + (tx + 16 * c) * C::kPitch + d);
+      for (int c = 0; c < 4; ++c) k[c] = *reinterpret_cast<const float4*>(s_k + (tx + 16 * c) * C::kPitch + d);
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -465,8 +529,15 @@ __global__ void __launch_bounds__(kSimtThreads) attn_tree_simt_kernel(const __gr
 #pragma unroll
       for (int c = 0; c < kCols; ++c) o[r][c] *= f;
     }
+    if (more && tid < kSimtTile) locate(page, row, s_next);
     __syncthreads();  // K is used up
-    load(vbase, s_at + kSimtTile);
+    if constexpr (kWide) {
+      if (more) load(s_k, kbase, s_next);
+      else cp_async_commit();  // a group either way
+      cp_async_wait<1>();
+    } else {
+      load(s_v, vbase, s_at + kSimtTile);
+    }
     __syncthreads();
     const bool drafts = pos0 + kSimtTile > cur.s.base;
     for (int t = 0; t < kSimtTile; t += 4) {
@@ -477,7 +548,7 @@ __global__ void __launch_bounds__(kSimtThreads) attn_tree_simt_kernel(const __gr
       for (int j = 0; j < kDP / 64; ++j)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const float4 v = *reinterpret_cast<const float4*>(s_kv + (t + k) * C::kPitch + j * 64 + tx * 4);
+          const float4 v = *reinterpret_cast<const float4*>(s_v + (t + k) * C::kPitch + j * 64 + tx * 4);
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const float w = k == 0 ? p[r].x : k == 1 ? p[r].y : k == 2 ? p[r].z : p[r].w;
@@ -518,8 +589,15 @@ __global__ void __launch_bounds__(kSimtThreads) attn_tree_simt_kernel(const __gr
       fresh = true;
     }
     __syncthreads();  // the tile's buffers are free
+    if (more) {
+      load(s_v, vbase, s_next + kSimtTile);
+      long long* at = s_at;
+      s_at = s_next;
+      s_next = at;
+    }
     if (++cur.t == cur.T) next_unit(a, cur, ahead, &fault);
   }
+  if constexpr (kWide) cp_async_wait_all();
   if (fault) atomicOr(&g_page_fault, fault);
 }
 
@@ -604,13 +682,6 @@ struct TcMaps {
   int lose;  // watchdog test build only: CTA 0's first K copy is for bytes that never come
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0)
-               : "memory");
-}
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
 // Whether the phase has completed, without waiting for it.
 __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
@@ -623,12 +694,6 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 template <bool kBf16, int kD, bool kTwo>
 __global__ void __launch_bounds__(TcCfg<kD, kTwo>::kThreads, TcCfg<kD, kTwo>::kCtas)
@@ -1497,6 +1562,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_tree_join_kernel(const _
 struct Plan {
   bool tc;  // the tensor-core kernel
   int kd;   // head dim the kernel is compiled for
+  bool wide;  // the other, fed by 16-byte copies
   bool two_tiles;  // a CTA takes two tiles of 128 rows at once (tensor cores)
   int unit_rows, row_tiles, tile;
   int box_rows, boxes;  // of a tile of K or V, by TMA; 0: 16-byte copies
@@ -1505,23 +1571,25 @@ struct Plan {
   size_t meta_at, ml_at, o_at, bytes;
 };
 
-// What the tensor-core kernel asks of the cache: 16-byte rows (and some).
-bool tc_takes(const AttnPagedCache* c) {
-  if (c->dtype == ATTN_F32 || c->D % 8 != 0 || c->num_pages == 0) return false;
+// Whether the cache's rows are read 16 bytes at a time.
+bool wide_rows(const AttnPagedCache* c) {
+  const int vec = c->dtype == ATTN_F32 ? 4 : 8;
+  if (c->D % vec != 0) return false;
   for (int i = 0; i < 3; ++i)
-    if (c->k_strides[i] % 8 != 0 || c->v_strides[i] % 8 != 0) return false;
+    if (c->k_strides[i] % vec != 0 || c->v_strides[i] % vec != 0) return false;
   return aligned_to(c->k, 16) && aligned_to(c->v, 16);
 }
 
-// `fast`: q and out allow the tensor-core kernel too.
+// `fast`: q and out allow 16-byte accesses, where the kernel needs them.
 Plan make_plan(const AttnPagedCache* c, bool fast, int Hq, int S, int sms) {
   Plan p;
   const int D = c->D;
   const long long rows = static_cast<long long>(Hq / c->heads) * S;
   int per_sm;
-  p.tc = fast && tc_takes(c);
+  const bool wide = fast && wide_rows(c);
+  p.tc = wide && c->dtype != ATTN_F32 && c->num_pages > 0;
   p.kd = D <= 64 ? 64 : D <= 128 ? 128 : 256;
-  p.two_tiles = false;
+  p.two_tiles = p.wide = false;
   if (p.tc) {
     p.two_tiles = p.kd <= 128 && rows > 128;
     p.unit_rows = p.two_tiles ? 256 : 128;
@@ -1550,7 +1618,8 @@ Plan make_plan(const AttnPagedCache* c, bool fast, int Hq, int S, int sms) {
   } else {
     p.unit_rows = kSimtRows;
     p.tile = kSimtTile;
-    per_sm = p.kd == 64 ? 5 : p.kd == 128 ? 3 : 2;
+    p.wide = wide && c->dtype == ATTN_F32;
+    per_sm = p.wide ? (p.kd == 64 ? 4 : p.kd == 128 ? 2 : 1) : p.kd == 64 ? 5 : p.kd == 128 ? 3 : 2;
   }
   p.row_tiles = static_cast<int>((rows + p.unit_rows - 1) / p.unit_rows);
   const long long capacity = static_cast<long long>(c->table_width) * c->page_size;
@@ -1644,19 +1713,19 @@ TcMaps make_maps(const AttnPagedCache* c, const Plan& p) {
   return m;
 }
 
-template <typename T, int kDP>
+template <typename T, int kDP, bool kWide>
 bool launch_simt(const TreeArgs& a, int grid, cudaStream_t stream) {
   static bool done[64] = {};
   static std::mutex mu;
-  return launch_big(attn_tree_simt_kernel<T, kDP>, mu, done, grid, kSimtThreads, SimtCfg<kDP>::kBytes, stream, a);
+  return launch_big(attn_tree_simt_kernel<T, kDP, kWide>, mu, done, grid, kSimtThreads, SimtCfg<kDP, kWide>::kBytes, stream, a);
 }
 
-template <typename T>
+template <typename T, bool kWide = false>
 bool launch_simt_d(const TreeArgs& a, const Plan& p, cudaStream_t stream) {
   switch (p.kd) {
-    case 64: return launch_simt<T, 64>(a, p.grid, stream);
-    case 128: return launch_simt<T, 128>(a, p.grid, stream);
-    default: return launch_simt<T, 256>(a, p.grid, stream);
+    case 64: return launch_simt<T, 64, kWide>(a, p.grid, stream);
+    case 128: return launch_simt<T, 128, kWide>(a, p.grid, stream);
+    default: return launch_simt<T, 256, kWide>(a, p.grid, stream);
   }
 }
 
@@ -1712,7 +1781,8 @@ extern "C" int launch_attn_tree(const AttnPagedCache* cache, const void* q, cons
     return ATTN_ERR_MISALIGNED;
   st = check_device();
   if (st != ATTN_OK) return st;
-  const bool fast = aligned_to(q, 16) && aligned_to(out, 16) && qs[0] % 8 == 0 && qs[1] % 8 == 0 && qs[2] % 8 == 0;
+  const bool fast = cache->dtype == ATTN_F32 ||
+                    (aligned_to(q, 16) && aligned_to(out, 16) && qs[0] % 8 == 0 && qs[1] % 8 == 0 && qs[2] % 8 == 0);
   const int sms = sm_count();
   float scale = softmax_scale;
   if (!(scale > 0.f) || !isfinite(scale)) scale = 1.0f / sqrtf(static_cast<float>(D));
@@ -1766,7 +1836,7 @@ extern "C" int launch_attn_tree(const AttnPagedCache* cache, const void* q, cons
   } else switch (cache->dtype) {
     case ATTN_F16: ok = launch_simt_d<__half>(a, p, stream); break;
     case ATTN_BF16: ok = launch_simt_d<__nv_bfloat16>(a, p, stream); break;
-    default: ok = launch_simt_d<float>(a, p, stream); break;
+    default: ok = p.wide ? launch_simt_d<float, true>(a, p, stream) : launch_simt_d<float>(a, p, stream); break;
   }
   if (!ok) return ATTN_ERR_LAUNCH;
   const int used = a.rows < p.unit_rows ? a.rows : p.unit_rows;
