@@ -469,6 +469,30 @@ def test_watchdog_fires_and_recovers(lens, D, Hq, S, ps):
     _close(out, tree_ref(q, k, v, table, ln, par), max(lens), BF16)
 
 
+@pytest.mark.parametrize("dtype,D", [(BF16, 64), (F16, 128), (F32, 64)])
+def test_layers_as_heads_of_one_cache(attn, dtype, D):
+    # three layers of two kv heads in one cache: each layer reads a view, one fork and one compaction move them all
+    S, Hq, ps = 6, 8, 16
+    k, v, table, ln = make_cache([150, 90], 6, D, ps, dtype)
+    dk, dv = k.cuda(), v.cuda()
+    P = k.shape[0]
+    refs = torch.zeros(P, dtype=torch.int32)
+    held = (ln + ps - 1) // ps
+    for b in range(2):
+        refs[table[b, :held[b]].long()] += 1
+    table, held, lens, missing = attn.kv_fork(dk, dv, table.cuda(), held.cuda(), ln.cuda(), refs.cuda(), ints([0, 1, 1]).cuda())
+    assert missing.tolist() == [0]
+    q, par = _q(3, Hq, S, D, dtype), _trees(3, S)
+    for layer in range(3):
+        heads = slice(2 * layer, 2 * layer + 2)
+        out = attn.attn_tree(q.cuda(), dk[:, heads], dv[:, heads], table, lens, par.cuda())
+        _close(out, tree_ref(q, dk[:, heads].cpu(), dv[:, heads].cpu(), table.cpu().clamp(min=0), lens.cpu(), par), 150, dtype)
+    for x, was in ((dk, k), (dv, v)):
+        # the copy of sequence 1's last page, all layers
+        new, old = int(table[2, 5]), int(table[1, 5])
+        assert new != old and torch.equal(x[new, :, :10], x[old, :, :10]) and torch.equal(x[old, :, :10].cpu(), was[old, :, :10])
+
+
 # ---------------------------------------------------------------------------
 # kv_compact
 # ---------------------------------------------------------------------------
