@@ -643,7 +643,7 @@ struct TcCfg {
   static constexpr int kMmaWarp = 4 * kStreams, kCopyWarp = kMmaWarp + 1;
   static constexpr int kThreads = kSoftThreads + 32 + 32 * kStreams;
   static constexpr uint32_t kTileBytes = kQTiles * kQBytes + (kKSlots + kVSlots) * kSlotBytes;
-  static constexpr size_t kCtlBytes = 3072;
+  static constexpr size_t kCtlBytes = 3 * 1024;
   static constexpr size_t kSmemBytes = kTileBytes + kCtlBytes;
   static_assert(kSmemBytes <= (kCtas == 1 ? 232448 : 115712), "shared memory of a CTA");
 };

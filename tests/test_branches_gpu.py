@@ -656,6 +656,21 @@ def test_fork(attn, B, n, W, P, ps, dtype, D, layout):
         assert attn.check_status(0) == 0
 
 
+def test_pools_of_more_pages_than_are_noted(attn):
+    # more counts than a warp keeps the bits of; the free pages few and at the end, and then many
+    rng, P = random.Random(5), 700_003
+    for free in ([P - 1 - 7 * i for i in range(40)], sorted(rng.sample(range(P), 300_000))):
+        refs = [1] * P
+        for p in free:
+            refs[p] = 0
+        table, held = [[-1] * 9 for _ in range(6)], [0] * 6
+        lens = [18, 1, 0, 11, 17, 16]
+        assert _resize(attn, table, held, lens, refs, 2) == [0] * 6
+        parents = [rng.randrange(6) for _ in range(9)]
+        _fork(attn, table, held, lens, refs, parents, 1, 8, 2, F16)
+        assert attn.check_status(0) == 0
+
+
 def test_fork_edges(attn):
     # a page that others hold is copied for the first child too; released pages are not given out by the call
     table, held, lens = [[0, 1], [0, 1], [2, -1]], [2, 2, 1], [20, 20, 16]
