@@ -107,7 +107,9 @@ __device__ __forceinline__ float inverse(float M, float L) {
 // ---------------------------------------------------------------------------
 
 // The tokens of a sequence: `len` in the cache, the last `n` from position
-// `base` on drafted (base < 0: the first of them are not there).
+// `base` on drafted (base < 0: the first of them are not there).  base is len
+// at most, so that a tile up to base is whole: drafted tokens that lie behind
+// the table's end are not there, wherever they lie.
 struct Seq {
   int len, n, base;
 };
@@ -128,7 +130,7 @@ __device__ __forceinline__ Seq seq_from(const TreeArgs& a, const RawSeq& r, int*
   Seq s;
   s.n = max(min(r.n, a.S), 0);
   s.len = max(min(r.len, a.c.capacity()), 0);
-  s.base = max(r.len, 0) - s.n;
+  s.base = min(max(r.len, 0) - s.n, s.len);
   if (r.n > a.S || r.len > a.c.capacity()) *fault |= kFaultPage;
   return s;
 }
