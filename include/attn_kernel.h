@@ -340,11 +340,20 @@ ATTN_API int launch_attn_tree(const AttnPagedCache* cache, const void* q, const 
  *             the sequence from then on (seq_lens is left as it is)
  * A list also ends at an entry that is not larger than the one before or names
  * no drafted token, which is reported as ATTN_ERR_BAD_PAGE.  Rows behind the
- * last kept token are left as they are, and so are page bounds: they still
- * bound the tokens.  Two sequences of a call must not write to one page.
+ * last kept token are left as they are.  Two sequences of a call must not write
+ * to one page.
+ *
+ * A key that moves to another page may lie outside that page's bounds.
+ * launch_kv_compact_bounds is the same call for a cache that has page bounds
+ * (as launch_kv_append, with the drafted tokens folded in): they take in the
+ * keys that come to a page.  After launch_kv_compact launch_kv_page_bounds
+ * makes them anew.  Null bounds: launch_kv_compact.
  */
 ATTN_API int launch_kv_compact(const AttnPagedCache* cache, const int* new_lens, const int* kept, long long kept_stride,
                                int n, int* lens, cudaStream_t stream);
+ATTN_API int launch_kv_compact_bounds(const AttnPagedCache* cache, const int* new_lens, const int* kept,
+                                      long long kept_stride, int n, int* lens, void* bounds,
+                                      const long long* bounds_strides, cudaStream_t stream);
 
 /*
  * Who holds which pages.  refs (int32 [num_pages]) counts the holders of each

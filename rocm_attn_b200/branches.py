@@ -73,7 +73,7 @@ def attn_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, blo
 
 
 def kv_compact(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
-               kept: torch.Tensor, new_lens: torch.Tensor) -> torch.Tensor:
+               kept: torch.Tensor, new_lens: torch.Tensor, bounds: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Move the drafted tokens that were accepted to the front of the drafted
     ones, in place.
 
@@ -81,12 +81,17 @@ def kv_compact(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.
     ``[B, n]``, drafted tokens in ascending order (a path of the tree); the first
     -1 ends a list.  With ``base = seq_lens[b] - new_lens[b]``, K and V of position
     ``base + kept[b, i]`` go to position ``base + i``; rows behind the last kept
-    token stay as they are.  Page bounds stay bounds of the tokens.  Two
-    sequences must not write to one page.
+    token stay as they are.  Two sequences must not write to one page.
+
+    bounds: optional page bounds (``kv_page_bounds``) that bound the drafted
+    tokens where they were, as ``kv_append`` with them leaves them; a page that
+    keys come to takes them in.  Where it is not given, a key that moves to
+    another page may lie outside that page's bounds, and ``kv_page_bounds`` has
+    to make them anew before ``kv_select_pages`` reads them.
 
     Returns the new lengths, int32 ``[B]``: base plus the tokens kept.
     """
-    return rocm_attn_ext.kv_compact(k_cache, v_cache, block_table, seq_lens, kept, new_lens)
+    return rocm_attn_ext.kv_compact(k_cache, v_cache, block_table, seq_lens, kept, new_lens, bounds)
 
 
 def kv_fork(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, held: torch.Tensor,

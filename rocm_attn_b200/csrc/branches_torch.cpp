@@ -72,7 +72,7 @@ Tensor attn_tree(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, 
 }
 
 Tensor kv_compact(const Tensor& k_cache, const Tensor& v_cache, const Tensor& block_table, const Tensor& seq_lens,
-                  const Tensor& kept, const Tensor& new_lens) {
+                  const Tensor& kept, const Tensor& new_lens, const OptTensor& bounds) {
   check_cache_tensor(k_cache, "k_cache");
   check_cache_tensor(v_cache, "v_cache");
   check_written(k_cache, "k_cache");
@@ -84,10 +84,16 @@ Tensor kv_compact(const Tensor& k_cache, const Tensor& v_cache, const Tensor& bl
   const Tensor list = int_rows(kept, "kept", c.c.B, dev, &stride);
   TORCH_CHECK(list.size(1) <= INT32_MAX, "sizes must fit in 32-bit integers");
   const Tensor n = int_vector(new_lens, "new_lens", c.c.B, "seq_lens", dev);
+  long long bs[3] = {0, 0, 0};
+  if (bounds) {
+    check_bounds(*bounds, c.c.num_pages, c.c.heads, c.c.D, k_cache, bs);
+    check_written(*bounds, "bounds");
+  }
   Tensor lens = torch::empty({c.c.B}, torch::dtype(torch::kInt32).device(dev));
   if (c.c.B > 0)
-    check_launch(launch_kv_compact(&c.c, n.data_ptr<int>(), list.data_ptr<int>(), stride,
-                                   static_cast<int>(list.size(1)), lens.data_ptr<int>(), stream_of(dev)),
+    check_launch(launch_kv_compact_bounds(&c.c, n.data_ptr<int>(), list.data_ptr<int>(), stride,
+                                          static_cast<int>(list.size(1)), lens.data_ptr<int>(),
+                                          bounds ? bounds->data_ptr() : nullptr, bs, stream_of(dev)),
                  "launch_kv_compact");
   return lens;
 }
@@ -151,7 +157,8 @@ void bind_branches(py::module& m) {
         py::arg("v_cache"), py::arg("block_table"), py::arg("seq_lens"), py::arg("parents") = py::none(),
         py::arg("new_lens") = py::none(), py::arg("scale") = -1.0);
   m.def("kv_compact", &kv_compact, "Move accepted drafted tokens to their places", py::arg("k_cache"),
-        py::arg("v_cache"), py::arg("block_table"), py::arg("seq_lens"), py::arg("kept"), py::arg("new_lens"));
+        py::arg("v_cache"), py::arg("block_table"), py::arg("seq_lens"), py::arg("kept"), py::arg("new_lens"),
+        py::arg("bounds") = py::none());
   m.def("kv_fork", &kv_fork, "Sequences that continue others, full pages shared", py::arg("k_cache"),
         py::arg("v_cache"), py::arg("block_table"), py::arg("held"), py::arg("seq_lens"), py::arg("refs"),
         py::arg("parents"));

@@ -19,6 +19,7 @@
 #include <limits.h>
 #include <stdint.h>
 
+#include "key_bounds.cuh"
 #include "paged_cache.h"
 #include "sm100_ptx.cuh"
 
@@ -34,11 +35,6 @@ constexpr int kFindThreads = kFindWarps * 32;
 constexpr int kStep = 256;  // pages a warp looks at in one turn
 constexpr int kTurnsKept = 8;  // turns whose bits are kept (half a million pages); others are looked at again
 constexpr int kCopyAhead = 4;  // rows a thread copies in one turn
-
-template <typename E, int kVec>
-struct alignas(sizeof(E) * kVec) Vec {
-  E v[kVec];
-};
 
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -472,15 +468,20 @@ struct CompactArgs {
   int n;
   int* lens;
   int cols;  // 16-byte (or element) columns of a row
+  void* bounds;             // page bounds, or null
+  long long b_p, b_h, b_m;  // their strides over (page, head, min/max)
 };
 
 // Warp (b, head), lane a column of K or V: a kept token's place is never behind
 // it, and the places of the tokens of one turn never among the sources of a later one, so
 // each lane moves its column by itself, the rows of a turn read before any of
-// them is written.
+// them is written.  kBounds: keys that change pages are folded into the bounds
+// of the page they come to, which has been appended to from its row 0 on and so
+// has bounds, by the lane that moves them (those that stay in a page are in its
+// bounds already).  E: the cache's type, or any of its size without bounds.
 constexpr int kMoveWarps = 4, kMoveAhead = 16;
 
-template <typename E, int kVec>
+template <typename E, int kVec, bool kBounds>
 __global__ void __launch_bounds__(kMoveWarps * 32) kv_compact_kernel(const __grid_constant__ CompactArgs a) {
   using V = Vec<E, kVec>;
   launch_dependents();
@@ -520,6 +521,7 @@ __global__ void __launch_bounds__(kMoveWarps * 32) kv_compact_kernel(const __gri
       to_page = paged_page(a.c, b, tp, &fault);
     }
     const unsigned moves = __ballot_sync(0xffffffffu, from_page >= 0 && to_page >= 0);
+    const unsigned crosses = __ballot_sync(0xffffffffu, from_page >= 0 && to_page >= 0 && from_page != to_page);
     for (int half = 0; half < 32; half += kMoveAhead) {
       if ((moves >> half & (0xffffffffu >> (32 - kMoveAhead))) == 0) continue;
       for (int c0 = 0; c0 < 2 * a.cols; c0 += 32) {
@@ -534,12 +536,33 @@ __global__ void __launch_bounds__(kMoveWarps * 32) kv_compact_kernel(const __gri
           const int in = __shfl_sync(0xffffffffu, from_row, half + p);
           if (live && (moves >> (half + p) & 1u)) row[p] = *reinterpret_cast<const V*>(x + pg * st[0] + in * st[2]);
         }
+        long long open = -1;  // the page whose bounds are to take in lo and hi
+        V lo = {}, hi = {};
+        auto close = [&] {
+          if (open < 0) return;
+          E* to = static_cast<E*>(a.bounds) + open * a.b_p + h * a.b_h + static_cast<long long>(c) * kVec;
+          V *to_lo = reinterpret_cast<V*>(to), *to_hi = reinterpret_cast<V*>(to + a.b_m);
+          if constexpr (kBounds) fold(lo, hi, *to_lo, *to_hi);
+          *to_lo = lo;
+          *to_hi = hi;
+        };
 #pragma unroll
         for (int p = 0; p < kMoveAhead; ++p) {
           const long long pg = __shfl_sync(0xffffffffu, to_page, half + p);
           const int in = __shfl_sync(0xffffffffu, to_row, half + p);
           if (live && (moves >> (half + p) & 1u)) *reinterpret_cast<V*>(x + pg * st[0] + in * st[2]) = row[p];
+          if constexpr (kBounds) {
+            if (!live || is_v || !(crosses >> (half + p) & 1u)) continue;
+            if (pg == open) {
+              fold(lo, hi, row[p], row[p]);
+            } else {
+              close();
+              open = pg;
+              lo = hi = row[p];
+            }
+          }
         }
+        if constexpr (kBounds) close();
       }
     }
     count += here;
@@ -587,13 +610,29 @@ ForkPlan fork_plan(const AttnPagedCache* c, int n) {
   return ForkPlan{0, old, copy, list, copies, order, order + round_up(sizeof(int) * listed)};
 }
 
-// Elements per access: 16 bytes where rows, strides and addresses of K and V
-// allow them, else one.
-int access_width(const AttnPagedCache* c) {
+// Elements per access: 16 bytes where rows, strides and addresses of K and V,
+// and of the page bounds if there are any, allow them, else one.
+int access_width(const AttnPagedCache* c, const void* bounds, const long long* bounds_strides) {
   const int vec = c->dtype == ATTN_F32 ? 4 : 8;
-  bool fits = c->D % vec == 0 && aligned_to(c->k, 16) && aligned_to(c->v, 16);
-  for (int i = 0; i < 3; ++i) fits = fits && c->k_strides[i] % vec == 0 && c->v_strides[i] % vec == 0;
+  bool fits = c->D % vec == 0 && aligned_to(c->k, 16) && aligned_to(c->v, 16) && aligned_to(bounds, 16);
+  for (int i = 0; i < 3; ++i)
+    fits = fits && c->k_strides[i] % vec == 0 && c->v_strides[i] % vec == 0 &&
+           (!bounds || bounds_strides[i] % vec == 0);
   return fits ? vec : 1;
+}
+
+// The checks of page bounds (none: null) that need no device.
+int check_bounds(const AttnPagedCache* c, const void* bounds, const long long* strides) {
+  if (!bounds) return ATTN_OK;
+  if (!strides || strides[0] < 0 || strides[1] < 0 || strides[2] < 0) return ATTN_ERR_INVALID_ARGUMENT;
+  return aligned_to(bounds, c->dtype == ATTN_F32 ? 4 : 2) ? ATTN_OK : ATTN_ERR_MISALIGNED;
+}
+
+template <typename E, int kVec, bool kBounds>
+bool launch_compact(const CompactArgs& a, cudaStream_t stream) {
+  const long long warps = static_cast<long long>(a.c.B) * a.c.heads;
+  return launch_after(kv_compact_kernel<E, kVec, kBounds>, dim3(static_cast<unsigned>((warps + kMoveWarps - 1) / kMoveWarps)),
+                      dim3(kMoveWarps * 32), 0, stream, 1, true, a);
 }
 
 }  // namespace
@@ -612,6 +651,12 @@ int page_word_read_clear_pages(cudaStream_t stream, int* host) {
 
 extern "C" int launch_kv_compact(const AttnPagedCache* cache, const int* new_lens, const int* kept,
                                  long long kept_stride, int n, int* lens, cudaStream_t stream) {
+  return launch_kv_compact_bounds(cache, new_lens, kept, kept_stride, n, lens, nullptr, nullptr, stream);
+}
+
+extern "C" int launch_kv_compact_bounds(const AttnPagedCache* cache, const int* new_lens, const int* kept,
+                                        long long kept_stride, int n, int* lens, void* bounds,
+                                        const long long* bounds_strides, cudaStream_t stream) {
   using namespace ra;
   CompactArgs a;
   int st = check_paged_cache(cache, kCacheK | kCacheV, &a.c);
@@ -620,6 +665,8 @@ extern "C" int launch_kv_compact(const AttnPagedCache* cache, const int* new_len
   if (cache->B == 0) return ATTN_OK;
   if (!new_lens || (n > 0 && !kept) || !lens) return ATTN_ERR_INVALID_ARGUMENT;
   if (!aligned_to(new_lens, 4) || !aligned_to(kept, 4) || !aligned_to(lens, 4)) return ATTN_ERR_MISALIGNED;
+  st = check_bounds(cache, bounds, bounds_strides);
+  if (st != ATTN_OK) return st;
   const long long blocks = (static_cast<long long>(cache->B) * cache->heads + kMoveWarps - 1) / kMoveWarps;
   if (blocks > 0x7fffffffLL) return ATTN_ERR_INVALID_ARGUMENT;
   st = check_device();
@@ -629,12 +676,23 @@ extern "C" int launch_kv_compact(const AttnPagedCache* cache, const int* new_len
   a.kept_stride = kept_stride;
   a.n = n;
   a.lens = lens;
-  const int vec = access_width(cache);
+  a.bounds = bounds;
+  a.b_p = a.b_h = a.b_m = 0;
+  if (bounds) a.b_p = bounds_strides[0], a.b_h = bounds_strides[1], a.b_m = bounds_strides[2];
+  const int vec = access_width(cache, bounds, bounds_strides);
   a.cols = cache->D / vec;
-  const dim3 grid(static_cast<unsigned>(blocks)), block(kMoveWarps * 32);
-  const auto kern = cache->dtype == ATTN_F32 ? (vec == 4 ? kv_compact_kernel<uint32_t, 4> : kv_compact_kernel<uint32_t, 1>)
-                                             : (vec == 8 ? kv_compact_kernel<uint16_t, 8> : kv_compact_kernel<uint16_t, 1>);
-  return launch_after(kern, grid, block, 0, stream, 1, true, a) ? ATTN_OK : ATTN_ERR_LAUNCH;
+  bool ok;
+  if (!bounds && cache->dtype == ATTN_F32)
+    ok = vec == 4 ? launch_compact<uint32_t, 4, false>(a, stream) : launch_compact<uint32_t, 1, false>(a, stream);
+  else if (!bounds)
+    ok = vec == 8 ? launch_compact<uint16_t, 8, false>(a, stream) : launch_compact<uint16_t, 1, false>(a, stream);
+  else if (cache->dtype == ATTN_F32)
+    ok = vec == 4 ? launch_compact<float, 4, true>(a, stream) : launch_compact<float, 1, true>(a, stream);
+  else if (cache->dtype == ATTN_F16)
+    ok = vec == 8 ? launch_compact<__half, 8, true>(a, stream) : launch_compact<__half, 1, true>(a, stream);
+  else
+    ok = vec == 8 ? launch_compact<__nv_bfloat16, 8, true>(a, stream) : launch_compact<__nv_bfloat16, 1, true>(a, stream);
+  return ok ? ATTN_OK : ATTN_ERR_LAUNCH;
 }
 
 extern "C" int kv_resize_workspace_bytes(const AttnPagedCache* cache, size_t* bytes) {
@@ -703,7 +761,7 @@ extern "C" int launch_kv_fork(const AttnPagedCache* cache, const int* held, int*
     if (!aligned_to(p, 4)) return ATTN_ERR_MISALIGNED;
   if (!aligned_to(workspace, 16)) return ATTN_ERR_MISALIGNED;
   const ForkPlan p = fork_plan(cache, n);
-  const int vec = access_width(cache);
+  const int vec = access_width(cache, nullptr, nullptr);
   a.cols = cache->D / vec;
   // Rows per thread: up to two turns of kCopyAhead, in large pages more.
   const long long per = 2LL * kCopyAhead * (256 / a.cols), chunks = (cache->page_size + per - 1) / per;

@@ -122,6 +122,17 @@ void check_cache_tensor(const Tensor& t, const char* name) {
   check_unit_inner(t, name);
 }
 
+// bounds [num_pages, Hkv, 2, D] like the cache's keys.
+void check_bounds(const Tensor& b, int64_t pages, int64_t heads, int64_t D, const Tensor& like, long long* strides) {
+  check_cuda(b, "bounds");
+  TORCH_CHECK(b.dim() == 4 && b.size(0) == pages && b.size(1) == heads && b.size(2) == 2 && b.size(3) == D,
+              "bounds must be [num_pages, Hkv, 2, D]");
+  TORCH_CHECK(b.scalar_type() == like.scalar_type(), "bounds must have the cache's dtype");
+  TORCH_CHECK(b.device() == like.device(), "bounds must be on the same device as the cache");
+  check_unit_inner(b, "bounds");
+  strides_of(b, 0, 3, strides);
+}
+
 Tensor workspace(size_t bytes, const c10::Device& dev) {
   return torch::empty({static_cast<int64_t>(bytes > 0 ? bytes : 16)}, torch::dtype(torch::kUInt8).device(dev));
 }

@@ -2,11 +2,12 @@
 their forms (test_branches_gpu.py) leave out, against the definitions
 (branches_ref.py)."""
 import math
+import random
 
 import pytest
 import torch
 
-from branches_ref import tree_ref
+from branches_ref import compact_ref, tree_ref
 from paged_ref import make_cache
 from test_branches_gpu import BF16, F16, F32, _close, _q, _trees, ints
 
@@ -40,3 +41,96 @@ def test_tree_lengths_behind_the_table(attn, ps, W, D, dtype, Hq, Hkv, S):
         out = attn.attn_tree(q.cuda(), k.cuda(), v.cuda(), table.cuda(), ln.cuda(), None if tree is None else tree.cuda())
         assert attn.check_status(0) == 8
         _close(out, tree_ref(q, k, v, table, ln, tree), cap, dtype)
+
+
+# ---------------------------------------------------------------------------
+# Page bounds after drafted tokens
+# ---------------------------------------------------------------------------
+
+
+def _check_bounds(bounds, k, table, lens):
+    """Whether every key of every sequence lies within the bounds of its page."""
+    ps = k.shape[2]
+    bounds, k = bounds.cpu().float(), k.cpu().float()
+    for b, n in enumerate(lens.tolist()):
+        for t in range(n):
+            p = int(table[b, t // ps])
+            assert (bounds[p, :, 0] <= k[p, :, t % ps]).all() and (k[p, :, t % ps] <= bounds[p, :, 1]).all()
+
+
+def _bounds_in(D, heads, pages, dtype, off):
+    """Storage for bounds, 16-byte aligned or not."""
+    x = torch.full((pages, heads, 2, D + off), math.nan, dtype=dtype, device="cuda")
+    return x[..., off:]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("D,ps,layout,off", [(64, 16, "hnd", 0), (128, 3, "nhd", 0), (256, 8, "hnd", 0), (80, 1, "hnd", 0),
+                                             (33, 4, "hnd", 0), (64, 5, "hnd", 1)])
+@pytest.mark.parametrize("S", [4, 40])
+def test_compact_keeps_page_bounds(attn, S, D, ps, layout, off, dtype):
+    # contexts that end anywhere in a page, drafted keys larger than those before, paths that end late in them
+    H, rng = 2, random.Random(S + D)
+    ctx = [15, 16, 0, 1, 31, 2 * ps, 3 * ps - 1]
+    B, new = len(ctx), [S, S, S, max(1, S - 1), 2, S, S]
+    lens = [c + n for c, n in zip(ctx, new)]
+    k, v, table, _ = make_cache(lens, H, D, ps, dtype, layout=layout, poison=False)
+    at, n = ints(ctx), ints(new)
+    kc, vc, t = k.cuda(), v.cuda(), table.cuda()
+    if layout == "nhd":
+        kc, vc = (x.transpose(1, 2).contiguous().transpose(1, 2) for x in (kc, vc))
+    bounds = _bounds_in(D, H, k.shape[0], dtype, off)
+    attn.kv_page_bounds(kc, t, at.cuda(), bounds=bounds)
+    x = (_q(B, H, S, D, dtype, 5).float() * torch.arange(1, S + 1)[:, None]).to(dtype).cuda()
+    attn.kv_append(x, x, kc, vc, t, ints(lens).cuda(), n.cuda(), bounds=bounds)
+    paths = [[S - 1]] + [sorted(rng.sample(range(m), rng.randint(0, m))) for m in new[1:]]
+    kept = ints([p + [-1] * (S - len(p)) for p in paths])
+    want, k, v = bounds.cpu().clone(), kc.cpu().clone(), vc.cpu().clone()
+    after = attn.kv_compact(kc, vc, t, ints(lens).cuda(), kept.cuda(), n.cuda(), bounds=bounds)
+    # the definition: a page that a key comes to takes it in
+    assert torch.equal(after.cpu(), compact_ref(k, v, table, ints(lens), kept, n))
+    assert torch.equal(kc.cpu(), k) and torch.equal(vc.cpu(), v)
+    for b in range(B):
+        for i, a in enumerate(kept[b].tolist()):
+            if a < 0:
+                break
+            p, r = int(table[b, (ctx[b] + i) // ps]), (ctx[b] + i) % ps
+            want[p, :, 0] = torch.minimum(want[p, :, 0], k[p, :, r])
+            want[p, :, 1] = torch.maximum(want[p, :, 1], k[p, :, r])
+    assert torch.equal(bounds.cpu().nan_to_num(7.0), want.nan_to_num(7.0))
+    _check_bounds(bounds, kc, table, after)
+    assert attn.check_status(0) == 0
+
+
+def test_selection_after_compaction_finds_the_moved_key(attn):
+    # 15 tokens, four drafted across the page's end, the last of them accepted: it comes to page 0, whose keys are
+    # small.  Selection of the pages that the next tokens read has to see it there.
+    ps, D = 16, 64
+    for dtype in (F16, BF16, F32):
+        kc, vc = (torch.zeros(8, 1, ps, D, dtype=dtype, device="cuda") for _ in range(2))
+        table = ints([[5, 2, 7, 0]]).cuda()
+        bounds = torch.zeros(8, 1, 2, D, dtype=dtype, device="cuda")
+        small = (_q(1, 1, 15, D, dtype) / 16).cuda()
+        attn.kv_append(small, small, kc, vc, table, ints([15]).cuda(), bounds=bounds)
+        drafts = (_q(1, 1, 4, D, dtype, 2) / 16).cuda()
+        drafts[0, 0, 3] = 4
+        attn.kv_append(drafts, drafts, kc, vc, table, ints([19]).cuda(), bounds=bounds)
+        lens = attn.kv_compact(kc, vc, table, ints([19]).cuda(), ints([[3]]).cuda(), ints([4]).cuda(), bounds=bounds)
+        assert lens.tolist() == [16] and bool((kc[5, 0, 15] == 4).all())
+        more = (_q(1, 1, 40, D, dtype, 3) / 8).cuda()
+        attn.kv_append(more, more, kc, vc, table, ints([56]).cuda(), bounds=bounds)
+        q = torch.ones(1, 1, 1, D, dtype=dtype, device="cuda")
+        assert attn.kv_select_pages(q, bounds, table, ints([56]).cuda(), ps, 2).tolist() == [[[0, 3]]]
+        assert bool((bounds[5, 0, 1] == 4).all())
+
+
+def test_compact_refuses_bounds_that_do_not_fit(attn):
+    k = torch.zeros(6, 2, 16, 64, dtype=F16, device="cuda")
+    t, n, kept, new = (ints(x).cuda() for x in ([[0, 1]], [20], [[1]], [4]))
+    good = torch.zeros(6, 2, 2, 64, dtype=F16, device="cuda")
+    for bad in (good[:5], good[:, :1], good[:, :, :1], good[..., :32], good.float(), good.cpu(), good[0],
+                good[:1].expand(6, 2, 2, 64), good.transpose(2, 3).contiguous().transpose(2, 3)):
+        with pytest.raises(RuntimeError, match="bounds"):
+            attn.kv_compact(k, k.clone(), t, n, kept, new, bounds=bad)
+    attn.kv_compact(k, k.clone(), t, n, kept, new, bounds=good)
+    assert attn.check_status(0) == 0
