@@ -396,11 +396,20 @@ ATTN_API int launch_kv_resize(const AttnPagedCache* cache, int* table, int* held
  * behind the pages it holds are left out and, like parents outside [-1, B) (taken
  * as -1), reported as ATTN_ERR_BAD_PAGE.  The written arrays must not overlap
  * the cache's table, lengths or held.
+ *
+ * launch_kv_fork_bounds is the same call for a cache that has page bounds (as
+ * launch_kv_append): those of a copied page go with its rows.  After
+ * launch_kv_fork the bounds of a copy are whatever the page had before, and
+ * launch_kv_page_bounds makes them anew.  Null bounds: launch_kv_fork.
  */
 ATTN_API int kv_fork_workspace_bytes(const AttnPagedCache* cache, int n, size_t* bytes);
 ATTN_API int launch_kv_fork(const AttnPagedCache* cache, const int* held, int* refs, const int* parents, int n,
                             int* new_table, int* new_held, int* new_lens, int* missing, void* workspace,
                             size_t workspace_bytes, cudaStream_t stream);
+ATTN_API int launch_kv_fork_bounds(const AttnPagedCache* cache, const int* held, int* refs, const int* parents, int n,
+                                   int* new_table, int* new_held, int* new_lens, int* missing, void* bounds,
+                                   const long long* bounds_strides, void* workspace, size_t workspace_bytes,
+                                   cudaStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -95,8 +95,8 @@ def kv_compact(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.
 
 
 def kv_fork(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, held: torch.Tensor,
-            seq_lens: torch.Tensor, refs: torch.Tensor,
-            parents: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+            seq_lens: torch.Tensor, refs: torch.Tensor, parents: torch.Tensor,
+            bounds: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """The sequences of the next step as continuations of the present ones:
     beams, or several samples of one prompt.
 
@@ -107,12 +107,17 @@ def kv_fork(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Ten
     present sequences give up what they hold, so ``refs``, changed in place,
     counts the new ones; pages that this frees are given out from the next call on.
 
+    bounds: optional page bounds (``kv_page_bounds``); those of a copied page go
+    with it.  Where it is not given, a copy's bounds are whatever the page had
+    before, and ``kv_page_bounds`` has to make them anew before ``kv_append``
+    folds keys into them or ``kv_select_pages`` reads them.
+
     Returns ``(block_table, held, seq_lens, missing)`` of the new sequences, int32
     ``[n, W]`` (-1 behind a row's pages), ``[n]``, ``[n]`` and ``[1]``.  If there are fewer free
     pages than copies, ``missing`` says how many are lacking, nothing is changed
     and the new sequences are empty; the given tensors are still valid then.
     """
-    return rocm_attn_ext.kv_fork(k_cache, v_cache, block_table, held, seq_lens, refs, parents)
+    return rocm_attn_ext.kv_fork(k_cache, v_cache, block_table, held, seq_lens, refs, parents, bounds)
 
 
 def kv_resize(block_table: torch.Tensor, held: torch.Tensor, seq_lens: torch.Tensor, refs: torch.Tensor,

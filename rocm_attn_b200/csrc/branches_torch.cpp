@@ -100,7 +100,8 @@ Tensor kv_compact(const Tensor& k_cache, const Tensor& v_cache, const Tensor& bl
 
 std::tuple<Tensor, Tensor, Tensor, Tensor> kv_fork(const Tensor& k_cache, const Tensor& v_cache,
                                                    const Tensor& block_table, const Tensor& held,
-                                                   const Tensor& seq_lens, const Tensor& refs, const Tensor& parents) {
+                                                   const Tensor& seq_lens, const Tensor& refs, const Tensor& parents,
+                                                   const OptTensor& bounds) {
   check_cache_tensor(k_cache, "k_cache");
   check_cache_tensor(v_cache, "v_cache");
   check_written(k_cache, "k_cache");
@@ -114,15 +115,21 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> kv_fork(const Tensor& k_cache, const 
   const Tensor from = int_tensor(parents, "parents", 1, dev).contiguous();
   TORCH_CHECK(from.size(0) <= INT32_MAX, "sizes must fit in 32-bit integers");
   const int n = static_cast<int>(from.size(0));
+  long long bs[3] = {0, 0, 0};
+  if (bounds) {
+    check_bounds(*bounds, c.c.num_pages, c.c.heads, c.c.D, k_cache, bs);
+    check_written(*bounds, "bounds");
+  }
   const auto ints = torch::dtype(torch::kInt32).device(dev);
   Tensor new_table = torch::empty({n, c.c.table_width}, ints), new_held = torch::empty({n}, ints),
          new_lens = torch::empty({n}, ints), missing = torch::empty({1}, ints);
   size_t bytes = 0;
   check_launch(kv_fork_workspace_bytes(&c.c, n, &bytes), "kv_fork_workspace_bytes");
   const Tensor space = workspace(bytes, dev);
-  check_launch(launch_kv_fork(&c.c, have.data_ptr<int>(), refs.data_ptr<int>(), from.data_ptr<int>(), n,
-                              new_table.data_ptr<int>(), new_held.data_ptr<int>(), new_lens.data_ptr<int>(),
-                              missing.data_ptr<int>(), space.data_ptr(), bytes, stream_of(dev)),
+  check_launch(launch_kv_fork_bounds(&c.c, have.data_ptr<int>(), refs.data_ptr<int>(), from.data_ptr<int>(), n,
+                                     new_table.data_ptr<int>(), new_held.data_ptr<int>(), new_lens.data_ptr<int>(),
+                                     missing.data_ptr<int>(), bounds ? bounds->data_ptr() : nullptr, bs,
+                                     space.data_ptr(), bytes, stream_of(dev)),
                "launch_kv_fork");
   return {new_table, new_held, new_lens, missing};
 }
@@ -161,7 +168,7 @@ void bind_branches(py::module& m) {
         py::arg("bounds") = py::none());
   m.def("kv_fork", &kv_fork, "Sequences that continue others, full pages shared", py::arg("k_cache"),
         py::arg("v_cache"), py::arg("block_table"), py::arg("held"), py::arg("seq_lens"), py::arg("refs"),
-        py::arg("parents"));
+        py::arg("parents"), py::arg("bounds") = py::none());
   m.def("kv_resize", &kv_resize, "Hold the pages that lengths need", py::arg("block_table"), py::arg("held"),
         py::arg("seq_lens"), py::arg("refs"), py::arg("page_size"));
 }

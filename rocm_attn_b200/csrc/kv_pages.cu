@@ -303,6 +303,8 @@ struct ForkArgs {
   int* order;         // workspace: free pages by rank
   int cols;           // 16-byte (or element) columns of a row
   int chunks;         // CTAs per head's K (or V) rows of a copied page
+  void* bounds;             // page bounds, or null: a copied page's go with it
+  long long b_p, b_h, b_m;  // their strides over (page, head, min/max)
 };
 
 // A new sequence's parent and what it takes from it: len tokens in `full` full
@@ -451,6 +453,14 @@ __global__ void __launch_bounds__(256) kv_fork_copy_kernel(const __grid_constant
 #pragma unroll
         for (int p = 0; p < kCopyAhead; ++p)
           if (r0 + p * step < what.y) *reinterpret_cast<V*>(x + to * st[0] + (r0 + p * step) * st[2]) = row[p];
+      }
+    }
+    if (a.bounds && !is_v && chunk == 0) {
+      E* y = static_cast<E*>(a.bounds) + h * a.b_h;
+      for (int e = threadIdx.x; e < 2 * a.cols; e += 256) {
+        const int m = e >= a.cols;
+        const long long off = m * a.b_m + static_cast<long long>(e - m * a.cols) * kVec;
+        *reinterpret_cast<V*>(y + to * a.b_p + off) = *reinterpret_cast<const V*>(y + from * a.b_p + off);
       }
     }
   }
@@ -747,6 +757,14 @@ extern "C" int kv_fork_workspace_bytes(const AttnPagedCache* cache, int n, size_
 extern "C" int launch_kv_fork(const AttnPagedCache* cache, const int* held, int* refs, const int* parents, int n,
                               int* new_table, int* new_held, int* new_lens, int* missing, void* workspace,
                               size_t workspace_bytes, cudaStream_t stream) {
+  return launch_kv_fork_bounds(cache, held, refs, parents, n, new_table, new_held, new_lens, missing, nullptr, nullptr,
+                               workspace, workspace_bytes, stream);
+}
+
+extern "C" int launch_kv_fork_bounds(const AttnPagedCache* cache, const int* held, int* refs, const int* parents, int n,
+                                     int* new_table, int* new_held, int* new_lens, int* missing, void* bounds,
+                                     const long long* bounds_strides, void* workspace, size_t workspace_bytes,
+                                     cudaStream_t stream) {
   using namespace ra;
   ForkArgs a;
   int st = check_paged_cache(cache, kCacheK | kCacheV, &a.c);
@@ -760,8 +778,10 @@ extern "C" int launch_kv_fork(const AttnPagedCache* cache, const int* held, int*
                         static_cast<const void*>(new_lens), static_cast<const void*>(missing)})
     if (!aligned_to(p, 4)) return ATTN_ERR_MISALIGNED;
   if (!aligned_to(workspace, 16)) return ATTN_ERR_MISALIGNED;
+  st = check_bounds(cache, bounds, bounds_strides);
+  if (st != ATTN_OK) return st;
   const ForkPlan p = fork_plan(cache, n);
-  const int vec = access_width(cache, nullptr, nullptr);
+  const int vec = access_width(cache, bounds, bounds_strides);
   a.cols = cache->D / vec;
   // Rows per thread: up to two turns of kCopyAhead, in large pages more.
   const long long per = 2LL * kCopyAhead * (256 / a.cols), chunks = (cache->page_size + per - 1) / per;
@@ -774,6 +794,9 @@ extern "C" int launch_kv_fork(const AttnPagedCache* cache, const int* held, int*
   a.parents = parents;
   a.refs = refs;
   a.n = n;
+  a.bounds = bounds;
+  a.b_p = a.b_h = a.b_m = 0;
+  if (bounds) a.b_p = bounds_strides[0], a.b_h = bounds_strides[1], a.b_m = bounds_strides[2];
   a.new_table = new_table;
   a.new_held = new_held;
   a.new_lens = new_lens;

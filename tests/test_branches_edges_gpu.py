@@ -134,3 +134,60 @@ def test_compact_refuses_bounds_that_do_not_fit(attn):
             attn.kv_compact(k, k.clone(), t, n, kept, new, bounds=bad)
     attn.kv_compact(k, k.clone(), t, n, kept, new, bounds=good)
     assert attn.check_status(0) == 0
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("D,ps,layout,off", [(64, 16, "hnd", 0), (128, 3, "nhd", 0), (256, 64, "hnd", 0), (80, 2, "hnd", 0),
+                                             (33, 4, "hnd", 0), (64, 5, "hnd", 1), (255, 7, "hnd", 0)])
+def test_fork_keeps_page_bounds(attn, D, ps, layout, off, dtype):
+    # beams of two prompts fork, append with bounds and fork again; free pages had other tokens before
+    H, P = 3, 60
+    rng = random.Random(D)
+    kc, vc = (torch.zeros(P, H, ps, D, dtype=dtype, device="cuda") for _ in range(2))
+    if layout == "nhd":
+        kc, vc = (x.transpose(1, 2).contiguous().transpose(1, 2) for x in (kc, vc))
+    bounds = _bounds_in(D, H, P, dtype, off)
+    bounds.zero_()  # too narrow for what will come
+    lens, refs = ints([4 * ps - 1, ps + 1]).cuda(), ints([0] * P).cuda()
+    table, held = torch.full((2, 9), -1, dtype=torch.int32, device="cuda"), ints([0, 0]).cuda()
+    assert not attn.kv_resize(table, held, lens, refs, ps).any()
+    x = _q(2, H, 4 * ps, D, dtype, 3).cuda()
+    attn.kv_append(x, x, kc, vc, table, lens, new_lens=lens, bounds=bounds)
+    parents = [0, 0, 1, 1, 0]
+    for turn in range(2 * ps if ps < 8 else 4):
+        was, free = bounds.clone(), refs == 0
+        old, old_lens, src = table.cpu(), lens.tolist(), list(parents)
+        table, held, lens, missing = attn.kv_fork(kc, vc, table, held, lens, refs, ints(parents).cuda(), bounds=bounds)
+        assert missing.tolist() == [0]
+        for i, a in enumerate(src):
+            last = old_lens[a] // ps
+            if old_lens[a] % ps and int(table[i, last]) != int(old[a, last]):
+                p = int(table[i, last])
+                assert bool(free[p]) and torch.equal(bounds[p], was[int(old[a, last])])
+                was[p] = bounds[p]
+        assert torch.equal(bounds.nan_to_num(7.0), was.nan_to_num(7.0))  # others stay as they are
+        _check_bounds(bounds, kc, table, lens)
+        lens = lens + 1
+        assert not attn.kv_resize(table, held, lens, refs, ps).any()
+        x = (turn + 2) * _q(5, H, 1, D, dtype, turn).cuda()
+        attn.kv_append(x, x, kc, vc, table, lens, bounds=bounds)
+        _check_bounds(bounds, kc, table, lens)
+        parents = [rng.randrange(5) for _ in range(5)]
+    # too few free pages: bounds stay as they are, too
+    refs.clamp_(min=1)
+    was = bounds.clone()
+    if (lens % ps).any():
+        *_, missing = attn.kv_fork(kc, vc, table, held, lens, refs, ints([0, 1, 2, 3, 4] * 2).cuda(), bounds=bounds)
+        assert missing.item() > 0 and torch.equal(bounds.nan_to_num(7.0), was.nan_to_num(7.0))
+    assert attn.check_status(0) == 0
+
+
+def test_fork_refuses_bounds_that_do_not_fit(attn):
+    k = torch.zeros(6, 2, 16, 64, dtype=F16, device="cuda")
+    t, h, n, r, p = (ints(x).cuda() for x in ([[0, 1]], [2], [20], [1, 1, 0, 0, 0, 0], [0, 0]))
+    good = torch.zeros(6, 2, 2, 64, dtype=F16, device="cuda")
+    for bad in (good[:5], good[:, :1], good[:, :, :1], good[..., :32], good.float(), good.cpu(), good[0],
+                good[:1].expand(6, 2, 2, 64)):
+        with pytest.raises(RuntimeError, match="bounds"):
+            attn.kv_fork(k, k.clone(), t, h, n, r, p, bounds=bad)
+    assert r.tolist() == [1, 1, 0, 0, 0, 0] and attn.check_status(0) == 0
