@@ -367,7 +367,9 @@ ATTN_API int launch_kv_compact_bounds(const AttnPagedCache* cache, const int* ne
  * for the sequences before it counted, takes none.  Changes
  * cache->block_table (through `table`, the same memory), held and refs;
  * missing (int32 [B]) receives the pages that a sequence lacked and did not
- * get, else 0.  Entries of the table behind those held are left as they are.
+ * get, else 0.  Entries of the table behind those held are left as they are:
+ * their pages may be other sequences' by then, and no operator can tell, so the
+ * lengths of later calls must not pass held[b] * page_size tokens.
  * cache->k and v are not used.
  *
  * Counts of held outside [0, table_width], lengths that need more pages than

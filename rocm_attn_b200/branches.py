@@ -15,17 +15,30 @@ here synchronises and captured calls follow them.  Free pages are given out
 from the lowest on, in the order of the sequences.  What is out of range
 (pages, lengths, parents) is never followed; ``check_status`` then returns 8.
 
-A step that drafts tokens::
+Lengths must not pass the pages that a sequence holds.  Entries of the table
+behind ``held[b]`` are what is left of pages that it has given back, and other
+sequences may hold those by now; no operator can tell.  So a program grows its
+lengths by what it got, not by what it asked for.  A step that drafts tokens::
 
-    missing = kv_resize(table, held, lens + S, refs, page_size)   # room for the drafts
-    lens += S
-    kv_append(k, v, k_cache, v_cache, table, lens)                # k/v [B, Hkv, S, D]
-    o = attn_tree(q, k_cache, v_cache, table, lens, parents)      # q [B, Hq, S, D]
+    kv_resize(table, held, lens + S, refs, page_size)             # room for the drafts
+    drafted = (held * page_size - lens).clamp(0, S)               # fewer than S where pages ran out
+    lens += drafted
+    kv_append(k, v, k_cache, v_cache, table, lens, drafted)       # k/v [B, Hkv, S, D]
+    o = attn_tree(q, k_cache, v_cache, table, lens, parents, drafted)  # q [B, Hq, S, D]
     lens = kv_compact(k_cache, v_cache, table, lens, accepted, drafted)
     kv_resize(table, held, lens, refs, page_size)                 # what the others held goes back
 
-and one of a beam search: ``kv_resize``, ``kv_append`` and ``attn_decode`` as for
-any token, then ``table, held, lens, missing = kv_fork(..., parents)``.
+and one of a beam search::
+
+    table, held, lens, missing = kv_fork(k_cache, v_cache, table, held, lens, refs, parents)
+    kv_resize(table, held, lens + 1, refs, page_size)
+    grown = (held * page_size - lens).clamp(0, 1)                 # 0 where pages ran out
+    lens += grown
+    kv_append(k, v, k_cache, v_cache, table, lens, grown)         # k/v [B, Hkv, 1, D]
+    o = attn_decode(q, k_cache, v_cache, table, lens)
+
+Nor may lengths be shortened into a page that other sequences hold (``kv_fork``
+shares full pages) and then grow there: appends would write to it.
 """
 from __future__ import annotations
 
@@ -115,7 +128,10 @@ def kv_fork(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Ten
     Returns ``(block_table, held, seq_lens, missing)`` of the new sequences, int32
     ``[n, W]`` (-1 behind a row's pages), ``[n]``, ``[n]`` and ``[1]``.  If there are fewer free
     pages than copies, ``missing`` says how many are lacking, nothing is changed
-    and the new sequences are empty; the given tensors are still valid then.
+    and the new sequences are empty; the given tensors are still valid then and
+    hold all their pages, so they had better be kept until ``missing`` has been
+    read.  One pair of cache tensors is served: layers that share a table are kept
+    as heads of one.
     """
     return rocm_attn_ext.kv_fork(k_cache, v_cache, block_table, held, seq_lens, refs, parents, bounds)
 
@@ -125,10 +141,12 @@ def kv_resize(block_table: torch.Tensor, held: torch.Tensor, seq_lens: torch.Ten
     """Make every sequence hold the pages that its length needs: pages behind
     are given back, pages that it lacks are taken from the free ones.  A length
     of zero gives back all.  Changes ``block_table``, ``held`` and ``refs`` in place;
-    entries of the table behind those held stay as they are.
+    entries of the table behind those held stay as they are, and lengths must not
+    reach them: their pages may be other sequences'.
 
     Pages that the call frees are given out from the next call on.  A sequence
     for which too few are free, those for the sequences before it counted, takes
-    none.  Returns int32 ``[B]``: the pages that such a sequence lacked, else 0.
+    none, and ``held[b] * page_size`` tokens are all it has room for.  Returns int32
+    ``[B]``: the pages that such a sequence lacked, else 0.
     """
     return rocm_attn_ext.kv_resize(block_table, held, seq_lens, refs, int(page_size))

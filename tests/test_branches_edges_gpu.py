@@ -191,3 +191,90 @@ def test_fork_refuses_bounds_that_do_not_fit(attn):
         with pytest.raises(RuntimeError, match="bounds"):
             attn.kv_fork(k, k.clone(), t, h, n, r, p, bounds=bad)
     assert r.tolist() == [1, 1, 0, 0, 0, 0] and attn.check_status(0) == 0
+
+
+# ---------------------------------------------------------------------------
+# Steps when pages run out
+# ---------------------------------------------------------------------------
+
+
+def _alone(cache, table, n):
+    """The tokens of a sequence, in order: [Hkv, n, D]."""
+    ps = cache.shape[2]
+    t = torch.arange(n)
+    return cache.cpu()[table.cpu()[t // ps].long(), :, t % ps].transpose(0, 1)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("Hq", [2, 8, 32])
+def test_drafts_without_pages_leave_other_sequences_alone(attn, Hq, dtype):
+    # sequence 0 has given a page back that sequence 1 holds by now, the pool is empty, and 0 drafts across its
+    # page's end, 2 within its page: the documented step writes to what they hold, and nowhere else
+    Hkv, ps, S, D = 2, 16, 7, 64
+    kc, vc = (torch.zeros(5, Hkv, ps, D, dtype=dtype, device="cuda") for _ in range(2))
+    table, held, refs = torch.full((3, 4), -1, dtype=torch.int32, device="cuda"), ints([0] * 3).cuda(), ints([0] * 5).cuda()
+    assert not attn.kv_resize(table, held, ints([30, 0, 0]).cuda(), refs, ps).any()
+    assert not attn.kv_resize(table, held, ints([13, 0, 0]).cuda(), refs, ps).any()
+    lens = ints([13, 48, 3]).cuda()
+    assert not attn.kv_resize(table, held, lens, refs, ps).any()
+    assert int(table[0, 1]) == int(table[1, 0]) and held.tolist() == [1, 3, 1] and refs.tolist() == [1] * 5
+    x = _q(3, Hkv, 48, D, dtype, 4)
+    attn.kv_append(x.cuda(), x.neg().cuda(), kc, vc, table, lens, new_lens=lens)
+    dense = [x[b, :, :n] for b, n in enumerate(lens.tolist())]
+
+    lacks = attn.kv_resize(table, held, lens + S, refs, ps)
+    drafted = (held * ps - lens).clamp(0, S)
+    lens += drafted
+    assert lacks.tolist() == [1, 1, 0] and drafted.tolist() == [3, 0, 7] and drafted.dtype == torch.int32
+    x, q, par = _q(3, Hkv, S, D, dtype, 5), _q(3, Hq, S, D, dtype, 6), _trees(3, S)
+    attn.kv_append(x.cuda(), x.neg().cuda(), kc, vc, table, lens, drafted)
+    out = attn.attn_tree(q.cuda(), kc, vc, table, lens, par.cuda(), drafted)
+    k = torch.zeros(3, Hkv, 48, D, dtype=dtype)
+    for b, n in enumerate(drafted.tolist()):
+        dense[b] = torch.cat([dense[b], x[b, :, :n]], 1)
+        assert torch.equal(_alone(kc, table[b], int(lens[b])), dense[b])
+        assert torch.equal(_alone(vc, table[b], int(lens[b])), dense[b].neg())
+        k[b, :, :dense[b].shape[1]] = dense[b]
+    _close(out, tree_ref(q, k, k.neg(), ints([[0], [1], [2]]), lens.cpu(), par, drafted.cpu()), 48, dtype)
+
+    lens = attn.kv_compact(kc, vc, table, lens, ints([[1, -1], [-1, -1], [2, 5]]).cuda(), drafted)
+    attn.kv_resize(table, held, lens, refs, ps)
+    assert lens.tolist() == [14, 48, 5] and refs.tolist() == [1] * 5
+    for b, at in ((0, list(range(13)) + [14]), (1, list(range(48))), (2, [0, 1, 2, 5, 8])):
+        assert torch.equal(_alone(kc, table[b], int(lens[b])), dense[b][:, at])
+    assert attn.check_status(0) == 0
+
+
+def test_beams_without_pages_leave_other_sequences_alone(attn):
+    # five pages, all held in the end: a beam at its page's end stays as it is while others go on
+    Hkv, ps, D = 2, 4, 64
+    kc, vc = (torch.zeros(5, Hkv, ps, D, dtype=BF16, device="cuda") for _ in range(2))
+    table, held, refs = torch.full((1, 4), -1, dtype=torch.int32, device="cuda"), ints([0]).cuda(), ints([0] * 5).cuda()
+    lens = ints([6]).cuda()
+    assert not attn.kv_resize(table, held, lens, refs, ps).any()
+    x = _q(1, Hkv, 6, D, BF16)
+    attn.kv_append(x.cuda(), x.cuda(), kc, vc, table, lens)
+    dense = [x[0]] * 3
+    table, held, lens, missing = attn.kv_fork(kc, vc, table, held, lens, refs, ints([0, 0, 0]).cuda())
+    assert missing.tolist() == [0]  # four pages are held now
+    for turn in range(5):
+        attn.kv_resize(table, held, lens + 1, refs, ps)
+        grown = (held * ps - lens).clamp(0, 1)
+        lens += grown
+        assert grown.tolist() == ([1, 1, 1] if turn < 2 else [1, 0, 0])
+        x, q = _q(3, Hkv, 1, D, BF16, turn), _q(3, 4, 1, D, BF16, turn + 9)
+        attn.kv_append(x.cuda(), x.cuda(), kc, vc, table, lens, grown)
+        out = attn.attn_decode(q.cuda(), kc, vc, table, lens)
+        dense = [torch.cat([d, x[b]], 1) if g else d for b, (d, g) in enumerate(zip(dense, grown.tolist()))]
+        for b in range(3):
+            n = dense[b].shape[1]
+            assert torch.equal(_alone(kc, table[b], int(lens[b])), dense[b])
+            one = dense[b][None]
+            _close(out[b:b + 1], tree_ref(q[b:b + 1], one, one, ints([[0]]), ints([n])), n, BF16)
+    # a fork that lacks pages: the given tensors go on
+    assert lens.tolist() == [11, 8, 8]
+    new = attn.kv_fork(kc, vc, table, held, lens, refs, ints([0, 0, 0]).cuda())
+    assert new[3].item() == 2 and not new[1].any() and not new[2].any()
+    for b in range(3):
+        assert torch.equal(_alone(kc, table[b], int(lens[b])), dense[b])
+    assert attn.check_status(0) == 0
