@@ -681,7 +681,7 @@ struct TcMaps {
   CUtensorMap k, v;
   int rows, boxes;  // rows of a box, boxes of a tile; 0: no boxes, 16-byte copies
   unsigned long long wait_ns;
-  int lose;  // watchdog test build only: CTA 0's first K copy is for bytes that never come
+  int lose;  // watchdog test build only: CTA 0's first K copy is for bytes that never come, or is never told
 };
 
 // Whether the phase has completed, without waiting for it.
@@ -988,7 +988,12 @@ __global__ void __launch_bounds__(TcCfg<kD, kTwo>::kThreads, TcCfg<kD, kTwo>::kC
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv) {
             if (!does[kv]) continue;
-            if (lane == 0) mbar_arrive(full(kv, told_slot[kv]));
+#ifdef RA_WATCHDOG_TEST
+            const bool lost = maps.lose && blockIdx.x == 0 && told == 0 && kv == 0;
+#else
+            constexpr bool lost = false;
+#endif
+            if (lane == 0 && !lost) mbar_arrive(full(kv, told_slot[kv]));
             if (++told_slot[kv] == (kv ? C::kVSlots : C::kKSlots)) told_slot[kv] = 0;
           }
         }

@@ -7,6 +7,7 @@ import random
 import pytest
 import torch
 
+import test_branches_gpu
 from branches_ref import compact_ref, tree_ref
 from paged_ref import make_cache
 from test_branches_gpu import BF16, F16, F32, _close, _q, _trees, ints
@@ -41,6 +42,13 @@ def test_tree_lengths_behind_the_table(attn, ps, W, D, dtype, Hq, Hkv, S):
         out = attn.attn_tree(q.cuda(), k.cuda(), v.cuda(), table.cuda(), ln.cuda(), None if tree is None else tree.cuda())
         assert attn.check_status(0) == 8
         _close(out, tree_ref(q, k, v, table, ln, tree), cap, dtype)
+
+
+@pytest.mark.parametrize("lens,D,Hq,S,ps", [([300, 40], 128, 8, 9, 7), ([2000, 700], 64, 4, 30, 100), ([900], 256, 4, 12, 1),
+                                            ([3000, 50], 128, 8, 50, 7), ([700], 64, 16, 40, 100), ([2500], 64, 8, 9, 7)])
+def test_watchdog_where_copies_are_of_16_bytes(attn, lens, D, Hq, S, ps):
+    # pages that no box of 8 rows divides: the first copy's arrival is not told
+    test_branches_gpu.test_watchdog_fires_and_recovers(lens, D, Hq, S, ps)
 
 
 # ---------------------------------------------------------------------------
