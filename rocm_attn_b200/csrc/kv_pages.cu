@@ -19,6 +19,8 @@
 #include <limits.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "key_bounds.cuh"
 #include "paged_cache.h"
 #include "sm100_ptx.cuh"
@@ -478,9 +480,14 @@ struct CompactArgs {
   int n;
   int* lens;
   int cols;  // 16-byte (or element) columns of a row
-  void* bounds;             // page bounds, or null
+};
+// (Apart, as a launch takes longer with them: 4.9 us from the host instead of 4.4.)
+struct CompactBoundsArgs : CompactArgs {
+  void* bounds;             // page bounds
   long long b_p, b_h, b_m;  // their strides over (page, head, min/max)
 };
+template <bool kBounds>
+using CompactArgsOf = typename std::conditional<kBounds, CompactBoundsArgs, CompactArgs>::type;
 
 // Warp (b, head), lane a column of K or V: a kept token's place is never behind
 // it, and the places of the tokens of one turn never among the sources of a later one, so
@@ -492,7 +499,7 @@ struct CompactArgs {
 constexpr int kMoveWarps = 4, kMoveAhead = 16;
 
 template <typename E, int kVec, bool kBounds>
-__global__ void __launch_bounds__(kMoveWarps * 32) kv_compact_kernel(const __grid_constant__ CompactArgs a) {
+__global__ void __launch_bounds__(kMoveWarps * 32) kv_compact_kernel(const __grid_constant__ CompactArgsOf<kBounds> a) {
   using V = Vec<E, kVec>;
   launch_dependents();
   grid_dependency_wait();
@@ -531,7 +538,9 @@ __global__ void __launch_bounds__(kMoveWarps * 32) kv_compact_kernel(const __gri
       to_page = paged_page(a.c, b, tp, &fault);
     }
     const unsigned moves = __ballot_sync(0xffffffffu, from_page >= 0 && to_page >= 0);
-    const unsigned crosses = __ballot_sync(0xffffffffu, from_page >= 0 && to_page >= 0 && from_page != to_page);
+    unsigned crosses = 0;  // those of them that change pages
+    if constexpr (kBounds)
+      crosses = __ballot_sync(0xffffffffu, from_page >= 0 && to_page >= 0 && from_page != to_page);
     for (int half = 0; half < 32; half += kMoveAhead) {
       if ((moves >> half & (0xffffffffu >> (32 - kMoveAhead))) == 0) continue;
       for (int c0 = 0; c0 < 2 * a.cols; c0 += 32) {
@@ -549,12 +558,14 @@ __global__ void __launch_bounds__(kMoveWarps * 32) kv_compact_kernel(const __gri
         long long open = -1;  // the page whose bounds are to take in lo and hi
         V lo = {}, hi = {};
         auto close = [&] {
-          if (open < 0) return;
-          E* to = static_cast<E*>(a.bounds) + open * a.b_p + h * a.b_h + static_cast<long long>(c) * kVec;
-          V *to_lo = reinterpret_cast<V*>(to), *to_hi = reinterpret_cast<V*>(to + a.b_m);
-          if constexpr (kBounds) fold(lo, hi, *to_lo, *to_hi);
-          *to_lo = lo;
-          *to_hi = hi;
+          if constexpr (kBounds) {
+            if (open < 0) return;
+            E* to = static_cast<E*>(a.bounds) + open * a.b_p + h * a.b_h + static_cast<long long>(c) * kVec;
+            V *to_lo = reinterpret_cast<V*>(to), *to_hi = reinterpret_cast<V*>(to + a.b_m);
+            fold(lo, hi, *to_lo, *to_hi);
+            *to_lo = lo;
+            *to_hi = hi;
+          }
         };
 #pragma unroll
         for (int p = 0; p < kMoveAhead; ++p) {
@@ -639,7 +650,8 @@ int check_bounds(const AttnPagedCache* c, const void* bounds, const long long* s
 }
 
 template <typename E, int kVec, bool kBounds>
-bool launch_compact(const CompactArgs& a, cudaStream_t stream) {
+bool launch_compact(const CompactBoundsArgs& args, cudaStream_t stream) {
+  const CompactArgsOf<kBounds>& a = args;
   const long long warps = static_cast<long long>(a.c.B) * a.c.heads;
   return launch_after(kv_compact_kernel<E, kVec, kBounds>, dim3(static_cast<unsigned>((warps + kMoveWarps - 1) / kMoveWarps)),
                       dim3(kMoveWarps * 32), 0, stream, 1, true, a);
@@ -668,7 +680,7 @@ extern "C" int launch_kv_compact_bounds(const AttnPagedCache* cache, const int* 
                                         long long kept_stride, int n, int* lens, void* bounds,
                                         const long long* bounds_strides, cudaStream_t stream) {
   using namespace ra;
-  CompactArgs a;
+  CompactBoundsArgs a;
   int st = check_paged_cache(cache, kCacheK | kCacheV, &a.c);
   if (st != ATTN_OK) return st;
   if (n < 0 || kept_stride < 0) return ATTN_ERR_INVALID_ARGUMENT;
