@@ -21,9 +21,8 @@
 //   up to 8, 16-bit   attn_decode's kernel, the rows as columns of mma.sync: 17
 //                     sequences of up to 2047 tokens, 16 kv heads of 64, five
 //                     rows 32.4 us, 35.5 here
-//   up to 128         tcgen05, tiles of 64 tokens, two CTAs per SM whose chains
-//                     of product, softmax and product fill each other's waits:
-//                     273 MB in 62 us, of which the join takes 3
+//   up to 128         tcgen05, tiles of 64 tokens, two CTAs per SM: 273 MB in 61
+//                     to 65 us on different GPUs, of which the join takes 3
 //   above             tcgen05, 256 rows in two streams over the same tiles of
 //                     128 tokens: K and V cross the copy engine once for both
 //   fp32, odd strides dot products on the plain cores
@@ -366,11 +365,12 @@ __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wai
 // .. 3}: scores of tokens tx + 16 {0 .. 3}, and of O the columns 4 tx + {0 .. 3}
 // + 64 j.  K and V lie in 32 bits, in a buffer each where copies of 16 bytes can
 // fill them (kWide: fp32, 16-byte rows), so that the next tile's come while this
-// one is worked on; else one after the other in one buffer.  fp32, us (in brackets
-// one buffer and an element per load): 3 sequences of 1500 tokens, 16/4 heads of
-// 64, 7 drafted 16.0 (30.5); 16 of up to 8192 96.9 (446); 16 of up to 4096, 32/8
-// heads of 128, 8 drafted 227 (808); 8 of up to 4096, 16/4 of 256 152 (596).  It
-// costs CTAs per SM (4, 2 and 1 at D = 64, 128 and 256 instead of 5, 3 and 2).
+// one is worked on; else one after the other in one buffer.  fp32, n sequences of
+// 1/n, 2/n ... of the given length, us (in brackets one buffer and an element per
+// load): 3 of 1500 tokens, 16/4 heads of 64, 7 drafted 16.0 (30.5); 16 of 8192 97
+// (446); 16 of 4096, 32/8 heads of 128, 8 drafted 227 (808); 8 of 4096, 16/4 of
+// 256, 8 drafted 152 (596).  16 bits, element by element: 16 of 4096, 32/8 heads of
+// 100, 8 drafted 374.  Two buffers cost CTAs per SM (4, 2 and 1 at D = 64, 128 and 256 instead of 5, 3 and 2).
 constexpr int kSimtThreads = 128, kSimtRows = 32, kSimtTile = 64;
 
 template <int kDP, bool kWide>
@@ -613,12 +613,19 @@ __global__ void __launch_bounds__(kSimtThreads) attn_tree_simt_kernel(const __gr
 // for 64 KB as an SM's share, the K and V of 128 tokens at D = 128.
 //   up to 128 rows   tiles of 64 tokens, two score buffers, so that S(j + 1) is
 //                    there when the softmax of tile j ends; two CTAs per SM (one
-//                    at D = 256) hide each other's waits and ends of units.
+//                    at D = 256).  With 64 rows each takes 3390 clocks for a tile,
+//                    the two of an SM 1690, where reading takes 1400 and the
+//                    chain of product, softmax and product alone 1600; no unit
+//                    is busy, and which wait it is has not been found.  One CTA with
+//                    two tiles in turn is slower (66 to 76 us for 62).
 //                    Q of the next unit is copied during this one where there
-//                    is room: a load takes some 5000 clocks beside so many copies.
+//                    is room (up to 64 rows; at D = 64 up to 128): a load takes
+//                    some 5000 clocks beside so many copies.
 //   more rows        256 at a time over the same tiles of 128 tokens: two
 //                    streams, each with its S and O in tensor memory and a
-//                    warpgroup for the softmax, one CTA per SM.
+//                    warpgroup for the softmax, one CTA per SM.  A tile's chain
+//                    is 3900 clocks; Q of the next unit is asked for when this
+//                    one has ended.
 // Warp roles: softmax warpgroups, then one warp of which a thread issues the
 // products, and one that copies K and V (one for each with two streams), page ids
 // looked up ahead: boxes of rows by TMA where 8 divides the page size, else by
@@ -1796,8 +1803,9 @@ extern "C" int launch_attn_tree(const AttnPagedCache* cache, const void* q, cons
   // Up to eight rows (which must lie evenly in memory) fill one column tile of
   // attn_decode's products, where a tile's softmax is not one warp's work of some
   // 1100 clocks: 8 rows, D = 128, that kernel / this one, us: one sequence of 4096
-  // tokens 14.3 / 19.5, 24 of up to 4096 57.0 / 62.5, 16 of up to 16384 138 / 154;
-  // 16 rows 19.9 / 19.7, 77.4 / 63.2, 172 / 155.
+  // tokens 14.6 / 17.3, of 517 10.4 / 9.8, 24 of up to 4096 55 to 60 / 54, 16 of up
+  // to 16384 124 to 133 / 133 to 139; five rows, D = 64, pages of 24 (no box of 16)
+  // 32.4 / 35.5.  16 rows: one of 4096 19.9 / 19.7, 24 77.4 / 63.2, 16 172 / 155.
   const bool even = S == 1 || Hq == 1 || qs[1] == S * qs[2];
   size_t few = 0;
   if (fast && even && decode_rows_plan(cache, Hq, S, sms, &few)) {
