@@ -201,6 +201,54 @@ def test_fork_refuses_bounds_that_do_not_fit(attn):
     assert r.tolist() == [1, 1, 0, 0, 0, 0] and attn.check_status(0) == 0
 
 
+@pytest.mark.parametrize("dtype,D", [(F16, 64), (BF16, 100), (F32, 128)])
+def test_captured_steps_keep_page_bounds(attn, dtype, D):
+    # one captured step (drafts, compaction, fork) over two layers kept as heads of one cache, replayed over changing
+    # data on another stream; each layer's compaction is given its heads of cache and bounds
+    ps, P, W, B, S, H = 8, 120, 9, 4, 6, 2
+    kc, vc = (torch.zeros(P, 2 * H, ps, D, dtype=dtype, device="cuda") for _ in range(2))
+    bounds = torch.zeros(P, 2 * H, 2, D, dtype=dtype, device="cuda")
+    table, held, refs = torch.full((B, W), -1, dtype=torch.int32, device="cuda"), ints([0] * B).cuda(), ints([0] * P).cuda()
+    lens, parents, kept = ints([0] * B).cuda(), ints([0] * B).cuda(), ints([[-1] * S] * B).cuda()
+    x = torch.zeros(B, 2 * H, S, D, dtype=dtype, device="cuda")
+    layers = [slice(0, H), slice(H, 2 * H)]
+
+    def step():
+        attn.kv_resize(table, held, lens + S, refs, ps)
+        drafted = (held * ps - lens).clamp(0, S)
+        lens.add_(drafted)
+        after = None
+        for h in layers:
+            attn.kv_append(x[:, h], x[:, h], kc[:, h], vc[:, h], table, lens, drafted, bounds=bounds[:, h])
+        for h in layers:
+            after = attn.kv_compact(kc[:, h], vc[:, h], table, lens, kept, drafted, bounds=bounds[:, h])
+        attn.kv_resize(table, held, after, refs, ps)
+        t, n, l, missing = attn.kv_fork(kc, vc, table, held, after, refs, parents, bounds=bounds)
+        table.copy_(t), held.copy_(n), lens.copy_(l)
+        return missing
+
+    side = torch.cuda.Stream()
+    step()  # from nothing to nothing: no token is kept
+    assert lens.tolist() == [0] * B and int(refs.sum()) == 0
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        missing = step()
+    rng, want = random.Random(D), [0] * B
+    for turn in range(10):
+        par = [rng.randrange(B) for _ in range(B)]
+        paths = [sorted(rng.sample(range(S), rng.randint(0, S - 1))) for _ in range(B)]
+        want = [want[p] + len(paths[p]) for p in par]
+        x.copy_((turn + 1) * _q(B, 2 * H, S, D, dtype, turn))
+        parents.copy_(ints(par)), kept.copy_(ints([p + [-1] * (S - len(p)) for p in paths]))
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            g.replay()
+        torch.cuda.current_stream().wait_stream(side)
+        assert missing.tolist() == [0] and lens.tolist() == want
+        _check_bounds(bounds, kc, table, lens)
+    assert max(want) > ps and attn.check_status(0) == 0
+
+
 # ---------------------------------------------------------------------------
 # Steps when pages run out
 # ---------------------------------------------------------------------------
